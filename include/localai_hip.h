@@ -263,6 +263,109 @@ int localai_hip_delta_net_step(float *state_dev, const float *q_dev, const float
                                const float *decay_dev, const float *beta_dev, float *core_dev, int heads,
                                int key_dim, int value_dim, void *stream);
 
+/* ---- paged key / value cache: several requests in one step ---------------- */
+
+/* One layer of a paged cache: value d of position p of kv head h of a request
+ * whose page table row is `row` is at
+ *   row[p / page_size] * page_stride + h * head_stride + (p % page_size) * pos_stride + d
+ * of k_dev and of v_dev (strides in values, the same for both). type: 0 fp32,
+ * 1 fp16, 30 bf16 (GGML numbers). page_size a power of two, at least 16;
+ * n_pages * page_size below 2^31; head_dim 64, 128 or 256; buffers 16-byte
+ * aligned, strides multiples of 16 bytes. The reference serves one request
+ * from a contiguous fp32 cache (engine/model.py:6-9), which is one page. */
+typedef struct localai_paged_cache {
+    void *k_dev, *v_dev;
+    int type, n_kv_heads, head_dim, page_size;
+    int64_t n_pages, page_stride, head_stride, pos_stride;
+} localai_paged_cache;
+
+/* Page tables and slots of a step's new tokens, from request lengths (all
+ * int32, on the device; nothing is read by the host). Request b has lengths[b]
+ * positions cached and gets fresh[b] >= 0 more; P(x) = ceil(x / page_size):
+ *   table[b][P(lengths[b]) ..] = the next pages of free[used ..], requests in order
+ *   starts[b] = sum of fresh before b;  starts[requests] = all new tokens
+ *   token t in [starts[b], starts[b + 1]): positions[t] = lengths[b] + t - starts[b],
+ *     slots[t] = table[b][positions[t] / page_size] * page_size + positions[t] % page_size
+ *   slots[t] = positions[t] = -1 for starts[requests] <= t < tokens
+ *   lengths_out[b] = lengths[b] + fresh[b];  used_out = used + pages handed out
+ * lengths_out may be lengths and used_out may be used; no other buffers may
+ * overlap. table is [requests, table_stride] of which max_pages columns are
+ * used; only the new pages' entries are written. free: a list of n_pages page
+ * ids, of which the first `used` are in use. *status is 0, or a sum of 1 (the
+ * pool has too few pages left), 2 (a negative length or count, or a request
+ * past max_pages), 4 (more than `tokens` new tokens): then no table entry,
+ * length or count changes, every start is 0, and every slot -1.
+ * A table entry or list that names no page of the pool gives slot -1.
+ * requests <= 4096; max_pages * page_size below 2^31. */
+int localai_hip_paged_extend(const int32_t *lengths_dev, const int32_t *fresh_dev, int64_t requests,
+                             int32_t *table_dev, int64_t table_stride, int64_t max_pages,
+                             const int32_t *free_dev, int64_t n_pages, const int32_t *used_dev, int page_size,
+                             int64_t tokens, int32_t *lengths_out_dev, int32_t *used_out_dev,
+                             int32_t *starts_dev, int32_t *slots_dev, int32_t *positions_dev,
+                             int32_t *status_dev, void *stream);
+
+/* The inverse: request b keeps its first min(keep[b], lengths[b]) positions
+ * (0: it has ended; fewer: drafted tokens are taken back). lengths, used,
+ * table and free are updated in place: pages that hold nothing any more
+ * return to the list in the order in which localai_hip_paged_extend would
+ * hand them out again, their table entries become -1. *status as above (2
+ * also for used > n_pages, 1 for more pages returned than in use): not 0
+ * means nothing changed. */
+int localai_hip_paged_shrink(int32_t *lengths_dev, const int32_t *keep_dev, int64_t requests, int32_t *table_dev,
+                             int64_t table_stride, int64_t max_pages, int32_t *free_dev, int64_t n_pages,
+                             int32_t *used_dev, int page_size, int32_t *status_dev, void *stream);
+
+/* Per new token t: q and k normed per head (engine/qwen35.py:158-182's q and k
+ * norms) and rotated (engine/model.py:203-210), q written to q_out_dev, k and
+ * the plain v to slot slots[t] of the cache, rounded to its type (nearest
+ * even; past fp16's range infinite):
+ *   y = x / sqrt(mean(x^2) + eps) * w     (q_w_dev / k_w_dev [head_dim]; NULL: y = x)
+ *   pairs (halves = 0): (y[2j], y[2j + 1]), halves = 1: (y[j], y[j + n_freq])
+ *     rotated by positions[t] * freq[j] radians, j < n_freq; the rest as it is
+ * freq_dev: fp64 [n_freq], 2 n_freq <= head_dim (n_freq 0: no rotation). fp32
+ * throughout but for the angle, which is fp64 until less than one turn is left.
+ * q [tokens, n_heads, head_dim], k, v [tokens, n_kv_heads, head_dim] fp32 with
+ * strides[0..7] = token and head stride of q, k, v, q_out in values (host
+ * array; multiples of 4; views of one fused projection will do). q_out may be
+ * q with q's strides. A token whose slot is outside [0, n_pages * page_size)
+ * is padding: it reads nothing and its row of q_out stays as it was. Slots of
+ * one call must differ from each other. All 16-byte aligned but the index and
+ * weight arrays. */
+int localai_hip_norm_rope_store(const float *q_dev, const float *k_dev, const float *v_dev, const int64_t *strides,
+                                int64_t tokens, int n_heads, const int32_t *positions_dev, const int32_t *slots_dev,
+                                const double *freq_dev, int n_freq, int halves, const float *q_w_dev,
+                                const float *k_w_dev, float eps, float *q_out_dev,
+                                const localai_paged_cache *cache, void *stream);
+
+/* Bytes of workspace localai_hip_paged_attention needs (partial results of
+ * split lengths); -1 for invalid sizes. Calls that may overlap in time need
+ * separate workspaces; its contents mean nothing between calls. */
+int64_t localai_hip_paged_attention_workspace_size(int64_t tokens, int64_t requests, int n_heads, int n_kv_heads,
+                                                   int head_dim);
+
+/* Attention of each request's new tokens over its pages (the tokens' own k and
+ * v already stored), the batched, paged form of localai_hip_attention_decode:
+ * token i of the n_b new ones of request b is at p = lengths[b] - n_b + i and
+ * sees s in [max(0, p + 1 - window), p] (window 0: from 0):
+ *   out_h = softmax_s(scale q_h . K[s]) V[s]      (query head h, kv head h / (n_heads / n_kv_heads))
+ *   out_h *= 1 / (1 + exp(-clip(gate_h, -80, 80)))                        (gate_dev not NULL)
+ * lengths count the new tokens. starts_dev [requests + 1]: request b's rows of
+ * q, gate and out are starts[b] .. starts[b + 1] - 1 (rows from
+ * starts[requests] on stay as they were); NULL: one row per request (tokens =
+ * requests). q, gate, out fp32 [tokens, n_heads, head_dim]. A row that sees
+ * nothing (length 0) is zeros. A row whose range reaches past max_pages or a
+ * page id outside [0, n_pages) is NaN, and nothing outside the cache is read.
+ * Cached values of unseen positions may be anything, NaN included.
+ * fp32 results: caches of 16 bits are read exactly, queries and probabilities
+ * keep at least 21 bits in the products. How a length is split depends on all
+ * requests of the call, so a row's last bits can differ between batches; the
+ * same call gives the same bits. */
+int localai_hip_paged_attention(const float *q_dev, int64_t tokens, int n_heads, const localai_paged_cache *cache,
+                                const int32_t *table_dev, int64_t table_stride, int64_t max_pages,
+                                const int32_t *lengths_dev, const int32_t *starts_dev, int64_t requests,
+                                int64_t window, float scale, const float *gate_dev, float *out_dev,
+                                void *workspace_dev, int64_t workspace_bytes, void *stream);
+
 /* ---- ZAYA router (engine/zaya.py:274-307) -------------------------------- */
 
 /* Everything of ZAYA's router after the first projection r0 = W_inp h

@@ -17,6 +17,13 @@ STATUS = {0: 'OK', 1: 'EARG', 2: 'ETYPE', 3: 'EHIP', 4: 'ENOMEM', 5: 'ESTATE'}
 _c_int, _c_i64, _vp = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
 _u8p, _f32p = ctypes.POINTER(ctypes.c_uint8), ctypes.POINTER(ctypes.c_float)
 
+class PagedCacheArg(ctypes.Structure):
+    """localai_paged_cache"""
+    _fields_ = [('k_dev', _vp), ('v_dev', _vp), ('type', _c_int), ('n_kv_heads', _c_int), ('head_dim', _c_int),
+                ('page_size', _c_int), ('n_pages', _c_i64), ('page_stride', _c_i64), ('head_stride', _c_i64),
+                ('pos_stride', _c_i64)]
+
+
 # name -> (restype, argtypes); mirrors include/localai_hip.h
 SIGNATURES = {
     'localai_hip_version': (_c_int, []),
@@ -61,6 +68,14 @@ SIGNATURES = {
     'localai_hip_attention_decode': (_c_int, [_vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_int, _c_int, _c_int,
                                               _c_i64, _vp, _vp, _vp, _c_i64, _vp]),
     'localai_hip_delta_net_step': (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp]),
+    'localai_hip_paged_extend': (_c_int, [_vp, _vp, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _c_int, _c_i64, _vp,
+                                          _vp, _vp, _vp, _vp, _vp, _vp]),
+    'localai_hip_paged_shrink': (_c_int, [_vp, _vp, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _c_int, _vp, _vp]),
+    'localai_hip_norm_rope_store': (_c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_int, _vp, _vp, _vp, _c_int, _c_int, _vp,
+                                             _vp, ctypes.c_float, _vp, ctypes.POINTER(PagedCacheArg), _vp]),
+    'localai_hip_paged_attention_workspace_size': (_c_i64, [_c_i64, _c_i64, _c_int, _c_int, _c_int]),
+    'localai_hip_paged_attention': (_c_int, [_vp, _c_i64, _c_int, ctypes.POINTER(PagedCacheArg), _vp, _c_i64, _c_i64,
+                                             _vp, _vp, _c_i64, _c_i64, ctypes.c_float, _vp, _vp, _vp, _c_i64, _vp]),
     'localai_hip_debug_fused_wait': (_c_int, [_c_int, _c_int]),
     'localai_hip_register_host': (_c_int, [_vp, ctypes.c_size_t]),
     'localai_hip_unregister_host': (_c_int, [_vp]),

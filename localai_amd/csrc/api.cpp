@@ -7,6 +7,7 @@
 #include <string>
 
 #include "internal.h"
+#include "paged.h"
 
 namespace lq {
 
@@ -601,6 +602,139 @@ int localai_hip_moe_forward(const float *h, int64_t T, int64_t H, const float *r
         return fail(LOCALAI_EARG, "moe: h and router_w must be 16-byte and workspace 256-byte aligned");
     if (int st = ensure_device()) return st;
     return launch_moe(h, T, H, rw, rb, E, k, gu, dn, out, topk_idx, topk_w, ws, (hipStream_t)stream);
+}
+
+// ---- paged key / value cache ----
+
+static int paged_sizes(const char *who, int64_t requests, int64_t table_stride, int64_t max_pages, int64_t n_pages,
+                       int page_size) {
+    const std::string w = who;
+    if (requests < 1 || requests > PAGED_MAX_REQUESTS) return fail(LOCALAI_EARG, w + ": requests must be in 1..4096");
+    if (page_size < 16 || (page_size & (page_size - 1)))
+        return fail(LOCALAI_EARG, w + ": page_size must be a power of two, at least 16");
+    if (n_pages < 1 || n_pages > INT32_MAX / page_size)
+        return fail(LOCALAI_EARG, w + ": n_pages * page_size must be in 1..2^31 - 1");
+    if (max_pages < 1 || max_pages > INT32_MAX / page_size || table_stride < max_pages)
+        return fail(LOCALAI_EARG, w + ": max_pages must be >= 1, at most table_stride, and max_pages * page_size below 2^31");
+    return LOCALAI_OK;
+}
+
+static int paged_cache_of(const char *who, const localai_paged_cache *c, PagedCache *out) {
+    const std::string w = who;
+    if (!c || !c->k_dev || !c->v_dev) return fail(LOCALAI_EARG, w + ": null cache");
+    if (c->type != PAGED_F32 && c->type != PAGED_F16 && c->type != PAGED_BF16)
+        return fail(LOCALAI_ETYPE, w + ": the cache holds fp32 (0), fp16 (1) or bf16 (30)");
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+        return fail(LOCALAI_ETYPE, w + ": head_dim 64, 128 or 256");
+    if (c->n_kv_heads < 1) return fail(LOCALAI_EARG, w + ": n_kv_heads must be >= 1");
+    if (int st = paged_sizes(who, 1, 1, 1, c->n_pages, c->page_size)) return st;
+    const int64_t unit = c->type == PAGED_F32 ? 4 : 8;
+    if (c->page_stride % unit || c->head_stride % unit || c->pos_stride % unit ||
+        ((reinterpret_cast<uintptr_t>(c->k_dev) | reinterpret_cast<uintptr_t>(c->v_dev)) & 15))
+        return fail(LOCALAI_EARG, w + ": cache buffers must be 16-byte aligned, strides multiples of 16 bytes");
+    if (c->pos_stride < c->head_dim || (c->n_kv_heads > 1 && c->head_stride < c->head_dim) ||
+        (c->n_pages > 1 && c->page_stride < c->head_dim))
+        return fail(LOCALAI_EARG, w + ": cache strides must be at least head_dim");
+    // offsets inside a page are 32-bit
+    if ((int64_t)(c->page_size - 1) * c->pos_stride + c->head_dim > INT32_MAX / 4)
+        return fail(LOCALAI_EARG, w + ": a page's positions must lie within 2 GiB");
+    *out = PagedCache{c->k_dev, c->v_dev, c->type, (int)c->n_pages, c->page_size,
+                      c->page_stride, c->head_stride, c->pos_stride};
+    return LOCALAI_OK;
+}
+
+int localai_hip_paged_extend(const int32_t *lengths, const int32_t *fresh, int64_t requests, int32_t *table,
+                             int64_t table_stride, int64_t max_pages, const int32_t *free_list, int64_t n_pages,
+                             const int32_t *used, int page_size, int64_t tokens, int32_t *lengths_out,
+                             int32_t *used_out, int32_t *starts, int32_t *slots, int32_t *positions,
+                             int32_t *status, void *stream) {
+    clear_error();
+    if (!lengths || !fresh || !table || !free_list || !used || !lengths_out || !used_out || !starts || !status ||
+        (tokens > 0 && (!slots || !positions)))
+        return fail(LOCALAI_EARG, "paged extend: null pointer");
+    if (tokens < 0 || tokens > INT32_MAX) return fail(LOCALAI_EARG, "paged extend: tokens must be in 0..2^31 - 1");
+    if (int st = paged_sizes("paged extend", requests, table_stride, max_pages, n_pages, page_size)) return st;
+    if (int st = ensure_device()) return st;
+    return launch_paged_extend(lengths, fresh, (int)requests, table, table_stride, (int)max_pages, free_list,
+                               (int)n_pages, used, page_size, tokens, lengths_out, used_out, starts, slots, positions,
+                               status, (hipStream_t)stream);
+}
+
+int localai_hip_paged_shrink(int32_t *lengths, const int32_t *keep, int64_t requests, int32_t *table,
+                             int64_t table_stride, int64_t max_pages, int32_t *free_list, int64_t n_pages,
+                             int32_t *used, int page_size, int32_t *status, void *stream) {
+    clear_error();
+    if (!lengths || !keep || !table || !free_list || !used || !status)
+        return fail(LOCALAI_EARG, "paged shrink: null pointer");
+    if (int st = paged_sizes("paged shrink", requests, table_stride, max_pages, n_pages, page_size)) return st;
+    if (int st = ensure_device()) return st;
+    return launch_paged_shrink(lengths, keep, (int)requests, table, table_stride, (int)max_pages, free_list,
+                               (int)n_pages, used, page_size, status, (hipStream_t)stream);
+}
+
+int localai_hip_norm_rope_store(const float *q, const float *k, const float *v, const int64_t *strides,
+                                int64_t tokens, int n_heads, const int32_t *positions, const int32_t *slots,
+                                const double *freq, int n_freq, int halves, const float *q_w, const float *k_w,
+                                float eps, float *q_out, const localai_paged_cache *cache, void *stream) {
+    clear_error();
+    PagedCache c;
+    if (int st = paged_cache_of("norm rope store", cache, &c)) return st;
+    if (tokens < 0 || tokens > INT32_MAX) return fail(LOCALAI_EARG, "norm rope store: tokens must be in 0..2^31 - 1");
+    if (n_heads < 1 || n_heads > 65536 || cache->n_kv_heads > 65536)
+        return fail(LOCALAI_EARG, "norm rope store: n_heads and n_kv_heads must be in 1..65536");
+    if (n_freq < 0 || 2 * (int64_t)n_freq > cache->head_dim || (n_freq && !freq))
+        return fail(LOCALAI_EARG, "norm rope store: 0 <= 2 n_freq <= head_dim, with n_freq frequencies");
+    if (halves != 0 && halves != 1) return fail(LOCALAI_EARG, "norm rope store: halves is 0 or 1");
+    if (!tokens) return LOCALAI_OK;
+    if (!q || !k || !v || !strides || !positions || !slots || !q_out)
+        return fail(LOCALAI_EARG, "norm rope store: null pointer");
+    for (int i = 0; i < 8; ++i)
+        if (strides[i] % 4 || strides[i] < 0)
+            return fail(LOCALAI_EARG, "norm rope store: strides must be multiples of 4 values");
+    const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
+                          reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(q_out);
+    if (all & 15) return fail(LOCALAI_EARG, "norm rope store: q, k, v and q_out must be 16-byte aligned");
+    if (int st = ensure_device()) return st;
+    return launch_norm_rope_store(q, k, v, strides, tokens, n_heads, cache->n_kv_heads, cache->head_dim, positions,
+                                  slots, freq, n_freq, halves ? 0 : 1, q_w, k_w, eps, q_out, c, (hipStream_t)stream);
+}
+
+int64_t localai_hip_paged_attention_workspace_size(int64_t tokens, int64_t requests, int n_heads, int n_kv,
+                                                   int head_dim) {
+    if (tokens < 0 || tokens > INT32_MAX || requests < 1 || requests > PAGED_MAX_REQUESTS || n_heads < 1 ||
+        n_heads > 65535 || n_kv < 1 || n_heads % n_kv || (head_dim != 64 && head_dim != 128 && head_dim != 256))
+        return -1;
+    return (int64_t)paged_attention_workspace_bytes(tokens, (int)requests, n_heads, n_kv, head_dim);
+}
+
+int localai_hip_paged_attention(const float *q, int64_t tokens, int n_heads, const localai_paged_cache *cache,
+                                const int32_t *table, int64_t table_stride, int64_t max_pages,
+                                const int32_t *lengths, const int32_t *starts, int64_t requests, int64_t window,
+                                float scale, const float *gate, float *out, void *ws, int64_t ws_bytes,
+                                void *stream) {
+    clear_error();
+    PagedCache c;
+    if (int st = paged_cache_of("paged attention", cache, &c)) return st;
+    if (int st = paged_sizes("paged attention", requests, table_stride, max_pages, cache->n_pages, cache->page_size))
+        return st;
+    if (tokens < 0 || tokens > INT32_MAX) return fail(LOCALAI_EARG, "paged attention: tokens must be in 0..2^31 - 1");
+    if (!starts && tokens != requests)
+        return fail(LOCALAI_EARG, "paged attention: without starts there is one token per request");
+    if (n_heads < 1 || n_heads > 65535 || n_heads % cache->n_kv_heads)
+        return fail(LOCALAI_EARG, "paged attention: n_heads must be a positive multiple of n_kv_heads (at most 65535)");
+    if (window < 0) return fail(LOCALAI_EARG, "paged attention: window must be >= 0");
+    if (!tokens) return LOCALAI_OK;
+    if (!q || !table || !lengths || !out) return fail(LOCALAI_EARG, "paged attention: null pointer");
+    const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(gate) |
+                          reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(ws);
+    if (all & 15) return fail(LOCALAI_EARG, "paged attention: every buffer must be 16-byte aligned");
+    const int64_t need = (int64_t)paged_attention_workspace_bytes(tokens, (int)requests, n_heads, cache->n_kv_heads,
+                                                                  cache->head_dim);
+    if (need > 0 && (!ws || ws_bytes < need)) return fail(LOCALAI_EARG, "paged attention: workspace too small");
+    if (int st = ensure_device()) return st;
+    const PagedQueries p{q, gate, out, tokens, n_heads, cache->n_kv_heads, cache->head_dim, (int)requests,
+                         table, lengths, starts, table_stride, (int)max_pages, window, scale};
+    return launch_paged_attention(p, c, ws, ws_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"
