@@ -296,7 +296,7 @@ typedef struct localai_paged_cache {
  * past max_pages), 4 (more than `tokens` new tokens): then no table entry,
  * length or count changes, every start is 0, and every slot -1.
  * A table entry or list that names no page of the pool gives slot -1.
- * requests <= 4096; max_pages * page_size below 2^31. */
+ * requests <= 4096; max_pages * page_size at most 2^30. */
 int localai_hip_paged_extend(const int32_t *lengths_dev, const int32_t *fresh_dev, int64_t requests,
                              int32_t *table_dev, int64_t table_stride, int64_t max_pages,
                              const int32_t *free_dev, int64_t n_pages, const int32_t *used_dev, int page_size,
@@ -355,7 +355,8 @@ int64_t localai_hip_paged_attention_workspace_size(int64_t tokens, int64_t reque
  * requests). q, gate, out fp32 [tokens, n_heads, head_dim]. A row that sees
  * nothing (length 0) is zeros. A row whose range reaches past max_pages or a
  * page id outside [0, n_pages) is NaN, and nothing outside the cache is read.
- * Cached values of unseen positions may be anything, NaN included.
+ * Cached values of positions that no new token of the request sees may be
+ * anything, NaN included. tokens <= 2^24, other limits as above.
  * fp32 results: caches of 16 bits are read exactly, queries and probabilities
  * keep at least 21 bits in the products. How a length is split depends on all
  * requests of the call, so a row's last bits can differ between batches; the

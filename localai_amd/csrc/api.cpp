@@ -614,8 +614,8 @@ static int paged_sizes(const char *who, int64_t requests, int64_t table_stride, 
         return fail(LOCALAI_EARG, w + ": page_size must be a power of two, at least 16");
     if (n_pages < 1 || n_pages > INT32_MAX / page_size)
         return fail(LOCALAI_EARG, w + ": n_pages * page_size must be in 1..2^31 - 1");
-    if (max_pages < 1 || max_pages > INT32_MAX / page_size || table_stride < max_pages)
-        return fail(LOCALAI_EARG, w + ": max_pages must be >= 1, at most table_stride, and max_pages * page_size below 2^31");
+    if (max_pages < 1 || max_pages > ((int64_t)1 << 30) / page_size || table_stride < max_pages)
+        return fail(LOCALAI_EARG, w + ": max_pages must be >= 1, at most table_stride, and max_pages * page_size at most 2^30");
     return LOCALAI_OK;
 }
 
@@ -701,7 +701,7 @@ int localai_hip_norm_rope_store(const float *q, const float *k, const float *v, 
 
 int64_t localai_hip_paged_attention_workspace_size(int64_t tokens, int64_t requests, int n_heads, int n_kv,
                                                    int head_dim) {
-    if (tokens < 0 || tokens > INT32_MAX || requests < 1 || requests > PAGED_MAX_REQUESTS || n_heads < 1 ||
+    if (tokens < 0 || tokens > 1 << 24 || requests < 1 || requests > PAGED_MAX_REQUESTS || n_heads < 1 ||
         n_heads > 65535 || n_kv < 1 || n_heads % n_kv || (head_dim != 64 && head_dim != 128 && head_dim != 256))
         return -1;
     return (int64_t)paged_attention_workspace_bytes(tokens, (int)requests, n_heads, n_kv, head_dim);
@@ -717,7 +717,7 @@ int localai_hip_paged_attention(const float *q, int64_t tokens, int n_heads, con
     if (int st = paged_cache_of("paged attention", cache, &c)) return st;
     if (int st = paged_sizes("paged attention", requests, table_stride, max_pages, cache->n_pages, cache->page_size))
         return st;
-    if (tokens < 0 || tokens > INT32_MAX) return fail(LOCALAI_EARG, "paged attention: tokens must be in 0..2^31 - 1");
+    if (tokens < 0 || tokens > 1 << 24) return fail(LOCALAI_EARG, "paged attention: tokens must be in 0..2^24");
     if (!starts && tokens != requests)
         return fail(LOCALAI_EARG, "paged attention: without starts there is one token per request");
     if (n_heads < 1 || n_heads > 65535 || n_heads % cache->n_kv_heads)

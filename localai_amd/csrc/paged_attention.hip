@@ -12,97 +12,661 @@ namespace lq {
 // + i; for query head h with kv head h / G:
 //   score_s = scale q_h . K[s],  s in [max(0, p + 1 - window), p]
 //   out_h   = sum_s softmax_s(score) V[s]     (times sigmoid(gate_h))
-// Nothing to see gives zeros; a page outside the pool, or a position past the
-// table, gives NaN, and nothing outside the cache is read.
+//
+// A wave takes 16 columns (query head, token) at once against tiles of
+// positions, all on MFMA:
+//   S^T [positions x columns] = K Q^T        O^T [d x columns] += V^T P^T
+// The result layout of the first product (lane: column l & 15, positions
+// 4 (l >> 4) + i) is the operand layout of the second once V's rows are taken
+// in the same order, so probabilities never leave their lane; a column's
+// running maximum and sum sit in the four lanes that hold it. K rows are read
+// as they lie (16 bytes of one position per lane); V rows too, 8 positions x 8
+// values per lane, transposed in registers by byte permutes.
+//
+// Precision: products of 16-bit caches are exact on MFMA, so only q and p are
+// rounded, and both are split: f16 into 2 pieces (22 bits; q scaled by a power
+// of two to [512, 1024), p by 2^14, so that small values keep their bits),
+// bf16 into 3 (24 bits). fp32 caches use fp32 MFMA. Sums, maxima and the
+// running statistics are fp32.
+//
+// Work: a block is TB tokens of one request, the columns of NT tiles; its
+// positions are cut into chunks, one per workgroup and kv head, of a length
+// that follows from all requests of the call (every wave sums the requests'
+// positions by itself, so the host reads nothing and a graph stays valid as
+// lengths grow). A workgroup's four waves take tiles in turn and meet in LDS;
+// blocks of several chunks are joined by a second launch.
 struct PagedArgs {
     PagedQueries p;
     PagedCache c;
-    int G, shift;
-    float scale2;      // scale * log2(e)
+    int G, GC, HG, tpt;  // query heads per kv head, per column group; groups; tokens per column tile
+    int shift, slots;    // workgroups per kv head and column group
+    float scale2;        // scale * log2(e)
+    float *part;         // [slots, n_kv, HG, 16 NT, HD] unscaled outputs of a chunk
+    float2 *ml;          // [slots, n_kv, HG, 16 NT] their maximum (base 2) and sum
+    int2 *rows;          // [tokens]: first slot << 6 | first column of the token's block, chunks
 };
 
-template <typename T, int HD>
-__global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
-    constexpr int N = HD / 64;
-    __shared__ float red_m[4], red_l[4], red_o[4][HD];
-    const int64_t t = blockIdx.x;
-    const int h = blockIdx.y, kh = h / a.G, lane = lane_id(), wave = wave_id();
-    int b = (int)t;
-    int64_t p = -1;
+typedef _Float16 pa_h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 pa_b8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ float bits_f(uint32_t v) { return __builtin_bit_cast(float, v); }
+__device__ __forceinline__ uint32_t f_bits(float v) { return __builtin_bit_cast(uint32_t, v); }
+
+// over lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float rows4_max(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(f_bits(v), f_bits(v), false, false);
+    v = fmaxf(bits_f(a[0]), bits_f(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(f_bits(v), f_bits(v), false, false);
+    return fmaxf(bits_f(b[0]), bits_f(b[1]));
+}
+__device__ __forceinline__ float rows4_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(f_bits(v), f_bits(v), false, false);
+    v = bits_f(a[0]) + bits_f(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(f_bits(v), f_bits(v), false, false);
+    return bits_f(b[0]) + bits_f(b[1]);
+}
+
+// inclusive scan over the wave's lanes
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+    v = dpp_add<0x111, 0xF>(v);
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);   // lane 15 of each row into the next
+    return dpp_add<0x143, 0xC>(v);   // lane 31 into the upper half
+}
+__device__ __forceinline__ float wave_total(float v) {
+    v += bits_f(dpp_u32<0xB1>(f_bits(v)));
+    v += bits_f(dpp_u32<0x4E>(f_bits(v)));
+    v += bits_f(dpp_u32<0x141>(f_bits(v)));
+    v += bits_f(dpp_u32<0x140>(f_bits(v)));
+    return rows4_sum(v);
+}
+
+// a block's share of one workgroup
+struct PagedWork {
+    int b, first, n;      // request, its first row, its new tokens
+    int length, r;        // its positions, block of its tokens
+    int c, chunks, slot0; // chunk, chunks of the block, the block's first slot
+};
+
+// The request's tokens, positions that its first token's window leaves, and blocks
+__device__ __forceinline__ void paged_request(const PagedArgs &a, int b, int TB, int *first, int *n, int *length,
+                                              int *span, int *blocks) {
+    int f = b, m = 1;
     if (a.p.starts) {
-        if (t >= a.p.starts[a.p.requests]) return;
-        int lo = 0, hi = a.p.requests - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (a.p.starts[mid] <= t) lo = mid;
-            else hi = mid - 1;
+        f = a.p.starts[b];
+        m = a.p.starts[b + 1] - f;
+    }
+    const int len = a.p.lengths[b] < 0 ? 0 : a.p.lengths[b];
+    m = m < 0 ? 0 : m;
+    *first = f;
+    *n = m;
+    *length = len;
+    int64_t s = len;
+    const int64_t seen = a.p.window + m - 1;     // positions that the request's tokens see at most
+    if (a.p.window > 0 && s > seen) s = seen;
+    *span = (int)s;
+    *blocks = (m + TB - 1) / TB;
+}
+
+// The work of slot `slot` (uniform over the wave); false if there is none
+__device__ __forceinline__ bool paged_work(const PagedArgs &a, int slot, int TB, int unit, PagedWork *w) {
+    const int lane = lane_id(), per = (a.p.requests + 63) >> 6;
+    const int b0 = lane * per, b1 = b0 + per < a.p.requests ? b0 + per : a.p.requests;
+    int first = 0, n = 0, length = 0, span = 0, blocks = 0;
+    float work = 0.0f, count = 0.0f;
+    for (int b = b0; b < b1; ++b) {
+        paged_request(a, b, TB, &first, &n, &length, &span, &blocks);
+        work += (float)blocks * (float)span;
+        count += (float)blocks;
+    }
+    work = wave_total(work);
+    count = wave_total(count);
+    // sum of blocks * ceil(span / C) <= work / C + count <= slots (1.001: the roundings of these sums)
+    const float room = fmaxf((float)a.slots - count, 1.0f);
+    const int C = ((int)fminf(work * 1.001f / room, 2.0e9f) / unit + 1) * unit;
+    int mine = 0;
+    for (int b = b0; b < b1; ++b) {
+        if (per > 1) paged_request(a, b, TB, &first, &n, &length, &span, &blocks);
+        const int ch = span <= C ? 1 : (span + C - 1) / C;
+        mine += blocks * ch;
+    }
+    const int upto = wave_scan(mine);
+    const uint64_t has = __ballot(upto > slot);
+    if (!has) return false;
+    const int owner = __builtin_ctzll(has);
+    int at = __builtin_amdgcn_readlane(upto - mine, owner);
+    int b = owner * per;
+    const int last = b + per - 1 < a.p.requests - 1 ? b + per - 1 : a.p.requests - 1;
+    for (;;) {       // uniform: the owner's requests one by one
+        paged_request(a, b, TB, &first, &n, &length, &span, &blocks);
+        const int ch = span <= C ? 1 : (span + C - 1) / C;
+        const int local = slot - at;
+        if (local < blocks * ch || b >= last) {
+            *w = PagedWork{b, first, n, length, local / ch, local % ch, ch, slot - local % ch};
+            return local < blocks * ch;
         }
-        b = lo;
-        p = (int64_t)a.p.lengths[b] - (a.p.starts[b + 1] - t);
-    } else {
-        p = (int64_t)a.p.lengths[b] - 1;
+        at += blocks * ch;
+        ++b;
     }
-    const int64_t lo = a.p.window > 0 && p + 1 > a.p.window ? p + 1 - a.p.window : 0;
-    const bool past = p >> a.shift >= a.p.max_pages;
-    const float *q = a.p.q + (t * a.p.n_heads + h) * HD + N * lane;
-    float qv[N], o[N], m = -INFINITY, l = 0.0f;
+}
+
+// ---- operand pieces by cache type
+
+template <typename T> struct PaType;
+template <> struct PaType<_Float16> {
+    static constexpr int pieces = 2, tile = 32;
+    static constexpr float p_bias = 14.0f;      // log2 of the probabilities' scale
+    static __device__ __forceinline__ lq_f4 mfma(const uint4 &x, const uint4 &y, lq_f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pa_h8, x), __builtin_bit_cast(pa_h8, y), c, 0,
+                                                      0, 0);
+    }
+    // 2 values into one word of each piece; what a piece's truncation drops, the next one has
+    static __device__ __forceinline__ void split(float x, float y, uint32_t *o) {
+        const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
+        const auto l = __builtin_amdgcn_cvt_pkrtz(x - (float)h[0], y - (float)h[1]);
+        o[0] = __builtin_bit_cast(uint32_t, h);
+        o[1] = __builtin_bit_cast(uint32_t, l);
+    }
+};
+template <> struct PaType<__bf16> {
+    static constexpr int pieces = 3, tile = 32;
+    static constexpr float p_bias = 0.0f;
+    static __device__ __forceinline__ lq_f4 mfma(const uint4 &x, const uint4 &y, lq_f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_b8, x), __builtin_bit_cast(pa_b8, y), c,
+                                                       0, 0, 0);
+    }
+    static __device__ __forceinline__ void split(float x, float y, uint32_t *o) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-        qv[e] = q[e] * a.scale2;
-        o[e] = 0.0f;
-    }
-    if (past) l = NAN;
-    for (int64_t s = past ? p + 1 : lo + wave; s <= p; s += 4) {
-        const int page = a.p.table[b * a.p.table_stride + (s >> a.shift)];
-        if (page < 0 || page >= a.c.n_pages) {
-            l = NAN;
-            break;
+        for (int i = 0; i < 3; ++i) {
+            o[i] = __builtin_amdgcn_perm(f_bits(y), f_bits(x), 0x07060302);
+            x -= bits_f(f_bits(x) & 0xffff0000u);
+            y -= bits_f(f_bits(y) & 0xffff0000u);
         }
-        const int64_t at = page * a.c.page_stride + kh * a.c.head_stride +
-                           (s & ((1 << a.shift) - 1)) * a.c.pos_stride + N * lane;
-        float d = 0.0f;
-#pragma unroll
-        for (int e = 0; e < N; ++e) d += qv[e] * (float)((const T *)a.c.k)[at + e];
-        d = group_sum<64>(d);
-        const float mn = fmaxf(m, d), f = m == -INFINITY ? 0.0f : exp2f(m - mn), w = exp2f(d - mn);
-        l = l * f + w;
-#pragma unroll
-        for (int e = 0; e < N; ++e) o[e] = o[e] * f + w * (float)((const T *)a.c.v)[at + e];
-        m = mn;
     }
+};
+template <> struct PaType<float> {
+    static constexpr int pieces = 1, tile = 16;
+    static constexpr float p_bias = 0.0f;
+};
+
+__device__ __forceinline__ float u4f(const uint4 &v, int i) { return bits_f(u4_get(v, i)); }
+
+template <typename T, int HD, int NT>
+__global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
+    using P = PaType<T>;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int TP = P::tile, NG = TP / 16;             // positions per tile, 16-position groups of it
+    constexpr int KW = HD * (int)sizeof(T) / 64;          // 16-byte loads of a K row's quarter
+    constexpr int EL = F32 || HD == 64 ? 4 : 8;           // adjacent values of a V row per lane
+    constexpr int SEG = HD / (16 * EL), NF = HD / 16;     // segments of a V row, output tiles
+    constexpr int VB = EL * (int)sizeof(T);               // bytes per lane and segment (8 or 16)
+    constexpr int PD = HD < 128 ? HD : 128;               // values of a column joined at once in LDS
+    __shared__ __align__(16) float red_o[4][16][PD + 4];
+    __shared__ float red_m[4][16 * NT], red_l[4][16 * NT];
+
+    const int x = (int)blockIdx.x, groups = a.p.n_kv * a.HG;
+    const int kh = x % a.p.n_kv, hg = (x / a.p.n_kv) % a.HG, slot = x / groups;
+    const int lane = lane_id(), wave = wave_id(), n = lane & 15, g = lane >> 4;
+    const int TB = NT * a.tpt;
+    PagedWork w;
+    if (!paged_work(a, slot, TB, 4 * TP, &w)) return;
+
+    // the block's positions: from its first token's window to its last token
+    const int p0 = w.length - w.n, i0 = w.r * TB, i1 = i0 + TB < w.n ? i0 + TB : w.n;
+    const int limit = a.p.max_pages << a.shift;           // positions that the table holds
+    int lo = 0, hi = p0 + i1;
+    if (a.p.window > 0 && (int64_t)p0 + i0 + 1 > a.p.window) lo = (int)(p0 + i0 + 1 - a.p.window);
+    hi = hi < limit ? hi : limit;
+    const int begin = lo & ~15;
+    const int len = hi > begin ? hi - begin : 0;
+    const int per = ((len + w.chunks - 1) / w.chunks + 4 * TP - 1) / (4 * TP) * (4 * TP);
+    const int64_t c0l = (int64_t)begin + (int64_t)w.c * per;
+    const int c0 = c0l < hi ? (int)c0l : hi, c1 = c0 + (int64_t)per < hi ? c0 + per : hi;
+
+    // columns: token and head of column 16 u + n, the positions it sees
+    int plo[NT], phi[NT], row[NT], head[NT];
+    float m[NT], l[NT];
+    const int ti = n / a.GC, hi_g = n % a.GC;
 #pragma unroll
-    for (int e = 0; e < N; ++e) red_o[wave][N * lane + e] = o[e];
-    if (lane == 0) {
-        red_m[wave] = m;
-        red_l[wave] = l;
+    for (int u = 0; u < NT; ++u) {
+        const int i = i0 + u * a.tpt + ti, h = hg * a.GC + hi_g;
+        const int t = w.first + i;
+        const bool in = ti < a.tpt && h < a.G && i < w.n && t >= 0 && t < a.p.tokens;
+        row[u] = in ? t : -1;
+        head[u] = kh * a.G + h;
+        phi[u] = in ? p0 + i : -1;
+        plo[u] = a.p.window > 0 && (int64_t)p0 + i + 1 > a.p.window ? (int)(p0 + i + 1 - a.p.window) : 0;
+        m[u] = -INFINITY;
+        l[u] = phi[u] >= limit ? NAN : 0.0f;
+    }
+
+    // q: lane (column n, group g) holds values [32 t + 8 g, + 8) (fp32 caches: 16 t + 4 g, + 4)
+    constexpr int QT = F32 ? HD / 16 : HD / 32;
+    uint4 q[NT][QT][P::pieces];
+    float unscale[NT];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+        const float *src = a.p.q + ((int64_t)(row[u] < 0 ? 0 : row[u]) * a.p.n_heads + (row[u] < 0 ? 0 : head[u])) * HD;
+        const float f = row[u] < 0 ? 0.0f : a.scale2;
+        unscale[u] = 1.0f;
+        if constexpr (F32) {
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                const float4 v = *reinterpret_cast<const float4 *>(src + 16 * t + 4 * g);
+                q[u][t][0] = make_uint4(f_bits(v.x * f), f_bits(v.y * f), f_bits(v.z * f), f_bits(v.w * f));
+            }
+        } else {
+            float v[QT][8];
+            float big = 0.0f;
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                const float4 v0 = *reinterpret_cast<const float4 *>(src + 32 * t + 8 * g);
+                const float4 v1 = *reinterpret_cast<const float4 *>(src + 32 * t + 8 * g + 4);
+                const float t8[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[t][e] = t8[e] * f;
+                    big = fmaxf(big, fabsf(v[t][e]));
+                }
+            }
+            if constexpr (P::pieces == 2) {
+                // the column's largest |q| to [512, 1024): exponent arithmetic, exact
+                big = rows4_max(big);
+                const int e = (int)((f_bits(big) >> 23) & 0xff);
+                const int up = e == 0 ? 100 : e == 255 ? 0 : 127 + 9 - e;   // zero or subnormal, inf: as near as it gets
+                const int u1 = up > 120 ? 120 : up < -120 ? -120 : up;
+                const float mul = bits_f((uint32_t)(127 + u1) << 23);
+                unscale[u] = bits_f((uint32_t)(127 - u1) << 23);
+#pragma unroll
+                for (int t = 0; t < QT; ++t)
+#pragma unroll
+                    for (int e8 = 0; e8 < 8; ++e8) v[t][e8] *= mul;
+            }
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                uint32_t o[P::pieces][4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t s[P::pieces];
+                    P::split(v[t][2 * e], v[t][2 * e + 1], s);
+#pragma unroll
+                    for (int i = 0; i < P::pieces; ++i) o[i][e] = s[i];
+                }
+#pragma unroll
+                for (int i = 0; i < P::pieces; ++i) q[u][t][i] = make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
+            }
+        }
+    }
+
+    lq_f4 acc[NT][NF];
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int f = 0; f < NF; ++f) acc[u][f] = lq_f4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    const int32_t *table = a.p.table + (int64_t)w.b * a.p.table_stride;
+    const char *kc = (const char *)a.c.k, *vc = (const char *)a.c.v;
+    const int64_t page_bytes = a.c.page_stride * (int64_t)sizeof(T), head_off = kh * a.c.head_stride * (int64_t)sizeof(T);
+    const int pos_bytes = (int)(a.c.pos_stride * (int64_t)sizeof(T)), mask = (1 << a.shift) - 1;
+    const int k_lane = n * pos_bytes + 16 * g;            // + 64 t
+    const int v_lane = 4 * g * pos_bytes + VB * n;        // + i pos_bytes + 16 VB seg
+
+    // pages of the wave's next 64 groups of 16 positions, one per lane
+    int pages = 0;
+    const int tiles = c1 > c0 ? (c1 - c0 + TP - 1) / TP : 0;
+    uint4 kr[NG][KW];
+    bool ok[NG];
+    int64_t off[NG];
+    auto fetch_pages = [&](int j) {       // j: index of the wave's tile, a multiple of 64 / NG
+        const int pos = c0 + ((j + lane / NG) * 4 + wave) * TP + 16 * (lane % NG);
+        pages = pos < c1 ? table[pos >> a.shift] : 0;
+    };
+    auto load_k = [&](int j) {
+        const int tb = c0 + (j * 4 + wave) * TP;
+#pragma unroll
+        for (int u = 0; u < NG; ++u) {
+            const int pos = tb + 16 * u;
+            const int page = __builtin_amdgcn_readlane(pages, (j * NG + u) & 63);
+            ok[u] = pos < c1 && page >= 0 && page < a.c.n_pages;
+            if (pos < c1 && !ok[u]) {     // columns that see a position of a page outside the pool
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    if (phi[t] >= pos && plo[t] < pos + 16) l[t] = NAN;
+            }
+            off[u] = (ok[u] ? (int64_t)page * page_bytes + (int64_t)(pos & mask) * pos_bytes : 0) + head_off;
+#pragma unroll
+            for (int t = 0; t < KW; ++t)
+                kr[u][t] = *reinterpret_cast<const uint4 *>(kc + off[u] + k_lane + 64 * t);
+        }
+    };
+
+    const int my = tiles > wave ? (tiles - wave + 3) / 4 : 0;   // tiles of this wave
+    if (my > 0) {
+        fetch_pages(0);
+        load_k(0);
+    }
+    for (int j = 0; j < my; ++j) {
+        const int tb = c0 + (j * 4 + wave) * TP;
+        bool good[NG];
+        // V: group u, position 4 g + i, segment s
+        uint32_t vr[NG][4][SEG][VB / 4];
+#pragma unroll
+        for (int u = 0; u < NG; ++u) {
+            good[u] = ok[u];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int s = 0; s < SEG; ++s) {
+                    const char *src = vc + off[u] + v_lane + i * pos_bytes + 16 * VB * s;
+                    if constexpr (VB == 16) {
+                        const uint4 t = *reinterpret_cast<const uint4 *>(src);
+                        vr[u][i][s][0] = t.x; vr[u][i][s][1] = t.y; vr[u][i][s][2] = t.z; vr[u][i][s][3] = t.w;
+                    } else {
+                        const uint2 t = *reinterpret_cast<const uint2 *>(src);
+                        vr[u][i][s][0] = t.x; vr[u][i][s][1] = t.y;
+                    }
+                }
+        }
+        // scores
+        lq_f4 sc[NT][NG];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int u = 0; u < NG; ++u) {
+                lq_f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < KW; ++k) {
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            s = __builtin_amdgcn_mfma_f32_16x16x4f32(u4f(kr[u][k], e), u4f(q[t][k][0], e), s, 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int i = P::pieces - 1; i >= 0; --i) s = P::mfma(kr[u][k], q[t][k][i], s);
+                    }
+                }
+                sc[t][u] = s;
+            }
+        const bool edge = tb < lo || tb + TP > hi;
+        if (j + 1 < my) {
+            if (((j + 1) * NG & 63) == 0) fetch_pages(j + 1);
+            load_k(j + 1);
+        }
+
+        // what no column sees may be anything: its V rows count as zero
+        if (edge || !good[0] || !good[NG - 1]) {
+#pragma unroll
+            for (int u = 0; u < NG; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int pos = tb + 16 * u + 4 * g + i;
+                    const bool zero = !good[u] || pos < lo || pos >= hi;
+#pragma unroll
+                    for (int s = 0; s < SEG; ++s)
+#pragma unroll
+                        for (int d = 0; d < VB / 4; ++d) vr[u][i][s][d] = zero ? 0u : vr[u][i][s][d];
+                }
+        }
+
+        // softmax: per column, this lane's positions 16 u + 4 g + i
+        uint4 pp[NT][P::pieces];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < NG; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int pos = tb + 16 * u + 4 * g + i;
+                    const float s = sc[t][u][i] * unscale[t];
+                    sc[t][u][i] = good[u] && pos >= plo[t] && pos <= phi[t] ? s : -INFINITY;
+                    top = fmaxf(top, sc[t][u][i]);
+                }
+            const float mn = fmaxf(m[t], rows4_max(top));
+            const float ref = mn == -INFINITY ? 0.0f : mn;
+            if (__any(mn > m[t])) {
+                const float f = __builtin_amdgcn_exp2f(m[t] - ref);
+                l[t] *= f;
+#pragma unroll
+                for (int o = 0; o < NF; ++o) acc[t][o] *= f;
+                m[t] = mn;
+            }
+            float p[NG][4];
+#pragma unroll
+            for (int u = 0; u < NG; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    p[u][i] = __builtin_amdgcn_exp2f(sc[t][u][i] - ref + P::p_bias);
+                    l[t] += p[u][i];
+                }
+            if constexpr (F32) {
+                pp[t][0] = make_uint4(f_bits(p[0][0]), f_bits(p[0][1]), f_bits(p[0][2]), f_bits(p[0][3]));
+            } else {
+                uint32_t o[4][P::pieces];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) P::split(p[e / 2][2 * (e % 2)], p[e / 2][2 * (e % 2) + 1], o[e]);
+#pragma unroll
+                for (int i = 0; i < P::pieces; ++i) pp[t][i] = make_uint4(o[0][i], o[1][i], o[2][i], o[3][i]);
+            }
+        }
+        // O^T: output tile f = EL s + e, row m of it is value 16 EL s + EL m + e
+#pragma unroll
+        for (int s = 0; s < SEG; ++s)
+#pragma unroll
+            for (int e = 0; e < EL; ++e) {
+                if constexpr (F32) {
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            acc[t][EL * s + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                bits_f(vr[0][i][s][e]), u4f(pp[t][0], i), acc[t][EL * s + e], 0, 0, 0);
+                } else {
+                    const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+                    uint4 v;
+                    v.x = __builtin_amdgcn_perm(vr[0][1][s][e / 2], vr[0][0][s][e / 2], sel);
+                    v.y = __builtin_amdgcn_perm(vr[0][3][s][e / 2], vr[0][2][s][e / 2], sel);
+                    v.z = __builtin_amdgcn_perm(vr[1][1][s][e / 2], vr[1][0][s][e / 2], sel);
+                    v.w = __builtin_amdgcn_perm(vr[1][3][s][e / 2], vr[1][2][s][e / 2], sel);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int i = P::pieces - 1; i >= 0; --i)
+                            acc[t][EL * s + e] = P::mfma(v, pp[t][i], acc[t][EL * s + e]);
+                }
+            }
+    }
+
+    // the waves meet
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const float ls = rows4_sum(l[t]);
+        if (g == 0) {
+            red_m[wave][16 * t + n] = m[t];
+            red_l[wave][16 * t + n] = ls;
+        }
+    }
+    const int64_t base = ((int64_t)slot * groups + kh * a.HG + hg) * (16 * NT);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int d0 = 0; d0 < HD; d0 += PD) {
+            __syncthreads();
+#pragma unroll
+            for (int s = d0 / (16 * EL); s < (d0 + PD) / (16 * EL); ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < EL; e += 4) {
+                        const int f = EL * s + e;
+                        *reinterpret_cast<float4 *>(&red_o[wave][n][16 * EL * s - d0 + EL * (4 * g + i) + e]) =
+                            make_float4(acc[t][f][i], acc[t][f + 1][i], acc[t][f + 2][i], acc[t][f + 3][i]);
+                    }
+            __syncthreads();
+            // 16 threads per column, PD / 16 values each
+            const int tid = (int)threadIdx.x, col = tid >> 4, dd = (tid & 15) * (PD / 16);
+            float M = red_m[0][16 * t + col];
+#pragma unroll
+            for (int v = 1; v < 4; ++v) M = fmaxf(M, red_m[v][16 * t + col]);
+            const float ref = M == -INFINITY ? 0.0f : M;
+            float L = 0.0f, o[PD / 16];
+#pragma unroll
+            for (int e = 0; e < PD / 16; ++e) o[e] = 0.0f;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const float f = __builtin_amdgcn_exp2f(red_m[v][16 * t + col] - ref);
+                L += f * red_l[v][16 * t + col];
+#pragma unroll
+                for (int e = 0; e < PD / 16; ++e) o[e] += f * red_o[v][col][dd + e];
+            }
+            const int cti = col / a.GC, ch = hg * a.GC + col % a.GC, i = i0 + t * a.tpt + cti, r = w.first + i;
+            if (!(cti < a.tpt && ch < a.G && i < w.n && r >= 0 && r < a.p.tokens)) continue;
+            if (w.chunks == 1) {
+                const int64_t at = ((int64_t)r * a.p.n_heads + kh * a.G + ch) * HD + d0 + dd;
+                const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+                for (int e = 0; e < PD / 16; e += 4) {
+                    float4 y = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+                    if (a.p.gate) {
+                        const float4 gt = *reinterpret_cast<const float4 *>(a.p.gate + at + e);
+                        y.x *= 1.0f / (1.0f + expf(-fminf(fmaxf(gt.x, -80.0f), 80.0f)));
+                        y.y *= 1.0f / (1.0f + expf(-fminf(fmaxf(gt.y, -80.0f), 80.0f)));
+                        y.z *= 1.0f / (1.0f + expf(-fminf(fmaxf(gt.z, -80.0f), 80.0f)));
+                        y.w *= 1.0f / (1.0f + expf(-fminf(fmaxf(gt.w, -80.0f), 80.0f)));
+                    }
+                    *reinterpret_cast<float4 *>(a.p.out + at + e) = y;
+                }
+            } else {
+                float *dst = a.part + (base + 16 * t + col) * HD + d0 + dd;
+#pragma unroll
+                for (int e = 0; e < PD / 16; e += 4)
+                    *reinterpret_cast<float4 *>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                if (d0 == 0 && (tid & 15) == 0) a.ml[base + 16 * t + col] = make_float2(M, L);
+            }
+            if (d0 == 0 && w.c == 0 && (tid & 15) == 0 && kh == 0 && hg == 0 && col % a.GC == 0)
+                a.rows[r] = make_int2(w.slot0 << 6 | (16 * t + col), w.chunks);
+        }
+}
+
+// Blocks of several chunks: out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c.
+// A workgroup takes one row and head; HD / 4 lanes hold its values, 4 each, and
+// the 256 / (HD / 4) such groups take chunks in turn and meet in LDS.
+template <int HD>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) {
+    constexpr int LPR = HD / 4, SL = 256 / LPR;
+    __shared__ __align__(16) float red_o[SL][HD];
+    __shared__ float red_m[SL], red_l[SL];
+    const int64_t t = blockIdx.x;
+    if (a.p.starts && t >= a.p.starts[a.p.requests]) return;
+    const int2 info = a.rows[t];
+    const int slot0 = info.x >> 6, chunks = info.y;
+    if (chunks <= 1 || slot0 < 0 || slot0 + chunks > a.slots) return;
+    const int h = (int)blockIdx.y, kh = h / a.G, hr = h % a.G, groups = a.p.n_kv * a.HG;
+    const int col = (info.x & 63) + hr % a.GC, tid = (int)threadIdx.x, d = 4 * (tid % LPR), sl = tid / LPR;
+    const int64_t first = ((int64_t)slot0 * groups + kh * a.HG + hr / a.GC) * cols + col;
+    const int64_t step = (int64_t)groups * cols;
+    float M = -INFINITY, L = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int c = sl; c < chunks; c += SL) {
+        const int64_t at = first + c * step;
+        const float2 ml = a.ml[at];
+        const float4 v = *reinterpret_cast<const float4 *>(a.part + at * HD + d);
+        const float mn = fmaxf(M, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
+        const float f = __builtin_amdgcn_exp2f(M - ref), w = __builtin_amdgcn_exp2f(ml.x - ref);
+        L = L * f + ml.y * w;
+        o.x = o.x * f + v.x * w;
+        o.y = o.y * f + v.y * w;
+        o.z = o.z * f + v.z * w;
+        o.w = o.w * f + v.w * w;
+        M = mn;
+    }
+    *reinterpret_cast<float4 *>(&red_o[sl][d]) = o;
+    if (tid % LPR == 0) {
+        red_m[sl] = M;
+        red_l[sl] = L;
     }
     __syncthreads();
-    const int d = (int)threadIdx.x;
-    if (d >= HD) return;
-    const float M = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
-    float os = 0.0f, ls = 0.0f;
-    for (int w = 0; w < 4; ++w) {
-        const float f = red_m[w] == -INFINITY ? 0.0f : exp2f(red_m[w] - M);
-        os += f * red_o[w][d];
-        ls += isnan(red_l[w]) ? NAN : f * red_l[w];
+    if (tid >= HD) return;
+    float top = -INFINITY, ls = 0.0f, os = 0.0f;
+    for (int i = 0; i < SL; ++i) top = fmaxf(top, red_m[i]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    for (int i = 0; i < SL; ++i) {
+        const float f = __builtin_amdgcn_exp2f(red_m[i] - ref);
+        ls += f * red_l[i];
+        os += f * red_o[i][tid];
     }
+    const int64_t at = (t * a.p.n_heads + h) * HD + tid;
     float y = ls == 0.0f ? 0.0f : os / ls;
-    const int64_t at = (t * a.p.n_heads + h) * HD + d;
     if (a.p.gate) y *= 1.0f / (1.0f + expf(-fminf(fmaxf(a.p.gate[at], -80.0f), 80.0f)));
     a.p.out[at] = y;
 }
 
-size_t paged_attention_workspace_bytes(int64_t, int, int, int, int) { return 0; }
+// How a call is laid out, from its host-known sizes alone
+struct PagedPlan {
+    int G, GC, HG, tpt, NT, slots, cols;
+    int64_t part, ml, rows, bytes;
+};
 
-int launch_paged_attention(const PagedQueries &p, const PagedCache &cache, void *, int64_t, hipStream_t s) {
-    const PagedArgs a{p, cache, p.n_heads / p.n_kv, page_shift(cache.page_size), p.scale * 1.44269504f};
-    const dim3 grid((unsigned)p.tokens, (unsigned)p.n_heads);
+constexpr int PAGED_GROUPS = 2048;    // workgroups that a call is cut into, if its blocks do not ask for more
+
+static PagedPlan paged_plan(int64_t tokens, int requests, int n_heads, int n_kv, int hd) {
+    PagedPlan p{};
+    p.G = n_heads / n_kv;
+    p.GC = p.G < 16 ? p.G : 16;
+    p.HG = (p.G + p.GC - 1) / p.GC;
+    p.tpt = 16 / p.GC;
+    p.NT = tokens > requests ? 2 : 1;
+    p.cols = 16 * p.NT;
+    const int TB = p.NT * p.tpt;
+    const int64_t most = (tokens + TB - 1) / TB + requests, blocks = most < tokens ? most : tokens;
+    const int64_t want = PAGED_GROUPS / ((int64_t)n_kv * p.HG);
+    const int64_t slots = want > 2 * blocks ? want : 2 * blocks;
+    p.slots = (int)slots;
+    auto up = [](int64_t b) { return (b + 255) & ~(int64_t)255; };
+    const int64_t recs = slots * n_kv * p.HG * p.cols;
+    p.part = 0;
+    p.ml = up(recs * hd * 4);
+    p.rows = p.ml + up(recs * 8);
+    p.bytes = p.rows + up(tokens * 8);
+    return p;
+}
+
+size_t paged_attention_workspace_bytes(int64_t tokens, int requests, int n_heads, int n_kv, int hd) {
+    return (size_t)paged_plan(tokens, requests, n_heads, n_kv, hd).bytes;
+}
+
+template <typename T, int HD>
+static void paged_launch(const PagedArgs &a, const PagedPlan &p, hipStream_t s) {
+    const dim3 grid((unsigned)((int64_t)p.slots * a.p.n_kv * p.HG));
+    if (p.NT == 1) hipLaunchKernelGGL((paged_attention_kernel<T, HD, 1>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((paged_attention_kernel<T, HD, 2>), grid, dim3(256), 0, s, a);
+}
+
+int launch_paged_attention(const PagedQueries &p, const PagedCache &cache, void *ws, int64_t, hipStream_t s) {
+    const PagedPlan l = paged_plan(p.tokens, p.requests, p.n_heads, p.n_kv, p.hd);
+    if ((int64_t)l.slots * p.n_kv * l.HG > INT32_MAX || l.slots >= 1 << 25)
+        return fail(LOCALAI_EARG, "paged attention: too many tokens times heads for one call");
+    char *w = (char *)ws;
+    const PagedArgs a{p, cache, l.G, l.GC, l.HG, l.tpt, page_shift(cache.page_size), l.slots,
+                      (float)(p.scale * 1.4426950408889634), (float *)(w + l.part), (float2 *)(w + l.ml),
+                      (int2 *)(w + l.rows)};
 #define LQ_PA(T, HD) \
-    if (p.hd == HD) hipLaunchKernelGGL((paged_attention_kernel<T, HD>), grid, dim3(256), 0, s, a);
+    if (p.hd == HD) paged_launch<T, HD>(a, l, s);
     if (cache.type == PAGED_F32) { LQ_PA(float, 64) LQ_PA(float, 128) LQ_PA(float, 256) }
     else if (cache.type == PAGED_F16) { LQ_PA(_Float16, 64) LQ_PA(_Float16, 128) LQ_PA(_Float16, 256) }
     else { LQ_PA(__bf16, 64) LQ_PA(__bf16, 128) LQ_PA(__bf16, 256) }
 #undef LQ_PA
+    LQ_HIP(hipGetLastError());
+    const dim3 grid((unsigned)p.tokens, (unsigned)p.n_heads);
+    if (p.hd == 64) hipLaunchKernelGGL(paged_join_kernel<64>, grid, dim3(256), 0, s, a, l.cols);
+    else if (p.hd == 128) hipLaunchKernelGGL(paged_join_kernel<128>, grid, dim3(256), 0, s, a, l.cols);
+    else hipLaunchKernelGGL(paged_join_kernel<256>, grid, dim3(256), 0, s, a, l.cols);
     LQ_HIP(hipGetLastError());
     return LOCALAI_OK;
 }
