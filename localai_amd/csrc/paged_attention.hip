@@ -2,6 +2,8 @@
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
 
+#include <cmath>
+
 #include "dev_common.h"
 #include "internal.h"
 #include "paged.h"
@@ -40,10 +42,11 @@ struct PagedArgs {
     PagedCache c;
     int G, GC, HG, tpt;  // query heads per kv head, per column group; groups; tokens per column tile
     int shift, slots;    // workgroups per kv head and column group
-    float scale2;        // scale * log2(e)
-    float *part;         // [slots, n_kv, HG, 16 NT, HD] unscaled outputs of a chunk
-    float2 *ml;          // [slots, n_kv, HG, 16 NT] their maximum (base 2) and sum
-    int2 *rows;          // [tokens]: first slot << 6 | first column of the token's block, chunks
+    float q_sign;        // sign of scale (0 for 0)
+    float scale2;        // |scale| * log2(e) (1 for 0)
+    float *part;         // [slots, n_kv, HG, columns of a block, HD] unscaled outputs of a chunk
+    float2 *ml;          // [slots, n_kv, HG, columns] their largest score and sum
+    int2 *rows;          // [tokens]: first slot << 8 | first column of the token's block, chunks
 };
 
 typedef _Float16 pa_h8 __attribute__((ext_vector_type(8)));
@@ -197,7 +200,21 @@ template <> struct PaType<float> {
 
 __device__ __forceinline__ float u4f(const uint4 &v, int i) { return bits_f(u4_get(v, i)); }
 
-template <typename T, int HD, int NT>
+__device__ __forceinline__ float4 gated(float4 y, const float *gate) {
+    const float4 g = *reinterpret_cast<const float4 *>(gate);
+    y.x *= 1.0f / (1.0f + expf(-fminf(fmaxf(g.x, -80.0f), 80.0f)));
+    y.y *= 1.0f / (1.0f + expf(-fminf(fmaxf(g.y, -80.0f), 80.0f)));
+    y.z *= 1.0f / (1.0f + expf(-fminf(fmaxf(g.z, -80.0f), 80.0f)));
+    y.w *= 1.0f / (1.0f + expf(-fminf(fmaxf(g.w, -80.0f), 80.0f)));
+    return y;
+}
+
+// NT: column tiles of a wave. APART false: the workgroup's waves share their
+// columns and take tiles of positions in turn (decode: few columns, long
+// lengths); true: each has columns of its own, over the same positions
+// (prompts: the four read the same K and V at about the same time, and
+// nothing has to be joined).
+template <typename T, int HD, int NT, bool APART>
 __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
     using P = PaType<T>;
     constexpr bool F32 = sizeof(T) == 4;
@@ -207,19 +224,22 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
     constexpr int SEG = HD / (16 * EL), NF = HD / 16;     // segments of a V row, output tiles
     constexpr int VB = EL * (int)sizeof(T);               // bytes per lane and segment (8 or 16)
     constexpr int PD = HD < 128 ? HD : 128;               // values of a column joined at once in LDS
-    __shared__ __align__(16) float red_o[4][16][PD + 4];
+    constexpr int WS = APART ? 1 : 4;                     // waves that share a chunk's tiles
+    constexpr int COLS = (APART ? 64 : 16) * NT;          // columns of a block
+    __shared__ __align__(16) float red_o[APART ? 1 : 4][APART ? 1 : 16][PD + 4];
     __shared__ float red_m[4][16 * NT], red_l[4][16 * NT];
 
     const int x = (int)blockIdx.x, groups = a.p.n_kv * a.HG;
     const int kh = x % a.p.n_kv, hg = (x / a.p.n_kv) % a.HG, slot = x / groups;
     const int lane = lane_id(), wave = wave_id(), n = lane & 15, g = lane >> 4;
-    const int TB = NT * a.tpt;
+    const int TW = NT * a.tpt, TB = APART ? 4 * TW : TW;  // tokens of a wave, of the block
     PagedWork w;
     if (!paged_work(a, slot, TB, 4 * TP, &w)) return;
 
-    // the block's positions: from its first token's window to its last token
-    const int p0 = w.length - w.n, i0 = w.r * TB, i1 = i0 + TB < w.n ? i0 + TB : w.n;
-    const int limit = a.p.max_pages << a.shift;           // positions that the table holds
+    // the block's positions: from its first token's window to its last token,
+    // and of these the chunk's
+    const int p0 = w.length - w.n, limit = a.p.max_pages << a.shift;   // positions that the table holds
+    int i0 = w.r * TB, i1 = i0 + TB < w.n ? i0 + TB : w.n;
     int lo = 0, hi = p0 + i1;
     if (a.p.window > 0 && (int64_t)p0 + i0 + 1 > a.p.window) lo = (int)(p0 + i0 + 1 - a.p.window);
     hi = hi < limit ? hi : limit;
@@ -227,7 +247,16 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
     const int len = hi > begin ? hi - begin : 0;
     const int per = ((len + w.chunks - 1) / w.chunks + 4 * TP - 1) / (4 * TP) * (4 * TP);
     const int64_t c0l = (int64_t)begin + (int64_t)w.c * per;
-    const int c0 = c0l < hi ? (int)c0l : hi, c1 = c0 + (int64_t)per < hi ? c0 + per : hi;
+    int c0 = c0l < hi ? (int)c0l : hi, c1 = c0 + (int64_t)per < hi ? c0 + per : hi;
+    if constexpr (APART) {         // the same for the wave's own tokens
+        i0 += wave * TW;
+        if (i0 >= w.n) return;
+        i1 = i0 + TW < w.n ? i0 + TW : w.n;
+        if (a.p.window > 0 && (int64_t)p0 + i0 + 1 > a.p.window) lo = (int)(p0 + i0 + 1 - a.p.window);
+        hi = p0 + i1 < limit ? p0 + i1 : limit;
+        if (c1 > hi) c1 = hi;
+        if (lo > c0) c0 += (lo - c0) & ~15;
+    }
 
     // columns: token and head of column 16 u + n, the positions it sees
     int plo[NT], phi[NT], row[NT], head[NT];
@@ -253,7 +282,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
         const float *src = a.p.q + ((int64_t)(row[u] < 0 ? 0 : row[u]) * a.p.n_heads + (row[u] < 0 ? 0 : head[u])) * HD;
-        const float f = row[u] < 0 ? 0.0f : a.scale2;
+        const float f = row[u] < 0 ? 0.0f : a.q_sign;
         unscale[u] = 1.0f;
         if constexpr (F32) {
 #pragma unroll
@@ -304,6 +333,10 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
         }
     }
 
+    float slope[NT];      // of the exponent over a score in the scaled q's units
+#pragma unroll
+    for (int u = 0; u < NT; ++u) slope[u] = fmaxf(a.scale2 * unscale[u], 1e-37f);   // never 0: -inf times it stays
+
     lq_f4 acc[NT][NF];
 #pragma unroll
     for (int u = 0; u < NT; ++u)
@@ -317,6 +350,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
     const int k_lane = n * pos_bytes + 16 * g;            // + 64 t
     const int v_lane = 4 * g * pos_bytes + VB * n;        // + i pos_bytes + 16 VB seg
 
+    const int wo = APART ? 0 : wave;
     // pages of the wave's next 64 groups of 16 positions, one per lane
     int pages = 0;
     const int tiles = c1 > c0 ? (c1 - c0 + TP - 1) / TP : 0;
@@ -324,11 +358,11 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
     bool ok[NG];
     int64_t off[NG];
     auto fetch_pages = [&](int j) {       // j: index of the wave's tile, a multiple of 64 / NG
-        const int pos = c0 + ((j + lane / NG) * 4 + wave) * TP + 16 * (lane % NG);
+        const int pos = c0 + ((j + lane / NG) * WS + wo) * TP + 16 * (lane % NG);
         pages = pos < c1 ? table[pos >> a.shift] : 0;
     };
     auto load_k = [&](int j) {
-        const int tb = c0 + (j * 4 + wave) * TP;
+        const int tb = c0 + (j * WS + wo) * TP;
 #pragma unroll
         for (int u = 0; u < NG; ++u) {
             const int pos = tb + 16 * u;
@@ -346,13 +380,13 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
         }
     };
 
-    const int my = tiles > wave ? (tiles - wave + 3) / 4 : 0;   // tiles of this wave
+    const int my = tiles > wo ? (tiles - wo + WS - 1) / WS : 0;   // tiles of this wave
     if (my > 0) {
         fetch_pages(0);
         load_k(0);
     }
     for (int j = 0; j < my; ++j) {
-        const int tb = c0 + (j * 4 + wave) * TP;
+        const int tb = c0 + (j * WS + wo) * TP;
         bool good[NG];
         // V: group u, position 4 g + i, segment s
         uint32_t vr[NG][4][SEG][VB / 4];
@@ -424,14 +458,13 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int pos = tb + 16 * u + 4 * g + i;
-                    const float s = sc[t][u][i] * unscale[t];
-                    sc[t][u][i] = good[u] && pos >= plo[t] && pos <= phi[t] ? s : -INFINITY;
+                    sc[t][u][i] = good[u] && pos >= plo[t] && pos <= phi[t] ? sc[t][u][i] : -INFINITY;
                     top = fmaxf(top, sc[t][u][i]);
                 }
             const float mn = fmaxf(m[t], rows4_max(top));
             const float ref = mn == -INFINITY ? 0.0f : mn;
             if (__any(mn > m[t])) {
-                const float f = __builtin_amdgcn_exp2f(m[t] - ref);
+                const float f = __builtin_amdgcn_exp2f((m[t] - ref) * slope[t]);
                 l[t] *= f;
 #pragma unroll
                 for (int o = 0; o < NF; ++o) acc[t][o] *= f;
@@ -442,7 +475,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
             for (int u = 0; u < NG; ++u)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    p[u][i] = __builtin_amdgcn_exp2f(sc[t][u][i] - ref + P::p_bias);
+                    p[u][i] = __builtin_amdgcn_exp2f((sc[t][u][i] - ref) * slope[t] + P::p_bias);
                     l[t] += p[u][i];
                 }
             if constexpr (F32) {
@@ -483,16 +516,47 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
             }
     }
 
+    const int64_t base = ((int64_t)slot * groups + kh * a.HG + hg) * COLS;
+    if constexpr (APART) {
+        // the lane's 4 x EL adjacent values of a segment, per column
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const float L = rows4_sum(l[t]);
+            if (row[t] < 0) continue;
+            const int col = (wave * NT + t) * 16 + n;
+            const float f = w.chunks > 1 ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
+            const int64_t at = ((int64_t)row[t] * a.p.n_heads + head[t]) * HD;
+            float *dst = w.chunks > 1 ? a.part + (base + col) * HD : a.p.out + at;
+#pragma unroll
+            for (int s = 0; s < SEG; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < EL; e += 4) {
+                        const int o = EL * s + e, d = 16 * EL * s + EL * (4 * g + i) + e;
+                        float4 y = make_float4(acc[t][o][i] * f, acc[t][o + 1][i] * f, acc[t][o + 2][i] * f,
+                                               acc[t][o + 3][i] * f);
+                        if (w.chunks == 1 && a.p.gate) y = gated(y, a.p.gate + at + d);
+                        *reinterpret_cast<float4 *>(dst + d) = y;
+                    }
+            if (g == 0) {
+                if (w.chunks > 1) a.ml[base + col] = make_float2(m[t] * unscale[t], L);
+                if (w.c == 0 && kh == 0 && hg == 0 && hi_g == 0)
+                    a.rows[row[t]] = make_int2(w.slot0 << 8 | col, w.chunks);
+            }
+        }
+        return;
+    }
+
     // the waves meet
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const float ls = rows4_sum(l[t]);
         if (g == 0) {
-            red_m[wave][16 * t + n] = m[t];
+            red_m[wave][16 * t + n] = m[t] * unscale[t];
             red_l[wave][16 * t + n] = ls;
         }
     }
-    const int64_t base = ((int64_t)slot * groups + kh * a.HG + hg) * (16 * NT);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -520,37 +584,27 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
             for (int e = 0; e < PD / 16; ++e) o[e] = 0.0f;
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-                const float f = __builtin_amdgcn_exp2f(red_m[v][16 * t + col] - ref);
+                const float f = __builtin_amdgcn_exp2f((red_m[v][16 * t + col] - ref) * a.scale2);
                 L += f * red_l[v][16 * t + col];
 #pragma unroll
                 for (int e = 0; e < PD / 16; ++e) o[e] += f * red_o[v][col][dd + e];
             }
             const int cti = col / a.GC, ch = hg * a.GC + col % a.GC, i = i0 + t * a.tpt + cti, r = w.first + i;
             if (!(cti < a.tpt && ch < a.G && i < w.n && r >= 0 && r < a.p.tokens)) continue;
-            if (w.chunks == 1) {
-                const int64_t at = ((int64_t)r * a.p.n_heads + kh * a.G + ch) * HD + d0 + dd;
-                const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            const int64_t at = ((int64_t)r * a.p.n_heads + kh * a.G + ch) * HD + d0 + dd;
+            float *dst = w.chunks > 1 ? a.part + (base + 16 * t + col) * HD + d0 + dd : a.p.out + at;
+            const float f = w.chunks > 1 ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
-                for (int e = 0; e < PD / 16; e += 4) {
-                    float4 y = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
-                    if (a.p.gate) {
-                        const float4 gt = *reinterpret_cast<const float4 *>(a.p.gate + at + e);
-                        y.x *= 1.0f / (1.0f + expf(-fminf(fmaxf(gt.x, -80.0f), 80.0f)));
-                        y.y *= 1.0f / (1.0f + expf(-fminf(fmaxf(gt.y, -80.0f), 80.0f)));
-                        y.z *= 1.0f / (1.0f + expf(-fminf(fmaxf(gt.z, -80.0f), 80.0f)));
-                        y.w *= 1.0f / (1.0f + expf(-fminf(fmaxf(gt.w, -80.0f), 80.0f)));
-                    }
-                    *reinterpret_cast<float4 *>(a.p.out + at + e) = y;
-                }
-            } else {
-                float *dst = a.part + (base + 16 * t + col) * HD + d0 + dd;
-#pragma unroll
-                for (int e = 0; e < PD / 16; e += 4)
-                    *reinterpret_cast<float4 *>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                if (d0 == 0 && (tid & 15) == 0) a.ml[base + 16 * t + col] = make_float2(M, L);
+            for (int e = 0; e < PD / 16; e += 4) {
+                float4 y = make_float4(o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f);
+                if (w.chunks == 1 && a.p.gate) y = gated(y, a.p.gate + at + e);
+                *reinterpret_cast<float4 *>(dst + e) = y;
             }
-            if (d0 == 0 && w.c == 0 && (tid & 15) == 0 && kh == 0 && hg == 0 && col % a.GC == 0)
-                a.rows[r] = make_int2(w.slot0 << 6 | (16 * t + col), w.chunks);
+            if (d0 == 0 && (tid & 15) == 0) {
+                if (w.chunks > 1) a.ml[base + 16 * t + col] = make_float2(M, L);
+                if (w.c == 0 && kh == 0 && hg == 0 && col % a.GC == 0)
+                    a.rows[r] = make_int2(w.slot0 << 8 | (16 * t + col), w.chunks);
+            }
         }
 }
 
@@ -565,10 +619,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) 
     const int64_t t = blockIdx.x;
     if (a.p.starts && t >= a.p.starts[a.p.requests]) return;
     const int2 info = a.rows[t];
-    const int slot0 = info.x >> 6, chunks = info.y;
+    const int slot0 = info.x >> 8, chunks = info.y;
     if (chunks <= 1 || slot0 < 0 || slot0 + chunks > a.slots) return;
     const int h = (int)blockIdx.y, kh = h / a.G, hr = h % a.G, groups = a.p.n_kv * a.HG;
-    const int col = (info.x & 63) + hr % a.GC, tid = (int)threadIdx.x, d = 4 * (tid % LPR), sl = tid / LPR;
+    const int col = (info.x & 255) + hr % a.GC, tid = (int)threadIdx.x, d = 4 * (tid % LPR), sl = tid / LPR;
     const int64_t first = ((int64_t)slot0 * groups + kh * a.HG + hr / a.GC) * cols + col;
     const int64_t step = (int64_t)groups * cols;
     float M = -INFINITY, L = 0.0f;
@@ -578,7 +632,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) 
         const float2 ml = a.ml[at];
         const float4 v = *reinterpret_cast<const float4 *>(a.part + at * HD + d);
         const float mn = fmaxf(M, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
-        const float f = __builtin_amdgcn_exp2f(M - ref), w = __builtin_amdgcn_exp2f(ml.x - ref);
+        const float f = __builtin_amdgcn_exp2f((M - ref) * a.scale2), w = __builtin_amdgcn_exp2f((ml.x - ref) * a.scale2);
         L = L * f + ml.y * w;
         o.x = o.x * f + v.x * w;
         o.y = o.y * f + v.y * w;
@@ -597,7 +651,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) 
     for (int i = 0; i < SL; ++i) top = fmaxf(top, red_m[i]);
     const float ref = top == -INFINITY ? 0.0f : top;
     for (int i = 0; i < SL; ++i) {
-        const float f = __builtin_amdgcn_exp2f(red_m[i] - ref);
+        const float f = __builtin_amdgcn_exp2f((red_m[i] - ref) * a.scale2);
         ls += f * red_l[i];
         os += f * red_o[i][tid];
     }
@@ -610,10 +664,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) 
 // How a call is laid out, from its host-known sizes alone
 struct PagedPlan {
     int G, GC, HG, tpt, NT, slots, cols;
+    bool apart;
     int64_t part, ml, rows, bytes;
 };
 
 constexpr int PAGED_GROUPS = 2048;    // workgroups that a call is cut into, if its blocks do not ask for more
+
+static int paged_env(const char *n, int d) { const char *e = getenv(n); return e ? atoi(e) : d; }
 
 static PagedPlan paged_plan(int64_t tokens, int requests, int n_heads, int n_kv, int hd) {
     PagedPlan p{};
@@ -621,11 +678,12 @@ static PagedPlan paged_plan(int64_t tokens, int requests, int n_heads, int n_kv,
     p.GC = p.G < 16 ? p.G : 16;
     p.HG = (p.G + p.GC - 1) / p.GC;
     p.tpt = 16 / p.GC;
-    p.NT = tokens > requests ? 2 : 1;
-    p.cols = 16 * p.NT;
-    const int TB = p.NT * p.tpt;
+    p.apart = tokens >= 16 * (int64_t)requests;
+    p.NT = hd == 256 || tokens <= requests ? 1 : 2;
+    p.cols = (p.apart ? 64 : 16) * p.NT;
+    const int TB = p.cols / 16 * p.tpt;
     const int64_t most = (tokens + TB - 1) / TB + requests, blocks = most < tokens ? most : tokens;
-    const int64_t want = PAGED_GROUPS / ((int64_t)n_kv * p.HG);
+    const int64_t want = paged_env("PG", PAGED_GROUPS) / ((int64_t)n_kv * p.HG);
     const int64_t slots = want > 2 * blocks ? want : 2 * blocks;
     p.slots = (int)slots;
     auto up = [](int64_t b) { return (b + 255) & ~(int64_t)255; };
@@ -643,18 +701,21 @@ size_t paged_attention_workspace_bytes(int64_t tokens, int requests, int n_heads
 
 template <typename T, int HD>
 static void paged_launch(const PagedArgs &a, const PagedPlan &p, hipStream_t s) {
+    constexpr int N2 = HD == 256 ? 1 : 2;
     const dim3 grid((unsigned)((int64_t)p.slots * a.p.n_kv * p.HG));
-    if (p.NT == 1) hipLaunchKernelGGL((paged_attention_kernel<T, HD, 1>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((paged_attention_kernel<T, HD, 2>), grid, dim3(256), 0, s, a);
+    if (p.apart) hipLaunchKernelGGL((paged_attention_kernel<T, HD, N2, true>), grid, dim3(256), 0, s, a);
+    else if (p.NT == 1) hipLaunchKernelGGL((paged_attention_kernel<T, HD, 1, false>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((paged_attention_kernel<T, HD, N2, false>), grid, dim3(256), 0, s, a);
 }
 
 int launch_paged_attention(const PagedQueries &p, const PagedCache &cache, void *ws, int64_t, hipStream_t s) {
     const PagedPlan l = paged_plan(p.tokens, p.requests, p.n_heads, p.n_kv, p.hd);
-    if ((int64_t)l.slots * p.n_kv * l.HG > INT32_MAX || l.slots >= 1 << 25)
+    if ((int64_t)l.slots * p.n_kv * l.HG > INT32_MAX || l.slots >= 1 << 23)
         return fail(LOCALAI_EARG, "paged attention: too many tokens times heads for one call");
     char *w = (char *)ws;
     const PagedArgs a{p, cache, l.G, l.GC, l.HG, l.tpt, page_shift(cache.page_size), l.slots,
-                      (float)(p.scale * 1.4426950408889634), (float *)(w + l.part), (float2 *)(w + l.ml),
+                      p.scale < 0 ? -1.0f : p.scale == 0 ? 0.0f : 1.0f,
+                      p.scale == 0 ? 1.0f : (float)(std::fabs((double)p.scale) * 1.4426950408889634), (float *)(w + l.part), (float2 *)(w + l.ml),
                       (int2 *)(w + l.rows)};
 #define LQ_PA(T, HD) \
     if (p.hd == HD) paged_launch<T, HD>(a, l, s);
