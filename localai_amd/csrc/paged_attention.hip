@@ -144,6 +144,12 @@ __device__ __forceinline__ bool paged_work(const PagedArgs &a, int slot, int TB,
     if (!has) return false;
     const int owner = __builtin_ctzll(has);
     int at = __builtin_amdgcn_readlane(upto - mine, owner);
+    if (per == 1) {      // the owner holds its only request
+        const int ch = span <= C ? 1 : (span + C - 1) / C, local = slot - at, uc = __builtin_amdgcn_readlane(ch, owner);
+        *w = PagedWork{owner, __builtin_amdgcn_readlane(first, owner), __builtin_amdgcn_readlane(n, owner),
+                       __builtin_amdgcn_readlane(length, owner), local / uc, local % uc, uc, slot - local % uc};
+        return true;
+    }
     int b = owner * per;
     const int last = b + per - 1 < a.p.requests - 1 ? b + per - 1 : a.p.requests - 1;
     for (;;) {       // uniform: the owner's requests one by one
@@ -275,19 +281,70 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
         l[u] = phi[u] >= limit ? NAN : 0.0f;
     }
 
-    // q: lane (column n, group g) holds values [32 t + 8 g, + 8) (fp32 caches: 16 t + 4 g, + 4)
-    constexpr int QT = F32 ? HD / 16 : HD / 32;
+    const int32_t *table = a.p.table + (int64_t)w.b * a.p.table_stride;
+    const char *kc = (const char *)a.c.k, *vc = (const char *)a.c.v;
+    const int64_t page_bytes = a.c.page_stride * (int64_t)sizeof(T), head_off = kh * a.c.head_stride * (int64_t)sizeof(T);
+    const int pos_bytes = (int)(a.c.pos_stride * (int64_t)sizeof(T)), mask = (1 << a.shift) - 1;
+    const int k_lane = n * pos_bytes + 16 * g;            // + 64 t
+    const int v_lane = 4 * g * pos_bytes + VB * n;        // + i pos_bytes + 16 VB seg
+
+    const int wo = APART ? 0 : wave;
+    // pages of the wave's next 64 groups of 16 positions, one per lane
+    int pages = 0;
+    const int tiles = c1 > c0 ? (c1 - c0 + TP - 1) / TP : 0;
+    uint4 kr[NG][KW];
+    bool ok[NG];
+    int64_t off[NG];
+    auto fetch_pages = [&](int j) {       // j: index of the wave's tile, a multiple of 64 / NG
+        const int pos = c0 + ((j + lane / NG) * WS + wo) * TP + 16 * (lane % NG);
+        pages = pos < c1 ? table[pos >> a.shift] : 0;
+    };
+    auto load_k = [&](int j) {
+        const int tb = c0 + (j * WS + wo) * TP;
+#pragma unroll
+        for (int u = 0; u < NG; ++u) {
+            const int pos = tb + 16 * u;
+            const int page = __builtin_amdgcn_readlane(pages, (j * NG + u) & 63);
+            ok[u] = pos < c1 && page >= 0 && page < a.c.n_pages;
+            if (pos < c1 && !ok[u]) {     // columns that see a position of a page outside the pool
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    if (phi[t] >= pos && plo[t] < pos + 16) l[t] = NAN;
+            }
+            off[u] = (ok[u] ? (int64_t)page * page_bytes + (int64_t)(pos & mask) * pos_bytes : 0) + head_off;
+#pragma unroll
+            for (int t = 0; t < KW; ++t)
+                kr[u][t] = *reinterpret_cast<const uint4 *>(kc + off[u] + k_lane + 64 * t);
+        }
+    };
+
+    const int my = tiles > wo ? (tiles - wo + WS - 1) / WS : 0;   // tiles of this wave
+    if (my > 0) fetch_pages(0);
+
+    // q: lane (column n, group g) holds values [32 t + 8 g, + 8) (fp32 caches:
+    // 16 t + 4 g, + 4). Requested before the first K, used after it is.
+    constexpr int QT = F32 ? HD / 16 : HD / 32, QL = F32 ? 1 : 2;
+    float4 q_raw[NT][QT][QL];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+        const float *src = a.p.q + ((int64_t)(row[u] < 0 ? 0 : row[u]) * a.p.n_heads + (row[u] < 0 ? 0 : head[u])) * HD;
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int e = 0; e < QL; ++e)
+                q_raw[u][t][e] = *reinterpret_cast<const float4 *>(src + 16 * QL * t + 4 * QL * g + 4 * e);
+    }
+    if (my > 0) load_k(0);
     uint4 q[NT][QT][P::pieces];
     float unscale[NT];
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-        const float *src = a.p.q + ((int64_t)(row[u] < 0 ? 0 : row[u]) * a.p.n_heads + (row[u] < 0 ? 0 : head[u])) * HD;
         const float f = row[u] < 0 ? 0.0f : a.q_sign;
         unscale[u] = 1.0f;
         if constexpr (F32) {
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
-                const float4 v = *reinterpret_cast<const float4 *>(src + 16 * t + 4 * g);
+                const float4 v = q_raw[u][t][0];
                 q[u][t][0] = make_uint4(f_bits(v.x * f), f_bits(v.y * f), f_bits(v.z * f), f_bits(v.w * f));
             }
         } else {
@@ -295,8 +352,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
             float big = 0.0f;
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
-                const float4 v0 = *reinterpret_cast<const float4 *>(src + 32 * t + 8 * g);
-                const float4 v1 = *reinterpret_cast<const float4 *>(src + 32 * t + 8 * g + 4);
+                const float4 v0 = q_raw[u][t][0], v1 = q_raw[u][t][QL - 1];
                 const float t8[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -343,48 +399,6 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
 #pragma unroll
         for (int f = 0; f < NF; ++f) acc[u][f] = lq_f4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    const int32_t *table = a.p.table + (int64_t)w.b * a.p.table_stride;
-    const char *kc = (const char *)a.c.k, *vc = (const char *)a.c.v;
-    const int64_t page_bytes = a.c.page_stride * (int64_t)sizeof(T), head_off = kh * a.c.head_stride * (int64_t)sizeof(T);
-    const int pos_bytes = (int)(a.c.pos_stride * (int64_t)sizeof(T)), mask = (1 << a.shift) - 1;
-    const int k_lane = n * pos_bytes + 16 * g;            // + 64 t
-    const int v_lane = 4 * g * pos_bytes + VB * n;        // + i pos_bytes + 16 VB seg
-
-    const int wo = APART ? 0 : wave;
-    // pages of the wave's next 64 groups of 16 positions, one per lane
-    int pages = 0;
-    const int tiles = c1 > c0 ? (c1 - c0 + TP - 1) / TP : 0;
-    uint4 kr[NG][KW];
-    bool ok[NG];
-    int64_t off[NG];
-    auto fetch_pages = [&](int j) {       // j: index of the wave's tile, a multiple of 64 / NG
-        const int pos = c0 + ((j + lane / NG) * WS + wo) * TP + 16 * (lane % NG);
-        pages = pos < c1 ? table[pos >> a.shift] : 0;
-    };
-    auto load_k = [&](int j) {
-        const int tb = c0 + (j * WS + wo) * TP;
-#pragma unroll
-        for (int u = 0; u < NG; ++u) {
-            const int pos = tb + 16 * u;
-            const int page = __builtin_amdgcn_readlane(pages, (j * NG + u) & 63);
-            ok[u] = pos < c1 && page >= 0 && page < a.c.n_pages;
-            if (pos < c1 && !ok[u]) {     // columns that see a position of a page outside the pool
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-                    if (phi[t] >= pos && plo[t] < pos + 16) l[t] = NAN;
-            }
-            off[u] = (ok[u] ? (int64_t)page * page_bytes + (int64_t)(pos & mask) * pos_bytes : 0) + head_off;
-#pragma unroll
-            for (int t = 0; t < KW; ++t)
-                kr[u][t] = *reinterpret_cast<const uint4 *>(kc + off[u] + k_lane + 64 * t);
-        }
-    };
-
-    const int my = tiles > wo ? (tiles - wo + WS - 1) / WS : 0;   // tiles of this wave
-    if (my > 0) {
-        fetch_pages(0);
-        load_k(0);
-    }
     for (int j = 0; j < my; ++j) {
         const int tb = c0 + (j * WS + wo) * TP;
         bool good[NG];
@@ -613,12 +627,12 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
 // the 256 / (HD / 4) such groups take chunks in turn and meet in LDS.
 template <int HD>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) {
-    constexpr int LPR = HD / 4, SL = 256 / LPR;
+    constexpr int LPR = HD / 4, SL = 256 / LPR, JOIN = 8;
     __shared__ __align__(16) float red_o[SL][HD];
     __shared__ float red_m[SL], red_l[SL];
     const int64_t t = blockIdx.x;
+    const int2 info = a.rows[t];     // means nothing behind the last token
     if (a.p.starts && t >= a.p.starts[a.p.requests]) return;
-    const int2 info = a.rows[t];
     const int slot0 = info.x >> 8, chunks = info.y;
     if (chunks <= 1 || slot0 < 0 || slot0 + chunks > a.slots) return;
     const int h = (int)blockIdx.y, kh = h / a.G, hr = h % a.G, groups = a.p.n_kv * a.HG;
@@ -627,17 +641,36 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) 
     const int64_t step = (int64_t)groups * cols;
     float M = -INFINITY, L = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int c = sl; c < chunks; c += SL) {
-        const int64_t at = first + c * step;
-        const float2 ml = a.ml[at];
-        const float4 v = *reinterpret_cast<const float4 *>(a.part + at * HD + d);
-        const float mn = fmaxf(M, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
-        const float f = __builtin_amdgcn_exp2f((M - ref) * a.scale2), w = __builtin_amdgcn_exp2f((ml.x - ref) * a.scale2);
-        L = L * f + ml.y * w;
-        o.x = o.x * f + v.x * w;
-        o.y = o.y * f + v.y * w;
-        o.z = o.z * f + v.z * w;
-        o.w = o.w * f + v.w * w;
+    for (int c0 = sl; c0 < chunks; c0 += SL * JOIN) {
+        // JOIN chunks requested at once; past the last one, the first again with weight 0
+        float2 ml[JOIN];
+        float4 v[JOIN];
+#pragma unroll
+        for (int i = 0; i < JOIN; ++i) {
+            const int c = c0 + i * SL;
+            const int64_t at = first + (c < chunks ? c : sl) * step;
+            ml[i] = a.ml[at];
+            v[i] = *reinterpret_cast<const float4 *>(a.part + at * HD + d);
+            if (c >= chunks) ml[i].x = -INFINITY;
+        }
+        float mn = M;
+#pragma unroll
+        for (int i = 0; i < JOIN; ++i) mn = fmaxf(mn, ml[i].x);
+        const float ref = mn == -INFINITY ? 0.0f : mn, f = __builtin_amdgcn_exp2f((M - ref) * a.scale2);
+        L *= f;
+        o.x *= f;
+        o.y *= f;
+        o.z *= f;
+        o.w *= f;
+#pragma unroll
+        for (int i = 0; i < JOIN; ++i) {
+            const float w = __builtin_amdgcn_exp2f((ml[i].x - ref) * a.scale2);
+            L += ml[i].y * w;
+            o.x += v[i].x * w;
+            o.y += v[i].y * w;
+            o.z += v[i].z * w;
+            o.w += v[i].w * w;
+        }
         M = mn;
     }
     *reinterpret_cast<float4 *>(&red_o[sl][d]) = o;
@@ -684,7 +717,7 @@ static PagedPlan paged_plan(int64_t tokens, int requests, int n_heads, int n_kv,
     const int TB = p.cols / 16 * p.tpt;
     const int64_t most = (tokens + TB - 1) / TB + requests, blocks = most < tokens ? most : tokens;
     const int64_t want = paged_env("PG", PAGED_GROUPS) / ((int64_t)n_kv * p.HG);
-    const int64_t slots = want > 2 * blocks ? want : 2 * blocks;
+    const int64_t slots = (want > 1 ? want : 1) + blocks;
     p.slots = (int)slots;
     auto up = [](int64_t b) { return (b + 255) & ~(int64_t)255; };
     const int64_t recs = slots * n_kv * p.HG * p.cols;
