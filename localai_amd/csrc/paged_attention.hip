@@ -21,13 +21,15 @@ namespace lq {
 // The result layout of the first product (lane: column l & 15, positions
 // 4 (l >> 4) + i) is the operand layout of the second once V's rows are taken
 // in the same order, so probabilities never leave their lane; a column's
-// running maximum and sum sit in the four lanes that hold it. K rows are read
+// running offset and sum sit in the four lanes that hold it; the offset follows
+// the maximum only when a score passes it by 2^8, which after the first tiles
+// is rare, so that most tiles rescale nothing. K rows are read
 // as they lie (16 bytes of one position per lane); V rows too, 8 positions x 8
 // values per lane, transposed in registers by byte permutes.
 //
 // Precision: products of 16-bit caches are exact on MFMA, so only q and p are
 // rounded, and both are split: f16 into 2 pieces (22 bits; q scaled by a power
-// of two to [512, 1024), p by 2^14, so that small values keep their bits),
+// of two to [512, 1024), p by 2^7, so that small values keep their bits),
 // bf16 into 3 (24 bits). fp32 caches use fp32 MFMA. Sums, maxima and the
 // running statistics are fp32.
 //
@@ -45,7 +47,7 @@ struct PagedArgs {
     float q_sign;        // sign of scale (0 for 0)
     float scale2;        // |scale| * log2(e) (1 for 0)
     float *part;         // [slots, n_kv, HG, columns of a block, HD] unscaled outputs of a chunk
-    float2 *ml;          // [slots, n_kv, HG, columns] their largest score and sum
+    float2 *ml;          // [slots, n_kv, HG, columns] their c and l
     int2 *rows;          // [tokens]: first slot << 8 | first column of the token's block, chunks
 };
 
@@ -170,7 +172,7 @@ __device__ __forceinline__ bool paged_work(const PagedArgs &a, int slot, int TB,
 template <typename T> struct PaType;
 template <> struct PaType<_Float16> {
     static constexpr int pieces = 2, tile = 32;
-    static constexpr float p_bias = 14.0f;      // log2 of the probabilities' scale
+    static constexpr float p_bias = 7.0f;       // log2 of a fresh maximum's probability; a stale one's: up to 15
     static __device__ __forceinline__ lq_f4 mfma(const uint4 &x, const uint4 &y, lq_f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pa_h8, x), __builtin_bit_cast(pa_h8, y), c, 0,
                                                       0, 0);
@@ -221,7 +223,7 @@ __device__ __forceinline__ float4 gated(float4 y, const float *gate) {
 // (prompts: the four read the same K and V at about the same time, and
 // nothing has to be joined).
 template <typename T, int HD, int NT, bool APART>
-__global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel(PagedArgs a) {
     using P = PaType<T>;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int TP = P::tile, NG = TP / 16;             // positions per tile, 16-position groups of it
@@ -266,7 +268,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
 
     // columns: token and head of column 16 u + n, the positions it sees
     int plo[NT], phi[NT], row[NT], head[NT];
-    float m[NT], l[NT];
+    float c[NT], l[NT];      // probabilities are 2^(score slope - c), l is their sum over this lane's positions
     const int ti = n / a.GC, hi_g = n % a.GC;
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
@@ -277,16 +279,20 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
         head[u] = kh * a.G + h;
         phi[u] = in ? p0 + i : -1;
         plo[u] = a.p.window > 0 && (int64_t)p0 + i + 1 > a.p.window ? (int)(p0 + i + 1 - a.p.window) : 0;
-        m[u] = -INFINITY;
+        c[u] = -INFINITY;
         l[u] = phi[u] >= limit ? NAN : 0.0f;
     }
+
+    // positions that every column sees: tiles inside need no mask
+    const int lo_in = a.p.window > 0 && (int64_t)p0 + i1 > a.p.window ? (int)(p0 + i1 - a.p.window) : 0;
+    const int hi_in = p0 + i0 + 1 < limit ? p0 + i0 + 1 : limit;
 
     const int32_t *table = a.p.table + (int64_t)w.b * a.p.table_stride;
     const char *kc = (const char *)a.c.k, *vc = (const char *)a.c.v;
     const int64_t page_bytes = a.c.page_stride * (int64_t)sizeof(T), head_off = kh * a.c.head_stride * (int64_t)sizeof(T);
     const int pos_bytes = (int)(a.c.pos_stride * (int64_t)sizeof(T)), mask = (1 << a.shift) - 1;
-    const int k_lane = n * pos_bytes + 16 * g;            // + 64 t
-    const int v_lane = 4 * g * pos_bytes + VB * n;        // + i pos_bytes + 16 VB seg
+    const uint32_t k_lane = (uint32_t)(n * pos_bytes + 16 * g);       // + 64 t
+    const uint32_t v_lane = (uint32_t)(4 * g * pos_bytes + VB * n);   // + i pos_bytes + 16 VB seg
 
     const int wo = APART ? 0 : wave;
     // pages of the wave's next 64 groups of 16 positions, one per lane
@@ -314,7 +320,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
             off[u] = (ok[u] ? (int64_t)page * page_bytes + (int64_t)(pos & mask) * pos_bytes : 0) + head_off;
 #pragma unroll
             for (int t = 0; t < KW; ++t)
-                kr[u][t] = *reinterpret_cast<const uint4 *>(kc + off[u] + k_lane + 64 * t);
+                kr[u][t] = *reinterpret_cast<const uint4 *>(kc + off[u] + 64 * t + k_lane);
         }
     };
 
@@ -411,7 +417,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int s = 0; s < SEG; ++s) {
-                    const char *src = vc + off[u] + v_lane + i * pos_bytes + 16 * VB * s;
+                    const char *src = vc + off[u] + i * (int64_t)pos_bytes + 16 * VB * s + v_lane;
                     if constexpr (VB == 16) {
                         const uint4 t = *reinterpret_cast<const uint4 *>(src);
                         vr[u][i][s][0] = t.x; vr[u][i][s][1] = t.y; vr[u][i][s][2] = t.z; vr[u][i][s][3] = t.w;
@@ -463,33 +469,39 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
         }
 
         // softmax: per column, this lane's positions 16 u + 4 g + i
+        if (tb < lo_in || tb + TP > hi_in || !good[0] || !good[NG - 1]) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int u = 0; u < NG; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int pos = tb + 16 * u + 4 * g + i;
+                        sc[t][u][i] = good[u] && pos >= plo[t] && pos <= phi[t] ? sc[t][u][i] : -INFINITY;
+                    }
+        }
         uint4 pp[NT][P::pieces];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            float top = -INFINITY;
+            float top = sc[t][0][0];
 #pragma unroll
-            for (int u = 0; u < NG; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int pos = tb + 16 * u + 4 * g + i;
-                    sc[t][u][i] = good[u] && pos >= plo[t] && pos <= phi[t] ? sc[t][u][i] : -INFINITY;
-                    top = fmaxf(top, sc[t][u][i]);
-                }
-            const float mn = fmaxf(m[t], rows4_max(top));
-            const float ref = mn == -INFINITY ? 0.0f : mn;
-            if (__any(mn > m[t])) {
-                const float f = __builtin_amdgcn_exp2f((m[t] - ref) * slope[t]);
+            for (int e = 1; e < 4 * NG; ++e) top = fmaxf(top, sc[t][e / 4][e % 4]);
+            // (c = -inf: any finite score)
+            if (__any(__builtin_fmaf(top, slope[t], -c[t]) > P::p_bias + 8.0f)) {
+                const float cn = fmaxf(c[t], __builtin_fmaf(rows4_max(top), slope[t], -P::p_bias));
+                const float f = __builtin_amdgcn_exp2f(c[t] - (cn == -INFINITY ? 0.0f : cn));
                 l[t] *= f;
 #pragma unroll
                 for (int o = 0; o < NF; ++o) acc[t][o] *= f;
-                m[t] = mn;
+                c[t] = cn;
             }
+            const float off = c[t] == -INFINITY ? 0.0f : c[t];
             float p[NG][4];
 #pragma unroll
             for (int u = 0; u < NG; ++u)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    p[u][i] = __builtin_amdgcn_exp2f((sc[t][u][i] - ref) * slope[t] + P::p_bias);
+                    p[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][u][i], slope[t], -off));
                     l[t] += p[u][i];
                 }
             if constexpr (F32) {
@@ -554,7 +566,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
                         *reinterpret_cast<float4 *>(dst + d) = y;
                     }
             if (g == 0) {
-                if (w.chunks > 1) a.ml[base + col] = make_float2(m[t] * unscale[t], L);
+                if (w.chunks > 1) a.ml[base + col] = make_float2(c[t], L);
                 if (w.c == 0 && kh == 0 && hg == 0 && hi_g == 0)
                     a.rows[row[t]] = make_int2(w.slot0 << 8 | col, w.chunks);
             }
@@ -567,7 +579,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
     for (int t = 0; t < NT; ++t) {
         const float ls = rows4_sum(l[t]);
         if (g == 0) {
-            red_m[wave][16 * t + n] = m[t] * unscale[t];
+            red_m[wave][16 * t + n] = c[t];
             red_l[wave][16 * t + n] = ls;
         }
     }
@@ -598,7 +610,7 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(PagedArgs a) {
             for (int e = 0; e < PD / 16; ++e) o[e] = 0.0f;
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-                const float f = __builtin_amdgcn_exp2f((red_m[v][16 * t + col] - ref) * a.scale2);
+                const float f = __builtin_amdgcn_exp2f(red_m[v][16 * t + col] - ref);
                 L += f * red_l[v][16 * t + col];
 #pragma unroll
                 for (int e = 0; e < PD / 16; ++e) o[e] += f * red_o[v][col][dd + e];
@@ -656,7 +668,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) 
         float mn = M;
 #pragma unroll
         for (int i = 0; i < JOIN; ++i) mn = fmaxf(mn, ml[i].x);
-        const float ref = mn == -INFINITY ? 0.0f : mn, f = __builtin_amdgcn_exp2f((M - ref) * a.scale2);
+        const float ref = mn == -INFINITY ? 0.0f : mn, f = __builtin_amdgcn_exp2f(M - ref);
         L *= f;
         o.x *= f;
         o.y *= f;
@@ -664,7 +676,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) 
         o.w *= f;
 #pragma unroll
         for (int i = 0; i < JOIN; ++i) {
-            const float w = __builtin_amdgcn_exp2f((ml[i].x - ref) * a.scale2);
+            const float w = __builtin_amdgcn_exp2f(ml[i].x - ref);
             L += ml[i].y * w;
             o.x += v[i].x * w;
             o.y += v[i].y * w;
@@ -684,7 +696,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) 
     for (int i = 0; i < SL; ++i) top = fmaxf(top, red_m[i]);
     const float ref = top == -INFINITY ? 0.0f : top;
     for (int i = 0; i < SL; ++i) {
-        const float f = __builtin_amdgcn_exp2f((red_m[i] - ref) * a.scale2);
+        const float f = __builtin_amdgcn_exp2f(red_m[i] - ref);
         ls += f * red_l[i];
         os += f * red_o[i][tid];
     }
@@ -701,7 +713,6 @@ struct PagedPlan {
     int64_t part, ml, rows, bytes;
 };
 
-constexpr int PAGED_GROUPS = 2048;    // workgroups that a call is cut into, if its blocks do not ask for more
 
 static int paged_env(const char *n, int d) { const char *e = getenv(n); return e ? atoi(e) : d; }
 
@@ -716,7 +727,8 @@ static PagedPlan paged_plan(int64_t tokens, int requests, int n_heads, int n_kv,
     p.cols = (p.apart ? 64 : 16) * p.NT;
     const int TB = p.cols / 16 * p.tpt;
     const int64_t most = (tokens + TB - 1) / TB + requests, blocks = most < tokens ? most : tokens;
-    const int64_t want = paged_env("PG", PAGED_GROUPS) / ((int64_t)n_kv * p.HG);
+    const int64_t per = (int64_t)n_kv * p.HG, round = paged_env("PG", (hd == 256 ? 256 : 512)) / per;
+    const int64_t want = p.apart ? round : round > 4 * blocks ? round : 4 * blocks;
     const int64_t slots = (want > 1 ? want : 1) + blocks;
     p.slots = (int)slots;
     auto up = [](int64_t b) { return (b + 255) & ~(int64_t)255; };
