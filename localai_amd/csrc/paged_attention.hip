@@ -217,12 +217,11 @@ __device__ __forceinline__ float4 gated(float4 y, const float *gate) {
     return y;
 }
 
-// NT: column tiles of a wave. APART false: the workgroup's waves share their
-// columns and take tiles of positions in turn (decode: few columns, long
-// lengths); true: each has columns of its own, over the same positions
-// (prompts: the four read the same K and V at about the same time, and
-// nothing has to be joined).
-template <typename T, int HD, int NT, bool APART>
+// NT: column tiles of a wave; WS: waves that share columns and take tiles of
+// positions in turn, meeting in LDS. WS 4 (decode): few columns, long lengths.
+// WS 2 and 1 (prompts): the workgroup has 2 or 4 sets of columns over the same
+// positions, whose waves read the same K and V at about the same time.
+template <typename T, int HD, int NT, int WS>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel(PagedArgs a) {
     using P = PaType<T>;
     constexpr bool F32 = sizeof(T) == 4;
@@ -232,15 +231,15 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     constexpr int SEG = HD / (16 * EL), NF = HD / 16;     // segments of a V row, output tiles
     constexpr int VB = EL * (int)sizeof(T);               // bytes per lane and segment (8 or 16)
     constexpr int PD = HD < 128 ? HD : 128;               // values of a column joined at once in LDS
-    constexpr int WS = APART ? 1 : 4;                     // waves that share a chunk's tiles
-    constexpr int COLS = (APART ? 64 : 16) * NT;          // columns of a block
-    __shared__ __align__(16) float red_o[APART ? 1 : 4][APART ? 1 : 16][PD + 4];
+    constexpr int SETS = 4 / WS, COLS = SETS * 16 * NT;   // sets of columns, columns of a block
+    __shared__ __align__(16) float red_o[WS > 1 ? 4 : 1][WS > 1 ? 16 : 1][PD + 4];
     __shared__ float red_m[4][16 * NT], red_l[4][16 * NT];
 
     const int x = (int)blockIdx.x, groups = a.p.n_kv * a.HG;
     const int kh = x % a.p.n_kv, hg = (x / a.p.n_kv) % a.HG, slot = x / groups;
     const int lane = lane_id(), wave = wave_id(), n = lane & 15, g = lane >> 4;
-    const int TW = NT * a.tpt, TB = APART ? 4 * TW : TW;  // tokens of a wave, of the block
+    const int TW = NT * a.tpt, TB = SETS * TW;            // tokens of a wave, of the block
+    const int set = wave / WS, wo = wave % WS;
     PagedWork w;
     if (!paged_work(a, slot, TB, 4 * TP, &w)) return;
 
@@ -256,10 +255,12 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     const int per = ((len + w.chunks - 1) / w.chunks + 4 * TP - 1) / (4 * TP) * (4 * TP);
     const int64_t c0l = (int64_t)begin + (int64_t)w.c * per;
     int c0 = c0l < hi ? (int)c0l : hi, c1 = c0 + (int64_t)per < hi ? c0 + per : hi;
-    if constexpr (APART) {         // the same for the wave's own tokens
-        i0 += wave * TW;
-        if (i0 >= w.n) return;
+    if constexpr (SETS > 1) {         // the same for the wave's own tokens
+        i0 += set * TW;
+        if (WS == 1 && i0 >= w.n) return;
+        if (i0 > w.n) i0 = w.n;       // none: no positions either
         i1 = i0 + TW < w.n ? i0 + TW : w.n;
+        if (i1 == i0) c1 = c0;
         if (a.p.window > 0 && (int64_t)p0 + i0 + 1 > a.p.window) lo = (int)(p0 + i0 + 1 - a.p.window);
         hi = p0 + i1 < limit ? p0 + i1 : limit;
         if (c1 > hi) c1 = hi;
@@ -294,7 +295,6 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     const uint32_t k_lane = (uint32_t)(n * pos_bytes + 16 * g);       // + 64 t
     const uint32_t v_lane = (uint32_t)(4 * g * pos_bytes + VB * n);   // + i pos_bytes + 16 VB seg
 
-    const int wo = APART ? 0 : wave;
     // pages of the wave's next 64 groups of 16 positions, one per lane
     int pages = 0;
     const int tiles = c1 > c0 ? (c1 - c0 + TP - 1) / TP : 0;
@@ -543,7 +543,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     }
 
     const int64_t base = ((int64_t)slot * groups + kh * a.HG + hg) * COLS;
-    if constexpr (APART) {
+    if constexpr (WS == 1) {
         // the lane's 4 x EL adjacent values of a segment, per column
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -599,56 +599,65 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
                             make_float4(acc[t][f][i], acc[t][f + 1][i], acc[t][f + 2][i], acc[t][f + 3][i]);
                     }
             __syncthreads();
-            // 16 threads per column, PD / 16 values each
-            const int tid = (int)threadIdx.x, col = tid >> 4, dd = (tid & 15) * (PD / 16);
-            float M = red_m[0][16 * t + col];
+            // 4 WS threads per column, VT values each
+            constexpr int VT = PD / (4 * WS);
+            const int tid = (int)threadIdx.x, cset = tid / 64 / WS, col = tid / (4 * WS) % 16, dd = tid % (4 * WS) * VT;
+            const int w0 = cset * WS;
+            float M = red_m[w0][16 * t + col];
 #pragma unroll
-            for (int v = 1; v < 4; ++v) M = fmaxf(M, red_m[v][16 * t + col]);
+            for (int v = 1; v < WS; ++v) M = fmaxf(M, red_m[w0 + v][16 * t + col]);
             const float ref = M == -INFINITY ? 0.0f : M;
-            float L = 0.0f, o[PD / 16];
+            float L = 0.0f, o[VT];
 #pragma unroll
-            for (int e = 0; e < PD / 16; ++e) o[e] = 0.0f;
+            for (int e = 0; e < VT; ++e) o[e] = 0.0f;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const float f = __builtin_amdgcn_exp2f(red_m[v][16 * t + col] - ref);
-                L += f * red_l[v][16 * t + col];
+            for (int v = 0; v < WS; ++v) {
+                const float f = __builtin_amdgcn_exp2f(red_m[w0 + v][16 * t + col] - ref);
+                L += f * red_l[w0 + v][16 * t + col];
 #pragma unroll
-                for (int e = 0; e < PD / 16; ++e) o[e] += f * red_o[v][col][dd + e];
+                for (int e = 0; e < VT; ++e) o[e] += f * red_o[w0 + v][col][dd + e];
             }
-            const int cti = col / a.GC, ch = hg * a.GC + col % a.GC, i = i0 + t * a.tpt + cti, r = w.first + i;
+            const int cti = col / a.GC, ch = hg * a.GC + col % a.GC;
+            const int i = w.r * TB + cset * TW + t * a.tpt + cti, r = w.first + i;
             if (!(cti < a.tpt && ch < a.G && i < w.n && r >= 0 && r < a.p.tokens)) continue;
             const int64_t at = ((int64_t)r * a.p.n_heads + kh * a.G + ch) * HD + d0 + dd;
-            float *dst = w.chunks > 1 ? a.part + (base + 16 * t + col) * HD + d0 + dd : a.p.out + at;
+            const int bc = (cset * NT + t) * 16 + col;
+            float *dst = w.chunks > 1 ? a.part + (base + bc) * HD + d0 + dd : a.p.out + at;
             const float f = w.chunks > 1 ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
-            for (int e = 0; e < PD / 16; e += 4) {
+            for (int e = 0; e < VT; e += 4) {
                 float4 y = make_float4(o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f);
                 if (w.chunks == 1 && a.p.gate) y = gated(y, a.p.gate + at + e);
                 *reinterpret_cast<float4 *>(dst + e) = y;
             }
-            if (d0 == 0 && (tid & 15) == 0) {
-                if (w.chunks > 1) a.ml[base + 16 * t + col] = make_float2(M, L);
+            if (d0 == 0 && dd == 0) {
+                if (w.chunks > 1) a.ml[base + bc] = make_float2(M, L);
                 if (w.c == 0 && kh == 0 && hg == 0 && col % a.GC == 0)
-                    a.rows[r] = make_int2(w.slot0 << 8 | (16 * t + col), w.chunks);
+                    a.rows[r] = make_int2(w.slot0 << 8 | bc, w.chunks);
             }
         }
 }
 
-// Blocks of several chunks: out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c.
-// A workgroup takes one row and head; HD / 4 lanes hold its values, 4 each, and
-// the 256 / (HD / 4) such groups take chunks in turn and meet in LDS.
-template <int HD>
+// Blocks of several chunks: out = sum_c 2^(c_c - C) o_c / sum_c 2^(c_c - C) l_c.
+// HD / 4 lanes hold a (row, head)'s values, 4 each. SL such groups share a row
+// and head, take chunks in turn and meet in LDS (few rows of many chunks), or
+// each has its own (SL 1: many rows, of which few have several chunks).
+template <int HD, int SL>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) {
-    constexpr int LPR = HD / 4, SL = 256 / LPR, JOIN = 8;
-    __shared__ __align__(16) float red_o[SL][HD];
+    constexpr int LPR = HD / 4, RP = 256 / LPR / SL, JOIN = 8;   // lanes, rows and heads of a workgroup
+    __shared__ __align__(16) float red_o[SL > 1 ? SL : 1][HD];
     __shared__ float red_m[SL], red_l[SL];
-    const int64_t t = blockIdx.x;
+    const int tid = (int)threadIdx.x, d = 4 * (tid % LPR), sl = SL > 1 ? tid / LPR : 0;
+    const int64_t rh = (int64_t)blockIdx.x * RP + (SL > 1 ? 0 : tid / LPR);
+    if (rh >= a.p.tokens * a.p.n_heads) return;
+    const int64_t t = rh / a.p.n_heads;
+    const int h = (int)(rh % a.p.n_heads);
     const int2 info = a.rows[t];     // means nothing behind the last token
     if (a.p.starts && t >= a.p.starts[a.p.requests]) return;
     const int slot0 = info.x >> 8, chunks = info.y;
     if (chunks <= 1 || slot0 < 0 || slot0 + chunks > a.slots) return;
-    const int h = (int)blockIdx.y, kh = h / a.G, hr = h % a.G, groups = a.p.n_kv * a.HG;
-    const int col = (info.x & 255) + hr % a.GC, tid = (int)threadIdx.x, d = 4 * (tid % LPR), sl = tid / LPR;
+    const int kh = h / a.G, hr = h % a.G, groups = a.p.n_kv * a.HG;
+    const int col = (info.x & 255) + hr % a.GC;
     const int64_t first = ((int64_t)slot0 * groups + kh * a.HG + hr / a.GC) * cols + col;
     const int64_t step = (int64_t)groups * cols;
     float M = -INFINITY, L = 0.0f;
@@ -685,6 +694,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) 
         }
         M = mn;
     }
+    const int64_t at = rh * HD;
+    if constexpr (SL == 1) {
+        const float f = L == 0.0f ? 0.0f : 1.0f / L;
+        float4 y = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+        if (a.p.gate) y = gated(y, a.p.gate + at + d);
+        *reinterpret_cast<float4 *>(a.p.out + at + d) = y;
+        return;
+    }
     *reinterpret_cast<float4 *>(&red_o[sl][d]) = o;
     if (tid % LPR == 0) {
         red_m[sl] = M;
@@ -693,26 +710,25 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) 
     __syncthreads();
     if (tid >= HD) return;
     float top = -INFINITY, ls = 0.0f, os = 0.0f;
+#pragma unroll
     for (int i = 0; i < SL; ++i) top = fmaxf(top, red_m[i]);
     const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
     for (int i = 0; i < SL; ++i) {
         const float f = __builtin_amdgcn_exp2f(red_m[i] - ref);
         ls += f * red_l[i];
         os += f * red_o[i][tid];
     }
-    const int64_t at = (t * a.p.n_heads + h) * HD + tid;
     float y = ls == 0.0f ? 0.0f : os / ls;
-    if (a.p.gate) y *= 1.0f / (1.0f + expf(-fminf(fmaxf(a.p.gate[at], -80.0f), 80.0f)));
-    a.p.out[at] = y;
+    if (a.p.gate) y *= 1.0f / (1.0f + expf(-fminf(fmaxf(a.p.gate[at + tid], -80.0f), 80.0f)));
+    a.p.out[at + tid] = y;
 }
 
 // How a call is laid out, from its host-known sizes alone
 struct PagedPlan {
-    int G, GC, HG, tpt, NT, slots, cols;
-    bool apart;
+    int G, GC, HG, tpt, NT, WS, slots, cols;
     int64_t part, ml, rows, bytes;
 };
-
 
 static int paged_env(const char *n, int d) { const char *e = getenv(n); return e ? atoi(e) : d; }
 
@@ -722,13 +738,25 @@ static PagedPlan paged_plan(int64_t tokens, int requests, int n_heads, int n_kv,
     p.GC = p.G < 16 ? p.G : 16;
     p.HG = (p.G + p.GC - 1) / p.GC;
     p.tpt = 16 / p.GC;
-    p.apart = tokens >= 16 * (int64_t)requests;
-    p.NT = hd == 256 || tokens <= requests ? 1 : 2;
-    p.cols = (p.apart ? 64 : 16) * p.NT;
-    const int TB = p.cols / 16 * p.tpt;
-    const int64_t most = (tokens + TB - 1) / TB + requests, blocks = most < tokens ? most : tokens;
+    const bool decode = tokens <= requests;
+    p.NT = hd == 256 || decode ? 1 : 2;
     const int64_t per = (int64_t)n_kv * p.HG, round = paged_env("PG", (hd == 256 ? 256 : 512)) / per;
-    const int64_t want = p.apart ? round : round > 4 * blocks ? round : 4 * blocks;
+    int64_t blocks = tokens;
+    for (p.WS = decode ? 4 : 1;; p.WS *= 2) {
+        p.cols = 64 / p.WS * p.NT;
+        const int TB = p.cols / 16 * p.tpt;
+        blocks = (tokens + TB - 1) / TB + requests;
+        if (blocks > tokens) blocks = tokens;
+        if (p.WS == 4 || (tokens >= requests * TB / 2 && blocks >= round)) break;
+    }
+    p.WS = paged_env("WS", p.WS);
+    {
+        p.cols = 64 / p.WS * p.NT;
+        const int TB = p.cols / 16 * p.tpt;
+        blocks = (tokens + TB - 1) / TB + requests;
+        if (blocks > tokens) blocks = tokens;
+    }
+    const int64_t want = p.WS < 4 ? paged_env("WANT", 256) / per : round > 4 * blocks ? round : 4 * blocks;
     const int64_t slots = (want > 1 ? want : 1) + blocks;
     p.slots = (int)slots;
     auto up = [](int64_t b) { return (b + 255) & ~(int64_t)255; };
@@ -748,9 +776,18 @@ template <typename T, int HD>
 static void paged_launch(const PagedArgs &a, const PagedPlan &p, hipStream_t s) {
     constexpr int N2 = HD == 256 ? 1 : 2;
     const dim3 grid((unsigned)((int64_t)p.slots * a.p.n_kv * p.HG));
-    if (p.apart) hipLaunchKernelGGL((paged_attention_kernel<T, HD, N2, true>), grid, dim3(256), 0, s, a);
-    else if (p.NT == 1) hipLaunchKernelGGL((paged_attention_kernel<T, HD, 1, false>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((paged_attention_kernel<T, HD, N2, false>), grid, dim3(256), 0, s, a);
+    if (p.WS == 1) hipLaunchKernelGGL((paged_attention_kernel<T, HD, N2, 1>), grid, dim3(256), 0, s, a);
+    else if (p.WS == 2) hipLaunchKernelGGL((paged_attention_kernel<T, HD, N2, 2>), grid, dim3(256), 0, s, a);
+    else if (p.NT == 1) hipLaunchKernelGGL((paged_attention_kernel<T, HD, 1, 4>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((paged_attention_kernel<T, HD, N2, 4>), grid, dim3(256), 0, s, a);
+}
+
+template <int HD>
+static void paged_join_launch(const PagedArgs &a, const PagedPlan &p, hipStream_t s) {
+    const int64_t rh = a.p.tokens * a.p.n_heads;
+    constexpr int GP = 1024 / HD;      // groups of HD / 4 lanes in a workgroup
+    if (rh <= 2048) hipLaunchKernelGGL((paged_join_kernel<HD, GP>), dim3((unsigned)rh), dim3(256), 0, s, a, p.cols);
+    else hipLaunchKernelGGL((paged_join_kernel<HD, 1>), dim3((unsigned)((rh + GP - 1) / GP)), dim3(256), 0, s, a, p.cols);
 }
 
 int launch_paged_attention(const PagedQueries &p, const PagedCache &cache, void *ws, int64_t, hipStream_t s) {
@@ -769,10 +806,9 @@ int launch_paged_attention(const PagedQueries &p, const PagedCache &cache, void 
     else { LQ_PA(__bf16, 64) LQ_PA(__bf16, 128) LQ_PA(__bf16, 256) }
 #undef LQ_PA
     LQ_HIP(hipGetLastError());
-    const dim3 grid((unsigned)p.tokens, (unsigned)p.n_heads);
-    if (p.hd == 64) hipLaunchKernelGGL(paged_join_kernel<64>, grid, dim3(256), 0, s, a, l.cols);
-    else if (p.hd == 128) hipLaunchKernelGGL(paged_join_kernel<128>, grid, dim3(256), 0, s, a, l.cols);
-    else hipLaunchKernelGGL(paged_join_kernel<256>, grid, dim3(256), 0, s, a, l.cols);
+    if (p.hd == 64) paged_join_launch<64>(a, l, s);
+    else if (p.hd == 128) paged_join_launch<128>(a, l, s);
+    else paged_join_launch<256>(a, l, s);
     LQ_HIP(hipGetLastError());
     return LOCALAI_OK;
 }
