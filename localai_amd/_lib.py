@@ -72,9 +72,9 @@ SIGNATURES = {
                                           _vp, _vp, _vp, _vp, _vp, _vp]),
     'localai_hip_paged_shrink': (_c_int, [_vp, _vp, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _c_int, _vp, _vp]),
     'localai_hip_norm_rope_store': (_c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_int, _vp, _vp, _vp, _c_int, _c_int, _vp,
-                                             _vp, ctypes.c_float, _vp, ctypes.POINTER(PagedCacheArg), _vp]),
+                                             _vp, ctypes.c_float, _vp, _vp, _vp]),
     'localai_hip_paged_attention_workspace_size': (_c_i64, [_c_i64, _c_i64, _c_int, _c_int, _c_int]),
-    'localai_hip_paged_attention': (_c_int, [_vp, _c_i64, _c_int, ctypes.POINTER(PagedCacheArg), _vp, _c_i64, _c_i64,
+    'localai_hip_paged_attention': (_c_int, [_vp, _c_i64, _c_int, _vp, _vp, _c_i64, _c_i64,
                                              _vp, _vp, _c_i64, _c_i64, ctypes.c_float, _vp, _vp, _vp, _c_i64, _vp]),
     'localai_hip_debug_fused_wait': (_c_int, [_c_int, _c_int]),
     'localai_hip_register_host': (_c_int, [_vp, ctypes.c_size_t]),

@@ -28,8 +28,8 @@ from __future__ import annotations
 
 import collections
 import contextlib
-import ctypes
-import math
+import functools
+import struct
 
 from . import _lib, device
 
@@ -39,6 +39,38 @@ _TYPES = {'torch.float32': 0, 'torch.float16': 1, 'torch.bfloat16': 30}
 _STATUS = ((1, 'the pool has too few pages left'),
            (2, 'a length or count is negative, or a request is longer than its page table'),
            (4, 'more new tokens than the step has places for'))
+
+_CACHE = struct.Struct('=QQiiiiqqqq')     # localai_paged_cache
+_STRIDES = struct.Struct('=8q')
+
+
+class _Run:
+    """What every call needs, looked up once: a step makes several calls per
+    layer, and looking the device up anew took half of their host time."""
+    lib = None
+
+    def __init__(self):
+        t = device.torch()
+        self.Tensor, self.empty = t.Tensor, t.empty
+        self.i32, self.f32, self.f64 = t.int32, t.float32, t.float64
+        self.types = {t.float32: 0, t.float16: 1, t.bfloat16: 30}
+        self.device = device.device()
+        self.index = self.device.index
+        self.raw_stream = getattr(t._C, '_cuda_getCurrentRawStream', None)
+        lib = _lib.load()
+        self.extend, self.shrink = lib.localai_hip_paged_extend, lib.localai_hip_paged_shrink
+        self.store, self.attention = lib.localai_hip_norm_rope_store, lib.localai_hip_paged_attention
+        self.workspace = functools.lru_cache(4096)(lib.localai_hip_paged_attention_workspace_size)
+
+
+_run = None
+
+
+def _r():
+    global _run
+    if _run is None:
+        _run = _Run()
+    return _run
 
 
 class Step(collections.namedtuple('Step', 'lengths used starts slots positions status')):
@@ -59,29 +91,44 @@ def check(status):
                            + ' (nothing was changed)')
 
 
-def _tensor(t, name, dtype, shape=None, contiguous=True):
+def _refuse(t, name, dtype, shape):
     torch = device.torch()
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f'{name} must be a device tensor')
-    if t.device.index != device.device().index:
-        raise ValueError(f'{name} is on {t.device}, the library on {device.device()}')
-    if t.dtype != dtype or (contiguous and not t.is_contiguous()):
-        raise TypeError(f'{name} must be a {"contiguous " if contiguous else ""}{dtype} tensor')
+    if t.device.index != _r().index:
+        raise ValueError(f'{name} is on {t.device}, the library on {_r().device}')
+    if t.dtype != dtype:
+        raise TypeError(f'{name} must be a {dtype} tensor')
     if shape is not None and tuple(t.shape) != tuple(shape):
         raise ValueError(f'{name} must be {list(shape)}, got {list(t.shape)}')
+    raise TypeError(f'{name} must be contiguous')
+
+
+def _device_tensor(t, name):
+    if not isinstance(t, device.torch().Tensor) or not t.is_cuda:
+        raise TypeError(f'{name} must be a device tensor')
     return t
+
+
+def _ptr(t, name, dtype, shape=None):
+    """Address of a contiguous tensor of this type and shape on the library's device."""
+    r = _run
+    if (isinstance(t, r.Tensor) and t.dtype is dtype and t.get_device() == r.index and t.is_contiguous()
+            and (shape is None or t.shape == shape)):
+        return t.data_ptr()
+    _refuse(t, name, dtype, shape)
 
 
 def _stream(stream):
     """hipStream_t of `stream`, or of the library device's current stream."""
-    torch = device.torch()
-    if stream is not None:
-        if stream.device.index != device.device().index:
-            raise ValueError(f'the stream is on {stream.device}, the library on {device.device()}')
-        return int(stream.cuda_stream)
-    raw = getattr(torch._C, '_cuda_getCurrentRawStream', None)
-    index = device.device().index
-    return raw(index) if raw else int(torch.cuda.current_stream(index).cuda_stream)
+    r = _run
+    if stream is None:
+        if r.raw_stream:
+            return r.raw_stream(r.index)
+        return int(device.torch().cuda.current_stream(r.index).cuda_stream)
+    if stream.device.index != r.index:
+        raise ValueError(f'the stream is on {stream.device}, the library on {r.device}')
+    return int(stream.cuda_stream)
 
 
 def _on(stream):
@@ -89,13 +136,41 @@ def _on(stream):
     return contextlib.nullcontext() if stream is None else device.torch().cuda.stream(stream)
 
 
+def _empty(stream, shape, dtype):
+    r = _run
+    if stream is None:
+        return r.empty(shape, dtype=dtype, device=r.device)
+    with _on(stream):
+        return r.empty(shape, dtype=dtype, device=r.device)
+
+
 def _table(table):
-    _tensor(table, 'table', device.torch().int32, contiguous=False)
-    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError('table must be [requests, pages] with adjacent pages')
-    if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
-        raise ValueError('rows of table overlap')
-    return max(table.stride(0), table.shape[1])
+    """(address, requests, pages, row stride) of a page table."""
+    r = _run
+    if not (isinstance(table, r.Tensor) and table.dtype is r.i32 and table.get_device() == r.index):
+        _refuse(table, 'table', r.i32, None)
+    if table.dim() != 2:
+        raise ValueError('table must be [requests, pages]')
+    n, width = table.shape
+    stride, step = table.stride()
+    if step != 1 and width > 1:
+        raise ValueError('a request\'s pages must be adjacent in table')
+    if stride < width:
+        if n > 1:
+            raise ValueError('rows of table overlap')
+        stride = width
+    return table.data_ptr(), n, width, stride
+
+
+def _step_buffers(r, stream, n, tokens, lengths=None, used=None):
+    """A Step of new tensors (but for lengths and used, if given), views of one allocation."""
+    own = lengths is None
+    buf = _empty(stream, (n + 2 + 2 * tokens + (n + 1 if own else 0),), r.i32)
+    if own:
+        starts, status, slots, positions, lengths, used = buf.split_with_sizes((n + 1, 1, tokens, tokens, n, 1))
+    else:
+        starts, status, slots, positions = buf.split_with_sizes((n + 1, 1, tokens, tokens))
+    return Step(lengths, used, starts, slots, positions, status)
 
 
 def extend(lengths, new, table, free, used, page_size, tokens, out=None, stream=None):
@@ -106,75 +181,69 @@ def extend(lengths, new, table, free, used, page_size, tokens, out=None, stream=
     used[0] of them in use; tokens: places for new tokens, at least as many as
     there are. Returns a Step; lengths and used change only if `out`, a Step
     to write to, holds them. All int32."""
-    torch = device.torch()
-    i32 = torch.int32
-    stride = _table(table)
-    n, width = table.shape
-    _tensor(lengths, 'lengths', i32, (n,))
-    _tensor(new, 'new', i32, (n,))
-    _tensor(free, 'free', i32)
-    _tensor(used, 'used', i32, (1,))
+    _device_tensor(table, 'table')
+    r = _r()
+    i32 = r.i32
+    at, n, width, stride = _table(table)
     tokens = int(tokens)
+    args = (_ptr(lengths, 'lengths', i32, (n,)), _ptr(new, 'new', i32, (n,)), n, at, stride, width,
+            _ptr(free, 'free', i32), free.numel(), _ptr(used, 'used', i32, (1,)), int(page_size), tokens)
+    if tokens < 0:
+        raise ValueError('tokens must not be negative')
     if out is None:
-        with _on(stream):
-            new_lengths, rest = torch.empty(n, dtype=i32, device=table.device), torch.empty(
-                n + 3, dtype=i32, device=table.device)
-            places = torch.empty((2, tokens), dtype=i32, device=table.device)
-        out = Step(new_lengths, rest[n + 1:n + 2], rest[:n + 1], places[0], places[1], rest[n + 2:])
+        out = _step_buffers(r, stream, n, tokens)
+        ptrs = [t.data_ptr() for t in out]
     else:
-        for t, name, shape in zip(out, Step._fields, ((n,), (1,), (n + 1,), (tokens,), (tokens,), (1,))):
-            _tensor(t, name, i32, shape)
-    _lib.check(_lib.load().localai_hip_paged_extend(
-        lengths.data_ptr(), new.data_ptr(), n, table.data_ptr(), stride, width, free.data_ptr(), free.numel(),
-        used.data_ptr(), int(page_size), tokens, out.lengths.data_ptr(), out.used.data_ptr(), out.starts.data_ptr(),
-        out.slots.data_ptr(), out.positions.data_ptr(), out.status.data_ptr(), _stream(stream)))
+        ptrs = [_ptr(t, name, i32, (size,)) for t, name, size in zip(out, Step._fields, (n, 1, n + 1, tokens, tokens, 1))]
+    status = r.extend(*args, *ptrs, _stream(stream))
+    if status:
+        _lib.check(status)
     return out
 
 
 def shrink(lengths, keep, table, free, used, page_size, stream=None):
     """Cut each request to its first keep positions (localai_hip_paged_shrink):
     lengths, table, free and used are updated in place. Returns the status [1]."""
-    torch = device.torch()
-    i32 = torch.int32
-    stride = _table(table)
-    n, width = table.shape
-    _tensor(lengths, 'lengths', i32, (n,))
-    _tensor(keep, 'keep', i32, (n,))
-    _tensor(free, 'free', i32)
-    _tensor(used, 'used', i32, (1,))
-    with _on(stream):
-        status = torch.empty(1, dtype=i32, device=table.device)
-    _lib.check(_lib.load().localai_hip_paged_shrink(
-        lengths.data_ptr(), keep.data_ptr(), n, table.data_ptr(), stride, width, free.data_ptr(), free.numel(),
-        used.data_ptr(), int(page_size), status.data_ptr(), _stream(stream)))
+    _device_tensor(table, 'table')
+    r = _r()
+    i32 = r.i32
+    at, n, width, stride = _table(table)
+    args = (_ptr(lengths, 'lengths', i32, (n,)), _ptr(keep, 'keep', i32, (n,)), n, at, stride, width,
+            _ptr(free, 'free', i32), free.numel(), _ptr(used, 'used', i32, (1,)), int(page_size))
+    status = _empty(stream, (1,), i32)
+    _lib.check(r.shrink(*args, status.data_ptr(), _stream(stream)))
     return status
 
 
 def _cache(k, v):
-    """localai_paged_cache of k, v [pages, kv heads, page size, head dim] (any strides with adjacent head values)."""
-    torch = device.torch()
-    _tensor(k, 'k_cache', k.dtype if isinstance(k, torch.Tensor) else None, contiguous=False)
-    _tensor(v, 'v_cache', k.dtype, k.shape, contiguous=False)
-    kind = _TYPES.get(str(k.dtype))
+    """(localai_paged_cache, kv heads, head dim) of k, v [pages, kv heads, page size, head dim] (any strides with
+    adjacent head values)."""
+    _device_tensor(k, 'k_cache')
+    r = _r()
+    kind = r.types.get(k.dtype)
     if kind is None:
         raise TypeError('the cache must be float32, float16 or bfloat16')
-    if k.dim() != 4 or k.stride(3) != 1 or k.stride() != v.stride():
+    if k.get_device() != r.index:
+        _refuse(k, 'k_cache', k.dtype, None)
+    if not (isinstance(v, r.Tensor) and v.dtype is k.dtype and v.get_device() == r.index and v.shape == k.shape):
+        _refuse(v, 'v_cache', k.dtype, k.shape)
+    strides = k.stride()
+    if len(strides) != 4 or strides[3] != 1 or v.stride() != strides:
         raise ValueError('k_cache and v_cache must be [pages, kv heads, page size, head dim] with the same strides '
                          'and adjacent head values')
     pages, nkv, page, hd = k.shape
-    return _lib.PagedCacheArg(k.data_ptr(), v.data_ptr(), kind, nkv, hd, page, pages, k.stride(0), k.stride(1),
-                              k.stride(2))
+    return _CACHE.pack(k.data_ptr(), v.data_ptr(), kind, nkv, hd, page, pages, *strides[:3]), nkv, hd
 
 
 def _rows(t, name, tokens, heads, hd):
-    """(pointer, token stride, head stride) of t [tokens, heads, hd] fp32."""
-    _tensor(t, name, device.torch().float32, contiguous=False)
-    if t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != hd or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f'{name} must be [{tokens}, {heads if heads is not None else "heads"}, {hd}], '
-                         f'got {list(t.shape)}')
-    if hd > 1 and t.stride(2) != 1:
+    """(address, token stride, head stride) of t [tokens, heads, hd] fp32."""
+    r = _run
+    if not (isinstance(t, r.Tensor) and t.dtype is r.f32 and t.get_device() == r.index and t.shape == (tokens, heads, hd)):
+        _refuse(t, name, r.f32, (tokens, heads, hd))
+    ts, hs, step = t.stride()
+    if step != 1:
         raise ValueError(f'{name} must have adjacent head values')
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    return t.data_ptr(), ts, hs
 
 
 def norm_rope_store(q, k, v, positions, slots, k_cache, v_cache, freq=None, q_weight=None, k_weight=None, eps=1e-6,
@@ -190,33 +259,31 @@ def norm_rope_store(q, k, v, positions, slots, k_cache, v_cache, freq=None, q_we
     q_weight, k_weight [head_dim]: the norms' weights, None for no norm.
     Returns q [tokens, heads, head_dim], in `out` if given (may be q); rows of
     padding are left as they were."""
-    torch = device.torch()
-    cache = _cache(k_cache, v_cache)
-    tokens, hd = q.shape[0], cache.head_dim
+    cache, nkv, hd = _cache(k_cache, v_cache)
+    r = _r()
+    f32 = r.f32
     if rope not in ('halves', 'pairs'):
         raise ValueError("rope must be 'halves' or 'pairs'")
-    qs = _rows(q, 'q', tokens, None, hd)
-    ks, vs = _rows(k, 'k', tokens, cache.n_kv_heads, hd), _rows(v, 'v', tokens, cache.n_kv_heads, hd)
-    heads = q.shape[1]
-    _tensor(positions, 'positions', torch.int32, (tokens,))
-    _tensor(slots, 'slots', torch.int32, (tokens,))
-    n = 0
-    if freq is not None:
-        _tensor(freq, 'freq', torch.float64)
-        n = freq.numel()
-    for w, name in ((q_weight, 'q_weight'), (k_weight, 'k_weight')):
-        if w is not None:
-            _tensor(w, name, torch.float32, (hd,))
+    _device_tensor(q, 'q')
+    if q.dim() != 3:
+        raise ValueError('q must be [tokens, heads, head_dim]')
+    tokens, heads, _ = q.shape
+    qp, *qs = _rows(q, 'q', tokens, heads, hd)
+    kp, *ks = _rows(k, 'k', tokens, nkv, hd)
+    vp, *vs = _rows(v, 'v', tokens, nkv, hd)
+    at = _ptr(positions, 'positions', r.i32, (tokens,)), _ptr(slots, 'slots', r.i32, (tokens,))
+    fp, n = (_ptr(freq, 'freq', r.f64), freq.numel()) if freq is not None else (None, 0)
+    qw = _ptr(q_weight, 'q_weight', f32, (hd,)) if q_weight is not None else None
+    kw = _ptr(k_weight, 'k_weight', f32, (hd,)) if k_weight is not None else None
     if out is None:
-        with _on(stream):
-            out = torch.empty((tokens, heads, hd), dtype=torch.float32, device=q.device)
-    os = _rows(out, 'out', tokens, heads, hd)
-    strides = (ctypes.c_int64 * 8)(*qs[1:], *ks[1:], *vs[1:], *os[1:])
-    p = lambda t: t.data_ptr() if t is not None else None
-    _lib.check(_lib.load().localai_hip_norm_rope_store(
-        qs[0], ks[0], vs[0], strides, tokens, heads, positions.data_ptr(), slots.data_ptr(), p(freq), n,
-        1 if rope == 'halves' else 0, p(q_weight), p(k_weight), float(eps), os[0], ctypes.byref(cache),
-        _stream(stream)))
+        out = _empty(stream, (tokens, heads, hd), f32)
+        op, os = out.data_ptr(), (heads * hd, hd)
+    else:
+        op, *os = _rows(out, 'out', tokens, heads, hd)
+    status = r.store(qp, kp, vp, _STRIDES.pack(*qs, *ks, *vs, *os), tokens, heads, *at, fp, n, rope == 'halves', qw, kw,
+                     eps, op, cache, _stream(stream))
+    if status:
+        _lib.check(status)
     return out
 
 
@@ -231,32 +298,30 @@ def attention(q, k_cache, v_cache, table, lengths, starts=None, window=0, scale=
     sqrt(head_dim) by default; gate: Qwen3.5's output gate, like q. Returns
     [tokens, heads, head_dim]; rows behind starts[-1] of a given `out` stay as
     they were."""
-    torch = device.torch()
-    cache = _cache(k_cache, v_cache)
-    if not isinstance(q, torch.Tensor) or q.dim() != 3:
-        raise ValueError('q must be a tensor [tokens, heads, head_dim]')
-    tokens, heads, hd = q.shape
-    f32 = torch.float32
-    _tensor(q, 'q', f32, (tokens, heads, cache.head_dim))
-    stride = _table(table)
-    n, width = table.shape
-    _tensor(lengths, 'lengths', torch.int32, (n,))
-    if starts is not None:
-        _tensor(starts, 'starts', torch.int32, (n + 1,))
-    if gate is not None:
-        _tensor(gate, 'gate', f32, q.shape)
-    lib = _lib.load()
-    need = int(lib.localai_hip_paged_attention_workspace_size(tokens, n, heads, cache.n_kv_heads, hd))
-    with _on(stream):
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-        if out is None:
-            out = torch.empty_like(q)
-    _tensor(out, 'out', f32, q.shape)
-    _lib.check(lib.localai_hip_paged_attention(
-        q.data_ptr(), tokens, heads, ctypes.byref(cache), table.data_ptr(), stride, width, lengths.data_ptr(),
-        starts.data_ptr() if starts is not None else None, n, int(max(window, 0)),
-        1.0 / math.sqrt(hd) if scale is None else float(scale), gate.data_ptr() if gate is not None else None,
-        out.data_ptr(), ws.data_ptr() if ws is not None else None, max(need, 0), _stream(stream)))
+    cache, nkv, hd = _cache(k_cache, v_cache)
+    r = _r()
+    f32 = r.f32
+    _device_tensor(q, 'q')
+    if q.dim() != 3:
+        raise ValueError('q must be [tokens, heads, head_dim]')
+    shape = tokens, heads, _ = q.shape
+    qp = _ptr(q, 'q', f32, (tokens, heads, hd))
+    tp, n, width, stride = _table(table)
+    lp = _ptr(lengths, 'lengths', r.i32, (n,))
+    sp = _ptr(starts, 'starts', r.i32, (n + 1,)) if starts is not None else None
+    gp = _ptr(gate, 'gate', f32, shape) if gate is not None else None
+    need = r.workspace(tokens, n, heads, nkv, hd)
+    ws = _empty(stream, (need,), device.torch().uint8) if need > 0 else None
+    if out is None:
+        out = _empty(stream, shape, f32)
+        op = out.data_ptr()
+    else:
+        op = _ptr(out, 'out', f32, shape)
+    status = r.attention(qp, tokens, heads, cache, tp, stride, width, lp, sp, n, window if window > 0 else 0,
+                         hd ** -0.5 if scale is None else scale, gp, op, ws.data_ptr() if need > 0 else None,
+                         need if need > 0 else 0, _stream(stream))
+    if status:
+        _lib.check(status)
     return out
 
 
@@ -291,13 +356,9 @@ class PagedKVCache:
     def extend(self, new, tokens, out=None, stream=None):
         """Places for new[b] tokens of each request (of `tokens` in all at most);
         the cache's own lengths and used move on."""
-        torch = device.torch()
-        n, dev = self.lengths.numel(), self.lengths.device
+        r = _r()
         if out is None:
-            with _on(stream):
-                rest = torch.empty(n + 2, dtype=torch.int32, device=dev)
-                places = torch.empty((2, int(tokens)), dtype=torch.int32, device=dev)
-            out = Step(self.lengths, self.used, rest[:n + 1], places[0], places[1], rest[n + 1:])
+            out = _step_buffers(r, stream, self.lengths.numel(), int(tokens), self.lengths, self.used)
         return extend(self.lengths, new, self.table, self.free, self.used, self.page_size, tokens, out, stream)
 
     def shrink(self, keep, stream=None):
