@@ -328,7 +328,7 @@ int localai_hip_paged_shrink(int32_t *lengths_dev, const int32_t *keep_dev, int6
  * strides[0..7] = token and head stride of q, k, v, q_out in values (host
  * array; multiples of 4; views of one fused projection will do). q_out may be
  * q with q's strides. A token whose slot is outside [0, n_pages * page_size)
- * is padding: it reads nothing and its row of q_out stays as it was. Slots of
+ * is padding: nothing is stored and its row of q_out stays as it was. Slots of
  * one call must differ from each other. All 16-byte aligned but the index and
  * weight arrays. */
 int localai_hip_norm_rope_store(const float *q_dev, const float *k_dev, const float *v_dev, const int64_t *strides,
