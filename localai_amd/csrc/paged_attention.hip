@@ -92,6 +92,8 @@ __device__ __forceinline__ float wave_total(float v) {
     return rows4_sum(v);
 }
 
+__device__ __forceinline__ int uniform_i(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // a block's share of one workgroup
 struct PagedWork {
     int b, first, n;      // request, its first row, its new tokens
@@ -180,7 +182,7 @@ template <> struct PaType<_Float16> {
     // 2 values into one word of each piece; what a piece's truncation drops, the next one has
     static __device__ __forceinline__ void split(float x, float y, uint32_t *o) {
         const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
-        const auto l = __builtin_amdgcn_cvt_pkrtz(x - (float)h[0], y - (float)h[1]);
+        const auto l = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], -1.0f, x), __builtin_fmaf((float)h[1], -1.0f, y));
         o[0] = __builtin_bit_cast(uint32_t, h);
         o[1] = __builtin_bit_cast(uint32_t, l);
     }
@@ -242,6 +244,9 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     const int set = wave / WS, wo = wave % WS;
     PagedWork w;
     if (!paged_work(a, slot, TB, 4 * TP, &w)) return;
+    // the same on every lane: kept in scalar registers, branches on it too
+    w.b = uniform_i(w.b); w.first = uniform_i(w.first); w.n = uniform_i(w.n); w.length = uniform_i(w.length);
+    w.r = uniform_i(w.r); w.c = uniform_i(w.c); w.chunks = uniform_i(w.chunks); w.slot0 = uniform_i(w.slot0);
 
     // the block's positions: from its first token's window to its last token,
     // and of these the chunk's
@@ -304,6 +309,8 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     auto fetch_pages = [&](int j) {       // j: index of the wave's tile, a multiple of 64 / NG
         const int pos = c0 + ((j + lane / NG) * WS + wo) * TP + 16 * (lane % NG);
         pages = pos < c1 ? table[pos >> a.shift] : 0;
+        // waited for here: at its use it would be waited for behind the V loads of a tile
+        asm volatile("" : "+v"(pages));
     };
     auto load_k = [&](int j) {
         const int tb = c0 + (j * WS + wo) * TP;
@@ -427,26 +434,25 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
                     }
                 }
         }
-        // scores
+        // scores: NT NG sums side by side, so that none waits for its own last product
         lq_f4 sc[NT][NG];
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int u = 0; u < NG; ++u) {
-                lq_f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int u = 0; u < NG; ++u) sc[t][u] = lq_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int k = 0; k < KW; ++k) {
-                    if constexpr (F32) {
+        for (int k = 0; k < KW; ++k)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            s = __builtin_amdgcn_mfma_f32_16x16x4f32(u4f(kr[u][k], e), u4f(q[t][k][0], e), s, 0, 0, 0);
-                    } else {
+            for (int i = F32 ? 3 : P::pieces - 1; i >= 0; --i)
 #pragma unroll
-                        for (int i = P::pieces - 1; i >= 0; --i) s = P::mfma(kr[u][k], q[t][k][i], s);
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int u = 0; u < NG; ++u) {
+                        if constexpr (F32)
+                            sc[t][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(u4f(kr[u][k], i), u4f(q[t][k][0], i),
+                                                                            sc[t][u], 0, 0, 0);
+                        else sc[t][u] = P::mfma(kr[u][k], q[t][k][i], sc[t][u]);
                     }
-                }
-                sc[t][u] = s;
-            }
         const bool edge = tb < lo || tb + TP > hi;
         if (j + 1 < my) {
             if (((j + 1) * NG & 63) == 0) fetch_pages(j + 1);
