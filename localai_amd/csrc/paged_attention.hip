@@ -53,6 +53,7 @@ struct PagedArgs {
 
 typedef _Float16 pa_h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 pa_b8 __attribute__((ext_vector_type(8)));
+typedef uint32_t pa_u4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float bits_f(uint32_t v) { return __builtin_bit_cast(float, v); }
 __device__ __forceinline__ uint32_t f_bits(float v) { return __builtin_bit_cast(uint32_t, v); }
@@ -175,7 +176,7 @@ template <typename T> struct PaType;
 template <> struct PaType<_Float16> {
     static constexpr int pieces = 2, tile = 32;
     static constexpr float p_bias = 7.0f;       // log2 of a fresh maximum's probability; a stale one's: up to 15
-    static __device__ __forceinline__ lq_f4 mfma(const uint4 &x, const uint4 &y, lq_f4 c) {
+    static __device__ __forceinline__ lq_f4 mfma(const pa_u4 &x, const pa_u4 &y, lq_f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pa_h8, x), __builtin_bit_cast(pa_h8, y), c, 0,
                                                       0, 0);
     }
@@ -190,7 +191,7 @@ template <> struct PaType<_Float16> {
 template <> struct PaType<__bf16> {
     static constexpr int pieces = 3, tile = 32;
     static constexpr float p_bias = 0.0f;
-    static __device__ __forceinline__ lq_f4 mfma(const uint4 &x, const uint4 &y, lq_f4 c) {
+    static __device__ __forceinline__ lq_f4 mfma(const pa_u4 &x, const pa_u4 &y, lq_f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_b8, x), __builtin_bit_cast(pa_b8, y), c,
                                                        0, 0, 0);
     }
@@ -208,7 +209,7 @@ template <> struct PaType<float> {
     static constexpr float p_bias = 0.0f;
 };
 
-__device__ __forceinline__ float u4f(const uint4 &v, int i) { return bits_f(u4_get(v, i)); }
+__device__ __forceinline__ float u4f(const pa_u4 &v, int i) { return bits_f(v[i]); }
 
 __device__ __forceinline__ float4 gated(float4 y, const float *gate) {
     const float4 g = *reinterpret_cast<const float4 *>(gate);
@@ -219,10 +220,18 @@ __device__ __forceinline__ float4 gated(float4 y, const float *gate) {
     return y;
 }
 
+// which 16-byte piece of row r of K holds piece 0, times 16 (rows of RB bytes, r < 16)
+template <int RB>
+__device__ __forceinline__ uint32_t swizzle(int r) {
+    return RB == 128 ? (uint32_t)(r >> 1) * 16 : (uint32_t)r * 16;
+}
+
 // NT: column tiles of a wave; WS: waves that share columns and take tiles of
 // positions in turn, meeting in LDS. WS 4 (decode): few columns, long lengths.
-// WS 2 and 1 (prompts): the workgroup has 2 or 4 sets of columns over the same
-// positions, whose waves read the same K and V at about the same time.
+// WS 2 (prompts): the workgroup has two sets of columns over the same positions,
+// whose waves read the same K and V at about the same time. (Four sets of one
+// wave each need no meeting, but leave a prompt of 2048 tokens half the
+// workgroups: 109 us against 100; one of 8192 takes 1081 against 1099.)
 template <typename T, int HD, int NT, int WS>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel(PagedArgs a) {
     using P = PaType<T>;
@@ -234,7 +243,17 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     constexpr int VB = EL * (int)sizeof(T);               // bytes per lane and segment (8 or 16)
     constexpr int PD = HD < 128 ? HD : 128;               // values of a column joined at once in LDS
     constexpr int SETS = 4 / WS, COLS = SETS * 16 * NT;   // sets of columns, columns of a block
-    __shared__ __align__(16) float red_o[WS > 1 ? 4 : 1][WS > 1 ? 16 : 1][PD + 4];
+    // K by way of LDS (prompts, f16): a wave reads whole rows, 8 lanes or more
+    // on one, and takes its fragments from its own part of LDS. Straight from
+    // memory a fragment load touches 64 pieces of 16 bytes, four times the
+    // cycles of the L1 (963 tokens over 2048 positions: 72.8 us against 68.9). A
+    // decode step waits for HBM and does not feel that; bf16 has no registers
+    // left for it (88 us without, 114 with), fp32 waits for its products.
+    constexpr int RB = HD * (int)sizeof(T), CPR = RB / 16, RPI = 64 / CPR;   // bytes, 16-byte pieces of a row; rows a load
+    constexpr bool KL = (WS < 4 || NT > 1) && P::pieces == 2;
+    constexpr int O_BYTES = 4 * 16 * (PD + 4) * 4, K_BYTES = KL ? 4 * NG * 16 * RB : 0;
+    __shared__ __align__(16) char lds[O_BYTES > K_BYTES ? O_BYTES : K_BYTES];
+    float (*red_o)[16][PD + 4] = reinterpret_cast<float (*)[16][PD + 4]>(lds);   // after the loop
     __shared__ float red_m[4][16 * NT], red_l[4][16 * NT];
 
     const int x = (int)blockIdx.x, groups = a.p.n_kv * a.HG;
@@ -246,6 +265,11 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     if (!paged_work(a, slot, TB, 4 * TP, &w)) return;
     // the same on every lane: kept in scalar registers, branches on it too
     w.b = uniform_i(w.b); w.first = uniform_i(w.first); w.n = uniform_i(w.n); w.length = uniform_i(w.length);
+    // a request's blocks, short (early tokens) to long: the first half as they
+    // come, the second from its end, so that a CU's workgroups add up to about
+    // the same
+    const int all = (w.n + TB - 1) / TB, half = (all + 1) / 2;
+    if (w.r >= half) w.r = all - 1 - (w.r - half);
     w.r = uniform_i(w.r); w.c = uniform_i(w.c); w.chunks = uniform_i(w.chunks); w.slot0 = uniform_i(w.slot0);
 
     // the block's positions: from its first token's window to its last token,
@@ -262,7 +286,6 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     int c0 = c0l < hi ? (int)c0l : hi, c1 = c0 + (int64_t)per < hi ? c0 + per : hi;
     if constexpr (SETS > 1) {         // the same for the wave's own tokens
         i0 += set * TW;
-        if (WS == 1 && i0 >= w.n) return;
         if (i0 > w.n) i0 = w.n;       // none: no positions either
         i1 = i0 + TW < w.n ? i0 + TW : w.n;
         if (i1 == i0) c1 = c0;
@@ -297,13 +320,14 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     const char *kc = (const char *)a.c.k, *vc = (const char *)a.c.v;
     const int64_t page_bytes = a.c.page_stride * (int64_t)sizeof(T), head_off = kh * a.c.head_stride * (int64_t)sizeof(T);
     const int pos_bytes = (int)(a.c.pos_stride * (int64_t)sizeof(T)), mask = (1 << a.shift) - 1;
-    const uint32_t k_lane = (uint32_t)(n * pos_bytes + 16 * g);       // + 64 t
+    const uint32_t k_lane = KL ? (uint32_t)(lane / CPR * pos_bytes + lane % CPR * 16)
+                               : (uint32_t)(n * pos_bytes + 16 * g);  // + 64 t
     const uint32_t v_lane = (uint32_t)(4 * g * pos_bytes + VB * n);   // + i pos_bytes + 16 VB seg
 
     // pages of the wave's next 64 groups of 16 positions, one per lane
     int pages = 0;
     const int tiles = c1 > c0 ? (c1 - c0 + TP - 1) / TP : 0;
-    uint4 kr[NG][KW];
+    pa_u4 kr[NG][KW];
     bool ok[NG];
     int64_t off[NG];
     auto fetch_pages = [&](int j) {       // j: index of the wave's tile, a multiple of 64 / NG
@@ -327,9 +351,16 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
             off[u] = (ok[u] ? (int64_t)page * page_bytes + (int64_t)(pos & mask) * pos_bytes : 0) + head_off;
 #pragma unroll
             for (int t = 0; t < KW; ++t)
-                kr[u][t] = *reinterpret_cast<const uint4 *>(kc + off[u] + 64 * t + k_lane);
+                kr[u][t] = *reinterpret_cast<const pa_u4 *>(
+                    kc + off[u] + (KL ? t * RPI * (int64_t)pos_bytes : 64 * t) + k_lane);
         }
     };
+
+    // a tile's rows of K in LDS, a row's pieces exchanged by the row (swizzle):
+    // a column of fragments then lies on all banks
+    char *k_lds = lds + (KL ? wave * NG * 16 * RB : 0);
+    const uint32_t k_put = (uint32_t)(lane / CPR * RB) + ((uint32_t)(lane % CPR * 16) ^ swizzle<RB>(lane / CPR));
+    const uint32_t k_get = (uint32_t)(16 * g) ^ swizzle<RB>(n);
 
     const int my = tiles > wo ? (tiles - wo + WS - 1) / WS : 0;   // tiles of this wave
     if (my > 0) fetch_pages(0);
@@ -348,7 +379,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
                 q_raw[u][t][e] = *reinterpret_cast<const float4 *>(src + 16 * QL * t + 4 * QL * g + 4 * e);
     }
     if (my > 0) load_k(0);
-    uint4 q[NT][QT][P::pieces];
+    pa_u4 q[NT][QT][P::pieces];
     float unscale[NT];
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
@@ -358,7 +389,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
                 const float4 v = q_raw[u][t][0];
-                q[u][t][0] = make_uint4(f_bits(v.x * f), f_bits(v.y * f), f_bits(v.z * f), f_bits(v.w * f));
+                q[u][t][0] = pa_u4{f_bits(v.x * f), f_bits(v.y * f), f_bits(v.z * f), f_bits(v.w * f)};
             }
         } else {
             float v[QT][8];
@@ -397,7 +428,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
                     for (int i = 0; i < P::pieces; ++i) o[i][e] = s[i];
                 }
 #pragma unroll
-                for (int i = 0; i < P::pieces; ++i) q[u][t][i] = make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
+                for (int i = 0; i < P::pieces; ++i) q[u][t][i] = pa_u4{o[i][0], o[i][1], o[i][2], o[i][3]};
             }
         }
     }
@@ -426,13 +457,21 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
                 for (int s = 0; s < SEG; ++s) {
                     const char *src = vc + off[u] + i * (int64_t)pos_bytes + 16 * VB * s + v_lane;
                     if constexpr (VB == 16) {
-                        const uint4 t = *reinterpret_cast<const uint4 *>(src);
+                        const pa_u4 t = *reinterpret_cast<const pa_u4 *>(src);
                         vr[u][i][s][0] = t.x; vr[u][i][s][1] = t.y; vr[u][i][s][2] = t.z; vr[u][i][s][3] = t.w;
                     } else {
                         const uint2 t = *reinterpret_cast<const uint2 *>(src);
                         vr[u][i][s][0] = t.x; vr[u][i][s][1] = t.y;
                     }
                 }
+        }
+        if constexpr (KL) {
+#pragma unroll
+            for (int u = 0; u < NG; ++u)
+#pragma unroll
+                for (int i = 0; i < KW; ++i)
+                    *reinterpret_cast<pa_u4 *>(k_lds + (16 * u + i * RPI) * RB + (k_put ^ swizzle<RB>(i * RPI))) =
+                        kr[u][i];
         }
         // scores: NT NG sums side by side, so that none waits for its own last product
         lq_f4 sc[NT][NG];
@@ -441,7 +480,13 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
 #pragma unroll
             for (int u = 0; u < NG; ++u) sc[t][u] = lq_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int k = 0; k < KW; ++k)
+        for (int k = 0; k < KW; ++k) {
+            pa_u4 kf[NG];
+#pragma unroll
+            for (int u = 0; u < NG; ++u) {
+                if constexpr (KL) kf[u] = *reinterpret_cast<const pa_u4 *>(k_lds + (16 * u + n) * RB + (k_get ^ (64 * k)));
+                else kf[u] = kr[u][k];
+            }
 #pragma unroll
             for (int i = F32 ? 3 : P::pieces - 1; i >= 0; --i)
 #pragma unroll
@@ -449,10 +494,11 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
 #pragma unroll
                     for (int u = 0; u < NG; ++u) {
                         if constexpr (F32)
-                            sc[t][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(u4f(kr[u][k], i), u4f(q[t][k][0], i),
+                            sc[t][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(u4f(kf[u], i), u4f(q[t][k][0], i),
                                                                             sc[t][u], 0, 0, 0);
-                        else sc[t][u] = P::mfma(kr[u][k], q[t][k][i], sc[t][u]);
+                        else sc[t][u] = P::mfma(kf[u], q[t][k][i], sc[t][u]);
                     }
+        }
         const bool edge = tb < lo || tb + TP > hi;
         if (j + 1 < my) {
             if (((j + 1) * NG & 63) == 0) fetch_pages(j + 1);
@@ -486,7 +532,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
                         sc[t][u][i] = good[u] && pos >= plo[t] && pos <= phi[t] ? sc[t][u][i] : -INFINITY;
                     }
         }
-        uint4 pp[NT][P::pieces];
+        pa_u4 pp[NT][P::pieces];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             float top = sc[t][0][0];
@@ -511,13 +557,13 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
                     l[t] += p[u][i];
                 }
             if constexpr (F32) {
-                pp[t][0] = make_uint4(f_bits(p[0][0]), f_bits(p[0][1]), f_bits(p[0][2]), f_bits(p[0][3]));
+                pp[t][0] = pa_u4{f_bits(p[0][0]), f_bits(p[0][1]), f_bits(p[0][2]), f_bits(p[0][3])};
             } else {
                 uint32_t o[4][P::pieces];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) P::split(p[e / 2][2 * (e % 2)], p[e / 2][2 * (e % 2) + 1], o[e]);
 #pragma unroll
-                for (int i = 0; i < P::pieces; ++i) pp[t][i] = make_uint4(o[0][i], o[1][i], o[2][i], o[3][i]);
+                for (int i = 0; i < P::pieces; ++i) pp[t][i] = pa_u4{o[0][i], o[1][i], o[2][i], o[3][i]};
             }
         }
         // O^T: output tile f = EL s + e, row m of it is value 16 EL s + EL m + e
@@ -534,7 +580,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
                                 bits_f(vr[0][i][s][e]), u4f(pp[t][0], i), acc[t][EL * s + e], 0, 0, 0);
                 } else {
                     const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
-                    uint4 v;
+                    pa_u4 v;
                     v.x = __builtin_amdgcn_perm(vr[0][1][s][e / 2], vr[0][0][s][e / 2], sel);
                     v.y = __builtin_amdgcn_perm(vr[0][3][s][e / 2], vr[0][2][s][e / 2], sel);
                     v.z = __builtin_amdgcn_perm(vr[1][1][s][e / 2], vr[1][0][s][e / 2], sel);
@@ -549,37 +595,6 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     }
 
     const int64_t base = ((int64_t)slot * groups + kh * a.HG + hg) * COLS;
-    if constexpr (WS == 1) {
-        // the lane's 4 x EL adjacent values of a segment, per column
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const float L = rows4_sum(l[t]);
-            if (row[t] < 0) continue;
-            const int col = (wave * NT + t) * 16 + n;
-            const float f = w.chunks > 1 ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
-            const int64_t at = ((int64_t)row[t] * a.p.n_heads + head[t]) * HD;
-            float *dst = w.chunks > 1 ? a.part + (base + col) * HD : a.p.out + at;
-#pragma unroll
-            for (int s = 0; s < SEG; ++s)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int e = 0; e < EL; e += 4) {
-                        const int o = EL * s + e, d = 16 * EL * s + EL * (4 * g + i) + e;
-                        float4 y = make_float4(acc[t][o][i] * f, acc[t][o + 1][i] * f, acc[t][o + 2][i] * f,
-                                               acc[t][o + 3][i] * f);
-                        if (w.chunks == 1 && a.p.gate) y = gated(y, a.p.gate + at + d);
-                        *reinterpret_cast<float4 *>(dst + d) = y;
-                    }
-            if (g == 0) {
-                if (w.chunks > 1) a.ml[base + col] = make_float2(c[t], L);
-                if (w.c == 0 && kh == 0 && hg == 0 && hi_g == 0)
-                    a.rows[row[t]] = make_int2(w.slot0 << 8 | col, w.chunks);
-            }
-        }
-        return;
-    }
-
     // the waves meet
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -730,13 +745,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) 
     a.p.out[at + tid] = y;
 }
 
+constexpr int PAGED_ROUND = 512;   // workgroups on the card at once, two a CU (head_dim 256: one)
+
 // How a call is laid out, from its host-known sizes alone
 struct PagedPlan {
     int G, GC, HG, tpt, NT, WS, slots, cols;
     int64_t part, ml, rows, bytes;
 };
-
-static int paged_env(const char *n, int d) { const char *e = getenv(n); return e ? atoi(e) : d; }
 
 static PagedPlan paged_plan(int64_t tokens, int requests, int n_heads, int n_kv, int hd) {
     PagedPlan p{};
@@ -745,24 +760,28 @@ static PagedPlan paged_plan(int64_t tokens, int requests, int n_heads, int n_kv,
     p.HG = (p.G + p.GC - 1) / p.GC;
     p.tpt = 16 / p.GC;
     const bool decode = tokens <= requests;
+    // two column tiles a wave where there are several tokens (one: 84 us for
+    // the 69 of 963 tokens of 32 heads of 128); head_dim 256 has no registers
+    // for two
     p.NT = hd == 256 || decode ? 1 : 2;
-    const int64_t per = (int64_t)n_kv * p.HG, round = paged_env("PG", (hd == 256 ? 256 : 512)) / per;
-    int64_t blocks = tokens;
-    for (p.WS = decode ? 4 : 1;; p.WS *= 2) {
-        p.cols = 64 / p.WS * p.NT;
-        const int TB = p.cols / 16 * p.tpt;
-        blocks = (tokens + TB - 1) / TB + requests;
-        if (blocks > tokens) blocks = tokens;
-        if (p.WS == 4 || (tokens >= requests * TB / 2 && blocks >= round)) break;
-    }
-    p.WS = paged_env("WS", p.WS);
-    {
-        p.cols = 64 / p.WS * p.NT;
-        const int TB = p.cols / 16 * p.tpt;
-        blocks = (tokens + TB - 1) / TB + requests;
-        if (blocks > tokens) blocks = tokens;
-    }
-    const int64_t want = p.WS < 4 ? paged_env("WANT", 256) / per : round > 4 * blocks ? round : 4 * blocks;
+    const auto blocks_of = [&](int WS) {
+        const int64_t TB = 4 / WS * p.NT * p.tpt, most = (tokens + TB - 1) / TB + requests;
+        return most < tokens ? most : tokens;
+    };
+    // two column sets where requests fill them and there are blocks for every
+    // CU: 32 requests of up to 512 tokens 141 us, 219 with one set of four
+    // waves; one of 64 tokens 28.5 against 27.8
+    const int64_t per = (int64_t)n_kv * p.HG;
+    p.WS = !decode && tokens >= requests * p.NT * p.tpt && blocks_of(2) * per >= 256 ? 2 : 4;
+    p.cols = 64 / p.WS * p.NT;
+    // Chunks: decode steps fill the card once (PAGED_ROUND: the workgroups that
+    // are resident; a second round costs 131072 positions of one request 102 us
+    // for 96), or have 4 per request, whose lengths differ (64 requests up to
+    // 8192: 116 us, 122 with 2). Prompts are cut only where one request is much
+    // longer than the rest.
+    const int64_t blocks = blocks_of(p.WS);
+    const int64_t round = (hd == 256 ? PAGED_ROUND / 2 : PAGED_ROUND) / per;
+    const int64_t want = p.WS == 2 ? 256 / per : round > 4 * blocks ? round : 4 * blocks;
     const int64_t slots = (want > 1 ? want : 1) + blocks;
     p.slots = (int)slots;
     auto up = [](int64_t b) { return (b + 255) & ~(int64_t)255; };
@@ -782,8 +801,7 @@ template <typename T, int HD>
 static void paged_launch(const PagedArgs &a, const PagedPlan &p, hipStream_t s) {
     constexpr int N2 = HD == 256 ? 1 : 2;
     const dim3 grid((unsigned)((int64_t)p.slots * a.p.n_kv * p.HG));
-    if (p.WS == 1) hipLaunchKernelGGL((paged_attention_kernel<T, HD, N2, 1>), grid, dim3(256), 0, s, a);
-    else if (p.WS == 2) hipLaunchKernelGGL((paged_attention_kernel<T, HD, N2, 2>), grid, dim3(256), 0, s, a);
+    if (p.WS == 2) hipLaunchKernelGGL((paged_attention_kernel<T, HD, N2, 2>), grid, dim3(256), 0, s, a);
     else if (p.NT == 1) hipLaunchKernelGGL((paged_attention_kernel<T, HD, 1, 4>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((paged_attention_kernel<T, HD, N2, 4>), grid, dim3(256), 0, s, a);
 }

@@ -410,6 +410,41 @@ def test_attention_piece_sizes(new):
     _attention((8, 2, 128), [300, 64, 301], 'bfloat16', new=new, seed=sum(new), window=40)
 
 
+# prompts large enough for the kernel's layout with two sets of columns a workgroup: (heads, lengths, new)
+PROMPTS = [((32, 32, 64), [300, 130, 70, 0], [200, 100, 70, 0]),
+           ((64, 32, 128), [150, 33, 260], [150, 33, 90]),
+           ((32, 32, 256), [90, 140, 41], [90, 100, 41]),
+           ((40, 2, 64), [210, 5, 1], [200, 5, 1]),
+           ((51, 17, 64), [310, 64], [260, 64])]
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('heads,lengths,new', PROMPTS)
+def test_attention_prompts(heads, lengths, new, dtype):
+    _attention(heads, lengths, dtype, new=new, behind=2, seed=heads[0])
+    _attention(heads, lengths, dtype, new=new, window=37, gate=True, page=64, seed=heads[0] + 1, token_major=True)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_attention_prompts_beside_a_long_request(dtype):
+    """One request far longer than the rest: its blocks are cut into chunks and joined, the others' are not."""
+    _attention((32, 32, 64), [6000, 130, 150], dtype, new=[3, 130, 120], seed=1)
+    _attention((64, 32, 128), [60, 2500, 60, 61], dtype, new=[60, 40, 60, 61], seed=2, page=32)
+
+
+def test_attention_prompts_with_bad_pages():
+    import torch
+    from localai_amd import paged
+    (q, kc, vc, table, dl), kw, y = _attention((32, 32, 64), [200, 150, 170], 'float16', new=[150, 150, 100], nan=False)
+    table = table.clone()
+    table[1, 4] = 10 ** 6                # positions 64 to 79 of request 1
+    bad = paged.attention(q, kc, vc, table, dl, **kw).cpu().numpy()
+    np.testing.assert_array_equal(bad[:150], y[:150])
+    np.testing.assert_array_equal(bad[300:], y[300:])
+    assert np.isnan(bad[150 + 64:300]).all()
+    np.testing.assert_array_equal(bad[150:150 + 64], y[150:150 + 64])   # tokens before the bad page do not see it
+
+
 def test_attention_fewer_positions_than_tokens_sees_nothing():
     """A length below the count of new tokens: the first of them lie before position 0 and are zeros."""
     _attention((8, 2, 64), [3, 40], 'float16', new=[5, 2], seed=1)
