@@ -51,8 +51,8 @@ class _Run:
 
     def __init__(self):
         t = device.torch()
-        self.Tensor, self.empty = t.Tensor, t.empty
-        self.i32, self.f32, self.f64 = t.int32, t.float32, t.float64
+        self.Tensor, self.empty, self.split = t.Tensor, t.empty, t.unsafe_split_with_sizes
+        self.u8, self.i32, self.f32, self.f64 = t.uint8, t.int32, t.float32, t.float64
         self.types = {t.float32: 0, t.float16: 1, t.bfloat16: 30}
         self.device = device.device()
         self.index = self.device.index
@@ -165,11 +165,11 @@ def _table(table):
 def _step_buffers(r, stream, n, tokens, lengths=None, used=None):
     """A Step of new tensors (but for lengths and used, if given), views of one allocation."""
     own = lengths is None
-    buf = _empty(stream, (n + 2 + 2 * tokens + (n + 1 if own else 0),), r.i32)
+    buf = _empty(stream, n + 2 + 2 * tokens + (n + 1 if own else 0), r.i32)
     if own:
-        starts, status, slots, positions, lengths, used = buf.split_with_sizes((n + 1, 1, tokens, tokens, n, 1))
+        starts, status, slots, positions, lengths, used = r.split(buf, (n + 1, 1, tokens, tokens, n, 1))
     else:
-        starts, status, slots, positions = buf.split_with_sizes((n + 1, 1, tokens, tokens))
+        starts, status, slots, positions = r.split(buf, (n + 1, 1, tokens, tokens))
     return Step(lengths, used, starts, slots, positions, status)
 
 
@@ -210,7 +210,7 @@ def shrink(lengths, keep, table, free, used, page_size, stream=None):
     at, n, width, stride = _table(table)
     args = (_ptr(lengths, 'lengths', i32, (n,)), _ptr(keep, 'keep', i32, (n,)), n, at, stride, width,
             _ptr(free, 'free', i32), free.numel(), _ptr(used, 'used', i32, (1,)), int(page_size))
-    status = _empty(stream, (1,), i32)
+    status = _empty(stream, 1, i32)
     _lib.check(r.shrink(*args, status.data_ptr(), _stream(stream)))
     return status
 
@@ -311,7 +311,7 @@ def attention(q, k_cache, v_cache, table, lengths, starts=None, window=0, scale=
     sp = _ptr(starts, 'starts', r.i32, (n + 1,)) if starts is not None else None
     gp = _ptr(gate, 'gate', f32, shape) if gate is not None else None
     need = r.workspace(tokens, n, heads, nkv, hd)
-    ws = _empty(stream, (need,), device.torch().uint8) if need > 0 else None
+    ws = _empty(stream, need, r.u8) if need > 0 else None
     if out is None:
         out = _empty(stream, shape, f32)
         op = out.data_ptr()
