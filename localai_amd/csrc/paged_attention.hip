@@ -119,11 +119,16 @@ __device__ __forceinline__ void paged_request(const PagedArgs &a, int b, int TB,
     const int64_t seen = a.p.window + m - 1;     // positions that the request's tokens see at most
     if (a.p.window > 0 && s > seen) s = seen;
     *span = (int)s;
-    *blocks = (m + TB - 1) / TB;
+    *blocks = m <= 1 ? m : (int)((uint32_t)(m + TB - 1) / (uint32_t)TB);
+}
+
+__device__ __forceinline__ int chunks_of(int span, int C) {
+    return span <= C ? 1 : (int)((uint32_t)(span + C - 1) / (uint32_t)C);
 }
 
 // The work of slot `slot` (uniform over the wave); false if there is none
-__device__ __forceinline__ bool paged_work(const PagedArgs &a, int slot, int TB, int unit, PagedWork *w) {
+template <int unit>
+__device__ __forceinline__ bool paged_work(const PagedArgs &a, int slot, int TB, PagedWork *w) {
     const int lane = lane_id(), per = (a.p.requests + 63) >> 6;
     const int b0 = lane * per, b1 = b0 + per < a.p.requests ? b0 + per : a.p.requests;
     int first = 0, n = 0, length = 0, span = 0, blocks = 0;
@@ -137,12 +142,11 @@ __device__ __forceinline__ bool paged_work(const PagedArgs &a, int slot, int TB,
     count = wave_total(count);
     // sum of blocks * ceil(span / C) <= work / C + count <= slots (1.001: the roundings of these sums)
     const float room = fmaxf((float)a.slots - count, 1.0f);
-    const int C = ((int)fminf(work * 1.001f / room, 2.0e9f) / unit + 1) * unit;
+    const int C = (int)((uint32_t)fminf(work * 1.001f * __builtin_amdgcn_rcpf(room), 2.0e9f) / unit + 1) * unit;
     int mine = 0;
     for (int b = b0; b < b1; ++b) {
         if (per > 1) paged_request(a, b, TB, &first, &n, &length, &span, &blocks);
-        const int ch = span <= C ? 1 : (span + C - 1) / C;
-        mine += blocks * ch;
+        mine += blocks * chunks_of(span, C);
     }
     const int upto = wave_scan(mine);
     const uint64_t has = __ballot(upto > slot);
@@ -150,17 +154,17 @@ __device__ __forceinline__ bool paged_work(const PagedArgs &a, int slot, int TB,
     const int owner = __builtin_ctzll(has);
     int at = __builtin_amdgcn_readlane(upto - mine, owner);
     if (per == 1) {      // the owner holds its only request
-        const int ch = span <= C ? 1 : (span + C - 1) / C, local = slot - at, uc = __builtin_amdgcn_readlane(ch, owner);
+        const int uc = __builtin_amdgcn_readlane(chunks_of(span, C), owner);
+        const uint32_t local = slot - at, r = uc == 1 ? local : local / (uint32_t)uc, c = local - r * uc;
         *w = PagedWork{owner, __builtin_amdgcn_readlane(first, owner), __builtin_amdgcn_readlane(n, owner),
-                       __builtin_amdgcn_readlane(length, owner), local / uc, local % uc, uc, slot - local % uc};
+                       __builtin_amdgcn_readlane(length, owner), (int)r, (int)c, uc, slot - (int)c};
         return true;
     }
     int b = owner * per;
     const int last = b + per - 1 < a.p.requests - 1 ? b + per - 1 : a.p.requests - 1;
     for (;;) {       // uniform: the owner's requests one by one
         paged_request(a, b, TB, &first, &n, &length, &span, &blocks);
-        const int ch = span <= C ? 1 : (span + C - 1) / C;
-        const int local = slot - at;
+        const int ch = chunks_of(span, C), local = slot - at;
         if (local < blocks * ch || b >= last) {
             *w = PagedWork{b, first, n, length, local / ch, local % ch, ch, slot - local % ch};
             return local < blocks * ch;
@@ -256,20 +260,24 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     float (*red_o)[16][PD + 4] = reinterpret_cast<float (*)[16][PD + 4]>(lds);   // after the loop
     __shared__ float red_m[4][16 * NT], red_l[4][16 * NT];
 
-    const int x = (int)blockIdx.x, groups = a.p.n_kv * a.HG;
-    const int kh = x % a.p.n_kv, hg = (x / a.p.n_kv) % a.HG, slot = x / groups;
+    // kv head fastest: with 8 of them (or a multiple) each one's workgroups share an XCD and its L2
+    const uint32_t x = blockIdx.x;
+    const int groups = a.p.n_kv * a.HG, slot = (int)(x / (uint32_t)a.p.n_kv), kh = (int)(x - (uint32_t)(slot * a.p.n_kv));
+    const int hg = (int)blockIdx.y;
     const int lane = lane_id(), wave = wave_id(), n = lane & 15, g = lane >> 4;
     const int TW = NT * a.tpt, TB = SETS * TW;            // tokens of a wave, of the block
     const int set = wave / WS, wo = wave % WS;
     PagedWork w;
-    if (!paged_work(a, slot, TB, 4 * TP, &w)) return;
+    if (!paged_work<4 * TP>(a, slot, TB, &w)) return;
     // the same on every lane: kept in scalar registers, branches on it too
     w.b = uniform_i(w.b); w.first = uniform_i(w.first); w.n = uniform_i(w.n); w.length = uniform_i(w.length);
     // a request's blocks, short (early tokens) to long: the first half as they
     // come, the second from its end, so that a CU's workgroups add up to about
     // the same
-    const int all = (w.n + TB - 1) / TB, half = (all + 1) / 2;
-    if (w.r >= half) w.r = all - 1 - (w.r - half);
+    if (w.r > 0) {
+        const int all = (int)((uint32_t)(w.n + TB - 1) / (uint32_t)TB), half = (all + 1) / 2;
+        if (w.r >= half) w.r = all - 1 - (w.r - half);
+    }
     w.r = uniform_i(w.r); w.c = uniform_i(w.c); w.chunks = uniform_i(w.chunks); w.slot0 = uniform_i(w.slot0);
 
     // the block's positions: from its first token's window to its last token,
@@ -281,7 +289,8 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     hi = hi < limit ? hi : limit;
     const int begin = lo & ~15;
     const int len = hi > begin ? hi - begin : 0;
-    const int per = ((len + w.chunks - 1) / w.chunks + 4 * TP - 1) / (4 * TP) * (4 * TP);
+    const int even = w.chunks == 1 ? len : (int)((uint32_t)(len + w.chunks - 1) / (uint32_t)w.chunks);
+    const int per = (even + 4 * TP - 1) & ~(4 * TP - 1);
     const int64_t c0l = (int64_t)begin + (int64_t)w.c * per;
     int c0 = c0l < hi ? (int)c0l : hi, c1 = c0 + (int64_t)per < hi ? c0 + per : hi;
     if constexpr (SETS > 1) {         // the same for the wave's own tokens
@@ -298,7 +307,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     // columns: token and head of column 16 u + n, the positions it sees
     int plo[NT], phi[NT], row[NT], head[NT];
     float c[NT], l[NT];      // probabilities are 2^(score slope - c), l is their sum over this lane's positions
-    const int ti = n / a.GC, hi_g = n % a.GC;
+    const int ti = (int)((uint32_t)n / (uint32_t)a.GC), hi_g = n - ti * a.GC;
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
         const int i = i0 + u * a.tpt + ti, h = hg * a.GC + hi_g;
@@ -812,7 +821,7 @@ size_t paged_attention_workspace_bytes(int64_t tokens, int requests, int n_heads
 template <typename T, int HD>
 static void paged_launch(const PagedArgs &a, const PagedPlan &p, hipStream_t s) {
     constexpr int N2 = HD == 256 ? 1 : 2;
-    const dim3 grid((unsigned)((int64_t)p.slots * a.p.n_kv * p.HG));
+    const dim3 grid((unsigned)((int64_t)p.slots * a.p.n_kv), (unsigned)p.HG);
     if (p.WS == 2) hipLaunchKernelGGL((paged_attention_kernel<T, HD, N2, 2>), grid, dim3(256), 0, s, a);
     else if (p.NT == 1) hipLaunchKernelGGL((paged_attention_kernel<T, HD, 1, 4>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((paged_attention_kernel<T, HD, N2, 4>), grid, dim3(256), 0, s, a);
