@@ -797,12 +797,14 @@ static PagedPlan paged_plan(int64_t tokens, int requests, int n_heads, int n_kv,
     p.cols = 64 / p.WS * p.NT;
     // Chunks: decode steps fill the card once (PAGED_ROUND: the workgroups that
     // are resident; a second round costs 131072 positions of one request 102 us
-    // for 96), or have 4 per request, whose lengths differ (64 requests up to
-    // 8192: 116 us, 122 with 2). Prompts are cut only where one request is much
-    // longer than the rest.
+    // for 98), or have 4 per request, whose lengths differ, but at most four
+    // rounds (64 requests up to 8192: 117 us, 123 with one round, 124 with
+    // eight). With head_dim 256, one workgroup a CU, a second round costs more
+    // than it evens out (16 requests over 1024: 18.7 us, 24.1 with two).
+    // Prompts are cut only where one request is much longer than the rest.
     const int64_t blocks = blocks_of(p.WS);
-    const int64_t round = (hd == 256 ? PAGED_ROUND / 2 : PAGED_ROUND) / per;
-    const int64_t want = p.WS == 2 ? 256 / per : round > 4 * blocks ? round : 4 * blocks;
+    const int64_t round = (hd == 256 ? PAGED_ROUND / 2 : PAGED_ROUND) / per, most = hd == 256 ? round : 4 * round;
+    const int64_t want = p.WS == 2 ? 256 / per : 4 * blocks < round ? round : 4 * blocks < most ? 4 * blocks : most;
     const int64_t slots = (want > 1 ? want : 1) + blocks;
     p.slots = (int)slots;
     auto up = [](int64_t b) { return (b + 255) & ~(int64_t)255; };
