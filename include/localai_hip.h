@@ -327,7 +327,7 @@ int localai_hip_paged_shrink(int32_t *lengths_dev, const int32_t *keep_dev, int6
  * q [tokens, n_heads, head_dim], k, v [tokens, n_kv_heads, head_dim] fp32 with
  * strides[0..7] = token and head stride of q, k, v, q_out in values (host
  * array; multiples of 4; views of one fused projection will do). q_out may be
- * q with q's strides. A token whose slot is outside [0, n_pages * page_size)
+ * q with q's strides; tokens below 2^24. A token whose slot is outside [0, n_pages * page_size)
  * is padding: nothing is stored and its row of q_out stays as it was. Slots of
  * one call must differ from each other. All 16-byte aligned but the index and
  * weight arrays. */
@@ -356,7 +356,10 @@ int64_t localai_hip_paged_attention_workspace_size(int64_t tokens, int64_t reque
  * nothing (length 0) is zeros. A row whose range reaches past max_pages or a
  * page id outside [0, n_pages) is NaN, and nothing outside the cache is read.
  * Cached values of positions that no new token of the request sees may be
- * anything, NaN included. tokens <= 2^24, other limits as above.
+ * anything, NaN included; an infinity or NaN in a position that a row sees
+ * makes the row's results NaN or infinite. scale must be finite. tokens below
+ * 2^24, other limits as above; EARG where tokens times heads are too many for
+ * one launch (2^24 workgroups).
  * fp32 results: caches of 16 bits are read exactly, queries and probabilities
  * keep at least 21 bits in the products. How a length is split depends on all
  * requests of the call, so a row's last bits can differ between batches; the

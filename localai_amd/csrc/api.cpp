@@ -1,6 +1,8 @@
 // extern "C" entry points: library state, errors, weight handles, dequant, matvec.
 #include <hip/hip_runtime.h>
 
+#include <cfloat>
+#include <cmath>
 #include <cstring>
 #include <atomic>
 #include <mutex>
@@ -679,7 +681,7 @@ int localai_hip_norm_rope_store(const float *q, const float *k, const float *v, 
     clear_error();
     PagedCache c;
     if (int st = paged_cache_of("norm rope store", cache, &c)) return st;
-    if (tokens < 0 || tokens > INT32_MAX) return fail(LOCALAI_EARG, "norm rope store: tokens must be in 0..2^31 - 1");
+    if (tokens < 0 || tokens >= 1 << 24) return fail(LOCALAI_EARG, "norm rope store: tokens must be in 0..2^24 - 1");
     if (n_heads < 1 || n_heads > 65536 || cache->n_kv_heads > 65536)
         return fail(LOCALAI_EARG, "norm rope store: n_heads and n_kv_heads must be in 1..65536");
     if (n_freq < 0 || 2 * (int64_t)n_freq > cache->head_dim || (n_freq && !freq))
@@ -701,7 +703,7 @@ int localai_hip_norm_rope_store(const float *q, const float *k, const float *v, 
 
 int64_t localai_hip_paged_attention_workspace_size(int64_t tokens, int64_t requests, int n_heads, int n_kv,
                                                    int head_dim) {
-    if (tokens < 0 || tokens > 1 << 24 || requests < 1 || requests > PAGED_MAX_REQUESTS || n_heads < 1 ||
+    if (tokens < 0 || tokens >= 1 << 24 || requests < 1 || requests > PAGED_MAX_REQUESTS || n_heads < 1 ||
         n_heads > 65535 || n_kv < 1 || n_heads % n_kv || (head_dim != 64 && head_dim != 128 && head_dim != 256))
         return -1;
     return (int64_t)paged_attention_workspace_bytes(tokens, (int)requests, n_heads, n_kv, head_dim);
@@ -717,12 +719,13 @@ int localai_hip_paged_attention(const float *q, int64_t tokens, int n_heads, con
     if (int st = paged_cache_of("paged attention", cache, &c)) return st;
     if (int st = paged_sizes("paged attention", requests, table_stride, max_pages, cache->n_pages, cache->page_size))
         return st;
-    if (tokens < 0 || tokens > 1 << 24) return fail(LOCALAI_EARG, "paged attention: tokens must be in 0..2^24");
+    if (tokens < 0 || tokens >= 1 << 24) return fail(LOCALAI_EARG, "paged attention: tokens must be in 0..2^24 - 1");
     if (!starts && tokens != requests)
         return fail(LOCALAI_EARG, "paged attention: without starts there is one token per request");
     if (n_heads < 1 || n_heads > 65535 || n_heads % cache->n_kv_heads)
         return fail(LOCALAI_EARG, "paged attention: n_heads must be a positive multiple of n_kv_heads (at most 65535)");
     if (window < 0) return fail(LOCALAI_EARG, "paged attention: window must be >= 0");
+    if (!(std::fabs(scale) <= FLT_MAX)) return fail(LOCALAI_EARG, "paged attention: scale must be finite");
     if (!tokens) return LOCALAI_OK;
     if (!q || !table || !lengths || !out) return fail(LOCALAI_EARG, "paged attention: null pointer");
     const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(gate) |

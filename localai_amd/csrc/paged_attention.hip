@@ -115,7 +115,8 @@ __device__ __forceinline__ void paged_request(const PagedArgs &a, int b, int TB,
     *first = f;
     *n = m;
     *length = len;
-    int64_t s = len;
+    const int limit = a.p.max_pages << a.shift;  // positions that the table holds
+    int64_t s = len < limit ? len : limit;
     const int64_t seen = a.p.window + m - 1;     // positions that the request's tokens see at most
     if (a.p.window > 0 && s > seen) s = seen;
     *span = (int)s;
@@ -694,12 +695,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) 
     if (rh >= a.p.tokens * a.p.n_heads) return;
     const int64_t t = rh / a.p.n_heads;
     const int h = (int)(rh % a.p.n_heads);
-    const int2 info = a.rows[t];     // means nothing behind the last token
-    if (a.p.starts && t >= a.p.starts[a.p.requests]) return;
+    const int2 info = a.rows[t];     // means nothing outside the requests' rows
+    if (a.p.starts && (t < a.p.starts[0] || t >= a.p.starts[a.p.requests])) return;
     const int slot0 = info.x >> 8, chunks = info.y;
-    if (chunks <= 1 || slot0 < 0 || slot0 + chunks > a.slots) return;
     const int kh = h / a.G, hr = h % a.G, groups = a.p.n_kv * a.HG;
     const int col = (info.x & 255) + hr % a.GC;
+    // (the last three hold for every row that starts gives to a request)
+    if (chunks <= 1 || slot0 < 0 || slot0 > a.slots - chunks || col >= cols) return;
     const int64_t first = ((int64_t)slot0 * groups + kh * a.HG + hr / a.GC) * cols + col;
     const int64_t step = (int64_t)groups * cols;
     float M = -INFINITY, L = 0.0f;
@@ -839,7 +841,9 @@ static void paged_join_launch(const PagedArgs &a, const PagedPlan &p, hipStream_
 
 int launch_paged_attention(const PagedQueries &p, const PagedCache &cache, void *ws, int64_t, hipStream_t s) {
     const PagedPlan l = paged_plan(p.tokens, p.requests, p.n_heads, p.n_kv, p.hd);
-    if ((int64_t)l.slots * p.n_kv * l.HG > INT32_MAX || l.slots >= 1 << 23)
+    // a launch has fewer than 2^24 workgroups of 256
+    if ((int64_t)l.slots * p.n_kv * l.HG >= 1 << 24 || l.slots >= 1 << 23 ||
+        p.tokens * p.n_heads >= (int64_t)(1024 / p.hd) << 24)
         return fail(LOCALAI_EARG, "paged attention: too many tokens times heads for one call");
     char *w = (char *)ws;
     const PagedArgs a{p, cache, l.G, l.GC, l.HG, l.tpt, page_shift(cache.page_size), l.slots,

@@ -353,12 +353,10 @@ class PagedKVCache:
         self.free.copy_(device.torch().arange(self.n_pages, dtype=self.free.dtype, device=self.free.device))
         self.used.zero_()
 
-    def extend(self, new, tokens, out=None, stream=None):
+    def extend(self, new, tokens, stream=None):
         """Places for new[b] tokens of each request (of `tokens` in all at most);
         the cache's own lengths and used move on."""
-        r = _r()
-        if out is None:
-            out = _step_buffers(r, stream, self.lengths.numel(), int(tokens), self.lengths, self.used)
+        out = _step_buffers(_r(), stream, self.lengths.numel(), int(tokens), self.lengths, self.used)
         return extend(self.lengths, new, self.table, self.free, self.used, self.page_size, tokens, out, stream)
 
     def shrink(self, keep, stream=None):

@@ -450,6 +450,30 @@ def test_attention_fewer_positions_than_tokens_sees_nothing():
     _attention((8, 2, 64), [3, 40], 'float16', new=[5, 2], seed=1)
 
 
+def test_attention_rows_ahead_of_the_first_request_stay():
+    import torch
+    from localai_amd import paged
+    (q, kc, vc, table, dl), kw, y = _attention((8, 2, 64), [2000, 40], 'float16', new=[3, 2], seed=5)
+    out = torch.full((9, 8, 64), 5.0, device='cuda')
+    qq = torch.cat([q[:1], q[:1], q, q[:2]])
+    paged.attention(qq, kc, vc, table, dl, starts=_ints([2, 5, 7]), out=out)
+    np.testing.assert_array_equal(out[2:7].cpu(), y)
+    assert (out[:2] == 5.0).all() and (out[7:] == 5.0).all()
+
+
+@pytest.mark.parametrize('scale', [0.0, -0.2])
+def test_attention_scale_of_zero_and_below(scale):
+    import torch
+    from localai_amd import paged
+    (q, kc, vc, table, dl), _, _ = _attention((8, 2, 64), [300, 1, 33], 'float16', seed=6)
+    y = paged.attention(q, kc, vc, table, dl, scale=scale).cpu().numpy()
+    for b, n in enumerate([300, 1, 33]):
+        k, v = (x[table[b, :-(-n // 16)].long()].transpose(1, 2).reshape(-1, 2, 64)[:n].double().cpu().numpy()
+                for x in (kc, vc))
+        want = opaged.attention(q[b:b + 1].cpu().numpy(), k, v, 1, scale)[0][0]
+        assert np.linalg.norm(y[b] - want) <= 1e-5 * np.linalg.norm(want)
+
+
 def test_attention_one_long_request():
     _attention((8, 2, 128), [70_001], 'float16', page=64, seed=2)
     _attention((4, 1, 64), [33_000, 5, 9000], 'bfloat16', page=16, seed=3)

@@ -83,15 +83,16 @@ def test_attention_arguments_are_refused():
     lib, c = _lib.load(), cache_arg()
 
     def call(q=ONE, tokens=2, heads=4, cache=ctypes.byref(c), table=ONE, stride=8, pages=8, lengths=ONE, starts=None,
-             requests=2, window=0, gate=None, out=ONE, ws=ONE, ws_bytes=1 << 40):
+             requests=2, window=0, scale=1.0, gate=None, out=ONE, ws=ONE, ws_bytes=1 << 40):
         return lib.localai_hip_paged_attention(q, tokens, heads, cache, table, stride, pages, lengths, starts,
-                                               requests, window, 1.0, gate, out, ws, ws_bytes, None)
+                                               requests, window, scale, gate, out, ws, ws_bytes, None)
 
     odd = ctypes.c_void_p(20)
     for change in (dict(q=None), dict(q=odd), dict(tokens=-1), dict(tokens=1 << 31), dict(heads=0), dict(heads=3),
                    dict(heads=65536), dict(cache=None), dict(table=None), dict(stride=7), dict(pages=0),
                    dict(pages=1 << 28, stride=1 << 28), dict(lengths=None), dict(requests=0), dict(requests=4097),
-                   dict(tokens=3), dict(window=-1), dict(gate=odd), dict(out=None), dict(out=odd), dict(ws=odd)):
+                   dict(tokens=3), dict(window=-1), dict(scale=float('nan')), dict(scale=float('inf')),
+                   dict(tokens=1 << 24, starts=ONE), dict(gate=odd), dict(out=None), dict(out=odd), dict(ws=odd)):
         assert call(**change) == 1, change
     need = lib.localai_hip_paged_attention_workspace_size(2, 2, 4, 2, 128)
     if need > 0:
@@ -112,7 +113,7 @@ def test_store_arguments_are_refused():
     odd = ctypes.c_void_p(20)
     for change in (dict(q=None), dict(k=None), dict(v=None), dict(q=odd), dict(k=odd), dict(v=odd), dict(out=odd),
                    dict(out=None), dict(strides=(512,) * 7 + (510,)), dict(strides=(-512,) + (512,) * 7),
-                   dict(tokens=-1), dict(heads=0), dict(positions=None), dict(slots=None), dict(freq=None),
+                   dict(tokens=-1), dict(tokens=1 << 24), dict(heads=0), dict(positions=None), dict(slots=None), dict(freq=None),
                    dict(n=65), dict(n=-1), dict(halves=2), dict(cache=None)):
         assert call(**change) == 1, change
     assert call(tokens=0) == 0
