@@ -726,6 +726,7 @@ int localai_hip_paged_attention(const float *q, int64_t tokens, int n_heads, con
         return fail(LOCALAI_EARG, "paged attention: n_heads must be a positive multiple of n_kv_heads (at most 65535)");
     if (window < 0) return fail(LOCALAI_EARG, "paged attention: window must be >= 0");
     if (!(std::fabs(scale) <= FLT_MAX)) return fail(LOCALAI_EARG, "paged attention: scale must be finite");
+    if (window > INT32_MAX) window = 0;     // more than there are positions: all of them
     if (!tokens) return LOCALAI_OK;
     if (!q || !table || !lengths || !out) return fail(LOCALAI_EARG, "paged attention: null pointer");
     const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(gate) |

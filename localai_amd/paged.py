@@ -186,6 +186,8 @@ def extend(lengths, new, table, free, used, page_size, tokens, out=None, stream=
     i32 = r.i32
     at, n, width, stride = _table(table)
     tokens = int(tokens)
+    if not 0 < page_size < 1 << 31:
+        raise ValueError('page_size must be a power of two, at least 16')
     args = (_ptr(lengths, 'lengths', i32, (n,)), _ptr(new, 'new', i32, (n,)), n, at, stride, width,
             _ptr(free, 'free', i32), free.numel(), _ptr(used, 'used', i32, (1,)), int(page_size), tokens)
     if tokens < 0:
@@ -208,6 +210,8 @@ def shrink(lengths, keep, table, free, used, page_size, stream=None):
     r = _r()
     i32 = r.i32
     at, n, width, stride = _table(table)
+    if not 0 < page_size < 1 << 31:
+        raise ValueError('page_size must be a power of two, at least 16')
     args = (_ptr(lengths, 'lengths', i32, (n,)), _ptr(keep, 'keep', i32, (n,)), n, at, stride, width,
             _ptr(free, 'free', i32), free.numel(), _ptr(used, 'used', i32, (1,)), int(page_size))
     status = _empty(stream, 1, i32)
@@ -317,7 +321,7 @@ def attention(q, k_cache, v_cache, table, lengths, starts=None, window=0, scale=
         op = out.data_ptr()
     else:
         op = _ptr(out, 'out', f32, shape)
-    status = r.attention(qp, tokens, heads, cache, tp, stride, width, lp, sp, n, window if window > 0 else 0,
+    status = r.attention(qp, tokens, heads, cache, tp, stride, width, lp, sp, n, min(int(window), 1 << 31) if window > 0 else 0,
                          hd ** -0.5 if scale is None else scale, gp, op, ws.data_ptr() if need > 0 else None,
                          need if need > 0 else 0, _stream(stream))
     if status:

@@ -461,6 +461,16 @@ def test_attention_rows_ahead_of_the_first_request_stay():
     assert (out[:2] == 5.0).all() and (out[7:] == 5.0).all()
 
 
+def test_attention_window_past_every_length():
+    import torch
+    from localai_amd import paged
+    args, kw, y = _attention((8, 2, 64), [300, 1, 33], 'float16', seed=6)
+    for window in (300, 2 ** 31 - 1, 2 ** 31, 2 ** 63 - 1, 2 ** 70, -1):
+        np.testing.assert_array_equal(paged.attention(*args, window=window).cpu(), y)
+    with pytest.raises(ValueError, match='page_size'):
+        paged.extend(args[4], args[4], args[3], args[4], args[4][:1], 2 ** 32 + 16, 4)
+
+
 @pytest.mark.parametrize('scale', [0.0, -0.2])
 def test_attention_scale_of_zero_and_below(scale):
     import torch
