@@ -853,10 +853,16 @@ int launch_paged_attention(const PagedQueries &p, const PagedCache &cache, void 
     // fill, four (fp32) or eight where the blocks fill them (64 requests up to
     // 500 positions bf16: 13.9 us whole, 19.8 in chunks of 128; 256 up to 2048:
     // 130 against 138; 16 requests of 1024 with head_dim 256: 18.8 in 256, 30.4
-    // whole). Tables that hold no more than that need no second launch.
+    // whole). Tables that hold no more than that, or 128 KB of a head's K, are
+    // not cut and need no second launch (one request, 32/8 heads of 128, chunks
+    // and join against whole: 512 positions f16 9.6 and 9.6 us, 1024 9.8 and
+    // 13.7; 256 fp32 9.9 and 10.4, 512 10.1 and 15.2; the launch costs an eager
+    // caller 2.4 us of host time too).
     const bool f32 = cache.type == PAGED_F32, full = l.blocks * p.n_kv * l.HG >= 256;
-    const int least = l.WS == 2 ? 1024 : full ? (f32 ? 256 : 1024) : (f32 ? 128 : 256);
-    const bool whole = (int64_t)p.max_pages * cache.page_size <= least;
+    const int limit = p.max_pages * cache.page_size, few = (128 << 10) / (p.hd * (f32 ? 4 : 2));
+    int least = l.WS == 2 ? 1024 : full ? (f32 ? 256 : 1024) : (f32 ? 128 : 256);
+    const bool whole = limit <= least || limit <= few;
+    if (whole) least = limit;
     const PagedArgs a{p, cache, l.G, l.GC, l.HG, l.tpt, page_shift(cache.page_size), l.slots, least,
                       p.scale < 0 ? -1.0f : p.scale == 0 ? 0.0f : 1.0f,
                       p.scale == 0 ? 1.0f : (float)(std::fabs((double)p.scale) * 1.4426950408889634), (float *)(w + l.part), (float2 *)(w + l.ml),

@@ -384,6 +384,19 @@ def test_attention_many_requests(n):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('n', [65, 130, 300])
+def test_attention_many_requests_of_several_chunks(n, dtype):
+    """More requests than a wave has lanes, some long: several requests per lane, each cut by its length."""
+    rng = np.random.default_rng(n)
+    lengths = np.exp(rng.uniform(0, np.log(2500), n)).astype(int).tolist()
+    lengths[3] = lengths[n - 1] = 0
+    lengths[7] = 2500
+    _attention((2, 1, 64), lengths, dtype, seed=n)
+    new = [min(x, y) for x, y in zip(lengths, rng.integers(0, 4, n).tolist())]
+    _attention((4, 2, 64), lengths, dtype, new=new, seed=n + 1, window=900)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('window', [1, 2, 17, 128, 1000, 2 ** 40])
 def test_attention_window(window, dtype):
     _attention((8, 2, 128), [1, 16, 700, 129, 2000], dtype, window=window, seed=window % 1000)
@@ -429,7 +442,7 @@ def test_attention_prompts(heads, lengths, new, dtype):
 def test_attention_prompts_beside_a_long_request(dtype):
     """One request far longer than the rest: its blocks are cut into chunks and joined, the others' are not."""
     _attention((32, 32, 64), [6000, 130, 150], dtype, new=[3, 130, 120], seed=1)
-    _attention((64, 32, 128), [60, 2500, 60, 61], dtype, new=[60, 40, 60, 61], seed=2, page=32)
+    _attention((64, 32, 128), [60, 2500, 60, 61], dtype, new=[60, 40, 60, 61], seed=2, page=32, gate=True)
 
 
 def test_attention_prompts_with_bad_pages():
