@@ -587,6 +587,25 @@ def test_attention_same_bits_again_and_on_another_stream():
         np.testing.assert_array_equal(x.cpu().numpy(), y)
 
 
+def test_attention_calls_at_once_on_two_streams():
+    """Calls that overlap in time have workspaces of their own."""
+    import torch
+    from localai_amd import paged
+    calls = [_attention((32, 8, 128), [3000, 900, 40], 'float16', seed=31),
+             _attention((32, 8, 128), [70, 2100, 1500], 'float16', seed=32)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(12):
+        for (args, kw, _), s, g in zip(calls, streams, got):
+            with torch.cuda.stream(s):
+                g.append(paged.attention(*args, **kw))
+    torch.cuda.synchronize()
+    for (_, _, y), g in zip(calls, got):
+        for x in g:
+            np.testing.assert_array_equal(x.cpu().numpy(), y)
+
+
 def test_refusals():
     import torch
     from localai_amd import _lib, paged
