@@ -295,7 +295,8 @@ typedef struct localai_paged_cache {
  * pool has too few pages left), 2 (a negative length or count, or a request
  * past max_pages), 4 (more than `tokens` new tokens): then no table entry,
  * length or count changes, every start is 0, and every slot -1.
- * A table entry or list that names no page of the pool gives slot -1.
+ * A table entry or list that names no page of the pool gives slot -1. A page
+ * belongs to one request at a time.
  * requests <= 4096; max_pages * page_size at most 2^30. */
 int localai_hip_paged_extend(const int32_t *lengths_dev, const int32_t *fresh_dev, int64_t requests,
                              int32_t *table_dev, int64_t table_stride, int64_t max_pages,

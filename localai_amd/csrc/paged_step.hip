@@ -22,6 +22,8 @@ namespace lq {
 // A fresh page starts at a position that is itself new, so the token there
 // writes the page's table entry, and no pass over pages is needed. Every
 // workgroup scans all requests (8 bytes each) and then takes its own tokens.
+// Bound by its launch and three dependent loads (lengths, the page, the store):
+// 4.0 us for one request, 4.8 for 256, 6.4 for 48 prompts of 36958 tokens.
 struct ExtendArgs {
     const int32_t *lengths, *fresh, *free, *used;
     int32_t *table;
@@ -239,6 +241,9 @@ int launch_paged_shrink(int32_t *lengths, const int32_t *keep, int requests, int
 // The angle is taken in fp64, in turns: position * (freq / 2 pi) less its
 // nearest whole number, whose rounding to fp32 leaves 2^-25 of a turn at any
 // position. Streams its rows once; a row is held by hd / 4 lanes, 4 values each.
+// Bound by memory for many tokens (8192 of 64 + 2 x 8 heads of 128, bf16 cache:
+// 124 us, 5.1 TB/s read and written) and by two dependent loads and the launch
+// for few (one token 3.8 us; 777 of 16 + 2 x 4 heads of 256, 35 MB: 12.3 us).
 struct StoreArgs {
     const float *q, *k, *v;
     int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;   // token and head strides
@@ -390,7 +395,7 @@ __global__ __launch_bounds__(256) void norm_rope_store_kernel(StoreArgs a) {
                 y[i][e] = plain ? v[e] : s * cs[e] + o * sn[e];
             }
         }
-        // in place, rows are read before any row of a later batch is written: each row is one wave's
+        // (in place: a row is read and written by one wave, and read first)
         if (first + NR * dr < rows) request(first + NR * dr);
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
