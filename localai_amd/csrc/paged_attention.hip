@@ -263,12 +263,19 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     // on one, and takes its fragments from its own part of LDS. Straight from
     // memory a fragment load touches 64 pieces of 16 bytes, four times the
     // cycles of the L1 (963 tokens over 2048 positions: 72.8 us against 68.9). A
-    // decode step waits for HBM and does not feel that; bf16 has no registers
-    // left for it (88 us without, 114 with), fp32 waits for its products.
+    // decode step waits for HBM and does not feel that; bf16's q takes the LDS
+    // for it, fp32 waits for its products.
     constexpr int RB = HD * (int)sizeof(T), CPR = RB / 16, RPI = 64 / CPR;   // bytes, 16-byte pieces of a row; rows a load
     constexpr bool KL = (WS < 4 || NT > 1) && P::pieces == 2;
+    constexpr int QT = F32 ? HD / 16 : HD / 32, QL = F32 ? 1 : 2;   // steps of a product over d; float4s of q for one
+    // q's three bf16 pieces of two column tiles stay in LDS, a copy for each
+    // set: in registers they spill (963 tokens over 2048 positions 86 us, 72
+    // so; 8192 tokens 1613 and 1372). f16's two fit, and are faster there (8192
+    // tokens 1096 us against 1157).
+    constexpr bool QS = P::pieces == 3 && NT == 2;
+    constexpr int Q_BYTES = QS ? SETS * NT * QT * P::pieces * 1024 : 0;
     constexpr int O_BYTES = 4 * 16 * (PD + 4) * 4, K_BYTES = KL ? 4 * NG * 16 * RB : 0;
-    __shared__ __align__(16) char lds[O_BYTES > K_BYTES ? O_BYTES : K_BYTES];
+    __shared__ __align__(16) char lds[O_BYTES > Q_BYTES + K_BYTES ? O_BYTES : Q_BYTES + K_BYTES];
     float (*red_o)[16][PD + 4] = reinterpret_cast<float (*)[16][PD + 4]>(lds);   // after the loop
     __shared__ float red_m[4][16 * NT], red_l[4][16 * NT];
 
@@ -379,7 +386,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
 
     // a tile's rows of K in LDS, a row's pieces exchanged by the row (swizzle):
     // a column of fragments then lies on all banks
-    char *k_lds = lds + (KL ? wave * NG * 16 * RB : 0);
+    char *k_lds = lds + Q_BYTES + (KL ? wave * NG * 16 * RB : 0);
     const uint32_t k_put = (uint32_t)(lane / CPR * RB) + ((uint32_t)(lane % CPR * 16) ^ swizzle<RB>(lane / CPR));
     const uint32_t k_get = (uint32_t)(16 * g) ^ swizzle<RB>(n);
 
@@ -388,7 +395,6 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
 
     // q: lane (column n, group g) holds values [32 t + 8 g, + 8) (fp32 caches:
     // 16 t + 4 g, + 4). Requested before the first K, used after it is.
-    constexpr int QT = F32 ? HD / 16 : HD / 32, QL = F32 ? 1 : 2;
     float4 q_raw[NT][QT][QL];
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
@@ -454,6 +460,18 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
         }
     }
 
+    pa_u4 *q_lds = reinterpret_cast<pa_u4 *>(lds) + (QS ? set * (NT * QT * P::pieces * 64) + lane : 0);
+    if constexpr (QS) {
+        if (wo == 0)
+#pragma unroll
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+                for (int t = 0; t < QT; ++t)
+#pragma unroll
+                    for (int i = 0; i < P::pieces; ++i) q_lds[((u * QT + t) * P::pieces + i) * 64] = q[u][t][i];
+        __syncthreads();
+    }
+
     float slope[NT];      // of the exponent over a score in the scaled q's units
 #pragma unroll
     for (int u = 0; u < NT; ++u) slope[u] = fmaxf(a.scale2 * unscale[u], 1e-37f);   // never 0: -inf times it stays
@@ -516,14 +534,18 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
 #pragma unroll
             for (int i = F32 ? 3 : P::pieces - 1; i >= 0; --i)
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+                for (int t = 0; t < NT; ++t) {
+                    pa_u4 qf;
+                    if constexpr (QS) qf = q_lds[((t * QT + k) * P::pieces + i) * 64];
+                    else qf = q[t][k][F32 ? 0 : i];
 #pragma unroll
                     for (int u = 0; u < NG; ++u) {
                         if constexpr (F32)
-                            part[t][u][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(u4f(kf[u], i), u4f(q[t][k][0], i),
+                            part[t][u][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(u4f(kf[u], i), u4f(qf, i),
                                                                                  part[t][u][i], 0, 0, 0);
-                        else part[t][u][0] = P::mfma(kf[u], q[t][k][i], part[t][u][0]);
+                        else part[t][u][0] = P::mfma(kf[u], qf, part[t][u][0]);
                     }
+                }
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
