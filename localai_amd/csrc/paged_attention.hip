@@ -514,8 +514,10 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
         }
         // scores: several sums side by side, so that no product waits for the
         // one before it; fp32's are four for each score, which also lowers their
-        // rounding error (output of 4096 positions: 4.4e-7 off in place of 1.3e-6)
-        constexpr int PS = F32 ? 4 : 1;
+        // rounding error (output of 4096 positions: 4.4e-7 off in place of 1.3e-6);
+        // 16-bit types sum q's first piece apart from the small others where
+        // registers allow
+        constexpr int PS = F32 ? 4 : NT == 1 || QS ? 2 : 1;
         lq_f4 sc[NT][NG], part[NT][NG][PS];
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -543,7 +545,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
                         if constexpr (F32)
                             part[t][u][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(u4f(kf[u], i), u4f(qf, i),
                                                                                  part[t][u][i], 0, 0, 0);
-                        else part[t][u][0] = P::mfma(kf[u], qf, part[t][u][0]);
+                        else part[t][u][i && PS > 1] = P::mfma(kf[u], qf, part[t][u][i && PS > 1]);
                     }
                 }
         }
@@ -552,7 +554,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
 #pragma unroll
             for (int u = 0; u < NG; ++u) {
                 if constexpr (F32) sc[t][u] = (part[t][u][0] + part[t][u][1]) + (part[t][u][2] + part[t][u][3]);
-                else sc[t][u] = part[t][u][0];
+                else sc[t][u] = PS > 1 ? part[t][u][0] + part[t][u][PS - 1] : part[t][u][0];
             }
         const bool edge = tb < lo || tb + TP > hi;
         if (j + 1 < my) {
