@@ -154,3 +154,11 @@ def test_python_checks_without_a_device():
         paged.norm_rope_store(x, x, x, z, z, x[None], x[None])
     with pytest.raises(RuntimeError, match='too few pages.*places'):
         paged.check(torch.tensor([5]))
+
+
+def test_packed_cache_argument_is_the_c_structure():
+    from localai_amd import paged
+    c = cache_arg(k_dev=0x1234567890, v_dev=0x987654320, type=30, page_stride=1 << 40)
+    fields = [getattr(c, n) for n, _ in c._fields_]
+    assert paged._CACHE.pack(*fields) == bytes(c)
+    assert paged._STRIDES.pack(*range(8)) == bytes((ctypes.c_int64 * 8)(*range(8)))
