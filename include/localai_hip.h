@@ -356,9 +356,10 @@ int64_t localai_hip_paged_attention_workspace_size(int64_t tokens, int64_t reque
  * requests). q, gate, out fp32 [tokens, n_heads, head_dim]. A row that sees
  * nothing (length 0) is zeros. A row whose range reaches past max_pages or a
  * page id outside [0, n_pages) is NaN, and nothing outside the cache is read.
- * Cached values of positions that no new token of the request sees may be
- * anything, NaN included; an infinity or NaN in a position that a row sees
- * makes the row's results NaN or infinite. scale must be finite. tokens below
+ * What positions that a row does not see hold does not reach it, infinities
+ * and NaN included. A v that is infinite or NaN makes that value of the rows
+ * that see it NaN or infinite, and no other; a NaN k makes the rows that see it
+ * NaN. scale must be finite. tokens below
  * 2^24, other limits as above; EARG where tokens times heads are too many for
  * one launch (2^24 workgroups).
  * fp32 results: caches of 16 bits are read exactly, queries and probabilities

@@ -188,8 +188,23 @@ __device__ __forceinline__ bool paged_work(const PagedArgs &a, int slot, int TB,
 
 // ---- operand pieces by cache type
 
+// a word of 16-bit values without those that are infinite or NaN
+template <uint32_t INF>
+__device__ __forceinline__ uint32_t finite16(uint32_t w) {
+    w = (w & 0x7fffu) >= INF ? w & 0xffff0000u : w;
+    return (w & 0x7fff0000u) >= INF << 16 ? w & 0xffffu : w;
+}
+// the larger magnitudes of two words of 16-bit values, half by half
+__device__ __forceinline__ uint32_t larger16(uint32_t m, uint32_t w) {
+    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, m),
+                                                                  __builtin_bit_cast(us2, w & 0x7fff7fffu)));
+}
+
+// larger, infinite: of words of the cache, whether one holds an infinity or NaN; finite: a word without them
 template <typename T> struct PaType;
 template <> struct PaType<_Float16> {
+    static constexpr uint32_t one = 0x3c00, inf = 0x7c00, magnitude = 0x7fff;
     static constexpr int pieces = 2, tile = 32;
     static constexpr float p_bias = 7.0f;       // log2 of a fresh maximum's probability; a stale one's: up to 15
     static __device__ __forceinline__ lq_f4 mfma(const pa_u4 &x, const pa_u4 &y, lq_f4 c) {
@@ -203,8 +218,12 @@ template <> struct PaType<_Float16> {
         o[0] = __builtin_bit_cast(uint32_t, h);
         o[1] = __builtin_bit_cast(uint32_t, l);
     }
+    static __device__ __forceinline__ uint32_t larger(uint32_t m, uint32_t w) { return larger16(m, w); }
+    static __device__ __forceinline__ bool infinite(uint32_t m) { return (m & 0xffffu) >= inf || m >= inf << 16; }
+    static __device__ __forceinline__ uint32_t finite(uint32_t w) { return finite16<inf>(w); }
 };
 template <> struct PaType<__bf16> {
+    static constexpr uint32_t one = 0x3f80, inf = 0x7f80, magnitude = 0x7fff;
     static constexpr int pieces = 3, tile = 32;
     static constexpr float p_bias = 0.0f;
     static __device__ __forceinline__ lq_f4 mfma(const pa_u4 &x, const pa_u4 &y, lq_f4 c) {
@@ -219,13 +238,74 @@ template <> struct PaType<__bf16> {
             y -= bits_f(f_bits(y) & 0xffff0000u);
         }
     }
+    static __device__ __forceinline__ uint32_t larger(uint32_t m, uint32_t w) { return larger16(m, w); }
+    static __device__ __forceinline__ bool infinite(uint32_t m) { return (m & 0xffffu) >= inf || m >= inf << 16; }
+    static __device__ __forceinline__ uint32_t finite(uint32_t w) { return finite16<inf>(w); }
 };
 template <> struct PaType<float> {
     static constexpr int pieces = 1, tile = 16;
     static constexpr float p_bias = 0.0f;
+    static constexpr uint32_t one = 0x3f800000u, inf = 0x7f800000u, magnitude = 0x7fffffffu;
+    static __device__ __forceinline__ uint32_t larger(uint32_t m, uint32_t w) {
+        w &= magnitude;
+        return m > w ? m : w;
+    }
+    static __device__ __forceinline__ bool infinite(uint32_t m) { return m >= inf; }
+    static __device__ __forceinline__ uint32_t finite(uint32_t w) { return (w & magnitude) >= inf ? 0u : w; }
 };
 
 __device__ __forceinline__ float u4f(const pa_u4 &v, int i) { return bits_f(v[i]); }
+
+// acc as the kernel below has it: NaN where V (vr, the tile whose first position
+// of this lane is pos) is infinite or NaN at a position that the column sees.
+// What is not finite (1 or 0) times what is seen (1 or 0) counts these.
+template <typename T, int NT, int NG, int SEG, int W, int NF>
+__device__ __forceinline__ void spoil_values(const uint32_t (&vr)[NG][4][SEG][W], lq_f4 (&acc)[NT][NF],
+                                             const int (&plo)[NT], const int (&phi)[NT], int pos) {
+    using P = PaType<T>;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int H = F32 ? 1 : 2;       // values of a word
+    const auto words = [](const uint32_t (&o)[NG][4]) {     // an operand, in the order of the probabilities
+        if constexpr (F32) return pa_u4{o[0][0], o[0][1], o[0][2], o[0][3]};
+        else return pa_u4{o[0][0] | o[0][1] << 16, o[0][2] | o[0][3] << 16, o[NG - 1][0] | o[NG - 1][1] << 16,
+                          o[NG - 1][2] | o[NG - 1][3] << 16};
+    };
+    pa_u4 sees[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        uint32_t o[NG][4];
+#pragma unroll
+        for (int u = 0; u < NG; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[u][i] = pos + 16 * u + i >= plo[t] && pos + 16 * u + i <= phi[t] ? P::one : 0u;
+        sees[t] = words(o);
+    }
+#pragma unroll
+    for (int s = 0; s < SEG; ++s)
+#pragma unroll
+        for (int e = 0; e < H * W; ++e) {
+            uint32_t o[NG][4];
+#pragma unroll
+            for (int u = 0; u < NG; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    o[u][i] = (vr[u][i][s][e / H] >> (F32 ? 0 : 16 * (e & 1)) & P::magnitude) >= P::inf ? P::one : 0u;
+            const pa_u4 bad = words(o);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                lq_f4 c = lq_f4{0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (F32) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        c = __builtin_amdgcn_mfma_f32_16x16x4f32(u4f(bad, i), u4f(sees[t], i), c, 0, 0, 0);
+                } else {
+                    c = P::mfma(bad, sees[t], c);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[t][H * W * s + e][i] = c[i] > 0.0f ? NAN : acc[t][H * W * s + e][i];
+            }
+        }
+}
 
 __device__ __forceinline__ float4 gated(float4 y, const float *gate) {
     const float4 g = *reinterpret_cast<const float4 *>(gate);
@@ -482,14 +562,10 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
 #pragma unroll
         for (int f = 0; f < NF; ++f) acc[u][f] = lq_f4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    for (int j = 0; j < my; ++j) {
-        const int tb = c0 + (j * WS + wo) * TP;
-        bool good[NG];
-        // V: group u, position 4 g + i, segment s
-        uint32_t vr[NG][4][SEG][VB / 4];
+    // V: group u, position 4 g + i, segment s
+    auto load_v = [&](uint32_t (&vr)[NG][4][SEG][VB / 4]) {
 #pragma unroll
-        for (int u = 0; u < NG; ++u) {
-            good[u] = ok[u];
+        for (int u = 0; u < NG; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -503,7 +579,19 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
                         vr[u][i][s][0] = t.x; vr[u][i][s][1] = t.y;
                     }
                 }
-        }
+    };
+    // the tile holds a position that some of the wave's columns see and others
+    // do not: the newest tokens' own, and what a window leaves behind
+    const auto apart = [&](int tb) { return (tb < lo_in && lo < lo_in) || (tb + TP > hi_in && hi_in < hi); };
+    bool spoilt = false;
+
+    for (int j = 0; j < my; ++j) {
+        const int tb = c0 + (j * WS + wo) * TP;
+        bool good[NG];
+        uint32_t vr[NG][4][SEG][VB / 4];
+#pragma unroll
+        for (int u = 0; u < NG; ++u) good[u] = ok[u];
+        load_v(vr);
         if constexpr (KL) {
 #pragma unroll
             for (int u = 0; u < NG; ++u)
@@ -575,6 +663,32 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
 #pragma unroll
                         for (int d = 0; d < VB / 4; ++d) vr[u][i][s][d] = zero ? 0u : vr[u][i][s][d];
                 }
+        }
+
+        // a probability of 0 keeps V out of a column only while V is finite:
+        // what is not (a store past f16's range makes it so) counts as zero
+        // here, and after the loop makes the values NaN that it does reach
+        if (apart(tb)) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int u = 0; u < NG; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int s = 0; s < SEG; ++s)
+#pragma unroll
+                        for (int d = 0; d < VB / 4; ++d) most = P::larger(most, vr[u][i][s][d]);
+            if (__any(P::infinite(most))) {
+                spoilt = true;
+#pragma unroll
+                for (int u = 0; u < NG; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int s = 0; s < SEG; ++s)
+#pragma unroll
+                            for (int d = 0; d < VB / 4; ++d) vr[u][i][s][d] = P::finite(vr[u][i][s][d]);
+            }
         }
 
         // softmax: per column, this lane's positions 16 u + 4 g + i
@@ -650,6 +764,29 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
                 }
             }
     }
+
+    if (spoilt)
+        for (int j = 0; j < my; ++j) {
+            const int tb = c0 + (j * WS + wo) * TP;
+            if (!apart(tb)) continue;
+#pragma unroll
+            for (int u = 0; u < NG; ++u) {
+                const int pos = tb + 16 * u, page = uniform_i(pos < c1 ? table[pos >> a.shift] : -1);
+                ok[u] = page >= 0 && page < a.c.n_pages;
+                off[u] = head_off + (ok[u] ? (int64_t)page * page_bytes + (int64_t)(pos & mask) * pos_bytes : 0);
+            }
+            uint32_t vr[NG][4][SEG][VB / 4];
+            load_v(vr);
+#pragma unroll
+            for (int u = 0; u < NG; ++u)       // the next chunk's, or of no page: columns that see such a page are NaN
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int s = 0; s < SEG; ++s)
+#pragma unroll
+                        for (int d = 0; d < VB / 4; ++d) vr[u][i][s][d] = ok[u] ? vr[u][i][s][d] : 0u;
+            spoil_values<T>(vr, acc, plo, phi, tb + 4 * g);
+        }
 
     const int64_t base = ((int64_t)slot * groups + kh * a.HG + hg) * COLS;
     // the waves meet

@@ -548,6 +548,47 @@ def test_attention_bad_pages_are_nan_and_others_unharmed(new, dtype):
         assert torch.isfinite(got[0]).all()
 
 
+# (heads, lengths, new, window): decode batches, drafts, prompts of one and of two column sets, head_dim 256
+LEAKS = [((8, 2, 128), [300, 64], [40, 9], 0), ((8, 2, 128), [300, 64], [40, 9], 19), ((6, 2, 64), [90, 33], [90, 33], 0),
+         ((16, 4, 256), [120, 50], [50, 7], 30), ((8, 2, 64), [70, 40, 20], [3, 0, 0], 0), ((8, 8, 64), [700], None, 80),
+         ((32, 32, 64), [300, 130, 70], [200, 100, 70], 0), ((64, 32, 128), [150, 33, 260], [150, 33, 90], 37),
+         ((9, 1, 128), [2500, 700], [20, 30], 0)]
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('heads,lengths,new,window', LEAKS)
+def test_attention_values_that_are_not_finite_reach_only_rows_that_see_them(heads, lengths, new, window, dtype):
+    """An infinity or NaN in v: that value of the rows and heads that see it is not finite, every other result keeps
+    its bits, whatever tokens share the row's tile. In k: the rows that see a NaN are NaN."""
+    from localai_amd import paged
+    nh, nkv, hd = heads
+    (q, kc, vc, table, dl), kw, y = _attention(heads, lengths, dtype, new=new, window=window, nan=False, seed=31)
+    pages, group = table.cpu().numpy(), nh // nkv
+    count, at = new or [1] * len(lengths), 0
+    rng = np.random.default_rng(7)
+    for b, (length, n) in enumerate(zip(lengths, count)):
+        first = length - n
+        spots = {length - 1, first, first + n // 2, max(0, first + 1 - (window or length)), max(0, first - 3)}
+        for s in sorted(spots):
+            kh, d, bad = int(rng.integers(nkv)), int(rng.integers(hd)), rng.choice([np.inf, -np.inf, np.nan])
+            place = (int(pages[b, s // 16]), kh, s % 16, d)
+            p = first + np.arange(n)
+            sees = np.zeros(len(q), bool)
+            sees[at:at + n] = (p >= s) & ((p - s < window) if window else True)
+            for cache, value in ((vc, float(bad)), (kc, float('nan'))):
+                kept = cache[place].clone()
+                cache[place] = value
+                got = paged.attention(q, kc, vc, table, dl, **kw).cpu().numpy()
+                cache[place] = kept
+                hit = np.zeros(y.shape, bool)
+                hit[sees, kh * group:(kh + 1) * group, slice(d, d + 1) if cache is vc else slice(None)] = True
+                assert not np.isfinite(got[hit]).any(), (b, s, value)
+                if cache is kc:
+                    assert np.isnan(got[hit]).all(), (b, s)
+                np.testing.assert_array_equal(got[~hit], y[~hit], err_msg=f'request {b} position {s} {value}')
+        at += n
+
+
 def test_attention_over_offsets_past_32_bits():
     """Pages and positions whose byte and value offsets pass 2^32: strides of a large buffer."""
     import torch
