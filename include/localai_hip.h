@@ -359,7 +359,9 @@ int64_t localai_hip_paged_attention_workspace_size(int64_t tokens, int64_t reque
  * What positions that a row does not see hold does not reach it, infinities
  * and NaN included. A v that is infinite or NaN makes that value of the rows
  * that see it NaN or infinite, and no other; a NaN k makes the rows that see it
- * NaN. scale must be finite. tokens below
+ * NaN; so does an infinite one, unless its score is -inf: a probability of 0.
+ * A row that sees positions with no score above -inf is NaN. scale must be
+ * finite. tokens below
  * 2^24, other limits as above; EARG where tokens times heads are too many for
  * one launch (2^24 workgroups).
  * fp32 results: caches of 16 bits are read exactly, queries and probabilities

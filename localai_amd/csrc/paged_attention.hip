@@ -835,25 +835,31 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
             const int cti = col / a.GC, ch = hg * a.GC + col % a.GC;
             const int i = w.r * TB + cset * TW + t * a.tpt + cti, r = w.first + i;
             if (!(cti < a.tpt && ch < a.G && i < w.n && r >= 0 && r < a.p.tokens)) continue;
+            // a token ahead of position 0 sees nothing: zeros, whatever chunks
+            // its block has. Any other has L > 0 unless all its scores are -inf,
+            // and is then NaN, 0 / 0.
+            const bool none = p0 + i < 0, whole = w.chunks == 1 || none;
+            if (none && w.c > 0) continue;
             const int64_t at = ((int64_t)r * a.p.n_heads + kh * a.G + ch) * HD + d0 + dd;
             const int bc = (cset * NT + t) * 16 + col;
-            float *dst = w.chunks > 1 ? a.part + (base + bc) * HD + d0 + dd : a.p.out + at;
-            const float f = w.chunks > 1 ? 1.0f : L == 0.0f ? 0.0f : 1.0f / L;
+            float *dst = whole ? a.p.out + at : a.part + (base + bc) * HD + d0 + dd;
+            const float f = !whole ? 1.0f : none ? 0.0f : 1.0f / L;
 #pragma unroll
             for (int e = 0; e < VT; e += 4) {
                 float4 y = make_float4(o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f);
-                if (w.chunks == 1 && a.p.gate) y = gated(y, a.p.gate + at + e);
+                if (whole && a.p.gate) y = gated(y, a.p.gate + at + e);
                 *reinterpret_cast<float4 *>(dst + e) = y;
             }
             if (d0 == 0 && dd == 0) {
-                if (w.chunks > 1) a.ml[base + bc] = make_float2(M, L);
+                if (!whole) a.ml[base + bc] = make_float2(M, L);
                 if (w.c == 0 && kh == 0 && hg == 0 && col % a.GC == 0)
-                    a.rows[r] = make_int2(w.slot0 << 8 | bc, w.chunks);
+                    a.rows[r] = make_int2(w.slot0 << 8 | bc, whole ? 1 : w.chunks);
             }
         }
 }
 
-// Blocks of several chunks: out = sum_c 2^(c_c - C) o_c / sum_c 2^(c_c - C) l_c.
+// Blocks of several chunks: out = sum_c 2^(c_c - C) o_c / sum_c 2^(c_c - C) l_c
+// (0 / 0, NaN, where all scores are -inf).
 // HD / 4 lanes hold a (row, head)'s values, 4 each. SL such groups share a row
 // and head, take chunks in turn and meet in LDS (few rows of many chunks), or
 // each has its own (SL 1: many rows, of which few have several chunks). Two
@@ -914,7 +920,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) 
     }
     const int64_t at = rh * HD;
     if constexpr (SL == 1) {
-        const float f = L == 0.0f ? 0.0f : 1.0f / L;
+        const float f = 1.0f / L;
         float4 y = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
         if (a.p.gate) y = gated(y, a.p.gate + at + d);
         *reinterpret_cast<float4 *>(a.p.out + at + d) = y;
@@ -937,7 +943,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) 
         ls += f * red_l[i];
         os += f * red_o[i][tid];
     }
-    float y = ls == 0.0f ? 0.0f : os / ls;
+    float y = os / ls;
     if (a.p.gate) y *= 1.0f / (1.0f + expf(-fminf(fmaxf(a.p.gate[at + tid], -80.0f), 80.0f)));
     a.p.out[at + tid] = y;
 }

@@ -589,6 +589,29 @@ def test_attention_values_that_are_not_finite_reach_only_rows_that_see_them(head
         at += n
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('heads,lengths,new', [((8, 2, 64), [1, 40], None), ((8, 2, 64), [2500, 900], None),
+                                               ((8, 8, 64), [600, 2500], [700, 300]), ((4, 2, 64), [290, 700], [300, 2]),
+                                               ((32, 32, 64), [300, 130], [320, 100])])
+def test_attention_rows_whose_scores_are_all_minus_infinity_are_nan(heads, lengths, new, dtype):
+    """Rows that see positions, but every score is -inf, are NaN as the softmax is; rows that see nothing are zeros,
+    whole or joined from chunks."""
+    import torch
+    from localai_amd import paged
+    nh, nkv, hd = heads
+    (q, kc, vc, table, dl), kw, y = _attention(heads, lengths, dtype, new=new, nan=False, seed=4)
+    q = q.clone()
+    q[:, :, 3] = 1.0
+    ids = table[0, :-(-lengths[0] // 16)].long()
+    kc[ids, :, :, 3] = float('-inf')
+    got = paged.attention(q, kc, vc, table, dl, **kw).cpu().numpy()
+    count = new or [1] * len(lengths)
+    none = max(0, count[0] - lengths[0])             # its rows ahead of position 0
+    assert (got[:none] == 0).all()
+    assert np.isnan(got[none:count[0]]).all()
+    assert np.isfinite(got[count[0]:]).all()
+
+
 def test_attention_over_offsets_past_32_bits():
     """Pages and positions whose byte and value offsets pass 2^32: strides of a large buffer."""
     import torch
