@@ -531,8 +531,13 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
                 for (int e = 0; e < 4; ++e) {
                     uint32_t s[P::pieces];
                     P::split(v[t][2 * e], v[t][2 * e + 1], s);
+                    // a second or third piece of 0 becomes the smallest of the
+                    // value's sign (at most 2^-33 of the column's largest in f16,
+                    // 2^-133 in bf16): times an infinite k it is the infinity that
+                    // the first piece gives, not NaN
+                    o[0][e] = s[0];
 #pragma unroll
-                    for (int i = 0; i < P::pieces; ++i) o[i][e] = s[i];
+                    for (int i = 1; i < P::pieces; ++i) o[i][e] = larger16(0x00010001u, s[i]) | (s[0] & 0x80008000u);
                 }
 #pragma unroll
                 for (int i = 0; i < P::pieces; ++i) q[u][t][i] = pa_u4{o[i][0], o[i][1], o[i][2], o[i][3]};

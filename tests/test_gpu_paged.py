@@ -612,6 +612,60 @@ def test_attention_rows_whose_scores_are_all_minus_infinity_are_nan(heads, lengt
     assert np.isfinite(got[count[0]:]).all()
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('heads,lengths,new', [((8, 2, 64), [1, 2, 40, 700], None), ((4, 2, 128), [3, 2500], [2, 1]),
+                                               ((32, 32, 64), [300, 130, 70], [200, 100, 70]),
+                                               ((64, 8, 128), [900, 60], [40, 60]), ((4, 4, 256), [20, 33], [5, 33])])
+def test_attention_infinite_scores(heads, lengths, new, dtype):
+    """An infinite k: a score of -inf has probability 0, one of inf makes the row NaN, and so does a row of nothing
+    but -inf (the softmax's 0 / 0). q's values are small multiples of 1/8: all their low bits are zero. Beside f16, a
+    value of q below 2^-34 of the largest is 0 (2^-24 where the largest is 2^9 to 2^10), and 0 times infinity NaN."""
+    import torch
+    from localai_amd import paged
+    nh, nkv, hd = heads
+    group = nh // nkv
+    (q, kc, vc, table, dl), kw, _ = _attention(heads, lengths, dtype, new=new, nan=False, seed=3)
+    q = torch.round(q * 4) / 8
+    q[:, :, 5] = torch.where(q[:, :, 5] == 0, 0.125, q[:, :, 5])
+    q[:, :, 9] *= 2.0 ** -40             # far below the row's largest
+    pages, count = table.cpu().numpy(), new or [1] * len(lengths)
+    rng = np.random.default_rng(8)
+
+    def place(b, s, kh, d):
+        return int(pages[b, s // 16]), kh, s % 16, d
+
+    planted = {}
+    for b, length in enumerate(lengths):
+        for s in {0, length // 2, length - 1}:
+            for kh in range(nkv):
+                d = int(rng.choice([5, 9]))
+                planted[b, s, kh] = d, float(rng.choice([np.inf, -np.inf]))
+                kc[place(b, s, kh, d)] = planted[b, s, kh][1]
+    got = paged.attention(q, kc, vc, table, dl, **kw).cpu().numpy()
+    qn, at, kinds = q.double().cpu().numpy(), 0, set()
+    if dtype == 'float16':
+        qn[:, :, 9] = 0
+    for b, (length, n) in enumerate(zip(lengths, count)):
+        k, v = (x[table[b, :-(-length // 16)].long()].transpose(1, 2).reshape(-1, nkv, hd)[:length].double().cpu().numpy()
+                for x in (kc, vc))
+        for i in range(n):
+            p = length - n + i
+            for h in range(nh):
+                with np.errstate(invalid='ignore'):
+                    score = k[:p + 1, h // group] @ qn[at + i, h] / np.sqrt(hd)
+                    w = np.exp(score - score.max())
+                y = got[at + i, h]
+                if not np.isfinite(score.max()):
+                    kinds.add(str(score.max()))
+                    assert np.isnan(y).all(), (b, i, h, score.max())
+                    continue
+                kinds.add('finite' if np.isfinite(score).all() else 'some')
+                want = (w / w.sum()) @ v[:p + 1, h // group]
+                assert np.linalg.norm(y - want) <= 1e-5 * np.linalg.norm(want), (b, i, h)
+        at += n
+    assert len(qn) < 40 or {'inf', 'some'} <= kinds      # (a few rows may all be NaN)
+
+
 def test_attention_over_offsets_past_32_bits():
     """Pages and positions whose byte and value offsets pass 2^32: strides of a large buffer."""
     import torch
