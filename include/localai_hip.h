@@ -365,9 +365,14 @@ int64_t localai_hip_paged_attention_workspace_size(int64_t tokens, int64_t reque
  * 2^24, other limits as above; EARG where tokens times heads are too many for
  * one launch (2^24 workgroups).
  * fp32 results: caches of 16 bits are read exactly, queries and probabilities
- * keep at least 21 bits in the products. How a length is split depends on all
- * requests of the call, so a row's last bits can differ between batches; the
- * same call gives the same bits. */
+ * are split into several values of 16 bits. Beside fp16 caches these are two: a
+ * value of q is off by at most 2^-21 of itself or 2^-33 of the largest of its
+ * row and head (one below 2^-34 of that counts as 0), a probability by 2^-21 of
+ * itself or 2^-31 of the row's largest. Beside bf16 caches they are three and
+ * hold all 24 bits. Sums of p v before the division pass what fp32 holds where
+ * 2^8 times the positions times |v| passes 2^128 (never beside fp16 caches).
+ * How a length is split depends on all requests of the call, so a row's last
+ * bits can differ between batches; the same call gives the same bits. */
 int localai_hip_paged_attention(const float *q_dev, int64_t tokens, int n_heads, const localai_paged_cache *cache,
                                 const int32_t *table_dev, int64_t table_stride, int64_t max_pages,
                                 const int32_t *lengths_dev, const int32_t *starts_dev, int64_t requests,

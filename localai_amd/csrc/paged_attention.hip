@@ -28,9 +28,10 @@ namespace lq {
 // values per lane, transposed in registers by byte permutes.
 //
 // Precision: products of 16-bit caches are exact on MFMA, so only q and p are
-// rounded, and both are split: f16 into 2 pieces (22 bits; q scaled by a power
-// of two to [512, 1024), p by 2^7, so that small values keep their bits),
-// bf16 into 3 (24 bits). fp32 caches use fp32 MFMA. Sums, maxima and the
+// rounded, and both are split: f16 into 2 pieces (22 bits while the second is
+// no subnormal; q is scaled by a power of two to [512, 1024) and p by 2^7, so
+// that what is lost below is 2^-33 of the largest |q| and 2^-31 of the largest
+// p), bf16 into 3 (24 bits). fp32 caches use fp32 MFMA. Sums, maxima and the
 // running statistics are fp32.
 //
 // Work: a block is TB tokens of one request, the columns of NT tiles; its
