@@ -308,13 +308,13 @@ __device__ __forceinline__ void spoil_values(const uint32_t (&vr)[NG][4][SEG][W]
         }
 }
 
+// sigmoid of the gate, clipped by comparisons: NaN stays
+__device__ __forceinline__ float gate_of(float g) {
+    return 1.0f / (1.0f + expf(-(g < -80.0f ? -80.0f : g > 80.0f ? 80.0f : g)));
+}
 __device__ __forceinline__ float4 gated(float4 y, const float *gate) {
     const float4 g = *reinterpret_cast<const float4 *>(gate);
-    y.x *= 1.0f / (1.0f + expf(-fminf(fmaxf(g.x, -80.0f), 80.0f)));
-    y.y *= 1.0f / (1.0f + expf(-fminf(fmaxf(g.y, -80.0f), 80.0f)));
-    y.z *= 1.0f / (1.0f + expf(-fminf(fmaxf(g.z, -80.0f), 80.0f)));
-    y.w *= 1.0f / (1.0f + expf(-fminf(fmaxf(g.w, -80.0f), 80.0f)));
-    return y;
+    return make_float4(y.x * gate_of(g.x), y.y * gate_of(g.y), y.z * gate_of(g.z), y.w * gate_of(g.w));
 }
 
 // which 16-byte piece of row r of K holds piece 0, times 16 (rows of RB bytes, r < 16)
@@ -853,7 +853,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
 #pragma unroll
             for (int e = 0; e < VT; e += 4) {
                 float4 y = make_float4(o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f);
-                if (whole && a.p.gate) y = gated(y, a.p.gate + at + e);
+                if (whole && !none && a.p.gate) y = gated(y, a.p.gate + at + e);
                 *reinterpret_cast<float4 *>(dst + e) = y;
             }
             if (d0 == 0 && dd == 0) {
@@ -950,7 +950,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) 
         os += f * red_o[i][tid];
     }
     float y = os / ls;
-    if (a.p.gate) y *= 1.0f / (1.0f + expf(-fminf(fmaxf(a.p.gate[at + tid], -80.0f), 80.0f)));
+    if (a.p.gate) y *= gate_of(a.p.gate[at + tid]);
     a.p.out[at + tid] = y;
 }
 

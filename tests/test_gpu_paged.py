@@ -666,6 +666,24 @@ def test_attention_infinite_scores(heads, lengths, new, dtype):
     assert len(qn) < 40 or {'inf', 'some'} <= kinds      # (a few rows may all be NaN)
 
 
+def test_attention_gate_that_is_not_a_number():
+    """The gate's clip keeps NaN; infinities are its ends."""
+    import torch
+    from localai_amd import paged
+    for lengths in ([30, 2500], [30, 40]):
+        (q, kc, vc, table, dl), kw, y = _attention((8, 2, 64), lengths, 'float16', gate=True, seed=2)
+        gate = kw['gate'].clone()
+        gate[0, 3, 7] = gate[1, 5, 60] = float('nan')
+        gate[0, 0, 0], gate[1, 0, 0] = float('inf'), float('-inf')
+        got = paged.attention(q, kc, vc, table, dl, gate=gate).cpu().numpy()
+        assert np.isnan(got[0, 3, 7]) and np.isnan(got[1, 5, 60])
+        assert np.isnan(got).sum() == 2
+        assert got[0, 0, 0] != 0 and abs(got[1, 0, 0]) <= abs(y[1, 0]).max() * 1e3 * np.exp(-80.0)
+    (q, kc, vc, table, dl), kw, y = _attention((8, 2, 64), [30, 0], 'float16', gate=True, seed=2)
+    got = paged.attention(q, kc, vc, table, dl, gate=torch.full_like(q, float('nan')))
+    assert torch.isnan(got[0]).all() and (got[1] == 0).all()           # a row that sees nothing is zeros
+
+
 def test_attention_over_offsets_past_32_bits():
     """Pages and positions whose byte and value offsets pass 2^32: strides of a large buffer."""
     import torch
