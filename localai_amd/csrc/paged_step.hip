@@ -392,7 +392,8 @@ __global__ __launch_bounds__(256) void norm_rope_store_kernel(StoreArgs a) {
                     o = row_of(r)[pd] * inv * weight[is_q ? 0 : 1][pd];
                 }
                 const float s = v[e] * inv * w4[e];
-                y[i][e] = plain ? v[e] : s * cs[e] + o * sn[e];
+                // (behind the rotated values s itself: 0 times a partner that is not finite is NaN)
+                y[i][e] = plain ? v[e] : d0 + e < 2 * a.n ? s * cs[e] + o * sn[e] : s;
             }
         }
         // (in place: a row is read and written by one wave, and read first)

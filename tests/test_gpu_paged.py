@@ -268,6 +268,36 @@ def test_norm_rope_store_at_far_positions(far):
     _store(9, (8, 2, 128), 'float32', 16, 'pairs', 64, True, far=far, seed=9)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rope,n', [('halves', 0), ('halves', 12), ('halves', 10), ('pairs', 12), ('pairs', 7),
+                                    ('pairs', 0)])
+def test_store_leaves_values_that_are_not_rotated_as_they_are(rope, n, dtype):
+    """Infinities, NaN and negative zeros behind the rotated values stay, and stay where they are."""
+    import torch
+    from localai_amd import paged
+    hd, nh, nkv, tokens = 64, 4, 2, 5
+    gen = torch.Generator('cuda').manual_seed(n)
+    q, k, v = (torch.randn((tokens, h, hd), generator=gen, device='cuda') for h in (nh, nkv, nkv))
+    freq = torch.from_numpy(100.0 ** (-np.arange(n) / max(n, 1))).cuda() if n else None
+    tt = getattr(torch, dtype)
+
+    def run(q, k):
+        kc, vc = (torch.zeros((1, nkv, 16, hd), dtype=tt, device='cuda') for _ in range(2))
+        y = paged.norm_rope_store(q, k, v, _ints(range(3, 3 + tokens)), _ints(range(tokens)), kc, vc, freq, rope=rope)
+        return y, kc[0, :, :tokens].transpose(0, 1)
+
+    clean = run(q, k)
+    for x in (q, k):
+        x[:, 0, 2 * n + 1], x[:, 1, 2 * n + 2], x[:, 1, hd - 1] = float('inf'), float('-inf'), float('nan')
+        x[:, 0, 2 * n + 6] = -0.0
+    for got, was, x in zip(run(q, k), clean, (q, k)):
+        assert torch.equal(got[..., :2 * n], was[..., :2 * n])
+        want = x[..., 2 * n:].to(got.dtype)
+        assert torch.equal(got[..., 2 * n:].isnan(), want.isnan())
+        assert torch.equal(got[..., 2 * n:].nan_to_num(7.0), want.nan_to_num(7.0))
+        assert torch.equal(torch.signbit(got[..., 2 * n:])[~want.isnan()], torch.signbit(want)[~want.isnan()])
+
+
 def test_store_rounds_as_the_type_does():
     """Values past fp16's range become infinite; zero rows keep the norm finite."""
     import torch
