@@ -328,10 +328,11 @@ int localai_hip_paged_shrink(int32_t *lengths_dev, const int32_t *keep_dev, int6
  * q [tokens, n_heads, head_dim], k, v [tokens, n_kv_heads, head_dim] fp32 with
  * strides[0..7] = token and head stride of q, k, v, q_out in values (host
  * array; multiples of 4; views of one fused projection will do). q_out may be
- * q with q's strides; tokens below 2^24. A token whose slot is outside [0, n_pages * page_size)
- * is padding: nothing is stored and its row of q_out stays as it was. Slots of
- * one call must differ from each other. All 16-byte aligned but the index and
- * weight arrays. */
+ * q with q's strides and shares memory with no other buffer; its rows may not
+ * overlap (EARG), nor may the cache's. tokens below 2^24. A token whose slot is
+ * outside [0, n_pages * page_size) is padding: nothing is stored and its row of
+ * q_out stays as it was. Slots of one call must differ from each other. All
+ * 16-byte aligned but the index and weight arrays. */
 int localai_hip_norm_rope_store(const float *q_dev, const float *k_dev, const float *v_dev, const int64_t *strides,
                                 int64_t tokens, int n_heads, const int32_t *positions_dev, const int32_t *slots_dev,
                                 const double *freq_dev, int n_freq, int halves, const float *q_w_dev,

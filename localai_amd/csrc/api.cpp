@@ -674,6 +674,20 @@ int localai_hip_paged_shrink(int32_t *lengths, const int32_t *keep, int64_t requ
                                (int)n_pages, used, page_size, status, (hipStream_t)stream);
 }
 
+// whether two of a [tokens, heads] set of rows of hd values share memory
+static bool rows_overlap(int64_t tokens, int64_t heads, int64_t ts, int64_t hs, int64_t hd) {
+    typedef __int128 wide;
+    if ((tokens > 1 && ts < hd) || (heads > 1 && hs < hd)) return true;
+    if (tokens == 1 || heads == 1) return false;
+    if (ts >= (wide)(heads - 1) * hs + hd || hs >= (wide)(tokens - 1) * ts + hd) return false;
+    // neither lies within one step of the other: the tokens just before and after h heads' distance
+    for (int64_t h = 1; h < heads; ++h) {
+        const wide x = (wide)h * hs, before = x / ts, left = x % ts;
+        if ((before < tokens && left < hd) || (before + 1 < tokens && ts - left < hd)) return true;
+    }
+    return false;
+}
+
 int localai_hip_norm_rope_store(const float *q, const float *k, const float *v, const int64_t *strides,
                                 int64_t tokens, int n_heads, const int32_t *positions, const int32_t *slots,
                                 const double *freq, int n_freq, int halves, const float *q_w, const float *k_w,
@@ -693,6 +707,8 @@ int localai_hip_norm_rope_store(const float *q, const float *k, const float *v, 
     for (int i = 0; i < 8; ++i)
         if (strides[i] % 4 || strides[i] < 0)
             return fail(LOCALAI_EARG, "norm rope store: strides must be multiples of 4 values");
+    if (rows_overlap(tokens, n_heads, strides[6], strides[7], cache->head_dim))
+        return fail(LOCALAI_EARG, "norm rope store: rows of q_out overlap");
     const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
                           reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(q_out);
     if (all & 15) return fail(LOCALAI_EARG, "norm rope store: q, k, v and q_out must be 16-byte aligned");

@@ -261,8 +261,9 @@ def norm_rope_store(q, k, v, positions, slots, k_cache, v_cache, freq=None, q_we
     size, head_dim] of one layer. freq: fp64 radians per position and rotated
     pair, or None; rope: 'halves' (j, j + n) or 'pairs' (2j, 2j + 1).
     q_weight, k_weight [head_dim]: the norms' weights, None for no norm.
-    Returns q [tokens, heads, head_dim], in `out` if given (may be q); rows of
-    padding are left as they were."""
+    Returns q [tokens, heads, head_dim], in `out` if given (q itself, or rows
+    that share no memory with each other or the rest); rows of padding are left
+    as they were."""
     cache, nkv, hd = _cache(k_cache, v_cache)
     r = _r()
     f32 = r.f32

@@ -298,6 +298,16 @@ def test_store_leaves_values_that_are_not_rotated_as_they_are(rope, n, dtype):
         assert torch.equal(torch.signbit(got[..., 2 * n:])[~want.isnan()], torch.signbit(want)[~want.isnan()])
 
 
+def test_store_refuses_outputs_that_overlap():
+    import torch
+    from localai_amd import _lib, paged
+    q, k = torch.zeros((2, 4, 64), device='cuda'), torch.zeros((2, 2, 64), device='cuda')
+    kc, vc = (torch.zeros((1, 2, 16, 64), device='cuda') for _ in range(2))
+    for out in (q[:1].expand(2, -1, -1), q[:, :1].expand(-1, 4, -1), torch.zeros(600, device='cuda').as_strided((2, 4, 64), (192, 64, 1))):
+        with pytest.raises(_lib.HipError, match='overlap'):
+            paged.norm_rope_store(q, k, k, _ints([0, 1]), _ints([0, 1]), kc, vc, out=out)
+
+
 def test_store_rounds_as_the_type_does():
     """Values past fp16's range become infinite; zero rows keep the norm finite."""
     import torch

@@ -119,6 +119,26 @@ def test_store_arguments_are_refused():
     assert call(tokens=0) == 0
 
 
+@pytest.mark.parametrize('tokens,heads,ts,hs,overlap', [
+    (2, 4, 512, 128, False), (2, 4, 128, 256, False), (1, 4, 0, 128, False), (3, 1, 128, 0, False), (1, 1, 0, 0, False),
+    (2, 4, 512, 512, True), (2, 4, 0, 128, True), (2, 4, 512, 0, True), (2, 4, 384, 128, True), (5, 4, 128, 512, True),
+    (4, 3, 384, 512, False), (5, 4, 384, 512, True), (5, 4, 384, 516, True), (2, 4, 64, 1024, True),
+    (1 << 20, 65536, 128, 1 << 27, False), (1 << 20, 65536, 128, (1 << 27) - 128, True)])
+def test_store_outputs_that_overlap_are_refused(tokens, heads, ts, hs, overlap):
+    """Every row writes its own memory: rows that share some would be written by two workgroups."""
+    import itertools
+    hd, lib = 128, _lib.load()
+    if tokens * heads < 100:
+        taken = [t * ts + h * hs for t, h in itertools.product(range(tokens), range(heads))]
+        assert overlap == any(abs(a - b) < hd for i, a in enumerate(taken) for b in taken[:i])
+    strides = (ctypes.c_int64 * 8)(512, 128, 512, 128, 512, 128, ts, hs)
+    c = cache_arg(n_kv_heads=1)
+    status = lib.localai_hip_norm_rope_store(ONE, ONE, ONE, strides, tokens, heads, ONE, ONE, None, 0, 0, None, None,
+                                             1e-6, ctypes.c_void_p(20), ctypes.byref(c), None)     # q_out: misaligned
+    assert status == 1
+    assert (b'overlap' in lib.localai_hip_last_error()) == overlap
+
+
 def test_table_arguments_are_refused():
     lib = _lib.load()
 
