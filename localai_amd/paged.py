@@ -22,7 +22,10 @@ The reference serves one request from one contiguous cache
 attention.attention_decode is that form. Arguments are device tensors, the
 work runs in the HIP library, and nothing is read back by the host but by
 check(). Every call may be captured in a graph; workspaces come from PyTorch's
-allocator call by call, so graphs and streams share none.
+allocator call by call, so graphs and streams share none. A call with `stream`
+runs there, allocates there, and holds the memory of its arguments (a Step made
+on another stream among them) until that stream has passed it; the streams' own
+order is the caller's.
 """
 from __future__ import annotations
 
@@ -136,6 +139,13 @@ def _on(stream):
     return contextlib.nullcontext() if stream is None else device.torch().cuda.stream(stream)
 
 
+def _hold(stream, *tensors):
+    """Memory of tensors freed before `stream` has passed this point is not given out again until it has."""
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
+
+
 def _empty(stream, shape, dtype):
     r = _run
     if stream is None:
@@ -200,6 +210,8 @@ def extend(lengths, new, table, free, used, page_size, tokens, out=None, stream=
     status = r.extend(*args, *ptrs, _stream(stream))
     if status:
         _lib.check(status)
+    if stream is not None:
+        _hold(stream, lengths, new, table, free, used, *out)
     return out
 
 
@@ -216,6 +228,8 @@ def shrink(lengths, keep, table, free, used, page_size, stream=None):
             _ptr(free, 'free', i32), free.numel(), _ptr(used, 'used', i32, (1,)), int(page_size))
     status = _empty(stream, 1, i32)
     _lib.check(r.shrink(*args, status.data_ptr(), _stream(stream)))
+    if stream is not None:
+        _hold(stream, lengths, keep, table, free, used)
     return status
 
 
@@ -289,6 +303,8 @@ def norm_rope_store(q, k, v, positions, slots, k_cache, v_cache, freq=None, q_we
                      eps, op, cache, _stream(stream))
     if status:
         _lib.check(status)
+    if stream is not None:
+        _hold(stream, q, k, v, positions, slots, k_cache, v_cache, freq, q_weight, k_weight, out)
     return out
 
 
@@ -327,6 +343,8 @@ def attention(q, k_cache, v_cache, table, lengths, starts=None, window=0, scale=
                          need if need > 0 else 0, _stream(stream))
     if status:
         _lib.check(status)
+    if stream is not None:
+        _hold(stream, q, k_cache, v_cache, table, lengths, starts, gate, out)
     return out
 
 

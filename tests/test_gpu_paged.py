@@ -782,6 +782,45 @@ def test_attention_calls_at_once_on_two_streams():
             np.testing.assert_array_equal(x.cpu().numpy(), y)
 
 
+def test_calls_on_another_stream_hold_their_arguments():
+    """A Step and inputs dropped while the other stream still waits: their memory is given out only after it."""
+    import torch
+    from localai_amd import paged
+    nh, nkv, hd = 8, 2, 64
+    gen = torch.Generator('cuda').manual_seed(3)
+    data = [torch.randn((40, h, hd), generator=gen, device='cuda') for h in (nh, nkv, nkv)]
+    freq, w = torch.rand(hd // 2, generator=gen, device='cuda', dtype=torch.float64), torch.ones(hd, device='cuda')
+    new, keep = _ints([30, 8]), [25, 0]
+    side = torch.cuda.Stream()
+
+    def run(stream):
+        cache = paged.PagedKVCache(1, nkv, hd, n_pages=8, page_size=16, requests=2, dtype=torch.float16)
+        q, k, v = (x.clone() for x in data)
+        step = cache.extend(new.clone(), 40)
+        if stream is not None:
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                torch.cuda._sleep(20_000_000)        # some 10 ms
+        q = cache.store(0, q, k, v, step, freq.clone(), w.clone(), w.clone(), stream=stream)
+        y = cache.attention(0, q, step, gate=data[0].clone(), stream=stream)
+        status = cache.shrink(_ints(keep), stream=stream)
+        more = paged.extend(cache.lengths, _ints([3, 4]), cache.table, cache.free, cache.used, 16, 7, stream=stream)
+        return cache, y, status, more
+
+    def results(cache, y, status, more):
+        return [x.cpu() for x in (cache.k, cache.v, cache.table, cache.lengths, cache.free, cache.used, y[:38], status, *more)]
+
+    want = results(*run(None))
+    torch.cuda.synchronize()
+    made = run(side)
+    held = [torch.full((n,), 2 ** 30, dtype=torch.int32, device='cuda') for n in
+            [2, 3, 8, 40, 83, 127, 128, 64, 40 * nh * hd, 40 * nkv * hd] for _ in range(8)]
+    torch.cuda.synchronize()
+    for a, b in zip(results(*made), want):
+        assert torch.equal(a, b)
+    del held
+
+
 def test_refusals():
     import torch
     from localai_amd import _lib, paged
