@@ -54,12 +54,13 @@ struct PagedArgs {
     PagedCache c;
     int G, GC, HG, tpt;  // query heads per kv head, per column group; groups; tokens per column tile
     int shift, slots;    // workgroups per kv head and column group
+    int extra, records;  // chunks past one a block, at most; chunks of cut blocks
     int least;           // shortest chunk
     float q_sign;        // sign of scale (0 for 0)
     float scale2;        // |scale| * log2(e) (1 for 0)
-    float *part;         // [slots, n_kv, HG, columns of a block, HD] unscaled outputs of a chunk
-    float2 *ml;          // [slots, n_kv, HG, columns] their c and l
-    int2 *rows;          // [tokens]: first slot << 8 | first column of the token's block, chunks
+    float *part;         // [records, n_kv, HG, columns of a block, HD] unscaled outputs of a cut block's chunk
+    float2 *ml;          // [records, n_kv, HG, columns] their c and l
+    int2 *rows;          // [tokens]: first record << 8 | first column of the token's block, chunks
 };
 
 typedef _Float16 pa_h8 __attribute__((ext_vector_type(8)));
@@ -110,7 +111,7 @@ __device__ __forceinline__ int uniform_i(int v) { return __builtin_amdgcn_readfi
 struct PagedWork {
     int b, first, n;      // request, its first row, its new tokens
     int length, r;        // its positions, block of its tokens
-    int c, chunks, slot0; // chunk, chunks of the block, the block's first slot
+    int c, chunks, rec0;  // chunk, chunks of the block, its first record if they are several
 };
 
 // The request's tokens, positions that its first token's window leaves, and blocks
@@ -152,25 +153,28 @@ __device__ __forceinline__ bool paged_work(const PagedArgs &a, int slot, int TB,
     }
     work = wave_total(work);
     count = wave_total(count);
-    // sum of blocks * ceil(span / C) <= work / C + count <= slots (1.001: the roundings of these sums)
-    const float room = fmaxf((float)a.slots - count, 1.0f);
+    // sum of blocks * (ceil(span / C) - 1) <= work / C <= room (1.001: the roundings of these sums), so
+    // that all fit the slots, and cut blocks, of at least two chunks each, 2 extra records
+    const float room = fmaxf(fminf((float)a.slots - count, (float)a.extra), 1.0f);
     const int fit = (int)((uint32_t)fminf(work * 1.001f * __builtin_amdgcn_rcpf(room), 2.0e9f) / unit + 1) * unit;
     const int C = fit > a.least ? fit : a.least;
-    int mine = 0;
+    int mine = 0, cut = 0;
     for (int b = b0; b < b1; ++b) {
         if (per > 1) paged_request(a, b, TB, &first, &n, &length, &span, &blocks);
-        mine += blocks * chunks_of(span, C);
+        const int ch = chunks_of(span, C);
+        mine += blocks * ch;
+        cut += ch > 1 ? blocks * ch : 0;
     }
-    const int upto = wave_scan(mine);
+    const int upto = wave_scan(mine), upto_cut = wave_scan(cut);
     const uint64_t has = __ballot(upto > slot);
     if (!has) return false;
     const int owner = __builtin_ctzll(has);
-    int at = __builtin_amdgcn_readlane(upto - mine, owner);
+    int at = __builtin_amdgcn_readlane(upto - mine, owner), rec = __builtin_amdgcn_readlane(upto_cut - cut, owner);
     if (per == 1) {      // the owner holds its only request
         const int uc = __builtin_amdgcn_readlane(chunks_of(span, C), owner);
         const uint32_t local = slot - at, r = uc == 1 ? local : local / (uint32_t)uc, c = local - r * uc;
         *w = PagedWork{owner, __builtin_amdgcn_readlane(first, owner), __builtin_amdgcn_readlane(n, owner),
-                       __builtin_amdgcn_readlane(length, owner), (int)r, (int)c, uc, slot - (int)c};
+                       __builtin_amdgcn_readlane(length, owner), (int)r, (int)c, uc, rec + (int)(local - c)};
         return true;
     }
     int b = owner * per;
@@ -179,10 +183,11 @@ __device__ __forceinline__ bool paged_work(const PagedArgs &a, int slot, int TB,
         paged_request(a, b, TB, &first, &n, &length, &span, &blocks);
         const int ch = chunks_of(span, C), local = slot - at;
         if (local < blocks * ch || b >= last) {
-            *w = PagedWork{b, first, n, length, local / ch, local % ch, ch, slot - local % ch};
+            *w = PagedWork{b, first, n, length, local / ch, local % ch, ch, rec + local - local % ch};
             return local < blocks * ch;
         }
         at += blocks * ch;
+        rec += ch > 1 ? blocks * ch : 0;
         ++b;
     }
 }
@@ -378,7 +383,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
         const int all = (int)((uint32_t)(w.n + TB - 1) / (uint32_t)TB), half = (all + 1) / 2;
         if (w.r >= half) w.r = all - 1 - (w.r - half);
     }
-    w.r = uniform_i(w.r); w.c = uniform_i(w.c); w.chunks = uniform_i(w.chunks); w.slot0 = uniform_i(w.slot0);
+    w.r = uniform_i(w.r); w.c = uniform_i(w.c); w.chunks = uniform_i(w.chunks); w.rec0 = uniform_i(w.rec0);
 
     // the block's positions: from its first token's window to its last token,
     // and of these the chunk's
@@ -794,7 +799,9 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
             spoil_values<T>(vr, acc, plo, phi, tb + 4 * g);
         }
 
-    const int64_t base = ((int64_t)slot * groups + kh * a.HG + hg) * COLS;
+    // (never so for starts that do not decrease and end within the tokens)
+    if (w.chunks > 1 && (w.rec0 < 0 || w.rec0 > a.records - w.chunks)) return;
+    const int64_t base = ((int64_t)(w.rec0 + w.c) * groups + kh * a.HG + hg) * COLS;
     // the waves meet
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -859,7 +866,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
             if (d0 == 0 && dd == 0) {
                 if (!whole) a.ml[base + bc] = make_float2(M, L);
                 if (w.c == 0 && kh == 0 && hg == 0 && col % a.GC == 0)
-                    a.rows[r] = make_int2(w.slot0 << 8 | bc, whole ? 1 : w.chunks);
+                    a.rows[r] = make_int2(w.rec0 << 8 | bc, whole ? 1 : w.chunks);
             }
         }
 }
@@ -883,12 +890,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a, int cols) 
     const int h = (int)(rh % a.p.n_heads);
     const int2 info = a.rows[t];     // means nothing outside the requests' rows
     if (a.p.starts && (t < a.p.starts[0] || t >= a.p.starts[a.p.requests])) return;
-    const int slot0 = info.x >> 8, chunks = info.y;
+    const int rec0 = info.x >> 8, chunks = info.y;
     const int kh = h / a.G, hr = h % a.G, groups = a.p.n_kv * a.HG;
     const int col = (info.x & 255) + hr % a.GC;
     // (the last three hold for every row that starts gives to a request)
-    if (chunks <= 1 || slot0 < 0 || slot0 > a.slots - chunks || col >= cols) return;
-    const int64_t first = ((int64_t)slot0 * groups + kh * a.HG + hr / a.GC) * cols + col;
+    if (chunks <= 1 || rec0 < 0 || rec0 > a.records - chunks || col >= cols) return;
+    const int64_t first = ((int64_t)rec0 * groups + kh * a.HG + hr / a.GC) * cols + col;
     const int64_t step = (int64_t)groups * cols;
     float M = -INFINITY, L = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -958,7 +965,7 @@ constexpr int PAGED_ROUND = 512;   // workgroups on the card at once, two a CU (
 
 // How a call is laid out, from its host-known sizes alone
 struct PagedPlan {
-    int G, GC, HG, tpt, NT, WS, slots, cols;
+    int G, GC, HG, tpt, NT, WS, slots, extra, records, cols;
     int64_t blocks, part, ml, rows, bytes;
 };
 
@@ -993,11 +1000,16 @@ static PagedPlan paged_plan(int64_t tokens, int requests, int n_heads, int n_kv,
     const int64_t blocks = blocks_of(p.WS);
     const int64_t round = (hd == 256 ? PAGED_ROUND / 2 : PAGED_ROUND) / per, most = hd == 256 ? round : 4 * round;
     const int64_t want = p.WS == 2 ? 256 / per : 4 * blocks < round ? round : 4 * blocks < most ? 4 * blocks : most;
-    const int64_t slots = (want > 1 ? want : 1) + blocks;
+    const int64_t extra = want > 1 ? want : 1, slots = extra + blocks, records = 2 * extra < slots ? 2 * extra : slots;
     p.slots = (int)slots;
+    p.extra = (int)extra;
+    p.records = (int)records;
     p.blocks = blocks;
     auto up = [](int64_t b) { return (b + 255) & ~(int64_t)255; };
-    const int64_t recs = slots * n_kv * p.HG * p.cols;
+    // partial results only for chunks of cut blocks: a prompt of 131072 tokens
+    // of 32 heads of 128, whose blocks are hardly ever cut, takes 18 MB, and
+    // 2.2 GB with a record for every slot
+    const int64_t recs = records * n_kv * p.HG * p.cols;
     p.part = 0;
     p.ml = up(recs * hd * 4);
     p.rows = p.ml + up(recs * 8);
@@ -1047,7 +1059,7 @@ int launch_paged_attention(const PagedQueries &p, const PagedCache &cache, void 
     int least = l.WS == 2 ? 1024 : full ? (f32 ? 256 : 1024) : (f32 ? 128 : 256);
     const bool whole = limit <= least || limit <= few;
     if (whole) least = limit;
-    const PagedArgs a{p, cache, l.G, l.GC, l.HG, l.tpt, page_shift(cache.page_size), l.slots, least,
+    const PagedArgs a{p, cache, l.G, l.GC, l.HG, l.tpt, page_shift(cache.page_size), l.slots, l.extra, l.records, least,
                       p.scale < 0 ? -1.0f : p.scale == 0 ? 0.0f : 1.0f,
                       p.scale == 0 ? 1.0f : (float)(std::fabs((double)p.scale) * 1.4426950408889634), (float *)(w + l.part), (float2 *)(w + l.ml),
                       (int2 *)(w + l.rows)};

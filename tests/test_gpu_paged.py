@@ -161,6 +161,27 @@ def test_shrink(n):
         assert int(d['used']) == oracle.used
 
 
+@pytest.mark.parametrize('n', [1, 5, 64, 1500])
+def test_shrink_says_that_it_was_done(n):
+    """Status 0 of drafts taken back and of a second cut, from a buffer that held something else."""
+    import torch
+    from localai_amd import paged
+    rng = np.random.default_rng(n + 1)
+    oracle, d = _tables(rng, rng.integers(0, 700, n).tolist(), 16, 60, 40 * n)
+    kept = list(oracle.lengths)
+    new = rng.integers(0, 90, n).tolist()
+    _extend_both(oracle, d, new, sum(new), 16, in_place=True)
+    for keep in (kept, rng.integers(0, 800, n).tolist(), [0] * n):
+        torch.full((1,), 77, dtype=torch.int32, device='cuda')
+        status = paged.shrink(d['lengths'], _ints(keep), d['table'], d['free'], d['used'], 16)
+        oracle.shrink(keep)
+        assert int(status) == 0
+        paged.check(status)
+        np.testing.assert_array_equal(d['lengths'].cpu(), oracle.lengths)
+        np.testing.assert_array_equal(d['free'].cpu(), oracle.free)
+    assert int(d['used']) == 0 and (d['table'] == -1).all()
+
+
 @pytest.mark.parametrize('fault,want', [('keep', 2), ('length', 2), ('used', 1), ('pool', 2)])
 def test_shrink_that_cannot_be_changes_nothing(fault, want):
     import torch
@@ -434,6 +455,40 @@ def test_attention_many_requests_of_several_chunks(n, dtype):
     _attention((2, 1, 64), lengths, dtype, seed=n)
     new = [min(x, y) for x, y in zip(lengths, rng.integers(0, 4, n).tolist())]
     _attention((4, 2, 64), lengths, dtype, new=new, seed=n + 1, window=900)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('n', [12, 64, 300])
+def test_attention_few_of_many_places(n, dtype):
+    """A batch whose places are mostly empty, of a few requests cut into many chunks, first, last and between."""
+    lengths = [0] * n
+    for b, x in ((0, 9000), (n // 3, 40), (n // 2, 3001), (n - 1, 6000)):
+        lengths[b] = x
+    _attention((8, 8, 64), lengths, dtype, page=64, seed=n)
+    _attention((4, 2, 128), lengths, dtype, page=64, new=[min(x, 2) for x in lengths], seed=n + 1)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('heads,tokens', [((2, 1, 64), 40), ((16, 16, 64), 40), ((8, 2, 128), 90)])
+def test_attention_many_requests_of_several_blocks(heads, tokens, dtype):
+    """More requests than a wave has lanes, several blocks of tokens each, some cut: with one and two column sets."""
+    rng = np.random.default_rng(tokens)
+    lengths = np.exp(rng.uniform(0, np.log(160), 70)).astype(int).tolist()
+    for b, x in ((2, 3000), (3, 2100), (69, 4000)):
+        lengths[b] = x
+    lengths[5] = lengths[68] = 0
+    new = [min(x, int(y)) for x, y in zip(lengths, rng.integers(1, tokens, 70))]
+    new[2] = new[69] = tokens
+    new[9] = 0
+    _attention(heads, lengths, dtype, page=32, new=new, seed=1, behind=2)
+    _attention(heads, lengths, dtype, page=32, new=new, seed=2, window=1500)
+
+
+@pytest.mark.parametrize('window', [0, 700])
+@pytest.mark.parametrize('heads', [(8, 8, 64), (32, 32, 64)])
+def test_attention_with_many_rows_of_padding(heads, window):
+    """Rows behind the last request count for the layout, not for the chunks."""
+    _attention(heads, [2500, 60, 1200], 'float16', new=[60, 60, 40], behind=2000, window=window, seed=3)
 
 
 @pytest.mark.parametrize('dtype', TYPES)

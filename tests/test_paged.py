@@ -102,6 +102,16 @@ def test_attention_arguments_are_refused():
     assert size(-1, 1, 4, 2, 128) == size(1, 0, 4, 2, 128) == size(1, 1, 4, 3, 128) == size(1, 1, 4, 2, 96) == -1
 
 
+@pytest.mark.parametrize('tokens,requests,heads,kv_heads,head_dim', [
+    (8192, 1, 32, 8, 128), (131072, 1, 32, 8, 128), (131072, 64, 64, 8, 128), (1 << 20, 4096, 16, 4, 256),
+    (4096, 4096, 32, 8, 128), (8192, 4096, 8, 8, 64), (1, 1, 32, 8, 128), (3, 2, 8, 2, 64)])
+def test_attention_workspace_holds_cut_blocks_only(tokens, requests, heads, kv_heads, head_dim):
+    """8 bytes a token, and partial results of at most twice the chunks that a call may cut (four rounds of two
+    workgroups for each of 256 CUs) of 32 columns: not of every block of a prompt."""
+    size = _lib.load().localai_hip_paged_attention_workspace_size(tokens, requests, heads, kv_heads, head_dim)
+    assert 0 < size <= 8 * tokens + 2 * 4 * 512 * 32 * (head_dim * 4 + 8) + 3 * 256
+
+
 def test_store_arguments_are_refused():
     lib, c = _lib.load(), cache_arg()
 
