@@ -754,7 +754,7 @@ int localai_hip_paged_attention(const float *q, int64_t tokens, int n_heads, con
     if (int st = ensure_device()) return st;
     const PagedQueries p{q, gate, out, tokens, n_heads, cache->n_kv_heads, cache->head_dim, (int)requests,
                          table, lengths, starts, table_stride, (int)max_pages, window, scale};
-    return launch_paged_attention(p, c, ws, ws_bytes, (hipStream_t)stream);
+    return launch_paged_attention(p, c, ws, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -49,6 +49,6 @@ struct PagedQueries {
     float scale;
 };
 size_t paged_attention_workspace_bytes(int64_t tokens, int requests, int n_heads, int n_kv, int hd);
-int launch_paged_attention(const PagedQueries &p, const PagedCache &cache, void *ws, int64_t ws_bytes, hipStream_t s);
+int launch_paged_attention(const PagedQueries &p, const PagedCache &cache, void *ws, hipStream_t s);
 
 }  // namespace lq

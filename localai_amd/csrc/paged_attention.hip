@@ -1023,11 +1023,11 @@ size_t paged_attention_workspace_bytes(int64_t tokens, int requests, int n_heads
 
 template <typename T, int HD>
 static void paged_launch(const PagedArgs &a, const PagedPlan &p, hipStream_t s) {
-    constexpr int N2 = HD == 256 ? 1 : 2;
+    constexpr int N2 = HD == 256 ? 1 : 2;       // as paged_plan chooses
     const dim3 grid((unsigned)((int64_t)p.slots * a.p.n_kv), (unsigned)p.HG);
     if (p.WS == 2) hipLaunchKernelGGL((paged_attention_kernel<T, HD, N2, 2>), grid, dim3(256), 0, s, a);
     else if (p.NT == 1) hipLaunchKernelGGL((paged_attention_kernel<T, HD, 1, 4>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((paged_attention_kernel<T, HD, N2, 4>), grid, dim3(256), 0, s, a);
+    else if constexpr (N2 == 2) hipLaunchKernelGGL((paged_attention_kernel<T, HD, 2, 4>), grid, dim3(256), 0, s, a);
 }
 
 template <int HD>
@@ -1038,7 +1038,7 @@ static void paged_join_launch(const PagedArgs &a, const PagedPlan &p, hipStream_
     else hipLaunchKernelGGL((paged_join_kernel<HD, 1>), dim3((unsigned)((rh + GP - 1) / GP)), dim3(256), 0, s, a, p.cols);
 }
 
-int launch_paged_attention(const PagedQueries &p, const PagedCache &cache, void *ws, int64_t, hipStream_t s) {
+int launch_paged_attention(const PagedQueries &p, const PagedCache &cache, void *ws, hipStream_t s) {
     const PagedPlan l = paged_plan(p.tokens, p.requests, p.n_heads, p.n_kv, p.hd);
     // a launch has fewer than 2^24 workgroups of 256
     if ((int64_t)l.slots * p.n_kv * l.HG >= 1 << 24 || l.slots >= 1 << 23 ||

@@ -36,9 +36,6 @@ import struct
 
 from . import _lib, device
 
-# torch dtype name -> the cache's GGML type number
-_TYPES = {'torch.float32': 0, 'torch.float16': 1, 'torch.bfloat16': 30}
-
 _STATUS = ((1, 'the pool has too few pages left'),
            (2, 'a length or count is negative, or a request is longer than its page table'),
            (4, 'more new tokens than the step has places for'))
@@ -56,7 +53,7 @@ class _Run:
         t = device.torch()
         self.Tensor, self.empty, self.split = t.Tensor, t.empty, t.unsafe_split_with_sizes
         self.u8, self.i32, self.f32, self.f64 = t.uint8, t.int32, t.float32, t.float64
-        self.types = {t.float32: 0, t.float16: 1, t.bfloat16: 30}
+        self.types = {t.float32: 0, t.float16: 1, t.bfloat16: 30}     # of a cache -> its GGML number
         self.device = device.device()
         self.index = self.device.index
         self.raw_stream = getattr(t._C, '_cuda_getCurrentRawStream', None)
@@ -357,7 +354,7 @@ class PagedKVCache:
         torch = device.torch()
         dev, i32 = device.device(), torch.int32
         dtype = dtype or torch.float32
-        if str(dtype) not in _TYPES:
+        if dtype not in _r().types:
             raise TypeError('the cache must be float32, float16 or bfloat16')
         if page_size < 16 or page_size & (page_size - 1):
             raise ValueError('page_size must be a power of two, at least 16')
