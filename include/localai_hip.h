@@ -354,7 +354,8 @@ int64_t localai_hip_paged_attention_workspace_size(int64_t tokens, int64_t reque
  * lengths count the new tokens. starts_dev [requests + 1]: request b's rows of
  * q, gate and out are starts[b] .. starts[b + 1] - 1 (rows from
  * starts[requests] on stay as they were); NULL: one row per request (tokens =
- * requests). q, gate, out fp32 [tokens, n_heads, head_dim]. A row that sees
+ * requests); they must not decrease or pass tokens. q, gate, out fp32 [tokens,
+ * n_heads, head_dim], out q itself or apart from every other buffer. A row that sees
  * nothing (length 0) is zeros. A row whose range reaches past max_pages or a
  * page id outside [0, n_pages) is NaN, and nothing outside the cache is read.
  * What positions that a row does not see hold does not reach it, infinities

@@ -274,7 +274,7 @@ def norm_rope_store(q, k, v, positions, slots, k_cache, v_cache, freq=None, q_we
     q_weight, k_weight [head_dim]: the norms' weights, None for no norm.
     Returns q [tokens, heads, head_dim], in `out` if given (q itself, or rows
     that share no memory with each other or the rest); rows of padding are left
-    as they were."""
+    as they were, in a new result whatever its memory held."""
     cache, nkv, hd = _cache(k_cache, v_cache)
     r = _r()
     f32 = r.f32
@@ -314,8 +314,9 @@ def attention(q, k_cache, v_cache, table, lengths, starts=None, window=0, scale=
     [requests + 1] (None: one token per request) as extend() leaves them;
     window: the last positions a token sees, 0 for all; scale: 1 /
     sqrt(head_dim) by default; gate: Qwen3.5's output gate, like q. Returns
-    [tokens, heads, head_dim]; rows behind starts[-1] of a given `out` stay as
-    they were."""
+    [tokens, heads, head_dim]; rows behind starts[-1] stay as they were in
+    `out`, and hold whatever was in the memory of a new result. `out` may be q;
+    it shares memory with nothing else."""
     cache, nkv, hd = _cache(k_cache, v_cache)
     r = _r()
     f32 = r.f32

@@ -806,6 +806,17 @@ def test_attention_over_offsets_past_32_bits():
     assert torch.equal(caches[0][2, :, 5], x[0].half()) and torch.equal(caches[1][2, :, 5], x[0].half())
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('heads,lengths,new', [((8, 2, 64), [3000, 5, 0], None), ((8, 2, 128), [2500, 64], [40, 9]),
+                                               ((32, 32, 64), [300, 130, 70], [200, 100, 70])])
+def test_attention_into_its_queries(heads, lengths, new, dtype):
+    from localai_amd import paged
+    (q, *rest), kw, y = _attention(heads, lengths, dtype, new=new, seed=14)
+    got = paged.attention(q, *rest, out=q, **kw)
+    assert got is q
+    np.testing.assert_array_equal(q.cpu().numpy(), y)
+
+
 def test_attention_same_bits_again_and_on_another_stream():
     import torch
     from localai_amd import paged
