@@ -79,13 +79,15 @@ class Step(collections.namedtuple('Step', 'lengths used starts slots positions s
     position (-1 behind the last token); status [1], 0 where all fitted."""
     __slots__ = ()
 
-    def check(self):
-        check(self.status)
+    def check(self, stream=None):
+        check(self.status, stream)
 
 
-def check(status):
-    """Wait for `status` (of extend or shrink) and raise if it is not 0."""
-    bits = int(status.item())
+def check(status, stream=None):
+    """Wait for `status` (of extend or shrink on `stream`, or on the current
+    stream) and raise if it is not 0."""
+    with _on(stream):
+        bits = int(status.item())
     if bits:
         raise RuntimeError('paged cache: ' + '; '.join(text for bit, text in _STATUS if bits & bit)
                            + ' (nothing was changed)')

@@ -887,6 +887,26 @@ def test_calls_on_another_stream_hold_their_arguments():
     del held
 
 
+def test_check_waits_for_the_stream_of_the_call():
+    import torch
+    from localai_amd import paged
+    cache = paged.PagedKVCache(1, 1, 64, n_pages=2, page_size=16, requests=1)
+    side, new, keep = torch.cuda.Stream(), _ints([40]), _ints([-1])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)        # some 10 ms
+    step = cache.extend(new, 40, stream=side)
+    with pytest.raises(RuntimeError, match='too few pages|longer than'):
+        step.check(stream=side)
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+    status = cache.shrink(keep, stream=side)
+    with pytest.raises(RuntimeError, match='negative'):
+        paged.check(status, side)
+    with torch.cuda.stream(side):
+        cache.extend(_ints([32]), 32).check()
+
+
 def test_refusals():
     import torch
     from localai_amd import _lib, paged
