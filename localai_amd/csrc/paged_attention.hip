@@ -46,9 +46,10 @@ namespace lq {
 // 6.0), 64 requests up to 8192, bf16 (594 MB), 110-113 us; below some 2000
 // positions by the launch and five dependent loads (7 us with one position).
 // Prompts are bound by the chain of products, softmax and products of a tile
-// while there are few of them (963 tokens over 2048 positions 66 us), by MFMA
-// when many (8192 tokens of 32 heads of 128 1.09 ms: 1017 TFLOP/s of f16 MFMA,
-// of which q's and p's second pieces are half).
+// while there are few of them (963 tokens over 2048 positions, 32 heads of 128:
+// f16 66 us, bf16 about 80, fp32 225), by MFMA when many (8192 tokens 1.09 to
+// 1.12 ms: 980 to 1010 TFLOP/s of f16 MFMA, of which q's and p's second pieces
+// are half).
 struct PagedArgs {
     PagedQueries p;
     PagedCache c;
@@ -355,7 +356,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     constexpr bool KL = (WS < 4 || NT > 1) && P::pieces == 2;
     constexpr int QT = F32 ? HD / 16 : HD / 32, QL = F32 ? 1 : 2;   // steps of a product over d; float4s of q for one
     // q's three bf16 pieces of two column tiles stay in LDS, a copy for each
-    // set: in registers they spill (963 tokens over 2048 positions 86 us, 72
+    // set: in registers they spill (555 tokens over 2048 positions 86 us, 72
     // so; 8192 tokens 1613 and 1372). f16's two fit, and are faster there (8192
     // tokens 1096 us against 1157).
     constexpr bool QS = P::pieces == 3 && NT == 2;
@@ -540,7 +541,8 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
                     // a second or third piece of 0 becomes the smallest of the
                     // value's sign (at most 2^-33 of the column's largest in f16,
                     // 2^-133 in bf16): times an infinite k it is the infinity that
-                    // the first piece gives, not NaN
+                    // the first piece gives, not NaN (16 requests of heads of 256
+                    // 18.9 -> 19.1 us, others within 1 %)
                     o[0][e] = s[0];
 #pragma unroll
                     for (int i = 1; i < P::pieces; ++i) o[i][e] = larger16(0x00010001u, s[i]) | (s[0] & 0x80008000u);
@@ -679,6 +681,8 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
         // a probability of 0 keeps V out of a column only while V is finite:
         // what is not (a store past f16's range makes it so) counts as zero
         // here, and after the loop makes the values NaN that it does reach
+        // (done here, that takes 15 to 26 registers more, which spill; looking
+        // costs 963 tokens 0.2 us, 0.4 under a window)
         if (apart(tb)) {
             uint32_t most = 0;
 #pragma unroll

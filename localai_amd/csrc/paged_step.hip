@@ -23,7 +23,8 @@ namespace lq {
 // writes the page's table entry, and no pass over pages is needed. Every
 // workgroup scans all requests (8 bytes each) and then takes its own tokens.
 // Bound by its launch and three dependent loads (lengths, the page, the store):
-// 4.0 us for one request, 4.8 for 256, 6.4 for 48 prompts of 36958 tokens.
+// 3.7 us for one request, 4.8 for 256, 6.4 for 48 prompts of 36958 tokens (8.7
+// with lengths updated in place, two launches).
 struct ExtendArgs {
     const int32_t *lengths, *fresh, *free, *used;
     int32_t *table;
@@ -165,7 +166,9 @@ int launch_paged_extend(const int32_t *lengths, const int32_t *fresh, int reques
 
 // The inverse: request b keeps its first min(keep_b, lengths_b) positions; the
 // pages behind them go back onto the front of the list, in the order in which
-// an extension would take them again, and their table entries become -1.
+// an extension would take them again, and their table entries become -1. One
+// workgroup: 3.7 us for few pages, 5.9 for 9984 of 64 requests, 61 for 142347 of
+// 256, 8 bytes moved a page by dependent loads.
 struct ShrinkArgs {
     int32_t *lengths;
     const int32_t *keep;
