@@ -647,7 +647,8 @@ def test_attention_bad_pages_are_nan_and_others_unharmed(new, dtype):
 LEAKS = [((8, 2, 128), [300, 64], [40, 9], 0), ((8, 2, 128), [300, 64], [40, 9], 19), ((6, 2, 64), [90, 33], [90, 33], 0),
          ((16, 4, 256), [120, 50], [50, 7], 30), ((8, 2, 64), [70, 40, 20], [3, 0, 0], 0), ((8, 8, 64), [700], None, 80),
          ((32, 32, 64), [300, 130, 70], [200, 100, 70], 0), ((64, 32, 128), [150, 33, 260], [150, 33, 90], 37),
-         ((9, 1, 128), [2500, 700], [20, 30], 0)]
+         ((9, 1, 128), [2500, 700], [20, 30], 0),
+         ((32, 32, 64), [2600, 300], [200, 160], 1500)]     # two column sets, cut, windows that end inside a chunk
 
 
 @pytest.mark.parametrize('dtype', TYPES)
