@@ -381,6 +381,89 @@ int localai_hip_paged_attention(const float *q_dev, int64_t tokens, int n_heads,
                                 int64_t window, float scale, const float *gate_dev, float *out_dev,
                                 void *workspace_dev, int64_t workspace_bytes, void *stream);
 
+/* ---- linear-attention layers: several requests in one step ---------------- */
+
+/* The requests of a call and the pool that holds their states. Request b's
+ * state is row slots[b] of the pool (NULL: row b), its new tokens are rows
+ * starts[b] .. starts[b + 1] - 1 of the activations (NULL: row b alone, and as
+ * many tokens as requests), lengths[b] counts these and all before: a request
+ * with lengths[b] <= starts[b + 1] - starts[b] starts from zeros, whatever its
+ * row holds (NULL: none does). slots, starts and lengths are as
+ * localai_hip_paged_extend leaves them, int32 on the device; nothing is read by
+ * the host. A request whose slot is outside [0, n_slots), and rows behind
+ * starts[requests], are left out: nothing of theirs is read but x, nothing
+ * written. Slots of one call must differ; starts must not decrease or pass
+ * tokens (what lies outside is cut off). requests <= 4096, tokens below 2^24. */
+typedef struct localai_delta_requests {
+    float *state_dev;
+    int64_t n_slots;
+    const int32_t *slots_dev, *starts_dev, *lengths_dev;
+    int64_t requests;
+} localai_delta_requests;
+
+/* The short causal convolution ahead of the delta rule
+ * (engine/qwen35.py:224-252's layers), per channel c and row t of a request:
+ *   y[t, c] = bias[c] + sum_{j < width} weight[c, j] x[t - (width - 1) + j, c]
+ *   out = y / (1 + exp(-y))   (silu 1; y itself: silu 0)
+ * Rows before the request's first are those its state keeps, [width - 1,
+ * channels] fp32 with the oldest first, which then holds its last width - 1
+ * rows. x, out: type 0 fp32, 1 fp16 or 30 bf16, [tokens, channels] with strides in values;
+ * weight [channels, width] and bias [channels] (NULL: 0) fp32. width 2..8.
+ * Sums in fp32, rounded once. out shares memory with no other buffer. */
+int localai_hip_delta_conv(const void *x_dev, int type, int64_t tokens, int64_t channels, int64_t x_stride,
+                           const float *weight_dev, const float *bias_dev, int width, int silu,
+                           const localai_delta_requests *requests, void *out_dev, int64_t out_stride,
+                           void *stream);
+
+/* Bytes of workspace localai_hip_delta_rule needs (starts: whether it gets
+ * starts_dev; 0 without); -1 for invalid sizes. Calls that may overlap in time
+ * need separate workspaces; its contents mean nothing between calls. */
+int64_t localai_hip_delta_rule_workspace_size(int64_t tokens, int64_t requests, int starts, int key_heads,
+                                              int value_heads, int key_dim, int value_dim);
+
+/* The gated delta rule (localai_hip_delta_net_step's step) over the new tokens
+ * of several requests, per value head h with S = state[h] [key_dim, value_dim]
+ * fp32, token after token, key head h / (value_heads / key_heads), or h mod
+ * key_heads where tiled is 1 (the order of GGUF files):
+ *   k^ = k / sqrt(|k|^2 + norm_eps);  q^ = scale q / sqrt(|q|^2 + norm_eps)
+ *   (norm_eps < 0: k^ = k, q^ = scale q)
+ *   g = decay[t, h];  b = beta[t, h]                       (a_dev, dt_bias_dev NULL)
+ *   g = a[h] log(1 + exp(decay[t, h] + dt_bias[h]));  b = 1 / (1 + exp(-beta[t, h]))
+ *   S <- exp(g) S;  d = b (v - S^T k^);  S <- S + k^ d^T;  out = S^T q^
+ * q, k [tokens, key_heads, key_dim], v, out [tokens, value_heads, value_dim] of
+ * type 0 fp32, 1 fp16 or 30 bf16; decay, beta [tokens, value_heads], a, dt_bias
+ * [value_heads] fp32. strides[0..9] (host array, in values): token and head
+ * stride of q, k, v, out (multiples of 4), token stride of decay and beta.
+ * key_dim 64, 128 or 256; value_dim a multiple of 16, at most 1024; q, k, v and
+ * out aligned to 4 values, state and workspace to 16 bytes. out shares memory
+ * with no other buffer. requests times value_heads times value_dim / 16 below 2^24.
+ * fp32 results whatever the type (out rounded once). What is not finite reaches
+ * the tokens behind it, of a v the one column alone, and none before it; which of NaN and
+ * infinity they show is not defined. */
+int localai_hip_delta_rule(const void *q_dev, const void *k_dev, const void *v_dev, int type,
+                           const int64_t *strides, int64_t tokens, int key_heads, int value_heads, int key_dim,
+                           int value_dim, const float *decay_dev, const float *beta_dev, const float *a_dev,
+                           const float *dt_bias_dev, int tiled, float norm_eps, float scale,
+                           const localai_delta_requests *requests, void *out_dev, void *workspace_dev,
+                           int64_t workspace_bytes, void *stream);
+
+/* Root-mean-square norm (engine/model.py:82) of rows [rows, heads, dim], each of
+ * dim values (heads 1: plain rows):
+ *   h = x + residual, kept in residual_dev           (residual_dev not NULL; fp32)
+ *   y = h / sqrt(mean(h^2) + eps) weight
+ *   y = y z / (1 + exp(-z)), z = gate                (gate_dev not NULL; x's type)
+ * x of type 0 fp32, 1 fp16 or 30 bf16; out of out_type 0, 1, 30 (rounded once),
+ * or 8: Q8_0 blocks, 34 bytes for 32 values, the scale d = fp16(max|y| / 127)
+ * and 32 times rint(y / d) (what localai_hip_dequant reads; a block with a value
+ * that is not finite is NaN; dim a multiple of 32). weight [dim] fp32.
+ * strides[0..7] (host array): row and head stride of x, residual, gate (in
+ * values) and out (in values; bytes for Q8_0). fp32 throughout. out may be x
+ * with x's type and strides; other buffers share no memory. rows times heads
+ * below 2^24, dim and heads at most 2^20. */
+int localai_hip_rms_norm(const void *x_dev, int type, const int64_t *strides, int64_t rows, int64_t heads,
+                         int64_t dim, const float *weight_dev, float eps, float *residual_dev,
+                         const void *gate_dev, void *out_dev, int out_type, void *stream);
+
 /* ---- ZAYA router (engine/zaya.py:274-307) -------------------------------- */
 
 /* Everything of ZAYA's router after the first projection r0 = W_inp h

@@ -24,6 +24,12 @@ class PagedCacheArg(ctypes.Structure):
                 ('pos_stride', _c_i64)]
 
 
+class DeltaRequestsArg(ctypes.Structure):
+    """localai_delta_requests"""
+    _fields_ = [('state_dev', _vp), ('n_slots', _c_i64), ('slots_dev', _vp), ('starts_dev', _vp), ('lengths_dev', _vp),
+                ('requests', _c_i64)]
+
+
 # name -> (restype, argtypes); mirrors include/localai_hip.h
 SIGNATURES = {
     'localai_hip_version': (_c_int, []),
@@ -76,6 +82,13 @@ SIGNATURES = {
     'localai_hip_paged_attention_workspace_size': (_c_i64, [_c_i64, _c_i64, _c_int, _c_int, _c_int]),
     'localai_hip_paged_attention': (_c_int, [_vp, _c_i64, _c_int, _vp, _vp, _c_i64, _c_i64,
                                              _vp, _vp, _c_i64, _c_i64, ctypes.c_float, _vp, _vp, _vp, _c_i64, _vp]),
+    'localai_hip_delta_conv': (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _vp, _vp, _c_int, _c_int, _vp, _vp, _c_i64,
+                                        _vp]),
+    'localai_hip_delta_rule_workspace_size': (_c_i64, [_c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int]),
+    'localai_hip_delta_rule': (_c_int, [_vp, _vp, _vp, _c_int, _vp, _c_i64, _c_int, _c_int, _c_int, _c_int, _vp, _vp, _vp,
+                                        _vp, _c_int, ctypes.c_float, ctypes.c_float, _vp, _vp, _vp, _c_i64, _vp]),
+    'localai_hip_rms_norm': (_c_int, [_vp, _c_int, _vp, _c_i64, _c_i64, _c_i64, _vp, ctypes.c_float, _vp, _vp, _vp, _c_int,
+                                      _vp]),
     'localai_hip_debug_fused_wait': (_c_int, [_c_int, _c_int]),
     'localai_hip_register_host': (_c_int, [_vp, ctypes.c_size_t]),
     'localai_hip_unregister_host': (_c_int, [_vp]),

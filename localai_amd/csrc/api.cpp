@@ -9,6 +9,7 @@
 #include <string>
 
 #include "internal.h"
+#include "delta.h"
 #include "paged.h"
 
 namespace lq {
@@ -755,6 +756,135 @@ int localai_hip_paged_attention(const float *q, int64_t tokens, int n_heads, con
     const PagedQueries p{q, gate, out, tokens, n_heads, cache->n_kv_heads, cache->head_dim, (int)requests,
                          table, lengths, starts, table_stride, (int)max_pages, window, scale};
     return launch_paged_attention(p, c, ws, (hipStream_t)stream);
+}
+
+// ---- linear-attention layers ----
+
+static bool delta_type(int type) { return type == DELTA_F32 || type == DELTA_F16 || type == DELTA_BF16; }
+
+static int delta_requests_of(const char *who, const localai_delta_requests *a, int64_t tokens, DeltaRequests *out) {
+    const std::string w = who;
+    if (!a || !a->state_dev) return fail(LOCALAI_EARG, w + ": null state");
+    if (tokens < 0 || tokens >= 1 << 24) return fail(LOCALAI_EARG, w + ": tokens must be in 0..2^24 - 1");
+    if (a->requests < 1 || a->requests > DELTA_MAX_REQUESTS)
+        return fail(LOCALAI_EARG, w + ": requests must be in 1..4096");
+    if (a->n_slots < 1) return fail(LOCALAI_EARG, w + ": n_slots must be at least 1");
+    if (!a->starts_dev && tokens != a->requests)
+        return fail(LOCALAI_EARG, w + ": without starts there is one token per request");
+    *out = DeltaRequests{a->state_dev, a->n_slots, a->slots_dev, a->starts_dev, a->lengths_dev, (int)a->requests,
+                         (int)tokens};
+    return LOCALAI_OK;
+}
+
+int localai_hip_delta_conv(const void *x, int type, int64_t tokens, int64_t channels, int64_t x_stride,
+                           const float *weight, const float *bias, int width, int silu,
+                           const localai_delta_requests *requests, void *out, int64_t out_stride, void *stream) {
+    clear_error();
+    DeltaRequests r;
+    if (int st = delta_requests_of("delta conv", requests, tokens, &r)) return st;
+    if (!delta_type(type)) return fail(LOCALAI_ETYPE, "delta conv: x and out are fp32 (0), fp16 (1) or bf16 (30)");
+    if (width < 2 || width > DELTA_MAX_WIDTH) return fail(LOCALAI_ETYPE, "delta conv: width 2..8");
+    if (channels < 1 || channels > 1 << 20) return fail(LOCALAI_EARG, "delta conv: channels must be in 1..2^20");
+    if (silu != 0 && silu != 1) return fail(LOCALAI_EARG, "delta conv: silu is 0 or 1");
+    if (r.n_slots > ((int64_t)1 << 50) / channels) return fail(LOCALAI_EARG, "delta conv: state too large");
+    if (!tokens) return LOCALAI_OK;
+    if (!x || !weight || !out) return fail(LOCALAI_EARG, "delta conv: null pointer");
+    if (x_stride < 0 || (tokens > 1 && out_stride < channels))
+        return fail(LOCALAI_EARG, "delta conv: x's stride must not be negative, rows of out must not overlap");
+    if (int st = ensure_device()) return st;
+    return launch_delta_conv(DeltaConv{x, out, weight, bias, x_stride, out_stride, channels, type, width, silu}, r,
+                             (hipStream_t)stream);
+}
+
+static int delta_rule_sizes(int64_t requests, int key_heads, int value_heads, int kd, int vd) {
+    if (key_heads < 1 || value_heads < 1 || value_heads > 4096 || value_heads % key_heads)
+        return fail(LOCALAI_EARG, "delta rule: value_heads must be a multiple of key_heads, at most 4096");
+    if (kd != 64 && kd != 128 && kd != 256) return fail(LOCALAI_ETYPE, "delta rule: key_dim 64, 128 or 256");
+    if (vd < 16 || vd > 1024 || vd % 16) return fail(LOCALAI_ETYPE, "delta rule: value_dim a multiple of 16, at most 1024");
+    if (requests * value_heads * (vd / 16) >= 1 << 24)     // workgroups of a launch
+        return fail(LOCALAI_EARG, "delta rule: too many requests times heads for one call");
+    return LOCALAI_OK;
+}
+
+int64_t localai_hip_delta_rule_workspace_size(int64_t tokens, int64_t requests, int starts, int key_heads,
+                                              int value_heads, int key_dim, int value_dim) {
+    if (tokens < 0 || tokens >= 1 << 24 || requests < 1 || requests > DELTA_MAX_REQUESTS ||
+        delta_rule_sizes(requests, key_heads, value_heads, key_dim, value_dim))
+        return -1;
+    return delta_rule_workspace_bytes(tokens, (int)requests, !starts, key_heads, value_heads, key_dim, value_dim);
+}
+
+int localai_hip_delta_rule(const void *q, const void *k, const void *v, int type, const int64_t *strides,
+                           int64_t tokens, int key_heads, int value_heads, int key_dim, int value_dim,
+                           const float *decay, const float *beta, const float *a, const float *dt_bias, int tiled,
+                           float norm_eps, float scale, const localai_delta_requests *requests, void *out, void *ws,
+                           int64_t ws_bytes, void *stream) {
+    clear_error();
+    DeltaRequests r;
+    if (int st = delta_requests_of("delta rule", requests, tokens, &r)) return st;
+    if (int st = delta_rule_sizes(r.requests, key_heads, value_heads, key_dim, value_dim)) return st;
+    if (!delta_type(type)) return fail(LOCALAI_ETYPE, "delta rule: q, k, v and out are fp32 (0), fp16 (1) or bf16 (30)");
+    if (tiled != 0 && tiled != 1) return fail(LOCALAI_EARG, "delta rule: tiled is 0 or 1");
+    if (!(std::fabs(scale) <= FLT_MAX) || !(norm_eps <= FLT_MAX))
+        return fail(LOCALAI_EARG, "delta rule: scale and norm_eps must be finite");
+    if ((a == nullptr) != (dt_bias == nullptr)) return fail(LOCALAI_EARG, "delta rule: a and dt_bias go together");
+    if (r.n_slots > ((int64_t)1 << 50) / ((int64_t)value_heads * key_dim * value_dim))
+        return fail(LOCALAI_EARG, "delta rule: state too large");
+    if (!tokens) return LOCALAI_OK;
+    if (!q || !k || !v || !strides || !decay || !beta || !out) return fail(LOCALAI_EARG, "delta rule: null pointer");
+    for (int i = 0; i < 10; ++i)
+        if (strides[i] < 0 || (i < 8 && strides[i] % 4))
+            return fail(LOCALAI_EARG, "delta rule: strides must not be negative, those of q, k, v and out multiples of 4 values");
+    if (rows_overlap(tokens, value_heads, strides[6], strides[7], value_dim))
+        return fail(LOCALAI_EARG, "delta rule: rows of out overlap");
+    const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
+                          reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out);
+    if (all & (type == DELTA_F32 ? 15 : 7))
+        return fail(LOCALAI_EARG, "delta rule: q, k, v and out must be aligned to 4 values");
+    if ((reinterpret_cast<uintptr_t>(r.state) | reinterpret_cast<uintptr_t>(ws)) & 15)
+        return fail(LOCALAI_EARG, "delta rule: the state and the workspace must be 16-byte aligned");
+    const int64_t need = delta_rule_workspace_bytes(tokens, r.requests, !r.starts, key_heads, value_heads, key_dim,
+                                                    value_dim);
+    if (need > 0 && (!ws || ws_bytes < need)) return fail(LOCALAI_EARG, "delta rule: workspace too small");
+    if (int st = ensure_device()) return st;
+    const DeltaRule p{q, k, v, out, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5],
+                      strides[6], strides[7], strides[8], strides[9], decay, beta, a, dt_bias,
+                      type, key_heads, value_heads, key_dim, value_dim, tiled, norm_eps, scale};
+    return launch_delta_rule(p, r, ws, (hipStream_t)stream);
+}
+
+int localai_hip_rms_norm(const void *x, int type, const int64_t *strides, int64_t rows, int64_t heads, int64_t dim,
+                         const float *weight, float eps, float *residual, const void *gate, void *out, int out_type,
+                         void *stream) {
+    clear_error();
+    const bool q8 = out_type == 8;
+    if (!delta_type(type)) return fail(LOCALAI_ETYPE, "rms norm: x and gate are fp32 (0), fp16 (1) or bf16 (30)");
+    if (!q8 && !delta_type(out_type))
+        return fail(LOCALAI_ETYPE, "rms norm: out is fp32 (0), fp16 (1), Q8_0 (8) or bf16 (30)");
+    if (rows < 0 || heads < 1 || dim < 1 || dim > 1 << 20 || heads > 1 << 20 || rows > ((1 << 24) - 1) / heads)
+        return fail(LOCALAI_EARG, "rms norm: dim and heads must be in 1..2^20, rows times heads below 2^24");
+    if (!(eps >= 0.0f && eps <= FLT_MAX)) return fail(LOCALAI_EARG, "rms norm: eps must be finite and not negative");
+    if (!rows) return LOCALAI_OK;
+    if (!x || !strides || !weight || !out) return fail(LOCALAI_EARG, "rms norm: null pointer");
+    for (int i = 0; i < 8; ++i)
+        if (strides[i] < 0) return fail(LOCALAI_EARG, "rms norm: strides must not be negative");
+    if (rows_overlap(rows, heads, strides[6], strides[7], q8 ? dim / 32 * 34 : dim) ||
+        (residual && rows_overlap(rows, heads, strides[2], strides[3], dim)))
+        return fail(LOCALAI_EARG, "rms norm: rows of out or of the residual overlap");
+    if (q8) {
+        const uintptr_t unit = type == DELTA_F32 ? 15 : 7;
+        if (dim % 32) return fail(LOCALAI_ETYPE, "rms norm: Q8_0 needs dim to be a multiple of 32");
+        if ((reinterpret_cast<uintptr_t>(x) & unit) || (reinterpret_cast<uintptr_t>(gate) & unit) ||
+            (reinterpret_cast<uintptr_t>(residual) & 15) || (reinterpret_cast<uintptr_t>(out) & 1))
+            return fail(LOCALAI_EARG, "rms norm: Q8_0 needs x, gate and residual aligned to 4 values, out to 2 bytes");
+        for (int i = 0; i < 8; ++i)
+            if (strides[i] % (i < 6 ? 4 : 2))
+                return fail(LOCALAI_EARG, "rms norm: Q8_0 needs strides of x, gate and residual that are multiples of 4, of out of 2");
+    }
+    if (int st = ensure_device()) return st;
+    return launch_rms_norm(RmsNorm{x, gate, out, residual, weight, strides[0], strides[1], strides[2], strides[3],
+                                   strides[4], strides[5], strides[6], strides[7], rows, heads, dim, type, out_type,
+                                   eps}, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,119 @@
+// The linear-attention layers of several requests: what the kernels of the
+// convolution and of the gated delta rule and their entry points share.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace lq {
+
+// activation types, by their GGML numbers
+enum { DELTA_F32 = 0, DELTA_F16 = 1, DELTA_BF16 = 30 };
+
+constexpr int DELTA_MAX_REQUESTS = 4096;
+constexpr int DELTA_MAX_WIDTH = 8;         // taps of the convolution
+
+// the requests of a call (localai_delta_requests)
+struct DeltaRequests {
+    float *state;
+    int64_t n_slots;
+    const int32_t *slots, *starts, *lengths;
+    int requests, tokens;
+};
+
+struct DeltaConv {
+    const void *x;
+    void *out;
+    const float *weight, *bias;
+    int64_t x_stride, out_stride, channels;
+    int type, width, silu;
+};
+int launch_delta_conv(const DeltaConv &c, const DeltaRequests &r, hipStream_t s);
+
+struct DeltaRule {
+    const void *q, *k, *v;
+    void *out;
+    int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs, g_ts, b_ts;   // token and head strides, in values
+    const float *decay, *beta, *a, *dt_bias;
+    int type, key_heads, value_heads, kd, vd, tiled;
+    float norm_eps, scale;      // norm_eps < 0: q and k as they are
+};
+int64_t delta_rule_workspace_bytes(int64_t tokens, int requests, bool step, int key_heads, int value_heads, int kd,
+                                   int vd);
+int launch_delta_rule(const DeltaRule &p, const DeltaRequests &r, void *ws, hipStream_t s);
+
+struct RmsNorm {
+    const void *x, *gate;
+    void *out;
+    float *residual;
+    const float *weight;
+    int64_t x_rs, x_hs, r_rs, r_hs, g_rs, g_hs, o_rs, o_hs;    // row and head strides, in values (Q8_0: bytes)
+    int64_t rows, heads, dim;
+    int type, out_type;
+    float eps;
+};
+int launch_rms_norm(const RmsNorm &n, hipStream_t s);
+
+#ifdef __HIPCC__
+// Request b's rows [first, first + count) and state row: a request without a
+// slot of the pool has none. Rows stay inside the call's whatever starts holds.
+struct DeltaSpan {
+    int first, count;
+    int64_t slot;
+    bool fresh;      // all of the request's tokens are new: it starts from zeros
+};
+__device__ __forceinline__ DeltaSpan delta_span(const DeltaRequests &r, int b) {
+    DeltaSpan d;
+    d.slot = r.slots ? r.slots[b] : b;
+    int first = b, end = b + 1;
+    if (r.starts) {
+        first = min(max(r.starts[b], 0), r.tokens);
+        end = min(max(r.starts[b + 1], first), r.tokens);
+    }
+    d.first = first;
+    d.count = d.slot >= 0 && d.slot < r.n_slots ? end - first : 0;
+    d.fresh = r.lengths && r.lengths[b] <= end - first;
+    return d;
+}
+
+// Requests cut into pieces of `size` rows: piece j of request b has the number
+// starts[b] / size + b + j, so no table is needed: a request of n rows has at
+// most (its last row / size - its first row / size + 1) pieces, and the next
+// request's numbers begin behind those. Numbers below tokens / size + requests.
+// Returns the piece's request, or -1 (no wave-wide value differs): the last b
+// with starts[b] / size + b <= piece, found 64 requests at a time.
+__device__ __forceinline__ int delta_request(const DeltaRequests &r, int piece, int size) {
+    const int lane = (int)(threadIdx.x & 63);
+    int b = -1;
+    for (int at = 0; at < r.requests; at += 64) {
+        const int i = at + lane;
+        const bool before = i < r.requests && min(max(r.starts[i], 0), r.tokens) / size + i <= piece;
+        const int n = __popcll(__ballot(before));
+        b += n;
+        if (n < 64) break;
+    }
+    return __builtin_amdgcn_readfirstlane(b);
+}
+
+template <typename T> struct DeltaVec;
+template <> struct DeltaVec<float> { typedef float4 raw; };
+template <> struct DeltaVec<_Float16> { typedef uint2 raw; };
+template <> struct DeltaVec<__bf16> { typedef uint2 raw; };
+
+// 4 adjacent values (aligned to 4 of them)
+template <typename T>
+__device__ __forceinline__ float4 delta_load4(const T *p) {
+    const auto raw = *reinterpret_cast<const typename DeltaVec<T>::raw *>(p);
+    T h[4];
+    __builtin_memcpy(h, &raw, sizeof(h));
+    return make_float4((float)h[0], (float)h[1], (float)h[2], (float)h[3]);
+}
+template <typename T>
+__device__ __forceinline__ void delta_store4(T *p, const float4 &y) {
+    T h[4] = {(T)y.x, (T)y.y, (T)y.z, (T)y.w};
+    typename DeltaVec<T>::raw raw;
+    __builtin_memcpy(&raw, h, sizeof(h));
+    *reinterpret_cast<typename DeltaVec<T>::raw *>(p) = raw;
+}
+#endif
+
+}  // namespace lq

@@ -1,4 +1,5 @@
-"""The matvec chain of one decode layer (localai_hip_layer_chain).
+"""The matvec chain of one decode layer (localai_hip_layer_chain), and the norm
+between layers for several rows.
 
 DecodeLayerChain holds the seven weight handles of the chain -- attn_output,
 ffn_gate, ffn_up, ffn_down of layer L and attn_q, attn_k, attn_v of layer
@@ -14,14 +15,19 @@ All of it stays on the device; nothing here computes on the host. By default
 the chain runs as four launches with the glue fused into the matvec kernels;
 set_mode(one_launch=True) selects the single launch with device-side waits
 between its stages.
+
+rms_norm is the norm of many tokens at once (localai_hip_rms_norm): with the
+residual's addition, with a gate, to any activation type or to Q8_0 blocks.
 """
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import numpy as np
 
 from . import _lib, device
+from .paged import _device_tensor, _empty, _hold, _ptr, _r, _refuse, _stream
 
 ORDER = ('attn_output', 'ffn_gate', 'ffn_up', 'ffn_down', 'attn_q', 'attn_k', 'attn_v')
 
@@ -78,3 +84,67 @@ class DecodeLayerChain:
         """Wait for `stream`; raise if a wait between stages ran out."""
         _lib.check(_lib.load().localai_hip_layer_error(device.ptr(self.ws),
                                                        ctypes.c_void_p(device.stream_ptr(stream))))
+
+
+_STRIDES = struct.Struct('=8q')
+_TYPES = {}
+
+
+def _norm_rows(t, name, dtype, shape):
+    """(address, row stride, head stride) of t [rows, dim] or [rows, heads, dim]."""
+    r = _r()
+    if not (isinstance(t, r.Tensor) and t.dtype is dtype and t.get_device() == r.index and t.shape == shape):
+        _refuse(t, name, dtype, shape)
+    stride = t.stride()
+    if stride[-1] != 1 and shape[-1] > 1:
+        raise ValueError(f'{name} must have adjacent values')
+    # (the stride of a dimension of one says nothing)
+    return (t.data_ptr(), stride[0] if shape[0] > 1 else 0,
+            stride[1] if len(shape) == 3 and shape[1] > 1 else 0)
+
+
+def rms_norm(x, weight, eps=1e-6, residual=None, gate=None, dtype=None, out=None, stream=None):
+    """Root-mean-square norm of rows (localai_hip_rms_norm).
+
+    x [rows, dim] or [rows, heads, dim]: fp32, f16 or bf16, any strides with
+    adjacent values, each row (of each head) normed by itself; weight [dim] fp32.
+    residual: fp32 of x's shape; x is added to it in place, and the sum is normed.
+    gate: of x's type and shape; the result is multiplied by gate / (1 + exp(-gate)).
+    dtype: the result's type, x's by default, or 'q8_0': uint8 [.., dim / 32 * 34],
+    GGML Q8_0 blocks (dequant.dequantize_device reads them; then dim is a multiple of 32,
+    and strides of 4 values). Returns the result, in `out` if given: x itself where the types are
+    the same, or memory of its own."""
+    _device_tensor(x, 'x')
+    r = _r()
+    if not _TYPES:
+        t = device.torch()
+        _TYPES.update({t.float32: 0, t.float16: 1, t.bfloat16: 30, 'q8_0': 8})
+    kind, out_type = _TYPES.get(x.dtype), _TYPES.get(x.dtype if dtype is None else dtype)
+    if kind is None:
+        raise TypeError('x must be float32, float16 or bfloat16')
+    if out_type is None:
+        raise TypeError("dtype must be float32, float16, bfloat16 or 'q8_0'")
+    shape = x.shape
+    if len(shape) not in (2, 3):
+        raise ValueError('x must be [rows, dim] or [rows, heads, dim]')
+    dim = shape[-1]
+    xp, *xs = _norm_rows(x, 'x', x.dtype, shape)
+    wp = _ptr(weight, 'weight', r.f32, (dim,))
+    rp, *rs = _norm_rows(residual, 'residual', r.f32, shape) if residual is not None else (None, 0, 0)
+    gp, *gs = _norm_rows(gate, 'gate', x.dtype, shape) if gate is not None else (None, 0, 0)
+    q8 = out_type == 8
+    if q8 and dim % 32:
+        raise ValueError("'q8_0' needs dim to be a multiple of 32")
+    out_shape = (*shape[:-1], dim // 32 * 34) if q8 else shape
+    out_dtype = r.u8 if q8 else x.dtype if dtype is None else dtype
+    if out is None:
+        out = _empty(stream, out_shape, out_dtype)
+    op, *os = _norm_rows(out, 'out', out_dtype, out_shape)
+    status = _lib.load().localai_hip_rms_norm(xp, kind, _STRIDES.pack(*xs, *rs, *gs, *os), shape[0],
+                                              shape[1] if len(shape) == 3 else 1, dim, wp, eps, rp, gp, op, out_type,
+                                              _stream(stream))
+    if status:
+        _lib.check(status)
+    if stream is not None:
+        _hold(stream, x, weight, residual, gate, out)
+    return out
