@@ -33,7 +33,7 @@ __device__ __forceinline__ int rule_key_head(const DeltaRule &p, int h) {
 // S' = e^g S, one pass over the rows gives S'^T k and S'^T q; the token's result
 // needs no second one: o = S'^T q^ + d (k^ . q^).
 template <typename T, int KD, int VS>
-__global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequests r) {
+__global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequests r, int most) {
     constexpr int LPR = VS / 4, RW = 64 / LPR, NR = KD * VS / 1024;   // lanes a row, rows a wave's pass, passes
     __shared__ __align__(16) float kq[2][2][KD];                       // by token parity: k, q
     __shared__ __align__(16) float red[2][4][2][VS];                   // by token parity, wave: S'^T k, S'^T q
@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequ
     const int64_t heads = (int64_t)p.value_heads * slices;
     const int b = (int)(blockIdx.x / heads), hs = (int)(blockIdx.x % heads), h = hs / slices;
     const DeltaSpan span = delta_span(r, b);
-    if (!span.count) return;
+    if (!span.count || span.count > most) return;
     const int tid = (int)threadIdx.x, lane = lane_id(), w = wave_id();
     const int c = lane % LPR * 4, c0 = hs % slices * VS, row0 = w * RW + lane / LPR, kh = rule_key_head(p, h);
     float *state = r.state + ((span.slot * p.value_heads + h) * KD + row0) * p.vd + c0 + c;
@@ -123,31 +123,645 @@ __global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequ
     for (int i = 0; i < NR; ++i) *reinterpret_cast<float4 *>(state + (int64_t)i * 4 * RW * p.vd) = S[i];
 }
 
+// ---------------------------------------------------------------- pieces of prompts
+//
+// 64 tokens at once. With G_i the sum of g over the piece's tokens up to i, and
+//   A_ij = b_i e^(G_i - G_j) k^_i . k^_j  (j < i)     P_ij = e^(G_i - G_j) q^_i . k^_j  (j <= i)
+// the rows d_i of all tokens solve (I + A) D = diag(b) (V - diag(e^G) K^ S), so
+//   D = T' (V - diag(e^G) K^ S),  T' = (I + A)^-1 diag(b)
+//   O = diag(e^G) Q^ S + P D
+//   S <- e^G_last S + (diag(e^(G_last - G)) K^)^T D
+// What does not depend on S (T', P, the factors, the operands' layout) is one
+// launch over all pieces and heads (delta_piece_kernel); the chain over a
+// request's pieces is a second one, each workgroup with 16 value columns of one
+// head, whose S stays in registers (delta_chain_kernel).
+//
+// Precision: everything is fp32's. MFMA takes bf16 operands, so each fp32 value
+// goes in as three bf16 pieces (24 bits), q and k of 16 bits as they are (bf16:
+// one piece, f16: two); of the products those up to 2^-16 of the largest are
+// kept. The norms' factors are applied to the sums (fp32 q and k: before). G is
+// summed in fp64, so that a difference keeps its bits behind a token that
+// forgets everything. The inverse goes by forward substitution in blocks of 16,
+// whose numbers stay as small as the rule's own.
+// A piece with a number that is not finite, or whose products would leave fp32's
+// range, goes through its tokens one by one instead: NaN times a zero of T' or
+// P would reach tokens before it.
+
+typedef __bf16 dr_b8 __attribute__((ext_vector_type(8)));
+typedef uint32_t dr_u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t dr_u2 __attribute__((ext_vector_type(2)));
+
+constexpr int PIECE = 64;
+constexpr int TRI = 6;                 // 16 x 32 blocks of a lower triangular 64 x 64: row tile w has w / 2 + 1
+constexpr float RULE_WILD = 1e15f;     // values of q, k, v (squared: of S) past it go token by token
+constexpr float RULE_FAINT = 1e-12f;   // so do k and q whose largest value is below it
+
+// pieces that hold a value of type T, and whether the norm's factor goes in first
+template <typename T> struct RuleType { static constexpr int NP = 1; };
+template <> struct RuleType<_Float16> { static constexpr int NP = 2; };
+template <> struct RuleType<float> { static constexpr int NP = 3; };
+
+// workspace of one window of pieces, in 1 KB blocks (64 lanes x 16 bytes: an MFMA operand)
+struct RuleWork {
+    dr_u4 *k, *q, *kt;     // [piece, key head][..][np][64]: row tile, step; kt: key tile, step
+    dr_u4 *t, *p;          // [piece, value head][TRI][3][64]
+    float *rows;           // [piece, value head][4][64]: e^G |k|^-1, e^G |q|^-1 scale, e^(G_last - G) |k|^-1; e^G_last, wild
+    int first, pieces;     // the window
+    int least;             // requests of fewer tokens are the token kernel's
+};
+
+__device__ __forceinline__ float dr_rows_sum(float v) {     // over lanes l, l ^ 16, l ^ 32, l ^ 48
+    const auto f = [](uint32_t u) { return __builtin_bit_cast(float, u); };
+    const auto u = [](float x) { return __builtin_bit_cast(uint32_t, x); };
+    const auto a = __builtin_amdgcn_permlane16_swap(u(v), u(v), false, false);
+    v = f(a[0]) + f(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(u(v), u(v), false, false);
+    return f(b[0]) + f(b[1]);
+}
+__device__ __forceinline__ float dr_rows_max(float v) {
+    const auto f = [](uint32_t u) { return __builtin_bit_cast(float, u); };
+    const auto u = [](float x) { return __builtin_bit_cast(uint32_t, x); };
+    const auto a = __builtin_amdgcn_permlane16_swap(u(v), u(v), false, false);
+    v = fmaxf(f(a[0]), f(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(u(v), u(v), false, false);
+    return fmaxf(f(b[0]), f(b[1]));
+}
+
+// x as N bf16 pieces, the first its nearest, the next what is left
+template <int N>
+__device__ __forceinline__ void dr_split(float x, __bf16 (&p)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        p[i] = (__bf16)x;
+        x -= (float)p[i];
+    }
+}
+template <int N>
+__device__ __forceinline__ void dr_split8(const float (&x)[8], dr_u4 (&y)[N]) {
+    __bf16 h[8][N];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dr_split<N>(x[e], h[e]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const dr_b8 v = {h[0][i], h[1][i], h[2][i], h[3][i], h[4][i], h[5][i], h[6][i], h[7][i]};
+        y[i] = __builtin_bit_cast(dr_u4, v);
+    }
+}
+__device__ __forceinline__ void dr_split4(const lq_f4 &x, dr_u2 (&y)[3]) {
+    __bf16 h[4][3];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) dr_split<3>(x[e], h[e]);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const __bf16 v[4] = {h[0][i], h[1][i], h[2][i], h[3][i]};
+        __builtin_memcpy(&y[i], v, 8);
+    }
+}
+
+__device__ __forceinline__ lq_f4 dr_mfma(const dr_u4 &a, const dr_u4 &b, const lq_f4 &c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dr_b8, a), __builtin_bit_cast(dr_b8, b), c, 0, 0, 0);
+}
+// c[0] += the first pieces' product, c[1] += the others' up to 2^-16 of it (NA, NB: pieces of a and b)
+template <int NA, int NB>
+__device__ __forceinline__ void dr_product(const dr_u4 (&a)[NA], const dr_u4 (&b)[NB], lq_f4 (&c)[2]) {
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            if (i + j < 3) c[i + j > 0] = dr_mfma(a[i], b[j], c[i + j > 0]);
+}
+
+// A workgroup prepares one piece for one key head and the value heads that read
+// it (blockIdx.y: one of them, where there are few pieces). Wave w owns rows
+// 16 w .. 16 w + 15. An operand's lane l holds row or column l & 15 and of each
+// 32 contracted values x the eight 4 (l >> 4) + 0..3 and 16 + 4 (l >> 4) + 0..3:
+// the layout in which MFMA leaves two tiles of results, so those are operands
+// as they are.
+template <typename T, int KD>
+__global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
+    constexpr int NP = RuleType<T>::NP, NS = KD / 32, LD = 68;
+    __shared__ __align__(16) dr_u4 ks[4][NS][NP][64];
+    __shared__ __align__(16) float am[PIECE][LD], tm[PIECE][LD];
+    __shared__ double gs[PIECE];
+    __shared__ float bs[PIECE], ik[PIECE], iq[PIECE], kn[PIECE];
+    __shared__ int wild_s[4];
+    const int local = (int)(blockIdx.x / p.key_heads), kh = (int)(blockIdx.x % p.key_heads);
+    const int piece = ws.first + local, b = delta_request(r, piece, PIECE);
+    if (b < 0) return;
+    const DeltaSpan span = delta_span(r, b);
+    const int j0 = (piece - (span.first / PIECE + b)) * PIECE, n = min(span.count - j0, PIECE);
+    if (j0 < 0 || n <= 0 || span.count < ws.least) return;
+    const int w = wave_id(), lane = lane_id(), m = lane & 15, g = lane >> 4;
+    const int64_t row0 = (int64_t)span.first + j0;
+    bool wild = false;
+    const bool norm = p.norm_eps >= 0.0f;
+    dr_u4 qf[NS][NP];
+    {
+        const bool in = 16 * w + m < n;
+        const T *rows[2] = {(const T *)p.k + (row0 + (in ? 16 * w + m : 0)) * p.k_ts + kh * p.k_hs,
+                            (const T *)p.q + (row0 + (in ? 16 * w + m : 0)) * p.q_ts + kh * p.q_hs};
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+            float x[NS][8], ss = 0.0f, top = 0.0f;
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float4 v = delta_load4(rows[o] + 32 * s + 16 * u + 4 * g);
+                    if (!in) v = make_float4(0, 0, 0, 0);
+                    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x[s][4 * u + i] = e[i];
+                        ss += e[i] * e[i];
+                        top = fmaxf(top, fabsf(e[i]));
+                        wild |= !(fabsf(e[i]) <= RULE_WILD);
+                    }
+                }
+            ss = dr_rows_sum(ss);
+            top = dr_rows_max(top);
+            wild |= top > 0.0f && top < RULE_FAINT;
+            float inv = norm ? 1.0f / sqrtf(ss + p.norm_eps) : 1.0f;
+            if (norm && !(inv <= 3.4e38f)) {     // a row of zeros and norm_eps 0: 0 / 0
+                wild |= in;
+                inv = 0.0f;
+            }
+            if (!o && g == 0) kn[16 * w + m] = ss * inv * inv;     // |k^|^2
+            if (NP == 3) {
+#pragma unroll
+                for (int s = 0; s < NS; ++s)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[s][e] *= inv;
+                inv = 1.0f;
+            }
+            if (g == 0) (o ? iq : ik)[16 * w + m] = inv;
+            dr_u4 *dst = (o ? ws.q : ws.k) + (((int64_t)local * p.key_heads + kh) * 4 + w) * NS * NP * 64 + lane;
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                dr_u4 y[NP];
+                dr_split8<NP>(x[s], y);
+#pragma unroll
+                for (int i = 0; i < NP; ++i) {
+                    if (o) qf[s][i] = y[i];
+                    else ks[w][s][i][lane] = y[i];
+                    if (blockIdx.y == 0) dst[(s * NP + i) * 64] = y[i];
+                }
+            }
+        }
+    }
+    __syncthreads();
+    // K^T: lane (key value 16 t + m, tokens 4 g + 0..3 and 16 + 4 g + 0..3 of 32)
+    if (blockIdx.y == 0) {
+        dr_u4 *dst = ws.kt + ((int64_t)local * p.key_heads + kh) * (KD / 16) * 2 * NP * 64 + lane;
+#pragma unroll
+        for (int i = 0; i < KD / 64; ++i) {
+            const int t = w * (KD / 64) + i;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int pc = 0; pc < NP; ++pc) {
+                    uint16_t h[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int token = 32 * s + 16 * (e >> 2) + 4 * g + (e & 3);
+                        const uint16_t *src = reinterpret_cast<const uint16_t *>(&ks[token >> 4][t >> 1][pc][(token & 15) + 16 * (m >> 2)]);
+                        h[e] = src[(m & 3) + 4 * (t & 1)];
+                    }
+                    dr_u4 y;
+                    __builtin_memcpy(&y, h, 16);
+                    dst[((t * 2 + s) * NP + pc) * 64] = y;
+                }
+        }
+    }
+    // k_i . k_j and q_i . k_j of row tile w, column tiles up to it
+    lq_f4 kk[4], qk[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        kk[j] = qk[j] = lq_f4{0, 0, 0, 0};
+        if (j <= w) {
+            lq_f4 a[2] = {}, c[2] = {};
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                dr_u4 x[NP], y[NP];
+#pragma unroll
+                for (int i = 0; i < NP; ++i) {
+                    x[i] = ks[w][s][i][lane];
+                    y[i] = ks[j][s][i][lane];
+                }
+                dr_product<NP, NP>(x, y, a);
+                dr_product<NP, NP>(qf[s], y, c);
+            }
+            kk[j] = a[0] + a[1];
+            qk[j] = c[0] + c[1];
+        }
+    }
+    const int group = p.value_heads / p.key_heads;
+    const int g0 = gridDim.y > 1 ? blockIdx.y : 0, g1 = gridDim.y > 1 ? g0 + 1 : group;
+    for (int gi = g0; gi < g1; ++gi) {
+        const int h = p.tiled ? gi * p.key_heads + kh : kh * group + gi;
+        const int64_t at = (int64_t)local * p.value_heads + h;
+        // gates, one token a lane (each wave for itself)
+        float2 gb = lane < n ? rule_gates(p, row0 + lane, h) : make_float2(0, 0);
+        // (a state that grows by itself would make T' grow to what the piece's sums cancel)
+        bool odd = wild || !(gb.y >= 0.0f && gb.y * kn[lane] <= 2.1f && gb.y <= 1e3f) || !(gb.x <= 0.3f);
+        double total = gb.x < -1e4f ? -1e4 : (double)gb.x;     // (e^-1e4 is 0; -inf less -inf would be NaN)
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const double up = __shfl_up(total, d, 64);
+            if (lane >= d) total += up;
+        }
+        // values of v that the piece's columns will meet: one column of a row a lane and pass
+        {
+            const T *vr = (const T *)p.v + row0 * p.v_ts + h * p.v_hs;
+            for (int i = (int)threadIdx.x; i < n * (p.vd / 4); i += 256) {
+                const float4 v = delta_load4(vr + (int64_t)(i / (p.vd / 4)) * p.v_ts + i % (p.vd / 4) * 4);
+                odd |= !(fabsf(v.x) <= RULE_WILD && fabsf(v.y) <= RULE_WILD && fabsf(v.z) <= RULE_WILD &&
+                         fabsf(v.w) <= RULE_WILD);
+            }
+        }
+        const bool any = __any(odd);
+        if (lane == 0) wild_s[w] = any;
+        if (w == 0) {
+            gs[lane] = total;
+            bs[lane] = gb.y;
+        }
+        __syncthreads();
+        const bool bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3];
+        if (w == 0) {
+            const float last = (float)gs[63], x = (float)total;
+            float *rows = ws.rows + at * 4 * PIECE;
+            rows[lane] = expf(x) * ik[lane];
+            rows[PIECE + lane] = expf(x) * iq[lane] * p.scale;
+            rows[2 * PIECE + lane] = expf((float)(gs[63] - total)) * ik[lane];
+            if (lane < 2) rows[3 * PIECE + lane] = lane ? (bad ? 1.0f : 0.0f) : expf(last);
+        }
+        if (bad) {      // nothing else of it is read
+            __syncthreads();
+            continue;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j > w) continue;
+            const int col = 16 * j + m;
+            const double gc = gs[col];
+            const float ikc = ik[col];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = 16 * w + 4 * g + e;
+                const float f = row >= col ? expf((float)(gs[row] - gc)) * ikc : 0.0f;
+                am[row][col] = row > col ? f * (bs[row] * ik[row]) * kk[j][e] : 0.0f;
+                tm[row][col] = row >= col ? f * (iq[row] * p.scale) * qk[j][e] : 0.0f;
+            }
+        }
+        __syncthreads();
+        // P's operands of row tile w (columns behind the tile's last are zero)
+        const auto give = [&](dr_u4 *dst, bool scaled) {
+            const int base = w == 0 ? 0 : w == 1 ? 1 : w == 2 ? 2 : 4;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (s > w / 2) continue;
+                float x[8];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int col = 32 * s + 16 * u + 4 * g;
+                    const float4 v = *reinterpret_cast<const float4 *>(&tm[16 * w + m][col]);
+                    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        x[4 * u + i] = 2 * s + u <= w ? scaled ? e[i] * bs[col + i] : e[i] : 0.0f;
+                }
+                dr_u4 y[3];
+                dr_split8<3>(x, y);
+#pragma unroll
+                for (int i = 0; i < 3; ++i) dst[((base + s) * 3 + i) * 64 + lane] = y[i];
+            }
+        };
+        give(ws.p + at * TRI * 3 * 64, false);
+        // the inverse of I + A: its diagonal block w, column m, by forward substitution
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float a0 = i == m ? 1.0f : 0.0f, a1 = 0.0f;
+#pragma unroll
+            for (int q4 = 0; q4 < (i + 3) / 4; ++q4) {
+                const float4 v = *reinterpret_cast<const float4 *>(&am[16 * w + i][16 * w + 4 * q4]);
+                const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (4 * q4 + u < i) (u & 1 ? a1 : a0) -= e[u] * x[4 * q4 + u];
+            }
+            x[i] = a0 + a1;
+        }
+        __syncthreads();     // P has been read
+        if (g == 0)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) tm[16 * w + i][16 * w + m] = x[i];
+        __syncthreads();
+        // blocks below it, of column tile w: T_iw = -T_ii (sum_u A_iu T_uw)
+        {
+            lq_f4 col[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) col[0][e] = tm[16 * w + 4 * g + e][16 * w + m];
+#pragma unroll
+            for (int i = 1; i < 4; ++i) {
+                if (w + i > 3) continue;
+                const int row = 16 * (w + i) + m;
+                lq_f4 sum = {0, 0, 0, 0}, res = {0, 0, 0, 0};
+#pragma unroll
+                for (int u = 0; u < i; ++u) {
+                    const float4 v = *reinterpret_cast<const float4 *>(&am[row][16 * (w + u) + 4 * g]);
+                    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) sum = __builtin_amdgcn_mfma_f32_16x16x4f32(e[c], col[u][c], sum, 0, 0, 0);
+                }
+                const float4 v = *reinterpret_cast<const float4 *>(&tm[row][16 * (w + i) + 4 * g]);
+                const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) res = __builtin_amdgcn_mfma_f32_16x16x4f32(e[c], sum[c], res, 0, 0, 0);
+                col[i] = -res;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tm[16 * (w + i) + 4 * g + c][16 * w + m] = col[i][c];
+            }
+        }
+        __syncthreads();
+        give(ws.t + at * TRI * 3 * 64, true);
+        __syncthreads();
+    }
+}
+
+// A workgroup carries 16 value columns of one head through a request's pieces of
+// the window. Wave w owns tokens 16 w .. + 15 of a piece and key values KD / 4 w
+// .. of S; operands that others made go through LDS: S, R = V - diag(e^G) K^ S,
+// D, and D scaled for S's sum.
+template <typename T, int KD>
+__global__ __launch_bounds__(256) void delta_chain_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
+    constexpr int NP = RuleType<T>::NP, NS = KD / 32, NT = KD / 64;
+    __shared__ __align__(16) dr_u4 ss[NS][3][64], rs[2][3][64], ds[2][3][64], us[2][3][64];
+    __shared__ float red[2][4][2][16], kq[2][2][KD];
+    __shared__ int wild_s[4];
+    const int group = p.value_heads / p.key_heads, slices = p.vd / 16;
+    // a key head's workgroups on one XCD: they read the same operands
+    const int xcd = blockIdx.x & 7, in = blockIdx.x >> 3, unit = in / (group * slices) * 8 + xcd, rest = in % (group * slices);
+    if (unit >= r.requests * p.key_heads) return;
+    const int b = unit / p.key_heads, kh = unit % p.key_heads, gi = rest / slices, c0 = rest % slices * 16;
+    const DeltaSpan span = delta_span(r, b);
+    if (!span.count || span.count < ws.least) return;
+    const int base = span.first / PIECE + b, pieces = (span.count + PIECE - 1) / PIECE;
+    const int from = max(ws.first - base, 0), to = min(ws.first + ws.pieces - base, pieces);
+    if (from >= to) return;
+    const int w = wave_id(), lane = lane_id(), m = lane & 15, g = lane >> 4;
+    const int h = p.tiled ? gi * p.key_heads + kh : kh * group + gi;
+    float *state = r.state + ((span.slot * p.value_heads + h) * KD + w * NT * 16) * p.vd + c0 + m;
+    lq_f4 S[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            S[t][e] = from == 0 && span.fresh ? 0.0f : state[(int64_t)(16 * t + 4 * g + e) * p.vd];
+    // S as operand, and whether its products stay in range
+    const auto share = [&]() {
+        bool odd = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            dr_u2 y[3];
+            dr_split4(S[t], y);
+            const int tile = w * NT + t;
+#pragma unroll
+            for (int i = 0; i < 3; ++i) reinterpret_cast<dr_u2 *>(&ss[tile >> 1][i][lane])[tile & 1] = y[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) odd |= !(fabsf(S[t][e]) <= RULE_WILD * RULE_WILD);
+        }
+        const bool any = __any(odd);
+        if (lane == 0) wild_s[w] = any;
+    };
+    const auto put = [&](dr_u4 (&dst)[2][3][64], const lq_f4 &x) {
+        dr_u2 y[3];
+        dr_split4(x, y);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) reinterpret_cast<dr_u2 *>(&dst[w >> 1][i][lane])[w & 1] = y[i];
+    };
+    // the wave's rows of a lower triangular operand times what LDS holds
+    const int tri = w == 0 ? 0 : w == 1 ? 1 : w == 2 ? 2 : 4;
+    share();
+    __syncthreads();
+    for (int j = from; j < to; ++j) {
+        const int local = base + j - ws.first, n = min(span.count - j * PIECE, PIECE);
+        const int64_t row0 = (int64_t)span.first + j * PIECE;
+        const int64_t at = (int64_t)local * p.value_heads + h, kat = (int64_t)local * p.key_heads + kh;
+        const float *rows = ws.rows + at * 4 * PIECE;
+        const bool bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3] | (rows[3 * PIECE + 1] != 0.0f);
+        if (__builtin_amdgcn_readfirstlane(bad)) {
+            // token by token, as delta_token_kernel
+            const T *kp = (const T *)p.k + row0 * p.k_ts + kh * p.k_hs, *qp = (const T *)p.q + row0 * p.q_ts + kh * p.q_hs;
+            for (int t = 0; t < n; ++t) {
+                const int par = t & 1;
+                constexpr int E = KD / 64;
+                float kk = 0.0f, qq = 0.0f, kdq = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float kv = (float)kp[t * p.k_ts + lane * E + e], qv = (float)qp[t * p.q_ts + lane * E + e];
+                    if (w == 0) kq[par][0][lane * E + e] = kv;
+                    if (w == 1) kq[par][1][lane * E + e] = qv;
+                    kk += kv * kv;
+                    qq += qv * qv;
+                    kdq += kv * qv;
+                }
+                kk = group_sum<64>(kk);
+                qq = group_sum<64>(qq);
+                kdq = group_sum<64>(kdq);
+                const float nk = p.norm_eps >= 0.0f ? 1.0f / sqrtf(kk + p.norm_eps) : 1.0f;
+                const float nq = (p.norm_eps >= 0.0f ? 1.0f / sqrtf(qq + p.norm_eps) : 1.0f) * p.scale;
+                const float2 gb = rule_gates(p, row0 + t, h);
+                const float f = expf(gb.x);
+                const float v = (float)((const T *)p.v)[(row0 + t) * p.v_ts + h * p.v_hs + c0 + m];
+                __syncthreads();
+                float pk = 0.0f, pq = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int row = (w * NT + i) * 16 + 4 * g + e;
+                        S[i][e] *= f;
+                        pk += S[i][e] * kq[par][0][row];
+                        pq += S[i][e] * kq[par][1][row];
+                    }
+                pk = dr_rows_sum(pk);
+                pq = dr_rows_sum(pq);
+                if (g == 0) {
+                    red[par][w][0][m] = pk;
+                    red[par][w][1][m] = pq;
+                }
+                __syncthreads();
+                pk = (red[par][0][0][m] + red[par][1][0][m]) + (red[par][2][0][m] + red[par][3][0][m]);
+                pq = (red[par][0][1][m] + red[par][1][1][m]) + (red[par][2][1][m] + red[par][3][1][m]);
+                const float d = (v - pk * nk) * gb.y;
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) S[i][e] += kq[par][0][(w * NT + i) * 16 + 4 * g + e] * nk * d;
+                if (threadIdx.x < 16)
+                    ((T *)p.out)[(row0 + t) * p.o_ts + h * p.o_hs + c0 + m] = (T)(pq * nq + d * (kdq * nk * nq));
+            }
+            __syncthreads();
+            share();
+            __syncthreads();
+            continue;
+        }
+        const dr_u4 *ko = ws.k + (kat * 4 + w) * NS * NP * 64 + lane, *qo = ws.q + (kat * 4 + w) * NS * NP * 64 + lane;
+        lq_f4 kS[2] = {}, qS[2] = {};
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            dr_u4 x[NP], y[NP], z[3];
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                x[i] = ko[(s * NP + i) * 64];
+                y[i] = qo[(s * NP + i) * 64];
+            }
+#pragma unroll
+            for (int i = 0; i < 3; ++i) z[i] = ss[s][i][lane];
+            dr_product<NP, 3>(x, z, kS);
+            dr_product<NP, 3>(y, z, qS);
+        }
+        // rows 16 w + 4 g + 0..3
+        const float4 cf = *reinterpret_cast<const float4 *>(rows + 16 * w + 4 * g);
+        const float4 of = *reinterpret_cast<const float4 *>(rows + PIECE + 16 * w + 4 * g);
+        const float4 sf = *reinterpret_cast<const float4 *>(rows + 2 * PIECE + 16 * w + 4 * g);
+        const float last = rows[3 * PIECE];
+        const float cv[4] = {cf.x, cf.y, cf.z, cf.w}, ov[4] = {of.x, of.y, of.z, of.w}, sv[4] = {sf.x, sf.y, sf.z, sf.w};
+        lq_f4 R, O[2] = {};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = 16 * w + 4 * g + e;
+            const float v = row < n ? (float)((const T *)p.v)[(row0 + row) * p.v_ts + h * p.v_hs + c0 + m] : 0.0f;
+            R[e] = v - cv[e] * (kS[0][e] + kS[1][e]);
+            O[0][e] = ov[e] * (qS[0][e] + qS[1][e]);
+        }
+        put(rs, R);
+        __syncthreads();
+        const auto lower = [&](const dr_u4 *op, const dr_u4 (&src)[2][3][64], lq_f4 (&c)[2]) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (s > w / 2) continue;
+                dr_u4 x[3], y[3];
+#pragma unroll
+                for (int i = 0; i < 3; ++i) {
+                    x[i] = op[((tri + s) * 3 + i) * 64 + lane];
+                    y[i] = src[s][i][lane];
+                }
+                dr_product<3, 3>(x, y, c);
+            }
+        };
+        lq_f4 D[2] = {};
+        lower(ws.t + at * TRI * 3 * 64, rs, D);
+        D[0] = D[0] + D[1];
+        put(ds, D[0]);
+        lq_f4 U;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) U[e] = D[0][e] * sv[e];
+        put(us, U);
+        __syncthreads();
+        const dr_u4 *kto = ws.kt + kat * (KD / 16) * 2 * NP * 64 + lane;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            lq_f4 c[2] = {};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[0][e] = last * S[t][e];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                dr_u4 x[NP], y[3];
+#pragma unroll
+                for (int i = 0; i < NP; ++i) x[i] = kto[(((w * NT + t) * 2 + s) * NP + i) * 64];
+#pragma unroll
+                for (int i = 0; i < 3; ++i) y[i] = us[s][i][lane];
+                dr_product<NP, 3>(x, y, c);
+            }
+            S[t] = c[0] + c[1];
+        }
+        share();
+        lower(ws.p + at * TRI * 3 * 64, ds, O);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = 16 * w + 4 * g + e;
+            if (row < n) ((T *)p.out)[(row0 + row) * p.o_ts + h * p.o_hs + c0 + m] = (T)(O[0][e] + O[1][e]);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) state[(int64_t)(16 * t + 4 * g + e) * p.vd] = S[t][e];
+}
+
+constexpr int RULE_LEAST = 5;              // tokens of a request below which the token kernel takes it
+constexpr int64_t RULE_WINDOW = 64 << 20;  // bytes of workspace that a window of pieces may fill
+
+static int64_t piece_bytes(int np, int key_heads, int value_heads, int kd) {
+    return (int64_t)key_heads * 3 * 2 * PIECE * kd * np + (int64_t)value_heads * (2 * TRI * 3 * 1024 + 4 * PIECE * 4);
+}
+// pieces of a call, and of a window
+static int64_t all_pieces(int64_t tokens, int requests) { return tokens / PIECE + requests; }
+static int64_t window_pieces(int64_t all, int64_t bytes) {
+    const int64_t most = RULE_WINDOW / bytes;
+    return all < most ? all : most > 1 ? most : 1;
+}
+
 int64_t delta_rule_workspace_bytes(int64_t tokens, int requests, bool step, int key_heads, int value_heads, int kd,
                                    int vd) {
-    return 0;
+    if (step) return 0;
+    const int64_t bytes = piece_bytes(3, key_heads, value_heads, kd);
+    return window_pieces(all_pieces(tokens, requests), bytes) * bytes;
 }
 
 template <typename T, int KD, int VS>
-static void token_launch(const DeltaRule &p, const DeltaRequests &r, hipStream_t s) {
+static void token_launch(const DeltaRule &p, const DeltaRequests &r, int most, hipStream_t s) {
     const int64_t groups = (int64_t)r.requests * p.value_heads * (p.vd / VS);
-    hipLaunchKernelGGL((delta_token_kernel<T, KD, VS>), dim3((unsigned)groups), dim3(256), 0, s, p, r);
+    hipLaunchKernelGGL((delta_token_kernel<T, KD, VS>), dim3((unsigned)groups), dim3(256), 0, s, p, r, most);
 }
 
 template <typename T, int KD>
-static void token_columns(const DeltaRule &p, const DeltaRequests &r, hipStream_t s) {
+static void token_columns(const DeltaRule &p, const DeltaRequests &r, int most, hipStream_t s) {
     const int64_t all = (int64_t)r.requests * p.value_heads * p.vd;     // value columns of the call
-    if (p.vd % 128 == 0 && all >= 128 * 512) token_launch<T, KD, 128>(p, r, s);
-    else if (p.vd % 64 == 0 && all >= 64 * 512) token_launch<T, KD, 64>(p, r, s);
-    else if (p.vd % 32 == 0 && all >= 32 * 256) token_launch<T, KD, 32>(p, r, s);
-    else token_launch<T, KD, 16>(p, r, s);
+    if (p.vd % 128 == 0 && all >= 128 * 512) token_launch<T, KD, 128>(p, r, most, s);
+    else if (p.vd % 64 == 0 && all >= 64 * 512) token_launch<T, KD, 64>(p, r, most, s);
+    else if (p.vd % 32 == 0 && all >= 32 * 256) token_launch<T, KD, 32>(p, r, most, s);
+    else token_launch<T, KD, 16>(p, r, most, s);
+}
+
+template <typename T, int KD>
+static void rule_launch(const DeltaRule &p, const DeltaRequests &r, void *ws, hipStream_t s) {
+    if (!r.starts) return token_columns<T, KD>(p, r, INT32_MAX, s);
+    constexpr int NP = RuleType<T>::NP;
+    const int64_t bytes = piece_bytes(NP, p.key_heads, p.value_heads, KD), all = all_pieces(r.tokens, r.requests);
+    const int64_t window = window_pieces(all, bytes);
+    RuleWork w{};
+    const int64_t operands = window * p.key_heads * 2 * PIECE * KD * NP, tri = window * p.value_heads * TRI * 3 * 1024;
+    char *at = (char *)ws;
+    w.k = (dr_u4 *)at;
+    w.q = (dr_u4 *)(at + operands);
+    w.kt = (dr_u4 *)(at + 2 * operands);
+    w.t = (dr_u4 *)(at + 3 * operands);
+    w.p = (dr_u4 *)(at + 3 * operands + tri);
+    w.rows = (float *)(at + 3 * operands + 2 * tri);
+    // (one request may also have few tokens: its pieces serve any number)
+    w.least = r.requests > 1 ? RULE_LEAST : 1;
+    if (w.least > 1) token_columns<T, KD>(p, r, w.least - 1, s);
+    const int group = p.value_heads / p.key_heads;
+    for (int64_t first = 0; first < all; first += window) {
+        w.first = (int)first;
+        w.pieces = (int)(all - first < window ? all - first : window);
+        const dim3 grid((unsigned)(w.pieces * p.key_heads), (unsigned)((int64_t)w.pieces * p.key_heads < 512 ? group : 1));
+        hipLaunchKernelGGL((delta_piece_kernel<T, KD>), grid, dim3(256), 0, s, p, r, w);
+        const int64_t units = ((int64_t)r.requests * p.key_heads + 7) / 8 * 8;
+        hipLaunchKernelGGL((delta_chain_kernel<T, KD>), dim3((unsigned)(units * group * (p.vd / 16))), dim3(256), 0, s, p, r,
+                           w);
+    }
 }
 
 template <typename T>
 static int rule_typed(const DeltaRule &p, const DeltaRequests &r, void *ws, hipStream_t s) {
-    if (p.kd == 64) token_columns<T, 64>(p, r, s);
-    else if (p.kd == 128) token_columns<T, 128>(p, r, s);
-    else token_columns<T, 256>(p, r, s);
+    if (p.kd == 64) rule_launch<T, 64>(p, r, ws, s);
+    else if (p.kd == 128) rule_launch<T, 128>(p, r, ws, s);
+    else rule_launch<T, 256>(p, r, ws, s);
     LQ_HIP(hipGetLastError());
     return LOCALAI_OK;
 }
