@@ -231,8 +231,14 @@ __device__ __forceinline__ void dr_product(const dr_u4 (&a)[NA], const dr_u4 (&b
             if (i + j < 3) c[i + j > 0] = dr_mfma(a[i], b[j], c[i + j > 0]);
 }
 
-// A workgroup prepares one piece for one key head and the value heads that read
-// it (blockIdx.y: one of them, where there are few pieces). Wave w owns rows
+// 2^x for fp64 x, to fp32's last bit or so however large x is
+__device__ __forceinline__ float dr_exp2(double x) {
+    const double whole = rint(x);
+    return ldexpf(__builtin_amdgcn_exp2f((float)(x - whole)), (int)fmax(whole, -400.0));
+}
+
+// A workgroup prepares one piece for one value head (blockIdx.y: the value heads
+// of a key head; the first writes the key head's operands). Wave w owns rows
 // 16 w .. 16 w + 15. An operand's lane l holds row or column l & 15 and of each
 // 32 contracted values x the eight 4 (l >> 4) + 0..3 and 16 + 4 (l >> 4) + 0..3:
 // the layout in which MFMA leaves two tiles of results, so those are operands
@@ -240,9 +246,13 @@ __device__ __forceinline__ void dr_product(const dr_u4 (&a)[NA], const dr_u4 (&b
 template <typename T, int KD>
 __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
     constexpr int NP = RuleType<T>::NP, NS = KD / 32, LD = 68;
-    __shared__ __align__(16) dr_u4 ks[4][NS][NP][64];
-    __shared__ __align__(16) float am[PIECE][LD], tm[PIECE][LD];
-    __shared__ double gs[PIECE];
+    // K's operands, then A and P / T
+    constexpr int KS = 4 * NS * NP * 64 * 16, MS = PIECE * LD * 4;
+    __shared__ __align__(16) char space[KS > 2 * MS ? KS : 2 * MS];
+    dr_u4 (&ks)[4][NS][NP][64] = *reinterpret_cast<dr_u4 (*)[4][NS][NP][64]>(space);
+    float (&am)[PIECE][LD] = *reinterpret_cast<float (*)[PIECE][LD]>(space);
+    float (&tm)[PIECE][LD] = *reinterpret_cast<float (*)[PIECE][LD]>(space + MS);
+    __shared__ double gs[PIECE];      // sums of g, in powers of two
     __shared__ float bs[PIECE], ik[PIECE], iq[PIECE], kn[PIECE];
     __shared__ int wild_s[4];
     const int local = (int)(blockIdx.x / p.key_heads), kh = (int)(blockIdx.x % p.key_heads);
@@ -252,14 +262,17 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
     const int j0 = (piece - (span.first / PIECE + b)) * PIECE, n = min(span.count - j0, PIECE);
     if (j0 < 0 || n <= 0 || span.count < ws.least) return;
     const int w = wave_id(), lane = lane_id(), m = lane & 15, g = lane >> 4;
-    const int64_t row0 = (int64_t)span.first + j0;
-    bool wild = false;
+    const int group = p.value_heads / p.key_heads, gi = blockIdx.y;
+    const int h = p.tiled ? gi * p.key_heads + kh : kh * group + gi;
+    const int64_t row0 = (int64_t)span.first + j0, at = (int64_t)local * p.value_heads + h;
     const bool norm = p.norm_eps >= 0.0f;
+    const float2 gb = lane < n ? rule_gates(p, row0 + lane, h) : make_float2(0, 0);     // one token a lane
+    bool wild = false;
     dr_u4 qf[NS][NP];
     {
         const bool in = 16 * w + m < n;
-        const T *rows[2] = {(const T *)p.k + (row0 + (in ? 16 * w + m : 0)) * p.k_ts + kh * p.k_hs,
-                            (const T *)p.q + (row0 + (in ? 16 * w + m : 0)) * p.q_ts + kh * p.q_hs};
+        const int64_t row = row0 + (in ? 16 * w + m : 0);
+        const T *rows[2] = {(const T *)p.k + row * p.k_ts + kh * p.k_hs, (const T *)p.q + row * p.q_ts + kh * p.q_hs};
 #pragma unroll
         for (int o = 0; o < 2; ++o) {
             float x[NS][8], ss = 0.0f, top = 0.0f;
@@ -304,14 +317,29 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
                 for (int i = 0; i < NP; ++i) {
                     if (o) qf[s][i] = y[i];
                     else ks[w][s][i][lane] = y[i];
-                    if (blockIdx.y == 0) dst[(s * NP + i) * 64] = y[i];
+                    if (gi == 0) dst[(s * NP + i) * 64] = y[i];
                 }
             }
         }
     }
+    // sums of g up to each token (e^-1e4 is 0; -inf less -inf would be NaN)
+    double total = (gb.x < -1e4f ? -1e4 : (double)gb.x) * 1.4426950408889634074;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const double up = __shfl_up(total, d, 64);
+        if (lane >= d) total += up;
+    }
+    if (w == 0) {
+        gs[lane] = total;
+        bs[lane] = gb.y;
+    }
+    // (a state that grows by itself would make T' grow to what the piece's sums cancel)
+    wild |= !(gb.y >= 0.0f && gb.y <= 1e3f) || !(gb.x <= 0.3f);
+    if (__any(wild) && lane == 0) wild_s[w] = 1;
+    else if (lane == 0) wild_s[w] = 0;
     __syncthreads();
     // K^T: lane (key value 16 t + m, tokens 4 g + 0..3 and 16 + 4 g + 0..3 of 32)
-    if (blockIdx.y == 0) {
+    if (gi == 0) {
         dr_u4 *dst = ws.kt + ((int64_t)local * p.key_heads + kh) * (KD / 16) * 2 * NP * 64 + lane;
 #pragma unroll
         for (int i = 0; i < KD / 64; ++i) {
@@ -320,19 +348,29 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int pc = 0; pc < NP; ++pc) {
-                    uint16_t h[8];
+                    uint16_t y[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const int token = 32 * s + 16 * (e >> 2) + 4 * g + (e & 3);
                         const uint16_t *src = reinterpret_cast<const uint16_t *>(&ks[token >> 4][t >> 1][pc][(token & 15) + 16 * (m >> 2)]);
-                        h[e] = src[(m & 3) + 4 * (t & 1)];
+                        y[e] = src[(m & 3) + 4 * (t & 1)];
                     }
-                    dr_u4 y;
-                    __builtin_memcpy(&y, h, 16);
-                    dst[((t * 2 + s) * NP + pc) * 64] = y;
+                    dr_u4 u;
+                    __builtin_memcpy(&u, y, 16);
+                    dst[((t * 2 + s) * NP + pc) * 64] = u;
                 }
         }
     }
+    const double last = gs[63];
+    const bool bad = (wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3]) || __any(!(gb.y * kn[lane] <= 2.1f));
+    if (w == 0) {
+        float *rows = ws.rows + at * 4 * PIECE;
+        rows[lane] = dr_exp2(total) * ik[lane];
+        rows[PIECE + lane] = dr_exp2(total) * iq[lane] * p.scale;
+        rows[2 * PIECE + lane] = dr_exp2(last - total) * ik[lane];
+        if (lane < 2) rows[3 * PIECE + lane] = lane ? (bad ? 1.0f : 0.0f) : dr_exp2(last);
+    }
+    if (bad) return;     // nothing else of it is read
     // k_i . k_j and q_i . k_j of row tile w, column tiles up to it
     lq_f4 kk[4], qk[4];
 #pragma unroll
@@ -355,146 +393,102 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
             qk[j] = c[0] + c[1];
         }
     }
-    const int group = p.value_heads / p.key_heads;
-    const int g0 = gridDim.y > 1 ? blockIdx.y : 0, g1 = gridDim.y > 1 ? g0 + 1 : group;
-    for (int gi = g0; gi < g1; ++gi) {
-        const int h = p.tiled ? gi * p.key_heads + kh : kh * group + gi;
-        const int64_t at = (int64_t)local * p.value_heads + h;
-        // gates, one token a lane (each wave for itself)
-        float2 gb = lane < n ? rule_gates(p, row0 + lane, h) : make_float2(0, 0);
-        // (a state that grows by itself would make T' grow to what the piece's sums cancel)
-        bool odd = wild || !(gb.y >= 0.0f && gb.y * kn[lane] <= 2.1f && gb.y <= 1e3f) || !(gb.x <= 0.3f);
-        double total = gb.x < -1e4f ? -1e4 : (double)gb.x;     // (e^-1e4 is 0; -inf less -inf would be NaN)
+    __syncthreads();     // K's operands have been read
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const double up = __shfl_up(total, d, 64);
-            if (lane >= d) total += up;
+    for (int j = 0; j < 4; ++j) {
+        if (j > w) continue;
+        const int col = 16 * j + m;
+        const double gc = gs[col];
+        const float ikc = ik[col];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = 16 * w + 4 * g + e;
+            const float f = row >= col ? dr_exp2(gs[row] - gc) * ikc : 0.0f;
+            am[row][col] = row > col ? f * (bs[row] * ik[row]) * kk[j][e] : 0.0f;
+            tm[row][col] = row >= col ? f * (iq[row] * p.scale) * qk[j][e] : 0.0f;
         }
-        // values of v that the piece's columns will meet: one column of a row a lane and pass
-        {
-            const T *vr = (const T *)p.v + row0 * p.v_ts + h * p.v_hs;
-            for (int i = (int)threadIdx.x; i < n * (p.vd / 4); i += 256) {
-                const float4 v = delta_load4(vr + (int64_t)(i / (p.vd / 4)) * p.v_ts + i % (p.vd / 4) * 4);
-                odd |= !(fabsf(v.x) <= RULE_WILD && fabsf(v.y) <= RULE_WILD && fabsf(v.z) <= RULE_WILD &&
-                         fabsf(v.w) <= RULE_WILD);
-            }
-        }
-        const bool any = __any(odd);
-        if (lane == 0) wild_s[w] = any;
-        if (w == 0) {
-            gs[lane] = total;
-            bs[lane] = gb.y;
-        }
-        __syncthreads();
-        const bool bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3];
-        if (w == 0) {
-            const float last = (float)gs[63], x = (float)total;
-            float *rows = ws.rows + at * 4 * PIECE;
-            rows[lane] = expf(x) * ik[lane];
-            rows[PIECE + lane] = expf(x) * iq[lane] * p.scale;
-            rows[2 * PIECE + lane] = expf((float)(gs[63] - total)) * ik[lane];
-            if (lane < 2) rows[3 * PIECE + lane] = lane ? (bad ? 1.0f : 0.0f) : expf(last);
-        }
-        if (bad) {      // nothing else of it is read
-            __syncthreads();
-            continue;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j > w) continue;
-            const int col = 16 * j + m;
-            const double gc = gs[col];
-            const float ikc = ik[col];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = 16 * w + 4 * g + e;
-                const float f = row >= col ? expf((float)(gs[row] - gc)) * ikc : 0.0f;
-                am[row][col] = row > col ? f * (bs[row] * ik[row]) * kk[j][e] : 0.0f;
-                tm[row][col] = row >= col ? f * (iq[row] * p.scale) * qk[j][e] : 0.0f;
-            }
-        }
-        __syncthreads();
-        // P's operands of row tile w (columns behind the tile's last are zero)
-        const auto give = [&](dr_u4 *dst, bool scaled) {
-            const int base = w == 0 ? 0 : w == 1 ? 1 : w == 2 ? 2 : 4;
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                if (s > w / 2) continue;
-                float x[8];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int col = 32 * s + 16 * u + 4 * g;
-                    const float4 v = *reinterpret_cast<const float4 *>(&tm[16 * w + m][col]);
-                    const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        x[4 * u + i] = 2 * s + u <= w ? scaled ? e[i] * bs[col + i] : e[i] : 0.0f;
-                }
-                dr_u4 y[3];
-                dr_split8<3>(x, y);
-#pragma unroll
-                for (int i = 0; i < 3; ++i) dst[((base + s) * 3 + i) * 64 + lane] = y[i];
-            }
-        };
-        give(ws.p + at * TRI * 3 * 64, false);
-        // the inverse of I + A: its diagonal block w, column m, by forward substitution
-        float x[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float a0 = i == m ? 1.0f : 0.0f, a1 = 0.0f;
-#pragma unroll
-            for (int q4 = 0; q4 < (i + 3) / 4; ++q4) {
-                const float4 v = *reinterpret_cast<const float4 *>(&am[16 * w + i][16 * w + 4 * q4]);
-                const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (4 * q4 + u < i) (u & 1 ? a1 : a0) -= e[u] * x[4 * q4 + u];
-            }
-            x[i] = a0 + a1;
-        }
-        __syncthreads();     // P has been read
-        if (g == 0)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) tm[16 * w + i][16 * w + m] = x[i];
-        __syncthreads();
-        // blocks below it, of column tile w: T_iw = -T_ii (sum_u A_iu T_uw)
-        {
-            lq_f4 col[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) col[0][e] = tm[16 * w + 4 * g + e][16 * w + m];
-#pragma unroll
-            for (int i = 1; i < 4; ++i) {
-                if (w + i > 3) continue;
-                const int row = 16 * (w + i) + m;
-                lq_f4 sum = {0, 0, 0, 0}, res = {0, 0, 0, 0};
-#pragma unroll
-                for (int u = 0; u < i; ++u) {
-                    const float4 v = *reinterpret_cast<const float4 *>(&am[row][16 * (w + u) + 4 * g]);
-                    const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) sum = __builtin_amdgcn_mfma_f32_16x16x4f32(e[c], col[u][c], sum, 0, 0, 0);
-                }
-                const float4 v = *reinterpret_cast<const float4 *>(&tm[row][16 * (w + i) + 4 * g]);
-                const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) res = __builtin_amdgcn_mfma_f32_16x16x4f32(e[c], sum[c], res, 0, 0, 0);
-                col[i] = -res;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tm[16 * (w + i) + 4 * g + c][16 * w + m] = col[i][c];
-            }
-        }
-        __syncthreads();
-        give(ws.t + at * TRI * 3 * 64, true);
-        __syncthreads();
     }
+    __syncthreads();
+    // the operands of row tile w of a lower triangular matrix (columns behind the tile's last are zero)
+    const auto give = [&](dr_u4 *dst, bool scaled) {
+        const int base = w == 0 ? 0 : w == 1 ? 1 : w == 2 ? 2 : 4;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            if (s > w / 2) continue;
+            float x[8];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int col = 32 * s + 16 * u + 4 * g;
+                const float4 v = *reinterpret_cast<const float4 *>(&tm[16 * w + m][col]);
+                const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    x[4 * u + i] = 2 * s + u <= w ? scaled ? e[i] * bs[col + i] : e[i] : 0.0f;
+            }
+            dr_u4 y[3];
+            dr_split8<3>(x, y);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) dst[((base + s) * 3 + i) * 64 + lane] = y[i];
+        }
+    };
+    give(ws.p + at * TRI * 3 * 64, false);
+    // the inverse of I + A: its diagonal block w, column m, by forward substitution
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float a0 = i == m ? 1.0f : 0.0f, a1 = 0.0f;
+#pragma unroll
+        for (int q4 = 0; q4 < (i + 3) / 4; ++q4) {
+            const float4 v = *reinterpret_cast<const float4 *>(&am[16 * w + i][16 * w + 4 * q4]);
+            const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (4 * q4 + u < i) (u & 1 ? a1 : a0) -= e[u] * x[4 * q4 + u];
+        }
+        x[i] = a0 + a1;
+    }
+    __syncthreads();     // P has been read
+    if (g == 0)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) tm[16 * w + i][16 * w + m] = x[i];
+    __syncthreads();
+    // blocks below it, of column tile w: T_iw = -T_ii (sum_u A_iu T_uw)
+    {
+        lq_f4 col[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) col[0][e] = tm[16 * w + 4 * g + e][16 * w + m];
+#pragma unroll
+        for (int i = 1; i < 4; ++i) {
+            if (w + i > 3) continue;
+            const int row = 16 * (w + i) + m;
+            lq_f4 sum = {0, 0, 0, 0}, res = {0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < i; ++u) {
+                const float4 v = *reinterpret_cast<const float4 *>(&am[row][16 * (w + u) + 4 * g]);
+                const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) sum = __builtin_amdgcn_mfma_f32_16x16x4f32(e[c], col[u][c], sum, 0, 0, 0);
+            }
+            const float4 v = *reinterpret_cast<const float4 *>(&tm[row][16 * (w + i) + 4 * g]);
+            const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) res = __builtin_amdgcn_mfma_f32_16x16x4f32(e[c], sum[c], res, 0, 0, 0);
+            col[i] = -res;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tm[16 * (w + i) + 4 * g + c][16 * w + m] = col[i][c];
+        }
+    }
+    __syncthreads();
+    give(ws.t + at * TRI * 3 * 64, true);
 }
 
 // A workgroup carries 16 value columns of one head through a request's pieces of
 // the window. Wave w owns tokens 16 w .. + 15 of a piece and key values KD / 4 w
 // .. of S; operands that others made go through LDS: S, R = V - diag(e^G) K^ S,
-// D, and D scaled for S's sum.
+// D, and D scaled for S's sum. Each operand of the next piece is requested as
+// soon as this piece's has been used.
 template <typename T, int KD>
-__global__ __launch_bounds__(256) void delta_chain_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
+__global__ __launch_bounds__(256, 1) void delta_chain_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
     constexpr int NP = RuleType<T>::NP, NS = KD / 32, NT = KD / 64;
     __shared__ __align__(16) dr_u4 ss[NS][3][64], rs[2][3][64], ds[2][3][64], us[2][3][64];
     __shared__ float red[2][4][2][16], kq[2][2][KD];
@@ -511,6 +505,61 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(DeltaRule p, DeltaRequ
     if (from >= to) return;
     const int w = wave_id(), lane = lane_id(), m = lane & 15, g = lane >> 4;
     const int h = p.tiled ? gi * p.key_heads + kh : kh * group + gi;
+    const int tri = w == 0 ? 0 : w == 1 ? 1 : w == 2 ? 2 : 4;      // of T' and P: row tile w
+    const int my = 16 * w + 4 * g;                                 // the lane's rows my .. my + 3 of a piece
+    const T *vp = (const T *)p.v + (int64_t)span.first * p.v_ts + h * p.v_hs + c0 + m;
+    T *op = (T *)p.out + (int64_t)span.first * p.o_ts + h * p.o_hs + c0 + m;
+
+    dr_u4 kf[NS][NP], qf[NS][NP], tf[2][3], pf[2][3], ktf[NT][2][NP];
+    float vf[4];
+    float4 cf, of, sf;
+    float2 lf;
+    const auto key = [&](int j) { return (int64_t)(base + j - ws.first) * p.key_heads + kh; };
+    const auto value = [&](int j) { return (int64_t)(base + j - ws.first) * p.value_heads + h; };
+    const auto ask_kq = [&](int j) {
+        const dr_u4 *k = ws.k + (key(j) * 4 + w) * NS * NP * 64 + lane, *q = ws.q + (key(j) * 4 + w) * NS * NP * 64 + lane;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                kf[s][i] = k[(s * NP + i) * 64];
+                qf[s][i] = q[(s * NP + i) * 64];
+            }
+    };
+    const auto ask_rows = [&](int j) {
+        const float *rows = ws.rows + value(j) * 4 * PIECE;
+        cf = *reinterpret_cast<const float4 *>(rows + my);
+        of = *reinterpret_cast<const float4 *>(rows + PIECE + my);
+        const int n = span.count - j * PIECE;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            vf[e] = my + e < n ? (float)vp[(int64_t)(j * PIECE + my + e) * p.v_ts] : 0.0f;
+    };
+    const auto ask_lower = [&](const dr_u4 *op4, dr_u4 (&x)[2][3]) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+            if (s <= w / 2)
+#pragma unroll
+                for (int i = 0; i < 3; ++i) x[s][i] = op4[((tri + s) * 3 + i) * 64 + lane];
+    };
+    const auto ask_kt = [&](int j) {
+        const dr_u4 *k = ws.kt + (key(j) * (KD / 16) + w * NT) * 2 * NP * 64 + lane;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < NP; ++i) ktf[t][s][i] = k[((t * 2 + s) * NP + i) * 64];
+        const float *rows = ws.rows + value(j) * 4 * PIECE;
+        sf = *reinterpret_cast<const float4 *>(rows + 2 * PIECE + my);
+        lf = *reinterpret_cast<const float2 *>(rows + 3 * PIECE);
+    };
+    ask_kq(from);
+    ask_rows(from);
+    ask_lower(ws.t + value(from) * TRI * 3 * 64, tf);
+    ask_kt(from);
+    ask_lower(ws.p + value(from) * TRI * 3 * 64, pf);
+
     float *state = r.state + ((span.slot * p.value_heads + h) * KD + w * NT * 16) * p.vd + c0 + m;
     lq_f4 S[NT];
 #pragma unroll
@@ -518,9 +567,7 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(DeltaRule p, DeltaRequ
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             S[t][e] = from == 0 && span.fresh ? 0.0f : state[(int64_t)(16 * t + 4 * g + e) * p.vd];
-    // S as operand, and whether its products stay in range
     const auto share = [&]() {
-        bool odd = false;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             dr_u2 y[3];
@@ -528,11 +575,7 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(DeltaRule p, DeltaRequ
             const int tile = w * NT + t;
 #pragma unroll
             for (int i = 0; i < 3; ++i) reinterpret_cast<dr_u2 *>(&ss[tile >> 1][i][lane])[tile & 1] = y[i];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) odd |= !(fabsf(S[t][e]) <= RULE_WILD * RULE_WILD);
         }
-        const bool any = __any(odd);
-        if (lane == 0) wild_s[w] = any;
     };
     const auto put = [&](dr_u4 (&dst)[2][3][64], const lq_f4 &x) {
         dr_u2 y[3];
@@ -540,18 +583,49 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(DeltaRule p, DeltaRequ
 #pragma unroll
         for (int i = 0; i < 3; ++i) reinterpret_cast<dr_u2 *>(&dst[w >> 1][i][lane])[w & 1] = y[i];
     };
-    // the wave's rows of a lower triangular operand times what LDS holds
-    const int tri = w == 0 ? 0 : w == 1 ? 1 : w == 2 ? 2 : 4;
+    // row tile w of a lower triangular operand times what LDS holds
+    const auto lower = [&](const dr_u4 (&x)[2][3], const dr_u4 (&src)[2][3][64], lq_f4 (&c)[2]) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+            if (s <= w / 2) {
+                dr_u4 y[3];
+#pragma unroll
+                for (int i = 0; i < 3; ++i) y[i] = src[s][i][lane];
+                dr_product<3, 3>(x[s], y, c);
+            }
+    };
     share();
     __syncthreads();
     for (int j = from; j < to; ++j) {
-        const int local = base + j - ws.first, n = min(span.count - j * PIECE, PIECE);
-        const int64_t row0 = (int64_t)span.first + j * PIECE;
-        const int64_t at = (int64_t)local * p.value_heads + h, kat = (int64_t)local * p.key_heads + kh;
-        const float *rows = ws.rows + at * 4 * PIECE;
-        const bool bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3] | (rows[3 * PIECE + 1] != 0.0f);
-        if (__builtin_amdgcn_readfirstlane(bad)) {
+        const int n = min(span.count - j * PIECE, PIECE), next = min(j + 1, to - 1);
+        lq_f4 kS[2] = {}, qS[2] = {};
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            dr_u4 z[3];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) z[i] = ss[s][i][lane];
+            dr_product<NP, 3>(kf[s], z, kS);
+            dr_product<NP, 3>(qf[s], z, qS);
+        }
+        ask_kq(next);
+        const float cv[4] = {cf.x, cf.y, cf.z, cf.w}, ov[4] = {of.x, of.y, of.z, of.w};
+        lq_f4 R, O[2] = {};
+        bool odd = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            R[e] = vf[e] - cv[e] * (kS[0][e] + kS[1][e]);
+            O[0][e] = ov[e] * (qS[0][e] + qS[1][e]);
+            odd |= !(fabsf(R[e]) <= RULE_WILD * RULE_WILD);     // v, or S, whose products with k are in it
+        }
+        put(rs, R);
+        odd |= lf.y != 0.0f;
+        const bool any = __any(odd);
+        if (lane == 0) wild_s[w] = any;
+        ask_rows(next);
+        __syncthreads();
+        if (__builtin_amdgcn_readfirstlane(wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3])) {
             // token by token, as delta_token_kernel
+            const int64_t row0 = (int64_t)span.first + j * PIECE;
             const T *kp = (const T *)p.k + row0 * p.k_ts + kh * p.k_hs, *qp = (const T *)p.q + row0 * p.q_ts + kh * p.q_hs;
             for (int t = 0; t < n; ++t) {
                 const int par = t & 1;
@@ -572,8 +646,7 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(DeltaRule p, DeltaRequ
                 const float nk = p.norm_eps >= 0.0f ? 1.0f / sqrtf(kk + p.norm_eps) : 1.0f;
                 const float nq = (p.norm_eps >= 0.0f ? 1.0f / sqrtf(qq + p.norm_eps) : 1.0f) * p.scale;
                 const float2 gb = rule_gates(p, row0 + t, h);
-                const float f = expf(gb.x);
-                const float v = (float)((const T *)p.v)[(row0 + t) * p.v_ts + h * p.v_hs + c0 + m];
+                const float f = expf(gb.x), v = (float)vp[(int64_t)(j * PIECE + t) * p.v_ts];
                 __syncthreads();
                 float pk = 0.0f, pq = 0.0f;
 #pragma unroll
@@ -600,90 +673,46 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(DeltaRule p, DeltaRequ
 #pragma unroll
                     for (int e = 0; e < 4; ++e) S[i][e] += kq[par][0][(w * NT + i) * 16 + 4 * g + e] * nk * d;
                 if (threadIdx.x < 16)
-                    ((T *)p.out)[(row0 + t) * p.o_ts + h * p.o_hs + c0 + m] = (T)(pq * nq + d * (kdq * nk * nq));
+                    op[(int64_t)(j * PIECE + t) * p.o_ts] = (T)(pq * nq + d * (kdq * nk * nq));
             }
-            __syncthreads();
             share();
+            ask_lower(ws.t + value(next) * TRI * 3 * 64, tf);
+            ask_kt(next);
+            ask_lower(ws.p + value(next) * TRI * 3 * 64, pf);
             __syncthreads();
             continue;
         }
-        const dr_u4 *ko = ws.k + (kat * 4 + w) * NS * NP * 64 + lane, *qo = ws.q + (kat * 4 + w) * NS * NP * 64 + lane;
-        lq_f4 kS[2] = {}, qS[2] = {};
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            dr_u4 x[NP], y[NP], z[3];
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                x[i] = ko[(s * NP + i) * 64];
-                y[i] = qo[(s * NP + i) * 64];
-            }
-#pragma unroll
-            for (int i = 0; i < 3; ++i) z[i] = ss[s][i][lane];
-            dr_product<NP, 3>(x, z, kS);
-            dr_product<NP, 3>(y, z, qS);
-        }
-        // rows 16 w + 4 g + 0..3
-        const float4 cf = *reinterpret_cast<const float4 *>(rows + 16 * w + 4 * g);
-        const float4 of = *reinterpret_cast<const float4 *>(rows + PIECE + 16 * w + 4 * g);
-        const float4 sf = *reinterpret_cast<const float4 *>(rows + 2 * PIECE + 16 * w + 4 * g);
-        const float last = rows[3 * PIECE];
-        const float cv[4] = {cf.x, cf.y, cf.z, cf.w}, ov[4] = {of.x, of.y, of.z, of.w}, sv[4] = {sf.x, sf.y, sf.z, sf.w};
-        lq_f4 R, O[2] = {};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int row = 16 * w + 4 * g + e;
-            const float v = row < n ? (float)((const T *)p.v)[(row0 + row) * p.v_ts + h * p.v_hs + c0 + m] : 0.0f;
-            R[e] = v - cv[e] * (kS[0][e] + kS[1][e]);
-            O[0][e] = ov[e] * (qS[0][e] + qS[1][e]);
-        }
-        put(rs, R);
-        __syncthreads();
-        const auto lower = [&](const dr_u4 *op, const dr_u4 (&src)[2][3][64], lq_f4 (&c)[2]) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                if (s > w / 2) continue;
-                dr_u4 x[3], y[3];
-#pragma unroll
-                for (int i = 0; i < 3; ++i) {
-                    x[i] = op[((tri + s) * 3 + i) * 64 + lane];
-                    y[i] = src[s][i][lane];
-                }
-                dr_product<3, 3>(x, y, c);
-            }
-        };
-        lq_f4 D[2] = {};
-        lower(ws.t + at * TRI * 3 * 64, rs, D);
+        lq_f4 D[2] = {}, U;
+        lower(tf, rs, D);
+        ask_lower(ws.t + value(next) * TRI * 3 * 64, tf);
         D[0] = D[0] + D[1];
         put(ds, D[0]);
-        lq_f4 U;
+        const float sv[4] = {sf.x, sf.y, sf.z, sf.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) U[e] = D[0][e] * sv[e];
         put(us, U);
         __syncthreads();
-        const dr_u4 *kto = ws.kt + kat * (KD / 16) * 2 * NP * 64 + lane;
+        dr_u4 y[2][3];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < 3; ++i) y[s][i] = us[s][i][lane];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             lq_f4 c[2] = {};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) c[0][e] = last * S[t][e];
+            for (int e = 0; e < 4; ++e) c[0][e] = lf.x * S[t][e];
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                dr_u4 x[NP], y[3];
-#pragma unroll
-                for (int i = 0; i < NP; ++i) x[i] = kto[(((w * NT + t) * 2 + s) * NP + i) * 64];
-#pragma unroll
-                for (int i = 0; i < 3; ++i) y[i] = us[s][i][lane];
-                dr_product<NP, 3>(x, y, c);
-            }
+            for (int s = 0; s < 2; ++s) dr_product<NP, 3>(ktf[t][s], y[s], c);
             S[t] = c[0] + c[1];
         }
+        ask_kt(next);
         share();
-        lower(ws.p + at * TRI * 3 * 64, ds, O);
+        lower(pf, ds, O);
+        ask_lower(ws.p + value(next) * TRI * 3 * 64, pf);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int row = 16 * w + 4 * g + e;
-            if (row < n) ((T *)p.out)[(row0 + row) * p.o_ts + h * p.o_hs + c0 + m] = (T)(O[0][e] + O[1][e]);
-        }
+        for (int e = 0; e < 4; ++e)
+            if (my + e < n) op[(int64_t)(j * PIECE + my + e) * p.o_ts] = (T)(O[0][e] + O[1][e]);
         __syncthreads();
     }
 #pragma unroll
@@ -749,7 +778,7 @@ static void rule_launch(const DeltaRule &p, const DeltaRequests &r, void *ws, hi
     for (int64_t first = 0; first < all; first += window) {
         w.first = (int)first;
         w.pieces = (int)(all - first < window ? all - first : window);
-        const dim3 grid((unsigned)(w.pieces * p.key_heads), (unsigned)((int64_t)w.pieces * p.key_heads < 512 ? group : 1));
+        const dim3 grid((unsigned)(w.pieces * p.key_heads), (unsigned)group);
         hipLaunchKernelGGL((delta_piece_kernel<T, KD>), grid, dim3(256), 0, s, p, r, w);
         const int64_t units = ((int64_t)r.requests * p.key_heads + 7) / 8 * 8;
         hipLaunchKernelGGL((delta_chain_kernel<T, KD>), dim3((unsigned)(units * group * (p.vd / 16))), dim3(256), 0, s, p, r,
