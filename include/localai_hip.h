@@ -433,7 +433,8 @@ int64_t localai_hip_delta_rule_workspace_size(int64_t tokens, int64_t requests, 
  * q, k [tokens, key_heads, key_dim], v, out [tokens, value_heads, value_dim] of
  * type 0 fp32, 1 fp16 or 30 bf16; decay, beta [tokens, value_heads], a, dt_bias
  * [value_heads] fp32. strides[0..9] (host array, in values): token and head
- * stride of q, k, v, out (multiples of 4), token stride of decay and beta.
+ * stride of q, k, v, out (multiples of 4; tokens' of v and out below 2^22), token
+ * stride of decay and beta.
  * key_dim 64, 128 or 256; value_dim a multiple of 16, at most 1024; q, k, v and
  * out aligned to 4 values, state and workspace to 16 bytes. out shares memory
  * with no other buffer. requests times value_heads times value_dim / 16 below 2^24.

@@ -835,6 +835,9 @@ int localai_hip_delta_rule(const void *q, const void *k, const void *v, int type
     for (int i = 0; i < 10; ++i)
         if (strides[i] < 0 || (i < 8 && strides[i] % 4))
             return fail(LOCALAI_EARG, "delta rule: strides must not be negative, those of q, k, v and out multiples of 4 values");
+    // (offsets within 64 tokens are 32-bit)
+    if (strides[4] >= 1 << 22 || strides[6] >= 1 << 22)
+        return fail(LOCALAI_EARG, "delta rule: token strides of v and out must be below 2^22 values");
     if (rows_overlap(tokens, value_heads, strides[6], strides[7], value_dim))
         return fail(LOCALAI_EARG, "delta rule: rows of out overlap");
     const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
@@ -848,7 +851,7 @@ int localai_hip_delta_rule(const void *q, const void *k, const void *v, int type
     if (need > 0 && (!ws || ws_bytes < need)) return fail(LOCALAI_EARG, "delta rule: workspace too small");
     if (int st = ensure_device()) return st;
     const DeltaRule p{q, k, v, out, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5],
-                      strides[6], strides[7], strides[8], strides[9], decay, beta, a, dt_bias,
+                      tokens > 1 ? strides[6] : value_dim, strides[7], strides[8], strides[9], decay, beta, a, dt_bias,
                       type, key_heads, value_heads, key_dim, value_dim, tiled, norm_eps, scale};
     return launch_delta_rule(p, r, ws, (hipStream_t)stream);
 }

@@ -62,17 +62,15 @@ struct DeltaSpan {
     bool fresh;      // all of the request's tokens are new: it starts from zeros
 };
 __device__ __forceinline__ DeltaSpan delta_span(const DeltaRequests &r, int b) {
-    DeltaSpan d;
-    d.slot = r.slots ? r.slots[b] : b;
+    const auto one = [](int x) { return __builtin_amdgcn_readfirstlane(x); };     // the same for the wave: scalar
+    const int slot = one(r.slots ? r.slots[b] : b);
     int first = b, end = b + 1;
     if (r.starts) {
-        first = min(max(r.starts[b], 0), r.tokens);
-        end = min(max(r.starts[b + 1], first), r.tokens);
+        first = min(max(one(r.starts[b]), 0), r.tokens);
+        end = min(max(one(r.starts[b + 1]), first), r.tokens);
     }
-    d.first = first;
-    d.count = d.slot >= 0 && d.slot < r.n_slots ? end - first : 0;
-    d.fresh = r.lengths && r.lengths[b] <= end - first;
-    return d;
+    return DeltaSpan{first, slot >= 0 && slot < r.n_slots ? end - first : 0, slot,
+                     r.lengths && one(r.lengths[b]) <= end - first};
 }
 
 // Requests cut into pieces of `size` rows: piece j of request b has the number

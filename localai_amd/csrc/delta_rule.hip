@@ -507,58 +507,61 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(DeltaRule p, DeltaR
     const int h = p.tiled ? gi * p.key_heads + kh : kh * group + gi;
     const int tri = w == 0 ? 0 : w == 1 ? 1 : w == 2 ? 2 : 4;      // of T' and P: row tile w
     const int my = 16 * w + 4 * g;                                 // the lane's rows my .. my + 3 of a piece
-    const T *vp = (const T *)p.v + (int64_t)span.first * p.v_ts + h * p.v_hs + c0 + m;
-    T *op = (T *)p.out + (int64_t)span.first * p.o_ts + h * p.o_hs + c0 + m;
+    // what a piece's operands lie at, moved on piece by piece (the same for the whole wave)
+    const int64_t key_step = (int64_t)p.key_heads * 4 * NS * NP * 1024, tri_step = (int64_t)p.value_heads * TRI * 3 * 1024;
+    const int64_t key0 = ((int64_t)(base + from - ws.first) * p.key_heads + kh) * 4 * NS * NP * 1024;
+    const int64_t val0 = (int64_t)(base + from - ws.first) * p.value_heads + h;
+    const char *kb = (const char *)ws.k + key0 + w * NS * NP * 1024, *qb = (const char *)ws.q + key0 + w * NS * NP * 1024;
+    const char *ktb = (const char *)ws.kt + key0 + w * NT * 2 * NP * 1024;
+    const char *tb = (const char *)ws.t + (val0 * TRI + tri) * 3 * 1024, *pb = (const char *)ws.p + (val0 * TRI + tri) * 3 * 1024;
+    const char *rb = (const char *)(ws.rows + val0 * 4 * PIECE);
+    const T *vb = (const T *)p.v + ((int64_t)span.first + from * PIECE) * p.v_ts + h * p.v_hs + c0;
+    T *ob = (T *)p.out + ((int64_t)span.first + from * PIECE) * p.o_ts + h * p.o_hs + c0;
+    const uint32_t lane16 = lane * 16, second = w < 2 ? 0 : 3072;      // (row tiles 0 and 1 have one block: it twice)
+    const int v_ts = (int)p.v_ts, o_ts = (int)p.o_ts;
+    int v_at[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v_at[e] = (my + e) * v_ts + m;
 
+    // Nothing between a request and its use is conditional but the waits stay
+    // exact only so: the compiler counts what is in flight.
     dr_u4 kf[NS][NP], qf[NS][NP], tf[2][3], pf[2][3], ktf[NT][2][NP];
-    float vf[4];
+    T vf[4];
     float4 cf, of, sf;
     float2 lf;
-    const auto key = [&](int j) { return (int64_t)(base + j - ws.first) * p.key_heads + kh; };
-    const auto value = [&](int j) { return (int64_t)(base + j - ws.first) * p.value_heads + h; };
-    const auto ask_kq = [&](int j) {
-        const dr_u4 *k = ws.k + (key(j) * 4 + w) * NS * NP * 64 + lane, *q = ws.q + (key(j) * 4 + w) * NS * NP * 64 + lane;
+    const auto block = [&](const char *at, int i) { return *reinterpret_cast<const dr_u4 *>(at + i * 1024 + lane16); };
+    const auto ask_kq = [&]() {
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
-                kf[s][i] = k[(s * NP + i) * 64];
-                qf[s][i] = q[(s * NP + i) * 64];
+                kf[s][i] = block(kb, s * NP + i);
+                qf[s][i] = block(qb, s * NP + i);
             }
     };
-    const auto ask_rows = [&](int j) {
-        const float *rows = ws.rows + value(j) * 4 * PIECE;
-        cf = *reinterpret_cast<const float4 *>(rows + my);
-        of = *reinterpret_cast<const float4 *>(rows + PIECE + my);
-        const int n = span.count - j * PIECE;
+    const auto ask_rows = [&](int n) {
+        cf = *reinterpret_cast<const float4 *>(rb + 4 * my);
+        of = *reinterpret_cast<const float4 *>(rb + 4 * PIECE + 4 * my);
+        sf = *reinterpret_cast<const float4 *>(rb + 8 * PIECE + 4 * my);
+        lf = *reinterpret_cast<const float2 *>(rb + 12 * PIECE);
+        // (rows behind the last one read the first)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            vf[e] = my + e < n ? (float)vp[(int64_t)(j * PIECE + my + e) * p.v_ts] : 0.0f;
+        for (int e = 0; e < 4; ++e) vf[e] = vb[my + e < n ? v_at[e] : m];
     };
-    const auto ask_lower = [&](const dr_u4 *op4, dr_u4 (&x)[2][3]) {
+    const auto ask_lower = [&](const char *at, dr_u4 (&x)[2][3]) {
 #pragma unroll
         for (int s = 0; s < 2; ++s)
-            if (s <= w / 2)
 #pragma unroll
-                for (int i = 0; i < 3; ++i) x[s][i] = op4[((tri + s) * 3 + i) * 64 + lane];
+            for (int i = 0; i < 3; ++i) x[s][i] = block(at + (s ? second : 0), i);
     };
-    const auto ask_kt = [&](int j) {
-        const dr_u4 *k = ws.kt + (key(j) * (KD / 16) + w * NT) * 2 * NP * 64 + lane;
+    const auto ask_kt = [&]() {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int i = 0; i < NP; ++i) ktf[t][s][i] = k[((t * 2 + s) * NP + i) * 64];
-        const float *rows = ws.rows + value(j) * 4 * PIECE;
-        sf = *reinterpret_cast<const float4 *>(rows + 2 * PIECE + my);
-        lf = *reinterpret_cast<const float2 *>(rows + 3 * PIECE);
+                for (int i = 0; i < NP; ++i) ktf[t][s][i] = block(ktb, (t * 2 + s) * NP + i);
     };
-    ask_kq(from);
-    ask_rows(from);
-    ask_lower(ws.t + value(from) * TRI * 3 * 64, tf);
-    ask_kt(from);
-    ask_lower(ws.p + value(from) * TRI * 3 * 64, pf);
 
     float *state = r.state + ((span.slot * p.value_heads + h) * KD + w * NT * 16) * p.vd + c0 + m;
     lq_f4 S[NT];
@@ -585,134 +588,159 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(DeltaRule p, DeltaR
     };
     // row tile w of a lower triangular operand times what LDS holds
     const auto lower = [&](const dr_u4 (&x)[2][3], const dr_u4 (&src)[2][3][64], lq_f4 (&c)[2]) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-            if (s <= w / 2) {
-                dr_u4 y[3];
-#pragma unroll
-                for (int i = 0; i < 3; ++i) y[i] = src[s][i][lane];
-                dr_product<3, 3>(x[s], y, c);
-            }
-    };
-    share();
-    __syncthreads();
-    for (int j = from; j < to; ++j) {
-        const int n = min(span.count - j * PIECE, PIECE), next = min(j + 1, to - 1);
-        lq_f4 kS[2] = {}, qS[2] = {};
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            dr_u4 z[3];
-#pragma unroll
-            for (int i = 0; i < 3; ++i) z[i] = ss[s][i][lane];
-            dr_product<NP, 3>(kf[s], z, kS);
-            dr_product<NP, 3>(qf[s], z, qS);
-        }
-        ask_kq(next);
-        const float cv[4] = {cf.x, cf.y, cf.z, cf.w}, ov[4] = {of.x, of.y, of.z, of.w};
-        lq_f4 R, O[2] = {};
-        bool odd = false;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            R[e] = vf[e] - cv[e] * (kS[0][e] + kS[1][e]);
-            O[0][e] = ov[e] * (qS[0][e] + qS[1][e]);
-            odd |= !(fabsf(R[e]) <= RULE_WILD * RULE_WILD);     // v, or S, whose products with k are in it
-        }
-        put(rs, R);
-        odd |= lf.y != 0.0f;
-        const bool any = __any(odd);
-        if (lane == 0) wild_s[w] = any;
-        ask_rows(next);
-        __syncthreads();
-        if (__builtin_amdgcn_readfirstlane(wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3])) {
-            // token by token, as delta_token_kernel
-            const int64_t row0 = (int64_t)span.first + j * PIECE;
-            const T *kp = (const T *)p.k + row0 * p.k_ts + kh * p.k_hs, *qp = (const T *)p.q + row0 * p.q_ts + kh * p.q_hs;
-            for (int t = 0; t < n; ++t) {
-                const int par = t & 1;
-                constexpr int E = KD / 64;
-                float kk = 0.0f, qq = 0.0f, kdq = 0.0f;
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float kv = (float)kp[t * p.k_ts + lane * E + e], qv = (float)qp[t * p.q_ts + lane * E + e];
-                    if (w == 0) kq[par][0][lane * E + e] = kv;
-                    if (w == 1) kq[par][1][lane * E + e] = qv;
-                    kk += kv * kv;
-                    qq += qv * qv;
-                    kdq += kv * qv;
-                }
-                kk = group_sum<64>(kk);
-                qq = group_sum<64>(qq);
-                kdq = group_sum<64>(kdq);
-                const float nk = p.norm_eps >= 0.0f ? 1.0f / sqrtf(kk + p.norm_eps) : 1.0f;
-                const float nq = (p.norm_eps >= 0.0f ? 1.0f / sqrtf(qq + p.norm_eps) : 1.0f) * p.scale;
-                const float2 gb = rule_gates(p, row0 + t, h);
-                const float f = expf(gb.x), v = (float)vp[(int64_t)(j * PIECE + t) * p.v_ts];
-                __syncthreads();
-                float pk = 0.0f, pq = 0.0f;
-#pragma unroll
-                for (int i = 0; i < NT; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int row = (w * NT + i) * 16 + 4 * g + e;
-                        S[i][e] *= f;
-                        pk += S[i][e] * kq[par][0][row];
-                        pq += S[i][e] * kq[par][1][row];
-                    }
-                pk = dr_rows_sum(pk);
-                pq = dr_rows_sum(pq);
-                if (g == 0) {
-                    red[par][w][0][m] = pk;
-                    red[par][w][1][m] = pq;
-                }
-                __syncthreads();
-                pk = (red[par][0][0][m] + red[par][1][0][m]) + (red[par][2][0][m] + red[par][3][0][m]);
-                pq = (red[par][0][1][m] + red[par][1][1][m]) + (red[par][2][1][m] + red[par][3][1][m]);
-                const float d = (v - pk * nk) * gb.y;
-#pragma unroll
-                for (int i = 0; i < NT; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) S[i][e] += kq[par][0][(w * NT + i) * 16 + 4 * g + e] * nk * d;
-                if (threadIdx.x < 16)
-                    op[(int64_t)(j * PIECE + t) * p.o_ts] = (T)(pq * nq + d * (kdq * nk * nq));
-            }
-            share();
-            ask_lower(ws.t + value(next) * TRI * 3 * 64, tf);
-            ask_kt(next);
-            ask_lower(ws.p + value(next) * TRI * 3 * 64, pf);
-            __syncthreads();
-            continue;
-        }
-        lq_f4 D[2] = {}, U;
-        lower(tf, rs, D);
-        ask_lower(ws.t + value(next) * TRI * 3 * 64, tf);
-        D[0] = D[0] + D[1];
-        put(ds, D[0]);
-        const float sv[4] = {sf.x, sf.y, sf.z, sf.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) U[e] = D[0][e] * sv[e];
-        put(us, U);
-        __syncthreads();
         dr_u4 y[2][3];
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int i = 0; i < 3; ++i) y[s][i] = us[s][i][lane];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            lq_f4 c[2] = {};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) c[0][e] = lf.x * S[t][e];
-#pragma unroll
-            for (int s = 0; s < 2; ++s) dr_product<NP, 3>(ktf[t][s], y[s], c);
-            S[t] = c[0] + c[1];
-        }
-        ask_kt(next);
+            for (int i = 0; i < 3; ++i) y[s][i] = src[s][i][lane];
+        dr_product<3, 3>(x[0], y[0], c);
+        if (w > 1) dr_product<3, 3>(x[1], y[1], c);
+    };
+    for (int j = from; j < to;) {
+        ask_kq();
+        ask_rows(span.count - j * PIECE);
+        ask_lower(tb, tf);
+        ask_kt();
+        ask_lower(pb, pf);
         share();
-        lower(pf, ds, O);
-        ask_lower(ws.p + value(next) * TRI * 3 * 64, pf);
+        __syncthreads();
+        for (; j < to; ++j) {
+            const int n = min(span.count - j * PIECE, PIECE);
+            const bool more = j + 1 < to;     // the last piece's are asked for again and not used
+            lq_f4 kS[2] = {}, qS[2] = {};
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (my + e < n) op[(int64_t)(j * PIECE + my + e) * p.o_ts] = (T)(O[0][e] + O[1][e]);
+            for (int s = 0; s < NS; ++s) {
+                dr_u4 z[3];
+#pragma unroll
+                for (int i = 0; i < 3; ++i) z[i] = ss[s][i][lane];
+                dr_product<NP, 3>(kf[s], z, kS);
+                dr_product<NP, 3>(qf[s], z, qS);
+            }
+            kb += more ? key_step : 0;
+            qb += more ? key_step : 0;
+            ask_kq();
+            const float cv[4] = {cf.x, cf.y, cf.z, cf.w}, ov[4] = {of.x, of.y, of.z, of.w};
+            lq_f4 R, O[2] = {};
+            bool odd = lf.y != 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                R[e] = (my + e < n ? (float)vf[e] : 0.0f) - cv[e] * (kS[0][e] + kS[1][e]);
+                O[0][e] = ov[e] * (qS[0][e] + qS[1][e]);
+                odd |= !(fabsf(R[e]) <= RULE_WILD * RULE_WILD);     // v, or S, whose products with k are in it
+            }
+            put(rs, R);
+            const bool any = __any(odd);
+            if (lane == 0) wild_s[w] = any;
+            const float last = lf.x;
+            const float sv[4] = {sf.x, sf.y, sf.z, sf.w};
+            vb += more ? PIECE * p.v_ts : 0;
+            rb += more ? (int64_t)p.value_heads * 16 * PIECE : 0;
+            ask_rows(more ? span.count - (j + 1) * PIECE : n);
+            __syncthreads();
+            lq_f4 D[2] = {}, U;
+            lower(tf, rs, D);
+            tb += more ? tri_step : 0;
+            ask_lower(tb, tf);
+            D[0] = D[0] + D[1];
+            put(ds, D[0]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) U[e] = D[0][e] * sv[e];
+            put(us, U);
+            __syncthreads();
+            const int bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3];
+            dr_u4 y[2][3];
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 3; ++i) y[s][i] = us[s][i][lane];
+            if (__builtin_amdgcn_readfirstlane(bad)) break;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                lq_f4 c[2] = {};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[0][e] = last * S[t][e];
+#pragma unroll
+                for (int s = 0; s < 2; ++s) dr_product<NP, 3>(ktf[t][s], y[s], c);
+                S[t] = c[0] + c[1];
+            }
+            ktb += more ? key_step : 0;
+            ask_kt();
+            share();
+            lower(pf, ds, O);
+            pb += more ? tri_step : 0;
+            ask_lower(pb, pf);
+            // (stores past the piece's last row are left out by the bound)
+            const auto dst = __builtin_amdgcn_make_buffer_rsrc(ob, 0, ((n - 1) * o_ts + 16) * (int)sizeof(T), 0x00027000);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const T y1 = (T)(O[0][e] + O[1][e]);
+                const int at = ((my + e) * o_ts + m) * (int)sizeof(T);
+                if constexpr (sizeof(T) == 4)
+                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, y1), dst, at, 0, 0);
+                else
+                    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, y1), dst, at, 0, 0);
+            }
+            ob += PIECE * p.o_ts;
+            __syncthreads();
+        }
+        if (j >= to) break;
+        // token by token, as delta_token_kernel: piece j, with S as it was (what was asked for of the next is asked again)
+        const int n = min(span.count - j * PIECE, PIECE);
+        const int64_t row0 = (int64_t)span.first + j * PIECE;
+        const T *kp = (const T *)p.k + row0 * p.k_ts + kh * p.k_hs, *qp = (const T *)p.q + row0 * p.q_ts + kh * p.q_hs;
+        const T *vp = (const T *)p.v + row0 * p.v_ts + h * p.v_hs + c0 + m;
+        for (int t = 0; t < n; ++t) {
+            const int par = t & 1;
+            constexpr int E = KD / 64;
+            float kk = 0.0f, qq = 0.0f, kdq = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float kv = (float)kp[t * p.k_ts + lane * E + e], qv = (float)qp[t * p.q_ts + lane * E + e];
+                if (w == 0) kq[par][0][lane * E + e] = kv;
+                if (w == 1) kq[par][1][lane * E + e] = qv;
+                kk += kv * kv;
+                qq += qv * qv;
+                kdq += kv * qv;
+            }
+            kk = group_sum<64>(kk);
+            qq = group_sum<64>(qq);
+            kdq = group_sum<64>(kdq);
+            const float nk = p.norm_eps >= 0.0f ? 1.0f / sqrtf(kk + p.norm_eps) : 1.0f;
+            const float nq = (p.norm_eps >= 0.0f ? 1.0f / sqrtf(qq + p.norm_eps) : 1.0f) * p.scale;
+            const float2 gb = rule_gates(p, row0 + t, h);
+            const float f = expf(gb.x), v = (float)vp[t * p.v_ts];
+            __syncthreads();
+            float pk = 0.0f, pq = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int row = (w * NT + i) * 16 + 4 * g + e;
+                    S[i][e] *= f;
+                    pk += S[i][e] * kq[par][0][row];
+                    pq += S[i][e] * kq[par][1][row];
+                }
+            pk = dr_rows_sum(pk);
+            pq = dr_rows_sum(pq);
+            if (g == 0) {
+                red[par][w][0][m] = pk;
+                red[par][w][1][m] = pq;
+            }
+            __syncthreads();
+            pk = (red[par][0][0][m] + red[par][1][0][m]) + (red[par][2][0][m] + red[par][3][0][m]);
+            pq = (red[par][0][1][m] + red[par][1][1][m]) + (red[par][2][1][m] + red[par][3][1][m]);
+            const float d = (v - pk * nk) * gb.y;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) S[i][e] += kq[par][0][(w * NT + i) * 16 + 4 * g + e] * nk * d;
+            if (threadIdx.x < 16) ob[(int64_t)t * p.o_ts + m] = (T)(pq * nq + d * (kdq * nk * nq));
+        }
+        if (++j >= to) break;
+        // T's, V's, K's and the factors' places are the next piece's already
+        ktb += key_step;
+        pb += tri_step;
+        ob += PIECE * p.o_ts;
         __syncthreads();
     }
 #pragma unroll
