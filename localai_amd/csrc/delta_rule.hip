@@ -127,14 +127,14 @@ __global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequ
 //
 // 64 tokens at once. With G_i the sum of g over the piece's tokens up to i, and
 //   A_ij = b_i e^(G_i - G_j) k^_i . k^_j  (j < i)     P_ij = e^(G_i - G_j) q^_i . k^_j  (j <= i)
-// the rows d_i of all tokens solve (I + A) D = diag(b) (V - diag(e^G) K^ S), so
-//   D = T' (V - diag(e^G) K^ S),  T' = (I + A)^-1 diag(b)
-//   O = diag(e^G) Q^ S + P D
-//   S <- e^G_last S + (diag(e^(G_last - G)) K^)^T D
-// What does not depend on S (T', P, the factors, the operands' layout) is one
-// launch over all pieces and heads (delta_piece_kernel); the chain over a
-// request's pieces is a second one, each workgroup with 16 value columns of one
-// head, whose S stays in registers (delta_chain_kernel).
+// the rows d_i of all tokens solve (I + A) D = diag(b) R, R = V - diag(e^G) K^ S, so
+// with T = (I + A)^-1 diag(b)
+//   O = diag(e^G) Q^ S + (P T) R
+//   S <- e^G_last S + K^T U,  U = diag(e^(G_last - G) / |k|) T R
+// What does not depend on S (P T, the scaled T, the factors, the operands'
+// layout) is one launch over all pieces and heads (delta_piece_kernel); the
+// chain over a request's pieces is a second one, each workgroup with 16 value
+// columns of one head, whose S stays in registers (delta_chain_kernel).
 //
 // Precision: everything is fp32's. MFMA takes bf16 operands, so each fp32 value
 // goes in as three bf16 pieces (24 bits), q and k of 16 bits as they are (bf16:
@@ -144,8 +144,8 @@ __global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequ
 // forgets everything. The inverse goes by forward substitution in blocks of 16,
 // whose numbers stay as small as the rule's own.
 // A piece with a number that is not finite, or whose products would leave fp32's
-// range, goes through its tokens one by one instead: NaN times a zero of T' or
-// P would reach tokens before it.
+// range, goes through its tokens one by one instead: NaN times a zero of T or
+// P T would reach tokens before it.
 
 typedef __bf16 dr_b8 __attribute__((ext_vector_type(8)));
 typedef uint32_t dr_u4 __attribute__((ext_vector_type(4)));
@@ -164,8 +164,8 @@ template <> struct RuleType<float> { static constexpr int NP = 3; };
 // workspace of one window of pieces, in 1 KB blocks (64 lanes x 16 bytes: an MFMA operand)
 struct RuleWork {
     dr_u4 *k, *q, *kt;     // [piece, key head][..][np][64]: row tile, step; kt: key tile, step
-    dr_u4 *t, *p;          // [piece, value head][TRI][3][64]
-    float *rows;           // [piece, value head][4][64]: e^G |k|^-1, e^G |q|^-1 scale, e^(G_last - G) |k|^-1; e^G_last, wild
+    dr_u4 *t, *p;          // [piece, value head][TRI][3][64]: scaled T, P T
+    float *rows;           // [piece, value head][3][64]: e^G / |k|, scale e^G / |q|; e^G_last, wild
     int first, pieces;     // the window
     int least;             // requests of fewer tokens are the token kernel's
 };
@@ -207,29 +207,37 @@ __device__ __forceinline__ void dr_split8(const float (&x)[8], dr_u4 (&y)[N]) {
         y[i] = __builtin_bit_cast(dr_u4, v);
     }
 }
+// Three pieces by cutting bits off: exact too, a third fewer instructions, and
+// the pieces one bit larger (the dropped products 2^-25 of the largest instead
+// of 2^-26: the other operand's pieces are the nearest).
 __device__ __forceinline__ void dr_split4(const lq_f4 &x, dr_u2 (&y)[3]) {
-    __bf16 h[4][3];
+    uint32_t h[3][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) dr_split<3>(x[e], h[e]);
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        const __bf16 v[4] = {h[0][i], h[1][i], h[2][i], h[3][i]};
-        __builtin_memcpy(&y[i], v, 8);
+    for (int e = 0; e < 4; ++e) {
+        const float a = x[e], b = a - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, a) & 0xffff0000u);
+        const float c = b - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, b) & 0xffff0000u);
+        h[0][e] = __builtin_bit_cast(uint32_t, a);
+        h[1][e] = __builtin_bit_cast(uint32_t, b);
+        h[2][e] = __builtin_bit_cast(uint32_t, c);
     }
+#pragma unroll
+    for (int i = 0; i < 3; ++i)     // the upper halves of two values
+        y[i] = dr_u2{__builtin_amdgcn_perm(h[i][1], h[i][0], 0x07060302u), __builtin_amdgcn_perm(h[i][3], h[i][2], 0x07060302u)};
 }
 
 __device__ __forceinline__ lq_f4 dr_mfma(const dr_u4 &a, const dr_u4 &b, const lq_f4 &c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dr_b8, a), __builtin_bit_cast(dr_b8, b), c, 0, 0, 0);
 }
-// c[0] += the first pieces' product, c[1] += the others' up to 2^-16 of it (NA, NB: pieces of a and b)
+// c[i] += the products of pieces i apart in size, up to 2^-16 of the largest (NA, NB: pieces of a and b)
 template <int NA, int NB>
-__device__ __forceinline__ void dr_product(const dr_u4 (&a)[NA], const dr_u4 (&b)[NB], lq_f4 (&c)[2]) {
+__device__ __forceinline__ void dr_product(const dr_u4 (&a)[NA], const dr_u4 (&b)[NB], lq_f4 (&c)[3]) {
 #pragma unroll
     for (int i = 0; i < NA; ++i)
 #pragma unroll
         for (int j = 0; j < NB; ++j)
-            if (i + j < 3) c[i + j > 0] = dr_mfma(a[i], b[j], c[i + j > 0]);
+            if (i + j < 3) c[i + j] = dr_mfma(a[i], b[j], c[i + j]);
 }
+__device__ __forceinline__ lq_f4 dr_total(const lq_f4 (&c)[3]) { return c[0] + (c[1] + c[2]); }
 
 // 2^x for fp64 x, to fp32's last bit or so however large x is
 __device__ __forceinline__ float dr_exp2(double x) {
@@ -246,14 +254,14 @@ __device__ __forceinline__ float dr_exp2(double x) {
 template <typename T, int KD>
 __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
     constexpr int NP = RuleType<T>::NP, NS = KD / 32, LD = 68;
-    // K's operands, then A and P / T
+    // K's operands, then A (later P, P T) and T
     constexpr int KS = 4 * NS * NP * 64 * 16, MS = PIECE * LD * 4;
     __shared__ __align__(16) char space[KS > 2 * MS ? KS : 2 * MS];
     dr_u4 (&ks)[4][NS][NP][64] = *reinterpret_cast<dr_u4 (*)[4][NS][NP][64]>(space);
     float (&am)[PIECE][LD] = *reinterpret_cast<float (*)[PIECE][LD]>(space);
     float (&tm)[PIECE][LD] = *reinterpret_cast<float (*)[PIECE][LD]>(space + MS);
     __shared__ double gs[PIECE];      // sums of g, in powers of two
-    __shared__ float bs[PIECE], ik[PIECE], iq[PIECE], kn[PIECE];
+    __shared__ float bs[PIECE], ik[PIECE], iq[PIECE], kn[PIECE], sc[PIECE];
     __shared__ int wild_s[4];
     const int local = (int)(blockIdx.x / p.key_heads), kh = (int)(blockIdx.x % p.key_heads);
     const int piece = ws.first + local, b = delta_request(r, piece, PIECE);
@@ -364,11 +372,11 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
     const double last = gs[63];
     const bool bad = (wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3]) || __any(!(gb.y * kn[lane] <= 2.1f));
     if (w == 0) {
-        float *rows = ws.rows + at * 4 * PIECE;
+        float *rows = ws.rows + at * 3 * PIECE;
         rows[lane] = dr_exp2(total) * ik[lane];
         rows[PIECE + lane] = dr_exp2(total) * iq[lane] * p.scale;
-        rows[2 * PIECE + lane] = dr_exp2(last - total) * ik[lane];
-        if (lane < 2) rows[3 * PIECE + lane] = lane ? (bad ? 1.0f : 0.0f) : dr_exp2(last);
+        if (lane < 2) rows[2 * PIECE + lane] = lane ? (bad ? 1.0f : 0.0f) : dr_exp2(last);
+        sc[lane] = dr_exp2(last - total) * ik[lane];
     }
     if (bad) return;     // nothing else of it is read
     // k_i . k_j and q_i . k_j of row tile w, column tiles up to it
@@ -377,7 +385,7 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
     for (int j = 0; j < 4; ++j) {
         kk[j] = qk[j] = lq_f4{0, 0, 0, 0};
         if (j <= w) {
-            lq_f4 a[2] = {}, c[2] = {};
+            lq_f4 a[3] = {}, c[3] = {};
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
                 dr_u4 x[NP], y[NP];
@@ -389,8 +397,8 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
                 dr_product<NP, NP>(x, y, a);
                 dr_product<NP, NP>(qf[s], y, c);
             }
-            kk[j] = a[0] + a[1];
-            qk[j] = c[0] + c[1];
+            kk[j] = dr_total(a);
+            qk[j] = dr_total(c);
         }
     }
     __syncthreads();     // K's operands have been read
@@ -405,33 +413,10 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
             const int row = 16 * w + 4 * g + e;
             const float f = row >= col ? dr_exp2(gs[row] - gc) * ikc : 0.0f;
             am[row][col] = row > col ? f * (bs[row] * ik[row]) * kk[j][e] : 0.0f;
-            tm[row][col] = row >= col ? f * (iq[row] * p.scale) * qk[j][e] : 0.0f;
+            qk[j][e] = row >= col ? f * (iq[row] * p.scale) * qk[j][e] : 0.0f;
         }
     }
     __syncthreads();
-    // the operands of row tile w of a lower triangular matrix (columns behind the tile's last are zero)
-    const auto give = [&](dr_u4 *dst, bool scaled) {
-        const int base = w == 0 ? 0 : w == 1 ? 1 : w == 2 ? 2 : 4;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            if (s > w / 2) continue;
-            float x[8];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int col = 32 * s + 16 * u + 4 * g;
-                const float4 v = *reinterpret_cast<const float4 *>(&tm[16 * w + m][col]);
-                const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    x[4 * u + i] = 2 * s + u <= w ? scaled ? e[i] * bs[col + i] : e[i] : 0.0f;
-            }
-            dr_u4 y[3];
-            dr_split8<3>(x, y);
-#pragma unroll
-            for (int i = 0; i < 3; ++i) dst[((base + s) * 3 + i) * 64 + lane] = y[i];
-        }
-    };
-    give(ws.p + at * TRI * 3 * 64, false);
     // the inverse of I + A: its diagonal block w, column m, by forward substitution
     float x[16];
 #pragma unroll
@@ -447,7 +432,6 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
         }
         x[i] = a0 + a1;
     }
-    __syncthreads();     // P has been read
     if (g == 0)
 #pragma unroll
         for (int i = 0; i < 16; ++i) tm[16 * w + i][16 * w + m] = x[i];
@@ -479,18 +463,77 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
         }
     }
     __syncthreads();
-    give(ws.t + at * TRI * 3 * 64, true);
+    // the operands of row tile w of a lower triangular matrix (columns behind the tile's last are zero),
+    // its columns times cols, its rows times by
+    const auto give = [&](const float (&src)[PIECE][LD], dr_u4 *dst, const float *cols, float by) {
+        const int base = w == 0 ? 0 : w == 1 ? 1 : w == 2 ? 2 : 4;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            if (s > w / 2) continue;
+            float y8[8];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int col = 32 * s + 16 * u + 4 * g;
+                const float4 v = *reinterpret_cast<const float4 *>(&src[16 * w + m][col]);
+                const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y8[4 * u + i] = 2 * s + u <= w ? e[i] * cols[col + i] * by : 0.0f;
+            }
+            dr_u4 y[3];
+            dr_split8<3>(y8, y);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) dst[((base + s) * 3 + i) * 64 + lane] = y[i];
+        }
+    };
+    give(tm, ws.t + at * TRI * 3 * 64, bs, sc[16 * w + m]);
+    // P over A
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j <= w)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) am[16 * w + 4 * g + e][16 * j + m] = qk[j][e];
+    __syncthreads();
+    // block (i, c) of P (I + A)^-1 is a sum over i - c + 1 blocks: five a wave
+    lq_f4 pt[4];
+    const uint32_t rows4 = w == 0 ? 0x03u : w == 1 ? 0x13u : w == 2 ? 0x32u : 0x1232u;
+    const uint32_t cols4 = w == 0 ? 0x00u : w == 1 ? 0x01u : w == 2 ? 0x20u : 0x1231u;
+    const int blocks = w < 3 ? 2 : 4;
+#pragma unroll
+    for (int o = 0; o < 4; ++o) {
+        pt[o] = lq_f4{0, 0, 0, 0};
+        if (o >= blocks) continue;
+        const int i = rows4 >> (4 * o) & 15, c = cols4 >> (4 * o) & 15;
+        for (int u = c; u <= i; ++u) {
+            const float4 v = *reinterpret_cast<const float4 *>(&am[16 * i + m][16 * u + 4 * g]);
+            const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                pt[o] = __builtin_amdgcn_mfma_f32_16x16x4f32(e[q], tm[16 * u + 4 * g + q][16 * c + m], pt[o], 0, 0, 0);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int o = 0; o < 4; ++o) {
+        if (o >= blocks) continue;
+        const int i = rows4 >> (4 * o) & 15, c = cols4 >> (4 * o) & 15;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) am[16 * i + 4 * g + e][16 * c + m] = pt[o][e];
+    }
+    __syncthreads();
+    give(am, ws.p + at * TRI * 3 * 64, bs, 1.0f);
 }
 
 // A workgroup carries 16 value columns of one head through a request's pieces of
-// the window. Wave w owns tokens 16 w .. + 15 of a piece and key values KD / 4 w
-// .. of S; operands that others made go through LDS: S, R = V - diag(e^G) K^ S,
-// D, and D scaled for S's sum. Each operand of the next piece is requested as
-// soon as this piece's has been used.
+// the window. Waves 0 to 3 are the chain: wave w has tokens 16 w .. + 15 of a
+// piece (R, U) and key values KD / 4 w .. of S. Waves 4 to 7 make the outputs of
+// the same tokens beside them. S, R and U go through LDS, three barriers a piece.
+// Each operand of the next piece is requested as soon as this piece's has been
+// used; nothing between a request and its use is conditional, so the compiler's
+// count of what is in flight is exact.
 template <typename T, int KD>
-__global__ __launch_bounds__(256, 1) void delta_chain_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
+__global__ __launch_bounds__(512, 1) void delta_chain_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
     constexpr int NP = RuleType<T>::NP, NS = KD / 32, NT = KD / 64;
-    __shared__ __align__(16) dr_u4 ss[NS][3][64], rs[2][3][64], ds[2][3][64], us[2][3][64];
+    __shared__ __align__(16) dr_u4 ss[NS][3][64], rs[2][3][64], us[2][3][64];
     __shared__ float red[2][4][2][16], kq[2][2][KD];
     __shared__ int wild_s[4];
     const int group = p.value_heads / p.key_heads, slices = p.vd / 16;
@@ -503,56 +546,124 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(DeltaRule p, DeltaR
     const int base = span.first / PIECE + b, pieces = (span.count + PIECE - 1) / PIECE;
     const int from = max(ws.first - base, 0), to = min(ws.first + ws.pieces - base, pieces);
     if (from >= to) return;
-    const int w = wave_id(), lane = lane_id(), m = lane & 15, g = lane >> 4;
+    const int wave = wave_id(), w = wave & 3, lane = lane_id(), m = lane & 15, g = lane >> 4;
+    const bool outputs = wave > 3;
     const int h = p.tiled ? gi * p.key_heads + kh : kh * group + gi;
-    const int tri = w == 0 ? 0 : w == 1 ? 1 : w == 2 ? 2 : 4;      // of T' and P: row tile w
+    const int tri = w == 0 ? 0 : w == 1 ? 1 : w == 2 ? 2 : 4;      // of T and P T: row tile w
     const int my = 16 * w + 4 * g;                                 // the lane's rows my .. my + 3 of a piece
-    // what a piece's operands lie at, moved on piece by piece (the same for the whole wave)
+
+    // where the wave's operands lie, moved on piece by piece
     const int64_t key_step = (int64_t)p.key_heads * 4 * NS * NP * 1024, tri_step = (int64_t)p.value_heads * TRI * 3 * 1024;
     const int64_t key0 = ((int64_t)(base + from - ws.first) * p.key_heads + kh) * 4 * NS * NP * 1024;
     const int64_t val0 = (int64_t)(base + from - ws.first) * p.value_heads + h;
-    const char *kb = (const char *)ws.k + key0 + w * NS * NP * 1024, *qb = (const char *)ws.q + key0 + w * NS * NP * 1024;
+    const char *xb = (const char *)(outputs ? ws.q : ws.k) + key0 + w * NS * NP * 1024;
     const char *ktb = (const char *)ws.kt + key0 + w * NT * 2 * NP * 1024;
-    const char *tb = (const char *)ws.t + (val0 * TRI + tri) * 3 * 1024, *pb = (const char *)ws.p + (val0 * TRI + tri) * 3 * 1024;
-    const char *rb = (const char *)(ws.rows + val0 * 4 * PIECE);
-    const T *vb = (const T *)p.v + ((int64_t)span.first + from * PIECE) * p.v_ts + h * p.v_hs + c0;
-    T *ob = (T *)p.out + ((int64_t)span.first + from * PIECE) * p.o_ts + h * p.o_hs + c0;
+    const char *tb = (const char *)(outputs ? ws.p : ws.t) + (val0 * TRI + tri) * 3 * 1024;
+    const char *rb = (const char *)(ws.rows + val0 * 3 * PIECE);
     const uint32_t lane16 = lane * 16, second = w < 2 ? 0 : 3072;      // (row tiles 0 and 1 have one block: it twice)
-    const int v_ts = (int)p.v_ts, o_ts = (int)p.o_ts;
-    int v_at[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v_at[e] = (my + e) * v_ts + m;
-
-    // Nothing between a request and its use is conditional but the waits stay
-    // exact only so: the compiler counts what is in flight.
-    dr_u4 kf[NS][NP], qf[NS][NP], tf[2][3], pf[2][3], ktf[NT][2][NP];
-    T vf[4];
-    float4 cf, of, sf;
-    float2 lf;
     const auto block = [&](const char *at, int i) { return *reinterpret_cast<const dr_u4 *>(at + i * 1024 + lane16); };
-    const auto ask_kq = [&]() {
+    dr_u4 xf[NS][NP], tf[2][3];     // K or Q; T or P T
+    const auto ask_x = [&]() {
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                kf[s][i] = block(kb, s * NP + i);
-                qf[s][i] = block(qb, s * NP + i);
-            }
+            for (int i = 0; i < NP; ++i) xf[s][i] = block(xb, s * NP + i);
     };
-    const auto ask_rows = [&](int n) {
-        cf = *reinterpret_cast<const float4 *>(rb + 4 * my);
-        of = *reinterpret_cast<const float4 *>(rb + 4 * PIECE + 4 * my);
-        sf = *reinterpret_cast<const float4 *>(rb + 8 * PIECE + 4 * my);
-        lf = *reinterpret_cast<const float2 *>(rb + 12 * PIECE);
-        // (rows behind the last one read the first)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) vf[e] = vb[my + e < n ? v_at[e] : m];
-    };
-    const auto ask_lower = [&](const char *at, dr_u4 (&x)[2][3]) {
+    const auto ask_t = [&]() {
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int i = 0; i < 3; ++i) x[s][i] = block(at + (s ? second : 0), i);
+            for (int i = 0; i < 3; ++i) tf[s][i] = block(tb + (s ? second : 0), i);
+    };
+    // K S or Q S of the wave's tokens
+    const auto with_state = [&]() {
+        lq_f4 c[3] = {};
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            dr_u4 z[3];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) z[i] = ss[s][i][lane];
+            dr_product<NP, 3>(xf[s], z, c);
+        }
+        return dr_total(c);
+    };
+    // T R or P T R of the wave's tokens
+    const auto with_rows = [&]() {
+        lq_f4 c[3] = {};
+        dr_u4 y[2][3];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < 3; ++i) y[s][i] = rs[s][i][lane];
+        dr_product<3, 3>(tf[0], y[0], c);
+        if (w > 1) dr_product<3, 3>(tf[1], y[1], c);
+        return dr_total(c);
+    };
+    const auto put = [&](dr_u4 (&dst)[2][3][64], const lq_f4 &x) {
+        dr_u2 y[3];
+        dr_split4(x, y);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) reinterpret_cast<dr_u2 *>(&dst[w >> 1][i][lane])[w & 1] = y[i];
+    };
+
+    if (outputs) {
+        T *ob = (T *)p.out + ((int64_t)span.first + from * PIECE) * p.o_ts + h * p.o_hs + c0;
+        const int o_ts = (int)p.o_ts;
+        float4 of;
+        const auto ask_rows = [&]() { of = *reinterpret_cast<const float4 *>(rb + 4 * PIECE + 4 * my); };
+        ask_x();
+        ask_rows();
+        ask_t();
+        for (int j = from; j < to; ++j) {
+            const int n = min(span.count - j * PIECE, PIECE);
+            const bool more = j + 1 < to;     // the last piece's are asked for again and not used
+            __syncthreads();     // S
+            const lq_f4 qS = with_state();
+            xb += more ? key_step : 0;
+            ask_x();
+            const float ov[4] = {of.x, of.y, of.z, of.w};
+            rb += more ? (int64_t)p.value_heads * 12 * PIECE : 0;
+            ask_rows();
+            __syncthreads();     // R
+            const lq_f4 pR = with_rows();
+            tb += more ? tri_step : 0;
+            ask_t();
+            __syncthreads();     // U
+            if (__builtin_amdgcn_readfirstlane(wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3])) {
+                for (int t = 0; t < 2 * n; ++t) __syncthreads();     // the others' token by token
+            } else {
+                // (stores past the piece's last row are left out by the bound)
+                const auto dst = __builtin_amdgcn_make_buffer_rsrc(ob, 0, ((n - 1) * o_ts + 16) * (int)sizeof(T), 0x00027000);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const T y = (T)(ov[e] * qS[e] + pR[e]);
+                    const int at = ((my + e) * o_ts + m) * (int)sizeof(T);
+                    if constexpr (sizeof(T) == 4)
+                        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, y), dst, at, 0, 0);
+                    else
+                        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, y), dst, at, 0, 0);
+                }
+            }
+            ob += PIECE * p.o_ts;
+        }
+        return;
+    }
+
+    const T *vb = (const T *)p.v + ((int64_t)span.first + from * PIECE) * p.v_ts + h * p.v_hs + c0;
+    const int v_ts = (int)p.v_ts;
+    int v_at[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v_at[e] = (my + e) * v_ts + m;
+    dr_u4 ktf[NT][2][NP];
+    T vf[4];
+    float4 cf;
+    float2 lf;
+    const auto ask_rows = [&](int n) {
+        cf = *reinterpret_cast<const float4 *>(rb + 4 * my);
+        lf = *reinterpret_cast<const float2 *>(rb + 8 * PIECE);
+        // (rows behind the last one read the first)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) vf[e] = vb[my + e < n ? v_at[e] : m];
     };
     const auto ask_kt = [&]() {
 #pragma unroll
@@ -562,7 +673,6 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(DeltaRule p, DeltaR
 #pragma unroll
                 for (int i = 0; i < NP; ++i) ktf[t][s][i] = block(ktb, (t * 2 + s) * NP + i);
     };
-
     float *state = r.state + ((span.slot * p.value_heads + h) * KD + w * NT * 16) * p.vd + c0 + m;
     lq_f4 S[NT];
 #pragma unroll
@@ -570,83 +680,45 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(DeltaRule p, DeltaR
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             S[t][e] = from == 0 && span.fresh ? 0.0f : state[(int64_t)(16 * t + 4 * g + e) * p.vd];
-    const auto share = [&]() {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            dr_u2 y[3];
-            dr_split4(S[t], y);
-            const int tile = w * NT + t;
-#pragma unroll
-            for (int i = 0; i < 3; ++i) reinterpret_cast<dr_u2 *>(&ss[tile >> 1][i][lane])[tile & 1] = y[i];
-        }
-    };
-    const auto put = [&](dr_u4 (&dst)[2][3][64], const lq_f4 &x) {
-        dr_u2 y[3];
-        dr_split4(x, y);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) reinterpret_cast<dr_u2 *>(&dst[w >> 1][i][lane])[w & 1] = y[i];
-    };
-    // row tile w of a lower triangular operand times what LDS holds
-    const auto lower = [&](const dr_u4 (&x)[2][3], const dr_u4 (&src)[2][3][64], lq_f4 (&c)[2]) {
-        dr_u4 y[2][3];
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int i = 0; i < 3; ++i) y[s][i] = src[s][i][lane];
-        dr_product<3, 3>(x[0], y[0], c);
-        if (w > 1) dr_product<3, 3>(x[1], y[1], c);
-    };
     for (int j = from; j < to;) {
-        ask_kq();
+        ask_x();
         ask_rows(span.count - j * PIECE);
-        ask_lower(tb, tf);
+        ask_t();
         ask_kt();
-        ask_lower(pb, pf);
-        share();
-        __syncthreads();
         for (; j < to; ++j) {
             const int n = min(span.count - j * PIECE, PIECE);
             const bool more = j + 1 < to;     // the last piece's are asked for again and not used
-            lq_f4 kS[2] = {}, qS[2] = {};
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                dr_u4 z[3];
+            for (int t = 0; t < NT; ++t) {
+                dr_u2 y[3];
+                dr_split4(S[t], y);
+                const int tile = w * NT + t;
 #pragma unroll
-                for (int i = 0; i < 3; ++i) z[i] = ss[s][i][lane];
-                dr_product<NP, 3>(kf[s], z, kS);
-                dr_product<NP, 3>(qf[s], z, qS);
+                for (int i = 0; i < 3; ++i) reinterpret_cast<dr_u2 *>(&ss[tile >> 1][i][lane])[tile & 1] = y[i];
             }
-            kb += more ? key_step : 0;
-            qb += more ? key_step : 0;
-            ask_kq();
-            const float cv[4] = {cf.x, cf.y, cf.z, cf.w}, ov[4] = {of.x, of.y, of.z, of.w};
-            lq_f4 R, O[2] = {};
+            __syncthreads();     // S
+            const lq_f4 kS = with_state();
+            xb += more ? key_step : 0;
+            ask_x();
+            const float cv[4] = {cf.x, cf.y, cf.z, cf.w}, last = lf.x;
+            lq_f4 R;
             bool odd = lf.y != 0.0f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                R[e] = (my + e < n ? (float)vf[e] : 0.0f) - cv[e] * (kS[0][e] + kS[1][e]);
-                O[0][e] = ov[e] * (qS[0][e] + qS[1][e]);
+                R[e] = (my + e < n ? (float)vf[e] : 0.0f) - cv[e] * kS[e];
                 odd |= !(fabsf(R[e]) <= RULE_WILD * RULE_WILD);     // v, or S, whose products with k are in it
             }
             put(rs, R);
             const bool any = __any(odd);
             if (lane == 0) wild_s[w] = any;
-            const float last = lf.x;
-            const float sv[4] = {sf.x, sf.y, sf.z, sf.w};
             vb += more ? PIECE * p.v_ts : 0;
-            rb += more ? (int64_t)p.value_heads * 16 * PIECE : 0;
+            rb += more ? (int64_t)p.value_heads * 12 * PIECE : 0;
             ask_rows(more ? span.count - (j + 1) * PIECE : n);
-            __syncthreads();
-            lq_f4 D[2] = {}, U;
-            lower(tf, rs, D);
+            __syncthreads();     // R
+            put(us, with_rows());
             tb += more ? tri_step : 0;
-            ask_lower(tb, tf);
-            D[0] = D[0] + D[1];
-            put(ds, D[0]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) U[e] = D[0][e] * sv[e];
-            put(us, U);
-            __syncthreads();
+            ask_t();
+            __syncthreads();     // U
             const int bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3];
             dr_u4 y[2][3];
 #pragma unroll
@@ -656,32 +728,15 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(DeltaRule p, DeltaR
             if (__builtin_amdgcn_readfirstlane(bad)) break;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                lq_f4 c[2] = {};
+                lq_f4 c[3] = {};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) c[0][e] = last * S[t][e];
 #pragma unroll
                 for (int s = 0; s < 2; ++s) dr_product<NP, 3>(ktf[t][s], y[s], c);
-                S[t] = c[0] + c[1];
+                S[t] = dr_total(c);
             }
             ktb += more ? key_step : 0;
             ask_kt();
-            share();
-            lower(pf, ds, O);
-            pb += more ? tri_step : 0;
-            ask_lower(pb, pf);
-            // (stores past the piece's last row are left out by the bound)
-            const auto dst = __builtin_amdgcn_make_buffer_rsrc(ob, 0, ((n - 1) * o_ts + 16) * (int)sizeof(T), 0x00027000);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const T y1 = (T)(O[0][e] + O[1][e]);
-                const int at = ((my + e) * o_ts + m) * (int)sizeof(T);
-                if constexpr (sizeof(T) == 4)
-                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, y1), dst, at, 0, 0);
-                else
-                    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, y1), dst, at, 0, 0);
-            }
-            ob += PIECE * p.o_ts;
-            __syncthreads();
         }
         if (j >= to) break;
         // token by token, as delta_token_kernel: piece j, with S as it was (what was asked for of the next is asked again)
@@ -689,6 +744,7 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(DeltaRule p, DeltaR
         const int64_t row0 = (int64_t)span.first + j * PIECE;
         const T *kp = (const T *)p.k + row0 * p.k_ts + kh * p.k_hs, *qp = (const T *)p.q + row0 * p.q_ts + kh * p.q_hs;
         const T *vp = (const T *)p.v + row0 * p.v_ts + h * p.v_hs + c0 + m;
+        T *op = (T *)p.out + row0 * p.o_ts + h * p.o_hs + c0 + m;
         for (int t = 0; t < n; ++t) {
             const int par = t & 1;
             constexpr int E = KD / 64;
@@ -734,14 +790,10 @@ __global__ __launch_bounds__(256, 1) void delta_chain_kernel(DeltaRule p, DeltaR
             for (int i = 0; i < NT; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) S[i][e] += kq[par][0][(w * NT + i) * 16 + 4 * g + e] * nk * d;
-            if (threadIdx.x < 16) ob[(int64_t)t * p.o_ts + m] = (T)(pq * nq + d * (kdq * nk * nq));
+            if (threadIdx.x < 16) op[(int64_t)t * p.o_ts] = (T)(pq * nq + d * (kdq * nk * nq));
         }
-        if (++j >= to) break;
-        // T's, V's, K's and the factors' places are the next piece's already
-        ktb += key_step;
-        pb += tri_step;
-        ob += PIECE * p.o_ts;
-        __syncthreads();
+        ++j;
+        ktb += key_step;     // (the other operands' places are the next piece's already)
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -753,7 +805,7 @@ constexpr int RULE_LEAST = 5;              // tokens of a request below which th
 constexpr int64_t RULE_WINDOW = 64 << 20;  // bytes of workspace that a window of pieces may fill
 
 static int64_t piece_bytes(int np, int key_heads, int value_heads, int kd) {
-    return (int64_t)key_heads * 3 * 2 * PIECE * kd * np + (int64_t)value_heads * (2 * TRI * 3 * 1024 + 4 * PIECE * 4);
+    return (int64_t)key_heads * 3 * 2 * PIECE * kd * np + (int64_t)value_heads * (2 * TRI * 3 * 1024 + 3 * PIECE * 4);
 }
 // pieces of a call, and of a window
 static int64_t all_pieces(int64_t tokens, int requests) { return tokens / PIECE + requests; }
@@ -809,7 +861,7 @@ static void rule_launch(const DeltaRule &p, const DeltaRequests &r, void *ws, hi
         const dim3 grid((unsigned)(w.pieces * p.key_heads), (unsigned)group);
         hipLaunchKernelGGL((delta_piece_kernel<T, KD>), grid, dim3(256), 0, s, p, r, w);
         const int64_t units = ((int64_t)r.requests * p.key_heads + 7) / 8 * 8;
-        hipLaunchKernelGGL((delta_chain_kernel<T, KD>), dim3((unsigned)(units * group * (p.vd / 16))), dim3(256), 0, s, p, r,
+        hipLaunchKernelGGL((delta_chain_kernel<T, KD>), dim3((unsigned)(units * group * (p.vd / 16))), dim3(512), 0, s, p, r,
                            w);
     }
 }
