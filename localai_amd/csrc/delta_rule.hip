@@ -130,11 +130,11 @@ __global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequ
 // the rows d_i of all tokens solve (I + A) D = diag(b) R, R = V - diag(e^G) K^ S, so
 // with T = (I + A)^-1 diag(b)
 //   O = diag(e^G) Q^ S + (P T) R
-//   S <- e^G_last S + K^T U,  U = diag(e^(G_last - G) / |k|) T R
-// What does not depend on S (P T, the scaled T, the factors, the operands'
-// layout) is one launch over all pieces and heads (delta_piece_kernel); the
-// chain over a request's pieces is a second one, each workgroup with 16 value
-// columns of one head, whose S stays in registers (delta_chain_kernel).
+//   S <- e^G_last S + W R,  W = K^T diag(e^(G_last - G)) T
+// What does not depend on S (W, P T, the factors, the operands' layout) is one
+// launch over all pieces and heads (delta_piece_kernel); the chain over a
+// request's pieces is a second one, each workgroup with 16 value columns of one
+// head, whose S stays in registers (delta_chain_kernel).
 //
 // Precision: everything is fp32's. MFMA takes bf16 operands, so each fp32 value
 // goes in as three bf16 pieces (24 bits), q and k of 16 bits as they are (bf16:
@@ -161,11 +161,24 @@ template <typename T> struct RuleType { static constexpr int NP = 1; };
 template <> struct RuleType<_Float16> { static constexpr int NP = 2; };
 template <> struct RuleType<float> { static constexpr int NP = 3; };
 
-// workspace of one window of pieces, in 1 KB blocks (64 lanes x 16 bytes: an MFMA operand)
+// Key values in the order of S's tiles of 16: tile t, row 4 g + e is key value
+// 32 (t / 2) + 8 g + 4 (t % 2) + e, so that a lane's eight values of two tiles are
+// adjacent in q and k. (64 key values: a tile a wave, the other half of its step zero.)
+template <int KD> struct RuleKeys {
+    static constexpr int TILES = KD / 16, NT = KD / 64;               // tiles, and of a wave
+    static constexpr int STEPS = KD == 64 ? 4 : KD / 32, NW = STEPS / 4;   // steps of 32 contracted values, and of a wave
+    static __device__ __forceinline__ int at(int tile, int row) {
+        return KD == 64 ? 16 * tile + row : 32 * (tile >> 1) + 8 * (row >> 2) + 4 * (tile & 1) + (row & 3);
+    }
+};
+
+// workspace of one window of pieces: byte offsets of arrays of 1 KB blocks (64 lanes x 16 bytes: an MFMA operand)
 struct RuleWork {
-    dr_u4 *k, *q, *kt;     // [piece, key head][..][np][64]: row tile, step; kt: key tile, step
-    dr_u4 *t, *p;          // [piece, value head][TRI][3][64]: scaled T, P T
-    float *rows;           // [piece, value head][3][64]: e^G / |k|, scale e^G / |q|; e^G_last, wild
+    char *base;
+    uint32_t bytes;
+    uint32_t k, q;         // [piece, key head][row tile][step][np]
+    uint32_t w, p;         // [piece, value head]: [key tile][2][3], [TRI][3]
+    uint32_t rows;         // [piece, value head][3][64] fp32: e^G / |k|, scale e^G / |q|; e^G_last, NaN: token by token
     int first, pieces;     // the window
     int least;             // requests of fewer tokens are the token kernel's
 };
@@ -245,6 +258,27 @@ __device__ __forceinline__ float dr_exp2(double x) {
     return ldexpf(__builtin_amdgcn_exp2f((float)(x - whole)), (int)fmax(whole, -400.0));
 }
 
+// four or eight adjacent values (aligned to four)
+template <typename T, int N>
+__device__ __forceinline__ void dr_load(const T *p, float (&x)[8]) {
+    struct __attribute__((packed, aligned(4 * sizeof(T)))) Raw { T v[N]; };
+    const Raw raw = *reinterpret_cast<const Raw *>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < N ? (float)raw.v[i < N ? i : 0] : 0.0f;
+}
+
+// one step of an inclusive sum over the wave's lanes, of fp64 values
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dr_add_from(double v) {
+    uint32_t u[2];
+    __builtin_memcpy(u, &v, 8);
+    u[0] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u[0], CTRL, ROWS, 0xF, false);
+    u[1] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u[1], CTRL, ROWS, 0xF, false);
+    double from;
+    __builtin_memcpy(&from, u, 8);
+    return v + from;
+}
+
 // A workgroup prepares one piece for one value head (blockIdx.y: the value heads
 // of a key head; the first writes the key head's operands). Wave w owns rows
 // 16 w .. 16 w + 15. An operand's lane l holds row or column l & 15 and of each
@@ -253,13 +287,15 @@ __device__ __forceinline__ float dr_exp2(double x) {
 // as they are.
 template <typename T, int KD>
 __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
-    constexpr int NP = RuleType<T>::NP, NS = KD / 32, LD = 68;
-    // K's operands, then A (later P, P T) and T
-    constexpr int KS = 4 * NS * NP * 64 * 16, MS = PIECE * LD * 4;
-    __shared__ __align__(16) char space[KS > 2 * MS ? KS : 2 * MS];
+    typedef RuleKeys<KD> Keys;
+    constexpr int NP = RuleType<T>::NP, NS = Keys::STEPS, NT = Keys::NT, LD = 68;
+    // K's operands, then A (later T's operands, P, P T) and T
+    constexpr int KS = 4 * NS * NP * 1024, AS = TRI * 3 * 1024, MS = PIECE * LD * 4;
+    __shared__ __align__(16) char space[KS > AS + MS ? KS : AS + MS];
     dr_u4 (&ks)[4][NS][NP][64] = *reinterpret_cast<dr_u4 (*)[4][NS][NP][64]>(space);
     float (&am)[PIECE][LD] = *reinterpret_cast<float (*)[PIECE][LD]>(space);
-    float (&tm)[PIECE][LD] = *reinterpret_cast<float (*)[PIECE][LD]>(space + MS);
+    dr_u4 (&to)[TRI][3][64] = *reinterpret_cast<dr_u4 (*)[TRI][3][64]>(space);
+    float (&tm)[PIECE][LD] = *reinterpret_cast<float (*)[PIECE][LD]>(space + AS);
     __shared__ double gs[PIECE];      // sums of g, in powers of two
     __shared__ float bs[PIECE], ik[PIECE], iq[PIECE], kn[PIECE], sc[PIECE];
     __shared__ int wild_s[4];
@@ -274,34 +310,35 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
     const int h = p.tiled ? gi * p.key_heads + kh : kh * group + gi;
     const int64_t row0 = (int64_t)span.first + j0, at = (int64_t)local * p.value_heads + h;
     const bool norm = p.norm_eps >= 0.0f;
-    const float2 gb = lane < n ? rule_gates(p, row0 + lane, h) : make_float2(0, 0);     // one token a lane
     bool wild = false;
     dr_u4 qf[NS][NP];
+    float2 gb;
     {
         const bool in = 16 * w + m < n;
         const int64_t row = row0 + (in ? 16 * w + m : 0);
-        const T *rows[2] = {(const T *)p.k + row * p.k_ts + kh * p.k_hs, (const T *)p.q + row * p.q_ts + kh * p.q_hs};
+        constexpr int V = KD == 64 ? 4 : 8;      // adjacent values of a lane's step
+        const T *rows[2] = {(const T *)p.k + row * p.k_ts + kh * p.k_hs + V * g, (const T *)p.q + row * p.q_ts + kh * p.q_hs + V * g};
+        float x[2][NS][8];
+#pragma unroll
+        for (int o = 0; o < 2; ++o)
+#pragma unroll
+            for (int s = 0; s < NS; ++s) dr_load<T, V>(rows[o] + 4 * V * s, x[o][s]);
+        gb = lane < n ? rule_gates(p, row0 + lane, h) : make_float2(0, 0);     // one token a lane
 #pragma unroll
         for (int o = 0; o < 2; ++o) {
-            float x[NS][8], ss = 0.0f, top = 0.0f;
+            float ss = 0.0f, top = 0.0f;
 #pragma unroll
             for (int s = 0; s < NS; ++s)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    float4 v = delta_load4(rows[o] + 32 * s + 16 * u + 4 * g);
-                    if (!in) v = make_float4(0, 0, 0, 0);
-                    const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        x[s][4 * u + i] = e[i];
-                        ss += e[i] * e[i];
-                        top = fmaxf(top, fabsf(e[i]));
-                        wild |= !(fabsf(e[i]) <= RULE_WILD);
-                    }
+                for (int e = 0; e < V; ++e) {
+                    x[o][s][e] = in ? x[o][s][e] : 0.0f;
+                    ss += x[o][s][e] * x[o][s][e];
+                    top = fmaxf(top, fabsf(x[o][s][e]));
                 }
             ss = dr_rows_sum(ss);
             top = dr_rows_max(top);
-            wild |= top > 0.0f && top < RULE_FAINT;
+            // (a NaN is in the sum, not in the largest)
+            wild |= !(ss <= RULE_WILD * RULE_WILD) || (top > 0.0f && top < RULE_FAINT);
             float inv = norm ? 1.0f / sqrtf(ss + p.norm_eps) : 1.0f;
             if (norm && !(inv <= 3.4e38f)) {     // a row of zeros and norm_eps 0: 0 / 0
                 wild |= in;
@@ -312,15 +349,15 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
 #pragma unroll
                 for (int s = 0; s < NS; ++s)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[s][e] *= inv;
+                    for (int e = 0; e < V; ++e) x[o][s][e] *= inv;
                 inv = 1.0f;
             }
             if (g == 0) (o ? iq : ik)[16 * w + m] = inv;
-            dr_u4 *dst = (o ? ws.q : ws.k) + (((int64_t)local * p.key_heads + kh) * 4 + w) * NS * NP * 64 + lane;
+            dr_u4 *dst = (dr_u4 *)(ws.base + (o ? ws.q : ws.k)) + (((int64_t)local * p.key_heads + kh) * 4 + w) * NS * NP * 64 + lane;
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
                 dr_u4 y[NP];
-                dr_split8<NP>(x[s], y);
+                dr_split8<NP>(x[o][s], y);
 #pragma unroll
                 for (int i = 0; i < NP; ++i) {
                     if (o) qf[s][i] = y[i];
@@ -332,53 +369,49 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
     }
     // sums of g up to each token (e^-1e4 is 0; -inf less -inf would be NaN)
     double total = (gb.x < -1e4f ? -1e4 : (double)gb.x) * 1.4426950408889634074;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const double up = __shfl_up(total, d, 64);
-        if (lane >= d) total += up;
-    }
+    total = dr_add_from<0x111, 0xF>(total);
+    total = dr_add_from<0x112, 0xF>(total);
+    total = dr_add_from<0x114, 0xF>(total);
+    total = dr_add_from<0x118, 0xF>(total);
+    total = dr_add_from<0x142, 0xA>(total);     // lane 15 of each row of lanes into the next
+    total = dr_add_from<0x143, 0xC>(total);     // lane 31 into the upper half
     if (w == 0) {
         gs[lane] = total;
         bs[lane] = gb.y;
     }
-    // (a state that grows by itself would make T' grow to what the piece's sums cancel)
+    // (a state that grows by itself would make T grow to what the piece's sums cancel)
     wild |= !(gb.y >= 0.0f && gb.y <= 1e3f) || !(gb.x <= 0.3f);
-    if (__any(wild) && lane == 0) wild_s[w] = 1;
-    else if (lane == 0) wild_s[w] = 0;
+    const bool any = __any(wild);
+    if (lane == 0) wild_s[w] = any;
     __syncthreads();
-    // K^T: lane (key value 16 t + m, tokens 4 g + 0..3 and 16 + 4 g + 0..3 of 32)
-    if (gi == 0) {
-        dr_u4 *dst = ws.kt + ((int64_t)local * p.key_heads + kh) * (KD / 16) * 2 * NP * 64 + lane;
-#pragma unroll
-        for (int i = 0; i < KD / 64; ++i) {
-            const int t = w * (KD / 64) + i;
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int pc = 0; pc < NP; ++pc) {
-                    uint16_t y[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int token = 32 * s + 16 * (e >> 2) + 4 * g + (e & 3);
-                        const uint16_t *src = reinterpret_cast<const uint16_t *>(&ks[token >> 4][t >> 1][pc][(token & 15) + 16 * (m >> 2)]);
-                        y[e] = src[(m & 3) + 4 * (t & 1)];
-                    }
-                    dr_u4 u;
-                    __builtin_memcpy(&u, y, 16);
-                    dst[((t * 2 + s) * NP + pc) * 64] = u;
-                }
-        }
-    }
     const double last = gs[63];
     const bool bad = (wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3]) || __any(!(gb.y * kn[lane] <= 2.1f));
     if (w == 0) {
-        float *rows = ws.rows + at * 3 * PIECE;
+        float *rows = (float *)(ws.base + ws.rows) + at * 3 * PIECE;
         rows[lane] = dr_exp2(total) * ik[lane];
         rows[PIECE + lane] = dr_exp2(total) * iq[lane] * p.scale;
-        if (lane < 2) rows[2 * PIECE + lane] = lane ? (bad ? 1.0f : 0.0f) : dr_exp2(last);
+        if (lane == 0) rows[2 * PIECE] = bad ? __builtin_nanf("") : dr_exp2(last);
         sc[lane] = dr_exp2(last - total) * ik[lane];
     }
     if (bad) return;     // nothing else of it is read
+    // K with tokens contracted: lane (key value (t, m), tokens 4 g + 0..3 and 16 + 4 g + 0..3 of 32), the wave's key tiles
+    dr_u4 kt[NT][2][NP];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const int t = w * NT + i, s1 = KD == 64 ? t : t >> 1, o1 = KD == 64 ? 0 : 4 * (t & 1);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int pc = 0; pc < NP; ++pc) {
+                uint16_t y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int tile = 2 * s + (e >> 2), token = 4 * g + (e & 3);
+                    y[e] = reinterpret_cast<const uint16_t *>(&ks[tile][s1][pc][token + 16 * (m >> 2)])[o1 + (m & 3)];
+                }
+                __builtin_memcpy(&kt[i][s][pc], y, 16);
+            }
+    }
     // k_i . k_j and q_i . k_j of row tile w, column tiles up to it
     lq_f4 kk[4], qk[4];
 #pragma unroll
@@ -401,19 +434,28 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
             qk[j] = dr_total(c);
         }
     }
+    double gr[4], gc[4];
+    float kr[4], qr[4], kc[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int row = 16 * w + 4 * g + e, col = 16 * e + m;
+        gr[e] = gs[row];
+        kr[e] = bs[row] * ik[row];
+        qr[e] = iq[row] * p.scale;
+        gc[e] = gs[col];
+        kc[e] = ik[col];
+    }
     __syncthreads();     // K's operands have been read
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         if (j > w) continue;
-        const int col = 16 * j + m;
-        const double gc = gs[col];
-        const float ikc = ik[col];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int row = 16 * w + 4 * g + e;
-            const float f = row >= col ? dr_exp2(gs[row] - gc) * ikc : 0.0f;
-            am[row][col] = row > col ? f * (bs[row] * ik[row]) * kk[j][e] : 0.0f;
-            qk[j][e] = row >= col ? f * (iq[row] * p.scale) * qk[j][e] : 0.0f;
+            const int row = 16 * w + 4 * g + e, col = 16 * j + m;
+            // (of far tokens the power's argument is rounded to 2^-24 of itself: less of the sum than 2^-25)
+            const float f = row >= col ? __builtin_amdgcn_exp2f((float)(gr[e] - gc[j])) * kc[j] : 0.0f;
+            am[row][col] = row > col ? f * kr[e] * kk[j][e] : 0.0f;
+            qk[j][e] = row >= col ? f * qr[e] * qk[j][e] : 0.0f;
         }
     }
     __syncthreads();
@@ -463,35 +505,57 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
         }
     }
     __syncthreads();
-    // the operands of row tile w of a lower triangular matrix (columns behind the tile's last are zero),
-    // its columns times cols, its rows times by
-    const auto give = [&](const float (&src)[PIECE][LD], dr_u4 *dst, const float *cols, float by) {
-        const int base = w == 0 ? 0 : w == 1 ? 1 : w == 2 ? 2 : 4;
+    // W^T = T^T diag K: the scaled T with tokens contracted, column tile c, tokens 32 s .., in A's place
+    for (int i = w; i < TRI; i += 4) {
+        const int c = i < 4 ? i >> 1 : i - 2, s = i < 4 ? i & 1 : 1;
+        const float bc = bs[16 * c + m];
+        float y8[8];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            if (s > w / 2) continue;
-            float y8[8];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int col = 32 * s + 16 * u + 4 * g;
-                const float4 v = *reinterpret_cast<const float4 *>(&src[16 * w + m][col]);
-                const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) y8[4 * u + i] = 2 * s + u <= w ? e[i] * cols[col + i] * by : 0.0f;
-            }
-            dr_u4 y[3];
-            dr_split8<3>(y8, y);
-#pragma unroll
-            for (int i = 0; i < 3; ++i) dst[((base + s) * 3 + i) * 64 + lane] = y[i];
+        for (int e = 0; e < 8; ++e) {
+            const int token = 32 * s + 16 * (e >> 2) + 4 * g + (e & 3);
+            y8[e] = 2 * s + (e >> 2) >= c ? tm[token][16 * c + m] * (bc * sc[token]) : 0.0f;
         }
-    };
-    give(tm, ws.t + at * TRI * 3 * 64, bs, sc[16 * w + m]);
-    // P over A
+        dr_u4 y[3];
+        dr_split8<3>(y8, y);
+#pragma unroll
+        for (int pc = 0; pc < 3; ++pc) to[i][pc][lane] = y[pc];
+    }
+    __syncthreads();
+    {
+        lq_f4 wt[NT][4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            lq_f4 acc[NT][3] = {};
+#pragma unroll
+            for (int s = c >> 1; s < 2; ++s) {
+                dr_u4 y[3];
+#pragma unroll
+                for (int pc = 0; pc < 3; ++pc) y[pc] = to[c < 2 ? 2 * c + s : c + 2][pc][lane];
+#pragma unroll
+                for (int i = 0; i < NT; ++i) dr_product<3, NP>(y, kt[i][s], acc[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < NT; ++i) wt[i][c] = dr_total(acc[i]);
+        }
+        dr_u4 *dst = (dr_u4 *)(ws.base + ws.w) + (at * Keys::TILES + w * NT) * 2 * 3 * 64 + lane;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const float y8[8] = {wt[i][2 * s][0], wt[i][2 * s][1], wt[i][2 * s][2], wt[i][2 * s][3],
+                                     wt[i][2 * s + 1][0], wt[i][2 * s + 1][1], wt[i][2 * s + 1][2], wt[i][2 * s + 1][3]};
+                dr_u4 y[3];
+                dr_split8<3>(y8, y);
+#pragma unroll
+                for (int pc = 0; pc < 3; ++pc) dst[((i * 2 + s) * 3 + pc) * 64] = y[pc];
+            }
+    }
+    __syncthreads();     // T's operands have been read
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         if (j <= w)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) am[16 * w + 4 * g + e][16 * j + m] = qk[j][e];
+            for (int e = 0; e < 4; ++e) am[16 * w + 4 * g + e][16 * j + m] = qk[j][e];     // P
     __syncthreads();
     // block (i, c) of P (I + A)^-1 is a sum over i - c + 1 blocks: five a wave
     lq_f4 pt[4];
@@ -520,20 +584,77 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
         for (int e = 0; e < 4; ++e) am[16 * i + 4 * g + e][16 * c + m] = pt[o][e];
     }
     __syncthreads();
-    give(am, ws.p + at * TRI * 3 * 64, bs, 1.0f);
+    // P T's operands of row tile w (columns behind the tile's last are zero)
+    dr_u4 *dst = (dr_u4 *)(ws.base + ws.p) + (at * TRI + (w < 2 ? w : 2 * w - 2)) * 3 * 64 + lane;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        if (s > w / 2) continue;
+        float y8[8];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int col = 32 * s + 16 * u + 4 * g;
+            const float4 v = *reinterpret_cast<const float4 *>(&am[16 * w + m][col]);
+            const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y8[4 * u + i] = 2 * s + u <= w ? e[i] * bs[col + i] : 0.0f;
+        }
+        dr_u4 y[3];
+        dr_split8<3>(y8, y);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) dst[(s * 3 + i) * 64] = y[i];
+    }
 }
 
+// Requests stay where they are written: moved ahead of the last use of what they
+// replace, they would need registers of their own and copies that wait for them
+// (measured: 8192 tokens, 2.1 us a piece with the compiler's order).
+__device__ __forceinline__ void dr_hold() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// v of N row tiles from tile t0 on, as R takes it (0 behind the last row)
+template <typename T, int N>
+struct RuleValues {
+    T v[N][4];
+    // rows of the call's v from the request's first one on, and how many there are
+    __device__ __forceinline__ void ask(const T *vb, int64_t ts, int row0, int rows) {
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[t][e] = vb[(int64_t)min(row0 + 16 * t + e, rows - 1) * ts];
+    }
+    __device__ __forceinline__ void give(lq_f4 (*dst)[64], int row0, int rows) {
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            lq_f4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = row0 + 16 * t + e < rows ? (float)v[t][e] : 0.0f;
+            dst[t][lane_id()] = x;
+        }
+    }
+};
+
 // A workgroup carries 16 value columns of one head through a request's pieces of
-// the window. Waves 0 to 3 are the chain: wave w has tokens 16 w .. + 15 of a
-// piece (R, U) and key values KD / 4 w .. of S. Waves 4 to 7 make the outputs of
-// the same tokens beside them. S, R and U go through LDS, three barriers a piece.
-// Each operand of the next piece is requested as soon as this piece's has been
-// used; nothing between a request and its use is conditional, so the compiler's
-// count of what is in flight is exact.
+// the window. Waves 0 to 3 are the chain: wave w holds a quarter of S's key
+// values as MFMA leaves them, which is the operand of its share of K S; the
+// shares meet in LDS, wave w makes R of tokens 16 w .. + 15, and all take R for
+// their quarter of W R. The waves behind them make the outputs of OT tiles of tokens
+// each beside them, from S and R in LDS (two halve what LDS has to give; of 256 key
+// values Q's pieces for one tile are what the registers hold). The last two bring
+// v, of every other piece each: from HBM, it takes longer than a piece (of 256 key
+// values the waves with the outputs do: a tenth wave would cost the others registers).
+// Two barriers a piece. Each operand of the next piece is requested as soon as this
+// piece's has been used; nothing between a request and its use is conditional, so
+// the compiler's count of what is in flight is exact.
+template <int KD> constexpr int RULE_OT = KD > 128 ? 1 : 2;
+constexpr int RULE_CHAIN = 512;      // threads
 template <typename T, int KD>
-__global__ __launch_bounds__(512, 1) void delta_chain_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
-    constexpr int NP = RuleType<T>::NP, NS = KD / 32, NT = KD / 64;
-    __shared__ __align__(16) dr_u4 ss[NS][3][64], rs[2][3][64], us[2][3][64];
+__global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
+    typedef RuleKeys<KD> Keys;
+    constexpr int NP = RuleType<T>::NP, NS = Keys::STEPS, NT = Keys::NT, NW = Keys::NW, OT = RULE_OT<KD>;
+    __shared__ __align__(16) dr_u4 ss[NS][3][64], rs[2][3][64];
+    __shared__ __align__(16) lq_f4 part[4][4][64], vs[2][4][64];
     __shared__ float red[2][4][2][16], kq[2][2][KD];
     __shared__ int wild_s[4];
     const int group = p.value_heads / p.key_heads, slices = p.vd / 16;
@@ -546,266 +667,323 @@ __global__ __launch_bounds__(512, 1) void delta_chain_kernel(DeltaRule p, DeltaR
     const int base = span.first / PIECE + b, pieces = (span.count + PIECE - 1) / PIECE;
     const int from = max(ws.first - base, 0), to = min(ws.first + ws.pieces - base, pieces);
     if (from >= to) return;
-    const int wave = wave_id(), w = wave & 3, lane = lane_id(), m = lane & 15, g = lane >> 4;
-    const bool outputs = wave > 3;
+    const int w = wave_id(), lane = lane_id(), m = lane & 15, g = lane >> 4;
     const int h = p.tiled ? gi * p.key_heads + kh : kh * group + gi;
-    const int tri = w == 0 ? 0 : w == 1 ? 1 : w == 2 ? 2 : 4;      // of T and P T: row tile w
-    const int my = 16 * w + 4 * g;                                 // the lane's rows my .. my + 3 of a piece
 
-    // where the wave's operands lie, moved on piece by piece
-    const int64_t key_step = (int64_t)p.key_heads * 4 * NS * NP * 1024, tri_step = (int64_t)p.value_heads * TRI * 3 * 1024;
-    const int64_t key0 = ((int64_t)(base + from - ws.first) * p.key_heads + kh) * 4 * NS * NP * 1024;
-    const int64_t val0 = (int64_t)(base + from - ws.first) * p.value_heads + h;
-    const char *xb = (const char *)(outputs ? ws.q : ws.k) + key0 + w * NS * NP * 1024;
-    const char *ktb = (const char *)ws.kt + key0 + w * NT * 2 * NP * 1024;
-    const char *tb = (const char *)(outputs ? ws.p : ws.t) + (val0 * TRI + tri) * 3 * 1024;
-    const char *rb = (const char *)(ws.rows + val0 * 3 * PIECE);
-    const uint32_t lane16 = lane * 16, second = w < 2 ? 0 : 3072;      // (row tiles 0 and 1 have one block: it twice)
-    const auto block = [&](const char *at, int i) { return *reinterpret_cast<const dr_u4 *>(at + i * 1024 + lane16); };
-    dr_u4 xf[NS][NP], tf[2][3];     // K or Q; T or P T
-    const auto ask_x = [&]() {
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-#pragma unroll
-            for (int i = 0; i < NP; ++i) xf[s][i] = block(xb, s * NP + i);
-    };
-    const auto ask_t = [&]() {
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int i = 0; i < 3; ++i) tf[s][i] = block(tb + (s ? second : 0), i);
-    };
-    // K S or Q S of the wave's tokens
-    const auto with_state = [&]() {
-        lq_f4 c[3] = {};
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            dr_u4 z[3];
-#pragma unroll
-            for (int i = 0; i < 3; ++i) z[i] = ss[s][i][lane];
-            dr_product<NP, 3>(xf[s], z, c);
+    const T *vb = (const T *)p.v + (int64_t)span.first * p.v_ts + h * p.v_hs + c0 + m;     // (vs[j & 1]: piece j's)
+    if (w >= 4 + 4 / OT) {
+        RuleValues<T, 4> v;
+        int mine = from + ((w ^ from) & 1);     // the next piece that is this wave's
+        v.ask(vb, p.v_ts, mine * PIECE + 4 * g, span.count);
+        for (int j = from - 1; j < to; ++j) {
+            if (j >= from) {
+                __syncthreads();     // S
+                __syncthreads();     // R: piece j's v has been read
+                const int bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3];
+                if (__builtin_amdgcn_readfirstlane(bad))
+                    for (int t = 0; t < 2 * min(span.count - j * PIECE, PIECE); ++t) __syncthreads();     // the others' token by token
+            }
+            if (mine == j + 1) {
+                v.give(vs[mine & 1], mine * PIECE + 4 * g, span.count);
+                mine += 2;
+                v.ask(vb, p.v_ts, mine * PIECE + 4 * g, span.count);
+            }
         }
-        return dr_total(c);
+        return;
+    }
+
+    // where the operands lie, moved on piece by piece
+    const auto wsrc = __builtin_amdgcn_make_buffer_rsrc(ws.base, 0, (int)ws.bytes, 0x00027000);
+    const uint32_t key_step = (uint32_t)p.key_heads * 4 * NS * NP * 1024, row_step = (uint32_t)p.value_heads * 12 * PIECE;
+    const uint32_t key0 = ((uint32_t)(base + from - ws.first) * p.key_heads + kh) * 4 * NS * NP * 1024;
+    const uint32_t val0 = (uint32_t)(base + from - ws.first) * p.value_heads + h;
+    uint32_t rb = ws.rows + val0 * 12 * PIECE;
+    const int lane16 = lane * 16;
+    const auto block = [&](uint32_t at, int i) {
+        return __builtin_bit_cast(dr_u4, __builtin_amdgcn_raw_buffer_load_b128(wsrc, lane16, (int)(at + i * 1024), 0));
     };
-    // T R or P T R of the wave's tokens
-    const auto with_rows = [&]() {
-        lq_f4 c[3] = {};
-        dr_u4 y[2][3];
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int i = 0; i < 3; ++i) y[s][i] = rs[s][i][lane];
-        dr_product<3, 3>(tf[0], y[0], c);
-        if (w > 1) dr_product<3, 3>(tf[1], y[1], c);
-        return dr_total(c);
-    };
-    const auto put = [&](dr_u4 (&dst)[2][3][64], const lq_f4 &x) {
-        dr_u2 y[3];
-        dr_split4(x, y);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) reinterpret_cast<dr_u2 *>(&dst[w >> 1][i][lane])[w & 1] = y[i];
+    // four factors of rows row .. row + 3 of set s
+    const auto factors = [&](int s, int row) {
+        return __builtin_bit_cast(lq_f4, __builtin_amdgcn_raw_buffer_load_b128(wsrc, 16 * g, (int)(rb + 4 * (s * PIECE + row)), 0));
     };
 
-    if (outputs) {
+    if (w > 3) {
+        const int o = (w - 4) * OT;                                    // row tiles o .. o + OT - 1
+        const bool upper = o > 1;                                      // their rows of P T have two blocks
+        uint32_t qb = ws.q + key0 + o * NS * NP * 1024;
+        uint32_t pb = ws.p + (val0 * TRI + (upper ? 2 * o - 2 : o)) * 3 * 1024;
+        const uint32_t tri_step = (uint32_t)p.value_heads * TRI * 3 * 1024;
         T *ob = (T *)p.out + ((int64_t)span.first + from * PIECE) * p.o_ts + h * p.o_hs + c0;
         const int o_ts = (int)p.o_ts;
-        float4 of;
-        const auto ask_rows = [&]() { of = *reinterpret_cast<const float4 *>(rb + 4 * PIECE + 4 * my); };
-        ask_x();
-        ask_rows();
-        ask_t();
+        dr_u4 qf[OT][NS][NP], pf[OT][2][3];
+        lq_f4 of[OT];
+        const auto ask_q = [&]() {
+#pragma unroll
+            for (int t = 0; t < OT; ++t)
+#pragma unroll
+                for (int s = 0; s < NS; ++s)
+#pragma unroll
+                    for (int i = 0; i < NP; ++i) qf[t][s][i] = block(qb, (t * NS + s) * NP + i);
+#pragma unroll
+            for (int t = 0; t < OT; ++t) of[t] = factors(1, 16 * (o + t));
+        };
+        const auto ask_p = [&]() {     // (row tiles 0 and 1 have one block: it twice)
+#pragma unroll
+            for (int t = 0; t < OT; ++t)
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) pf[t][s][i] = block(pb, (upper ? 2 * t + s : t) * 3 + i);
+        };
+        RuleValues<T, OT> v;      // of 256 key values
+        ask_q();
+        dr_hold();
+        ask_p();
+        dr_hold();
+        if constexpr (KD > 128) {
+            v.ask(vb, p.v_ts, from * PIECE + 16 * o + 4 * g, span.count);
+            v.give(vs[from & 1] + o, from * PIECE + 16 * o + 4 * g, span.count);
+            v.ask(vb, p.v_ts, (from + 1) * PIECE + 16 * o + 4 * g, span.count);
+        }
         for (int j = from; j < to; ++j) {
             const int n = min(span.count - j * PIECE, PIECE);
             const bool more = j + 1 < to;     // the last piece's are asked for again and not used
             __syncthreads();     // S
-            const lq_f4 qS = with_state();
-            xb += more ? key_step : 0;
-            ask_x();
-            const float ov[4] = {of.x, of.y, of.z, of.w};
-            rb += more ? (int64_t)p.value_heads * 12 * PIECE : 0;
-            ask_rows();
+            lq_f4 O[OT];
+            {
+                lq_f4 c[OT][3] = {};
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    dr_u4 z[3];
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) z[i] = ss[s][i][lane];
+#pragma unroll
+                    for (int t = 0; t < OT; ++t) dr_product<NP, 3>(qf[t][s], z, c[t]);
+                }
+#pragma unroll
+                for (int t = 0; t < OT; ++t) O[t] = dr_total(c[t]) * of[t];
+            }
+            dr_hold();
+            qb += more ? key_step : 0;
+            rb += more ? row_step : 0;
+            ask_q();
             __syncthreads();     // R
-            const lq_f4 pR = with_rows();
-            tb += more ? tri_step : 0;
-            ask_t();
-            __syncthreads();     // U
-            if (__builtin_amdgcn_readfirstlane(wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3])) {
+            const int bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3];
+            {
+                lq_f4 c[OT][3] = {};
+                dr_u4 y[2][3];
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) y[s][i] = rs[s][i][lane];
+#pragma unroll
+                for (int t = 0; t < OT; ++t) {
+                    dr_product<3, 3>(pf[t][0], y[0], c[t]);
+                    if (upper) dr_product<3, 3>(pf[t][1], y[1], c[t]);
+                    O[t] = O[t] + dr_total(c[t]);
+                }
+            }
+            dr_hold();
+            pb += more ? tri_step : 0;
+            ask_p();
+            dr_hold();
+            if (__builtin_amdgcn_readfirstlane(bad)) {
                 for (int t = 0; t < 2 * n; ++t) __syncthreads();     // the others' token by token
             } else {
                 // (stores past the piece's last row are left out by the bound)
                 const auto dst = __builtin_amdgcn_make_buffer_rsrc(ob, 0, ((n - 1) * o_ts + 16) * (int)sizeof(T), 0x00027000);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const T y = (T)(ov[e] * qS[e] + pR[e]);
-                    const int at = ((my + e) * o_ts + m) * (int)sizeof(T);
-                    if constexpr (sizeof(T) == 4)
-                        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, y), dst, at, 0, 0);
-                    else
-                        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, y), dst, at, 0, 0);
-                }
+                for (int t = 0; t < OT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const T y = (T)O[t][e];
+                        const int at = ((16 * (o + t) + 4 * g + e) * o_ts + m) * (int)sizeof(T);
+                        if constexpr (sizeof(T) == 4)
+                            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, y), dst, at, 0, 0);
+                        else
+                            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, y), dst, at, 0, 0);
+                    }
             }
             ob += PIECE * p.o_ts;
+            if constexpr (KD > 128) {
+                v.give(vs[(j + 1) & 1] + o, (j + 1) * PIECE + 16 * o + 4 * g, span.count);
+                v.ask(vb, p.v_ts, (j + 2) * PIECE + 16 * o + 4 * g, span.count);
+            }
         }
         return;
     }
 
-    const T *vb = (const T *)p.v + ((int64_t)span.first + from * PIECE) * p.v_ts + h * p.v_hs + c0;
-    const int v_ts = (int)p.v_ts;
-    int v_at[4];
+    uint32_t kb = ws.k + key0 + w * NW * NP * 1024;
+    uint32_t wb = ws.w + (val0 * Keys::TILES + w * NT) * 2 * 3 * 1024;
+    const uint32_t w_step = (uint32_t)p.value_heads * Keys::TILES * 2 * 3 * 1024;
+    dr_u4 kf[4][NW][NP], wf[NT][2][3];
+    lq_f4 cf;
+    float lf;
+    const auto ask_k = [&]() {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v_at[e] = (my + e) * v_ts + m;
-    dr_u4 ktf[NT][2][NP];
-    T vf[4];
-    float4 cf;
-    float2 lf;
-    const auto ask_rows = [&](int n) {
-        cf = *reinterpret_cast<const float4 *>(rb + 4 * my);
-        lf = *reinterpret_cast<const float2 *>(rb + 8 * PIECE);
-        // (rows behind the last one read the first)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) vf[e] = vb[my + e < n ? v_at[e] : m];
+            for (int s = 0; s < NW; ++s)
+#pragma unroll
+                for (int i = 0; i < NP; ++i) kf[t][s][i] = block(kb, (t * NS + s) * NP + i);
     };
-    const auto ask_kt = [&]() {
+    const auto ask_rows = [&]() {
+        cf = factors(0, 16 * w);
+        lf = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(wsrc, 0, (int)(rb + 8 * PIECE), 0));
+    };
+    const auto ask_w = [&]() {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int i = 0; i < NP; ++i) ktf[t][s][i] = block(ktb, (t * 2 + s) * NP + i);
+                for (int i = 0; i < 3; ++i) wf[t][s][i] = block(wb, (t * 2 + s) * 3 + i);
     };
-    float *state = r.state + ((span.slot * p.value_heads + h) * KD + w * NT * 16) * p.vd + c0 + m;
+    float *state = r.state + (span.slot * p.value_heads + h) * (int64_t)KD * p.vd + c0 + m;
     lq_f4 S[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            S[t][e] = from == 0 && span.fresh ? 0.0f : state[(int64_t)(16 * t + 4 * g + e) * p.vd];
-    for (int j = from; j < to;) {
-        ask_x();
-        ask_rows(span.count - j * PIECE);
-        ask_t();
-        ask_kt();
-        for (; j < to; ++j) {
-            const int n = min(span.count - j * PIECE, PIECE);
-            const bool more = j + 1 < to;     // the last piece's are asked for again and not used
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                dr_u2 y[3];
-                dr_split4(S[t], y);
-                const int tile = w * NT + t;
-#pragma unroll
-                for (int i = 0; i < 3; ++i) reinterpret_cast<dr_u2 *>(&ss[tile >> 1][i][lane])[tile & 1] = y[i];
-            }
-            __syncthreads();     // S
-            const lq_f4 kS = with_state();
-            xb += more ? key_step : 0;
-            ask_x();
-            const float cv[4] = {cf.x, cf.y, cf.z, cf.w}, last = lf.x;
-            lq_f4 R;
-            bool odd = lf.y != 0.0f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                R[e] = (my + e < n ? (float)vf[e] : 0.0f) - cv[e] * kS[e];
-                odd |= !(fabsf(R[e]) <= RULE_WILD * RULE_WILD);     // v, or S, whose products with k are in it
-            }
-            put(rs, R);
-            const bool any = __any(odd);
-            if (lane == 0) wild_s[w] = any;
-            vb += more ? PIECE * p.v_ts : 0;
-            rb += more ? (int64_t)p.value_heads * 12 * PIECE : 0;
-            ask_rows(more ? span.count - (j + 1) * PIECE : n);
-            __syncthreads();     // R
-            put(us, with_rows());
-            tb += more ? tri_step : 0;
-            ask_t();
-            __syncthreads();     // U
-            const int bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3];
-            dr_u4 y[2][3];
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int i = 0; i < 3; ++i) y[s][i] = us[s][i][lane];
-            if (__builtin_amdgcn_readfirstlane(bad)) break;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                lq_f4 c[3] = {};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) c[0][e] = last * S[t][e];
-#pragma unroll
-                for (int s = 0; s < 2; ++s) dr_product<NP, 3>(ktf[t][s], y[s], c);
-                S[t] = dr_total(c);
-            }
-            ktb += more ? key_step : 0;
-            ask_kt();
-        }
-        if (j >= to) break;
-        // token by token, as delta_token_kernel: piece j, with S as it was (what was asked for of the next is asked again)
+            S[t][e] = from == 0 && span.fresh ? 0.0f : state[(int64_t)Keys::at(w * NT + t, 4 * g + e) * p.vd];
+    ask_k();
+    dr_hold();
+    ask_rows();
+    dr_hold();
+    ask_w();
+    dr_hold();
+    for (int j = from; j < to; ++j) {
         const int n = min(span.count - j * PIECE, PIECE);
-        const int64_t row0 = (int64_t)span.first + j * PIECE;
-        const T *kp = (const T *)p.k + row0 * p.k_ts + kh * p.k_hs, *qp = (const T *)p.q + row0 * p.q_ts + kh * p.q_hs;
-        const T *vp = (const T *)p.v + row0 * p.v_ts + h * p.v_hs + c0 + m;
-        T *op = (T *)p.out + row0 * p.o_ts + h * p.o_hs + c0 + m;
-        for (int t = 0; t < n; ++t) {
-            const int par = t & 1;
-            constexpr int E = KD / 64;
-            float kk = 0.0f, qq = 0.0f, kdq = 0.0f;
+        const bool more = j + 1 < to;     // the last piece's are asked for again and not used
+        lq_f4 c[4] = {};
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float kv = (float)kp[t * p.k_ts + lane * E + e], qv = (float)qp[t * p.q_ts + lane * E + e];
-                if (w == 0) kq[par][0][lane * E + e] = kv;
-                if (w == 1) kq[par][1][lane * E + e] = qv;
-                kk += kv * kv;
-                qq += qv * qv;
-                kdq += kv * qv;
+        for (int s = 0; s < NW; ++s) {
+            dr_u2 lo[3], hi[3] = {};
+            dr_split4(S[NT > 1 ? 2 * s : 0], lo);
+            if (NT > 1) dr_split4(S[NT > 1 ? 2 * s + 1 : 0], hi);
+            dr_u4 z[3];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                z[i] = dr_u4{lo[i][0], lo[i][1], hi[i][0], hi[i][1]};
+                ss[w * NW + s][i][lane] = z[i];
             }
-            kk = group_sum<64>(kk);
-            qq = group_sum<64>(qq);
-            kdq = group_sum<64>(kdq);
-            const float nk = p.norm_eps >= 0.0f ? 1.0f / sqrtf(kk + p.norm_eps) : 1.0f;
-            const float nq = (p.norm_eps >= 0.0f ? 1.0f / sqrtf(qq + p.norm_eps) : 1.0f) * p.scale;
-            const float2 gb = rule_gates(p, row0 + t, h);
-            const float f = expf(gb.x), v = (float)vp[t * p.v_ts];
-            __syncthreads();
-            float pk = 0.0f, pq = 0.0f;
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
+            for (int i = 2; i >= 0; --i)     // the smallest products first
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int row = (w * NT + i) * 16 + 4 * g + e;
-                    S[i][e] *= f;
-                    pk += S[i][e] * kq[par][0][row];
-                    pq += S[i][e] * kq[par][1][row];
-                }
-            pk = dr_rows_sum(pk);
-            pq = dr_rows_sum(pq);
-            if (g == 0) {
-                red[par][w][0][m] = pk;
-                red[par][w][1][m] = pq;
-            }
-            __syncthreads();
-            pk = (red[par][0][0][m] + red[par][1][0][m]) + (red[par][2][0][m] + red[par][3][0][m]);
-            pq = (red[par][0][1][m] + red[par][1][1][m]) + (red[par][2][1][m] + red[par][3][1][m]);
-            const float d = (v - pk * nk) * gb.y;
+                for (int u = 0; u < NP; ++u)
+                    if (u <= i)
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) S[i][e] += kq[par][0][(w * NT + i) * 16 + 4 * g + e] * nk * d;
-            if (threadIdx.x < 16) op[(int64_t)t * p.o_ts] = (T)(pq * nq + d * (kdq * nk * nq));
+                        for (int t = 0; t < 4; ++t) c[t] = dr_mfma(kf[t][s][u], z[i - u], c[t]);
         }
-        ++j;
-        ktb += key_step;     // (the other operands' places are the next piece's already)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) part[w][t][lane] = c[t];
+        dr_hold();
+        kb += more ? key_step : 0;
+        ask_k();
+        __syncthreads();     // S
+        const lq_f4 kS = (part[0][w][lane] + part[1][w][lane]) + (part[2][w][lane] + part[3][w][lane]);
+        const lq_f4 R = vs[j & 1][w][lane] - cf * kS;
+        lq_f4 next[NT];
+        bool odd = lf != lf;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) next[t] = lf * S[t];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd |= !(fabsf(R[e]) <= RULE_WILD * RULE_WILD);     // v, or S, whose products with k are in it
+        dr_u2 x[3];
+        dr_split4(R, x);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) reinterpret_cast<dr_u2 *>(&rs[w >> 1][i][lane])[w & 1] = x[i];
+        const bool any = __any(odd);
+        if (lane == 0) wild_s[w] = any;
+        dr_hold();
+        rb += more ? row_step : 0;
+        ask_rows();
+        __syncthreads();     // R
+        const int bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3];
+        dr_u4 y[2][3];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < 3; ++i) y[s][i] = rs[s][i][lane];
+        if (__builtin_amdgcn_readfirstlane(bad)) {
+            // token by token, as delta_token_kernel: piece j, with S as it was
+            const int64_t row0 = (int64_t)span.first + j * PIECE;
+            const T *kp = (const T *)p.k + row0 * p.k_ts + kh * p.k_hs, *qp = (const T *)p.q + row0 * p.q_ts + kh * p.q_hs;
+            const T *vp = (const T *)p.v + row0 * p.v_ts + h * p.v_hs + c0 + m;
+            T *op = (T *)p.out + row0 * p.o_ts + h * p.o_hs + c0 + m;
+            for (int t = 0; t < n; ++t) {
+                const int par = t & 1;
+                constexpr int E = KD / 64;
+                float kk = 0.0f, qq = 0.0f, kdq = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float kv = (float)kp[t * p.k_ts + lane * E + e], qv = (float)qp[t * p.q_ts + lane * E + e];
+                    if (w == 0) kq[par][0][lane * E + e] = kv;
+                    if (w == 1) kq[par][1][lane * E + e] = qv;
+                    kk += kv * kv;
+                    qq += qv * qv;
+                    kdq += kv * qv;
+                }
+                kk = group_sum<64>(kk);
+                qq = group_sum<64>(qq);
+                kdq = group_sum<64>(kdq);
+                const float nk = p.norm_eps >= 0.0f ? 1.0f / sqrtf(kk + p.norm_eps) : 1.0f;
+                const float nq = (p.norm_eps >= 0.0f ? 1.0f / sqrtf(qq + p.norm_eps) : 1.0f) * p.scale;
+                const float2 gb = rule_gates(p, row0 + t, h);
+                const float f = expf(gb.x), v = (float)vp[t * p.v_ts];
+                __syncthreads();
+                float pk = 0.0f, pq = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int row = Keys::at(w * NT + i, 4 * g + e);
+                        S[i][e] *= f;
+                        pk += S[i][e] * kq[par][0][row];
+                        pq += S[i][e] * kq[par][1][row];
+                    }
+                pk = dr_rows_sum(pk);
+                pq = dr_rows_sum(pq);
+                if (g == 0) {
+                    red[par][w][0][m] = pk;
+                    red[par][w][1][m] = pq;
+                }
+                __syncthreads();
+                pk = (red[par][0][0][m] + red[par][1][0][m]) + (red[par][2][0][m] + red[par][3][0][m]);
+                pq = (red[par][0][1][m] + red[par][1][1][m]) + (red[par][2][1][m] + red[par][3][1][m]);
+                const float d = (v - pk * nk) * gb.y;
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) S[i][e] += kq[par][0][Keys::at(w * NT + i, 4 * g + e)] * nk * d;
+                if (threadIdx.x < 16) op[(int64_t)t * p.o_ts] = (T)(pq * nq + d * (kdq * nk * nq));
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                lq_f4 d[3] = {next[t]};
+#pragma unroll
+                for (int s = 0; s < 2; ++s) dr_product<3, 3>(wf[t][s], y[s], d);
+                S[t] = dr_total(d);
+            }
+        }
+        dr_hold();
+        wb += more ? w_step : 0;
+        ask_w();
+        dr_hold();
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) state[(int64_t)(16 * t + 4 * g + e) * p.vd] = S[t][e];
+        for (int e = 0; e < 4; ++e) state[(int64_t)Keys::at(w * NT + t, 4 * g + e) * p.vd] = S[t][e];
 }
 
 constexpr int RULE_LEAST = 5;              // tokens of a request below which the token kernel takes it
 constexpr int64_t RULE_WINDOW = 64 << 20;  // bytes of workspace that a window of pieces may fill
 
+static int64_t key_bytes(int np, int kd) { return 4 * (kd == 64 ? 4 : kd / 32) * np * 1024; }     // a piece's K, or Q
 static int64_t piece_bytes(int np, int key_heads, int value_heads, int kd) {
-    return (int64_t)key_heads * 3 * 2 * PIECE * kd * np + (int64_t)value_heads * (2 * TRI * 3 * 1024 + 3 * PIECE * 4);
+    return 2 * key_heads * key_bytes(np, kd) + value_heads * ((kd / 16 * 2 + TRI) * 3 * 1024 + 12 * PIECE);
 }
 // pieces of a call, and of a window
 static int64_t all_pieces(int64_t tokens, int requests) { return tokens / PIECE + requests; }
@@ -843,14 +1021,15 @@ static void rule_launch(const DeltaRule &p, const DeltaRequests &r, void *ws, hi
     const int64_t bytes = piece_bytes(NP, p.key_heads, p.value_heads, KD), all = all_pieces(r.tokens, r.requests);
     const int64_t window = window_pieces(all, bytes);
     RuleWork w{};
-    const int64_t operands = window * p.key_heads * 2 * PIECE * KD * NP, tri = window * p.value_heads * TRI * 3 * 1024;
-    char *at = (char *)ws;
-    w.k = (dr_u4 *)at;
-    w.q = (dr_u4 *)(at + operands);
-    w.kt = (dr_u4 *)(at + 2 * operands);
-    w.t = (dr_u4 *)(at + 3 * operands);
-    w.p = (dr_u4 *)(at + 3 * operands + tri);
-    w.rows = (float *)(at + 3 * operands + 2 * tri);
+    const int64_t keys = window * p.key_heads * key_bytes(NP, KD), tiles = window * p.value_heads * 3 * 1024;
+    uint32_t at = 0;     // (a window is far below 4 GB)
+    w.base = (char *)ws;
+    w.k = at;
+    w.q = at += (uint32_t)keys;
+    w.w = at += (uint32_t)keys;
+    w.p = at += (uint32_t)(tiles * (KD / 16 * 2));
+    w.rows = at += (uint32_t)(tiles * TRI);
+    w.bytes = (uint32_t)(window * bytes);
     // (one request may also have few tokens: its pieces serve any number)
     w.least = r.requests > 1 ? RULE_LEAST : 1;
     if (w.least > 1) token_columns<T, KD>(p, r, w.least - 1, s);
@@ -861,7 +1040,7 @@ static void rule_launch(const DeltaRule &p, const DeltaRequests &r, void *ws, hi
         const dim3 grid((unsigned)(w.pieces * p.key_heads), (unsigned)group);
         hipLaunchKernelGGL((delta_piece_kernel<T, KD>), grid, dim3(256), 0, s, p, r, w);
         const int64_t units = ((int64_t)r.requests * p.key_heads + 7) / 8 * 8;
-        hipLaunchKernelGGL((delta_chain_kernel<T, KD>), dim3((unsigned)(units * group * (p.vd / 16))), dim3(512), 0, s, p, r,
+        hipLaunchKernelGGL((delta_chain_kernel<T, KD>), dim3((unsigned)(units * group * (p.vd / 16))), dim3(RULE_CHAIN), 0, s, p, r,
                            w);
     }
 }
