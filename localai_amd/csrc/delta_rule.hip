@@ -605,10 +605,15 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
     }
 }
 
-// Requests stay where they are written: moved ahead of the last use of what they
-// replace, they would need registers of their own and copies that wait for them
-// (measured: 8192 tokens, 2.1 us a piece with the compiler's order).
-__device__ __forceinline__ void dr_hold() {
+// Requests stay behind what makes the values x, the last uses of what they
+// replace: moved ahead of one, they need registers of their own, and copies at the
+// loop's end that wait for all of them (8192 tokens, 32 heads of 128: 2.0 us a piece
+// so, ___ as it is).
+template <typename X>
+__device__ __forceinline__ void dr_pin(X &x) { asm volatile("" : "+v"(x)); }
+template <typename... X>
+__device__ __forceinline__ void dr_hold(X &...x) {
+    (dr_pin(x), ...);
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
 }
@@ -700,7 +705,9 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
     uint32_t rb = ws.rows + val0 * 12 * PIECE;
     const int lane16 = lane * 16;
     const auto block = [&](uint32_t at, int i) {
-        return __builtin_bit_cast(dr_u4, __builtin_amdgcn_raw_buffer_load_b128(wsrc, lane16, (int)(at + i * 1024), 0));
+        const auto x = __builtin_amdgcn_raw_buffer_load_b128(wsrc, lane16, (int)(at + i * 1024), 0);
+        dr_hold();     // in this order everywhere: a wait has to hold for each way to it
+        return __builtin_bit_cast(dr_u4, x);
     };
     // four factors of rows row .. row + 3 of set s
     const auto factors = [&](int s, int row) {
@@ -708,14 +715,16 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
     };
 
     if (w > 3) {
-        const int o = (w - 4) * OT;                                    // row tiles o .. o + OT - 1
-        const bool upper = o > 1;                                      // their rows of P T have two blocks
-        uint32_t qb = ws.q + key0 + o * NS * NP * 1024;
-        uint32_t pb = ws.p + (val0 * TRI + (upper ? 2 * o - 2 : o)) * 3 * 1024;
+        // the row tiles: of two waves 0 and 3, 1 and 2, which have three blocks of P T together
+        const int o = w - 4;
+        const auto tile = [&](int t) { return t ? 3 - o : o; };
+        const bool upper = o > 1;                                      // its one tile has two blocks
+        uint32_t qb = ws.q + key0, pb = ws.p + val0 * TRI * 3 * 1024;
         const uint32_t tri_step = (uint32_t)p.value_heads * TRI * 3 * 1024;
         T *ob = (T *)p.out + ((int64_t)span.first + from * PIECE) * p.o_ts + h * p.o_hs + c0;
         const int o_ts = (int)p.o_ts;
-        dr_u4 qf[OT][NS][NP], pf[OT][2][3];
+        constexpr int PB = OT + 1;      // blocks of P T: the first tile's, the last one's two
+        dr_u4 qf[OT][NS][NP], pf[PB][3];
         lq_f4 of[OT];
         const auto ask_q = [&]() {
 #pragma unroll
@@ -723,17 +732,18 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
 #pragma unroll
                 for (int s = 0; s < NS; ++s)
 #pragma unroll
-                    for (int i = 0; i < NP; ++i) qf[t][s][i] = block(qb, (t * NS + s) * NP + i);
+                    for (int i = 0; i < NP; ++i) qf[t][s][i] = block(qb + tile(t) * NS * NP * 1024, s * NP + i);
 #pragma unroll
-            for (int t = 0; t < OT; ++t) of[t] = factors(1, 16 * (o + t));
+            for (int t = 0; t < OT; ++t) of[t] = factors(1, 16 * tile(t));
         };
-        const auto ask_p = [&]() {     // (row tiles 0 and 1 have one block: it twice)
+        // where a tile's blocks begin: 0, 1, 2, 4
+        const auto first = [](int t) { return t < 2 ? t : 2 * t - 2; };
+        const auto ask_p = [&]() {     // (OT 1: row tiles 0 and 1 have one block, it twice)
 #pragma unroll
-            for (int t = 0; t < OT; ++t)
+            for (int s = 0; s < PB; ++s)
 #pragma unroll
-                for (int s = 0; s < 2; ++s)
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) pf[t][s][i] = block(pb, (upper ? 2 * t + s : t) * 3 + i);
+                for (int i = 0; i < 3; ++i)
+                    pf[s][i] = block(pb + 3072 * (OT == 1 ? first(o) + (upper ? s : 0) : s ? first(3 - o) + s - 1 : o), i);
         };
         RuleValues<T, OT> v;      // of 256 key values
         ask_q();
@@ -761,9 +771,11 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
                     for (int t = 0; t < OT; ++t) dr_product<NP, 3>(qf[t][s], z, c[t]);
                 }
 #pragma unroll
-                for (int t = 0; t < OT; ++t) O[t] = dr_total(c[t]) * of[t];
+                for (int t = 0; t < OT; ++t) {
+                    O[t] = dr_total(c[t]) * of[t];
+                    dr_hold(O[t]);
+                }
             }
-            dr_hold();
             qb += more ? key_step : 0;
             rb += more ? row_step : 0;
             ask_q();
@@ -778,12 +790,12 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
                     for (int i = 0; i < 3; ++i) y[s][i] = rs[s][i][lane];
 #pragma unroll
                 for (int t = 0; t < OT; ++t) {
-                    dr_product<3, 3>(pf[t][0], y[0], c[t]);
-                    if (upper) dr_product<3, 3>(pf[t][1], y[1], c[t]);
+                    dr_product<3, 3>(pf[t], y[0], c[t]);
+                    if (OT == 1 ? upper : t) dr_product<3, 3>(pf[t + 1], y[1], c[t]);
                     O[t] = O[t] + dr_total(c[t]);
+                    dr_hold(O[t]);
                 }
             }
-            dr_hold();
             pb += more ? tri_step : 0;
             ask_p();
             dr_hold();
@@ -797,7 +809,7 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const T y = (T)O[t][e];
-                        const int at = ((16 * (o + t) + 4 * g + e) * o_ts + m) * (int)sizeof(T);
+                        const int at = ((16 * tile(t) + 4 * g + e) * o_ts + m) * (int)sizeof(T);
                         if constexpr (sizeof(T) == 4)
                             __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, y), dst, at, 0, 0);
                         else
@@ -813,6 +825,7 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
         return;
     }
 
+    __builtin_amdgcn_s_setprio(3);      // ahead of the other waves, which have time to spare
     uint32_t kb = ws.k + key0 + w * NW * NP * 1024;
     uint32_t wb = ws.w + (val0 * Keys::TILES + w * NT) * 2 * 3 * 1024;
     const uint32_t w_step = (uint32_t)p.value_heads * Keys::TILES * 2 * 3 * 1024;
@@ -846,131 +859,142 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             S[t][e] = from == 0 && span.fresh ? 0.0f : state[(int64_t)Keys::at(w * NT + t, 4 * g + e) * p.vd];
-    ask_k();
-    dr_hold();
-    ask_rows();
-    dr_hold();
-    ask_w();
-    dr_hold();
-    for (int j = from; j < to; ++j) {
-        const int n = min(span.count - j * PIECE, PIECE);
-        const bool more = j + 1 < to;     // the last piece's are asked for again and not used
-        lq_f4 c[4] = {};
-#pragma unroll
-        for (int s = 0; s < NW; ++s) {
-            dr_u2 lo[3], hi[3] = {};
-            dr_split4(S[NT > 1 ? 2 * s : 0], lo);
-            if (NT > 1) dr_split4(S[NT > 1 ? 2 * s + 1 : 0], hi);
-            dr_u4 z[3];
-#pragma unroll
-            for (int i = 0; i < 3; ++i) {
-                z[i] = dr_u4{lo[i][0], lo[i][1], hi[i][0], hi[i][1]};
-                ss[w * NW + s][i][lane] = z[i];
-            }
-#pragma unroll
-            for (int i = 2; i >= 0; --i)     // the smallest products first
-#pragma unroll
-                for (int u = 0; u < NP; ++u)
-                    if (u <= i)
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) c[t] = dr_mfma(kf[t][s][u], z[i - u], c[t]);
-        }
-#pragma unroll
-        for (int t = 0; t < 4; ++t) part[w][t][lane] = c[t];
-        dr_hold();
-        kb += more ? key_step : 0;
+    for (int j = from; j < to;) {
         ask_k();
-        __syncthreads();     // S
-        const lq_f4 kS = (part[0][w][lane] + part[1][w][lane]) + (part[2][w][lane] + part[3][w][lane]);
-        const lq_f4 R = vs[j & 1][w][lane] - cf * kS;
-        lq_f4 next[NT];
-        bool odd = lf != lf;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) next[t] = lf * S[t];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) odd |= !(fabsf(R[e]) <= RULE_WILD * RULE_WILD);     // v, or S, whose products with k are in it
-        dr_u2 x[3];
-        dr_split4(R, x);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) reinterpret_cast<dr_u2 *>(&rs[w >> 1][i][lane])[w & 1] = x[i];
-        const bool any = __any(odd);
-        if (lane == 0) wild_s[w] = any;
         dr_hold();
-        rb += more ? row_step : 0;
         ask_rows();
-        __syncthreads();     // R
-        const int bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3];
-        dr_u4 y[2][3];
+        dr_hold();
+        ask_w();
+        dr_hold();
+        for (; j < to; ++j) {
+            const bool more = j + 1 < to;     // the last piece's are asked for again and not used
+            lq_f4 c[4] = {};
+            kb += more ? key_step : 0;
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+            for (int s = 0; s < NW; ++s) {
+                dr_u2 lo[3], hi[3] = {};
+                dr_split4(S[NT > 1 ? 2 * s : 0], lo);
+                if (NT > 1) dr_split4(S[NT > 1 ? 2 * s + 1 : 0], hi);
+                dr_u4 z[3];
 #pragma unroll
-            for (int i = 0; i < 3; ++i) y[s][i] = rs[s][i][lane];
-        if (__builtin_amdgcn_readfirstlane(bad)) {
-            // token by token, as delta_token_kernel: piece j, with S as it was
-            const int64_t row0 = (int64_t)span.first + j * PIECE;
-            const T *kp = (const T *)p.k + row0 * p.k_ts + kh * p.k_hs, *qp = (const T *)p.q + row0 * p.q_ts + kh * p.q_hs;
-            const T *vp = (const T *)p.v + row0 * p.v_ts + h * p.v_hs + c0 + m;
-            T *op = (T *)p.out + row0 * p.o_ts + h * p.o_hs + c0 + m;
-            for (int t = 0; t < n; ++t) {
-                const int par = t & 1;
-                constexpr int E = KD / 64;
-                float kk = 0.0f, qq = 0.0f, kdq = 0.0f;
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float kv = (float)kp[t * p.k_ts + lane * E + e], qv = (float)qp[t * p.q_ts + lane * E + e];
-                    if (w == 0) kq[par][0][lane * E + e] = kv;
-                    if (w == 1) kq[par][1][lane * E + e] = qv;
-                    kk += kv * kv;
-                    qq += qv * qv;
-                    kdq += kv * qv;
+                for (int i = 0; i < 3; ++i) {
+                    z[i] = dr_u4{lo[i][0], lo[i][1], hi[i][0], hi[i][1]};
+                    ss[w * NW + s][i][lane] = z[i];
                 }
-                kk = group_sum<64>(kk);
-                qq = group_sum<64>(qq);
-                kdq = group_sum<64>(kdq);
-                const float nk = p.norm_eps >= 0.0f ? 1.0f / sqrtf(kk + p.norm_eps) : 1.0f;
-                const float nq = (p.norm_eps >= 0.0f ? 1.0f / sqrtf(qq + p.norm_eps) : 1.0f) * p.scale;
-                const float2 gb = rule_gates(p, row0 + t, h);
-                const float f = expf(gb.x), v = (float)vp[t * p.v_ts];
-                __syncthreads();
-                float pk = 0.0f, pq = 0.0f;
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
+                for (int i = 2; i >= 0; --i)     // the smallest products first
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int row = Keys::at(w * NT + i, 4 * g + e);
-                        S[i][e] *= f;
-                        pk += S[i][e] * kq[par][0][row];
-                        pq += S[i][e] * kq[par][1][row];
-                    }
-                pk = dr_rows_sum(pk);
-                pq = dr_rows_sum(pq);
-                if (g == 0) {
-                    red[par][w][0][m] = pk;
-                    red[par][w][1][m] = pq;
-                }
-                __syncthreads();
-                pk = (red[par][0][0][m] + red[par][1][0][m]) + (red[par][2][0][m] + red[par][3][0][m]);
-                pq = (red[par][0][1][m] + red[par][1][1][m]) + (red[par][2][1][m] + red[par][3][1][m]);
-                const float d = (v - pk * nk) * gb.y;
+                    for (int u = 0; u < NP; ++u)
+                        if (u <= i)
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
+                            for (int t = 0; t < 4; ++t) {
+                                c[t] = dr_mfma(kf[t][s][u], z[i - u], c[t]);
+                                if (i == 0) {     // piece 0 is the last use of a tile's pieces
+                                    dr_hold();
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) S[i][e] += kq[par][0][Keys::at(w * NT + i, 4 * g + e)] * nk * d;
-                if (threadIdx.x < 16) op[(int64_t)t * p.o_ts] = (T)(pq * nq + d * (kdq * nk * nq));
+                                    for (int v = 0; v < NP; ++v) kf[t][s][v] = block(kb, (t * NS + s) * NP + v);
+                                    dr_hold();
+                                }
+                            }
             }
-        } else {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) part[w][t][lane] = c[t];
+            __syncthreads();     // S
+            const lq_f4 kS = (part[0][w][lane] + part[1][w][lane]) + (part[2][w][lane] + part[3][w][lane]);
+            const lq_f4 R = vs[j & 1][w][lane] - cf * kS;
+            lq_f4 next[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) next[t] = lf * S[t];
+            // of v, or of S, whose products with k are in it; NaN where lf is
+            const float size = fabsf(R[0]) + fabsf(R[1]) + fabsf(R[2]) + (fabsf(R[3]) + lf);
+            dr_u2 x[3];
+            dr_split4(R, x);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) reinterpret_cast<dr_u2 *>(&rs[w >> 1][i][lane])[w & 1] = x[i];
+            const bool any = __any(!(size <= RULE_WILD * RULE_WILD));
+            if (lane == 0) wild_s[w] = any;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) dr_hold(next[t]);
+            rb += more ? row_step : 0;
+            ask_rows();
+            __syncthreads();     // R
+            const int bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3];
+            dr_u4 y[2][3];
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 3; ++i) y[s][i] = rs[s][i][lane];
+            wb += more ? w_step : 0;
+            if (__builtin_amdgcn_readfirstlane(bad)) break;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 lq_f4 d[3] = {next[t]};
 #pragma unroll
-                for (int s = 0; s < 2; ++s) dr_product<3, 3>(wf[t][s], y[s], d);
+                for (int s = 0; s < 2; ++s) {
+                    dr_product<3, 3>(wf[t][s], y[s], d);
+                    dr_hold(d[0], d[1], d[2]);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) wf[t][s][i] = block(wb, (t * 2 + s) * 3 + i);
+                    dr_hold();
+                }
                 S[t] = dr_total(d);
             }
         }
-        dr_hold();
-        wb += more ? w_step : 0;
-        ask_w();
-        dr_hold();
+        if (j >= to) break;
+        // token by token, as delta_token_kernel: piece j, with S as it was
+        const int n = min(span.count - j * PIECE, PIECE);
+        const int64_t row0 = (int64_t)span.first + j * PIECE;
+        const T *kp = (const T *)p.k + row0 * p.k_ts + kh * p.k_hs, *qp = (const T *)p.q + row0 * p.q_ts + kh * p.q_hs;
+        const T *vp = (const T *)p.v + row0 * p.v_ts + h * p.v_hs + c0 + m;
+        T *op = (T *)p.out + row0 * p.o_ts + h * p.o_hs + c0 + m;
+        for (int t = 0; t < n; ++t) {
+            const int par = t & 1;
+            constexpr int E = KD / 64;
+            float kk = 0.0f, qq = 0.0f, kdq = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float kv = (float)kp[t * p.k_ts + lane * E + e], qv = (float)qp[t * p.q_ts + lane * E + e];
+                if (w == 0) kq[par][0][lane * E + e] = kv;
+                if (w == 1) kq[par][1][lane * E + e] = qv;
+                kk += kv * kv;
+                qq += qv * qv;
+                kdq += kv * qv;
+            }
+            kk = group_sum<64>(kk);
+            qq = group_sum<64>(qq);
+            kdq = group_sum<64>(kdq);
+            const float nk = p.norm_eps >= 0.0f ? 1.0f / sqrtf(kk + p.norm_eps) : 1.0f;
+            const float nq = (p.norm_eps >= 0.0f ? 1.0f / sqrtf(qq + p.norm_eps) : 1.0f) * p.scale;
+            const float2 gb = rule_gates(p, row0 + t, h);
+            const float f = expf(gb.x), v = (float)vp[t * p.v_ts];
+            __syncthreads();
+            float pk = 0.0f, pq = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int row = Keys::at(w * NT + i, 4 * g + e);
+                    S[i][e] *= f;
+                    pk += S[i][e] * kq[par][0][row];
+                    pq += S[i][e] * kq[par][1][row];
+                }
+            pk = dr_rows_sum(pk);
+            pq = dr_rows_sum(pq);
+            if (g == 0) {
+                red[par][w][0][m] = pk;
+                red[par][w][1][m] = pq;
+            }
+            __syncthreads();
+            pk = (red[par][0][0][m] + red[par][1][0][m]) + (red[par][2][0][m] + red[par][3][0][m]);
+            pq = (red[par][0][1][m] + red[par][1][1][m]) + (red[par][2][1][m] + red[par][3][1][m]);
+            const float d = (v - pk * nk) * gb.y;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) S[i][e] += kq[par][0][Keys::at(w * NT + i, 4 * g + e)] * nk * d;
+            if (threadIdx.x < 16) op[(int64_t)t * p.o_ts] = (T)(pq * nq + d * (kdq * nk * nq));
+        }
+        ++j;     // (the operands' places are the next piece's already)
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
