@@ -5,6 +5,8 @@
 //   S <- e^g S;  d = beta (v - S^T k^);  S <- S + k^ d^T;  o = S^T q^
 // g = decay, beta as given, or from projections: g = a softplus(decay + dt_bias),
 // beta = 1 / (1 + exp(-beta)). fp32 throughout; o rounded once to its type.
+#include <algorithm>
+
 #include "delta.h"
 #include "dev_common.h"
 #include "internal.h"
@@ -608,7 +610,7 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
 // Requests stay behind what makes the values x, the last uses of what they
 // replace: moved ahead of one, they need registers of their own, and copies at the
 // loop's end that wait for all of them (8192 tokens, 32 heads of 128: 2.0 us a piece
-// so, ___ as it is).
+// so, 1.8 as it is).
 template <typename X>
 __device__ __forceinline__ void dr_pin(X &x) { asm volatile("" : "+v"(x)); }
 template <typename... X>
@@ -1009,18 +1011,14 @@ static int64_t key_bytes(int np, int kd) { return 4 * (kd == 64 ? 4 : kd / 32) *
 static int64_t piece_bytes(int np, int key_heads, int value_heads, int kd) {
     return 2 * key_heads * key_bytes(np, kd) + value_heads * ((kd / 16 * 2 + TRI) * 3 * 1024 + 12 * PIECE);
 }
-// pieces of a call, and of a window
 static int64_t all_pieces(int64_t tokens, int requests) { return tokens / PIECE + requests; }
-static int64_t window_pieces(int64_t all, int64_t bytes) {
-    const int64_t most = RULE_WINDOW / bytes;
-    return all < most ? all : most > 1 ? most : 1;
-}
 
+// room for a window of fp32's pieces; 16-bit types' are smaller, so theirs may be longer
 int64_t delta_rule_workspace_bytes(int64_t tokens, int requests, bool step, int key_heads, int value_heads, int kd,
                                    int vd) {
     if (step) return 0;
-    const int64_t bytes = piece_bytes(3, key_heads, value_heads, kd);
-    return window_pieces(all_pieces(tokens, requests), bytes) * bytes;
+    const int64_t bytes = piece_bytes(3, key_heads, value_heads, kd), all = all_pieces(tokens, requests);
+    return std::min(all, std::max<int64_t>(RULE_WINDOW / bytes, 1)) * bytes;
 }
 
 template <typename T, int KD, int VS>
@@ -1043,7 +1041,7 @@ static void rule_launch(const DeltaRule &p, const DeltaRequests &r, void *ws, hi
     if (!r.starts) return token_columns<T, KD>(p, r, INT32_MAX, s);
     constexpr int NP = RuleType<T>::NP;
     const int64_t bytes = piece_bytes(NP, p.key_heads, p.value_heads, KD), all = all_pieces(r.tokens, r.requests);
-    const int64_t window = window_pieces(all, bytes);
+    const int64_t window = std::min(all, delta_rule_workspace_bytes(r.tokens, r.requests, false, p.key_heads, p.value_heads, KD, p.vd) / bytes);
     RuleWork w{};
     const int64_t keys = window * p.key_heads * key_bytes(NP, KD), tiles = window * p.value_heads * 3 * 1024;
     uint32_t at = 0;     // (a window is far below 4 GB)
