@@ -156,7 +156,7 @@ typedef uint32_t dr_u2 __attribute__((ext_vector_type(2)));
 constexpr int PIECE = 64;
 constexpr int TRI = 6;                 // 16 x 32 blocks of a lower triangular 64 x 64: row tile w has w / 2 + 1
 constexpr float RULE_WILD = 1e15f;     // values of q, k, v (squared: of S) past it go token by token
-constexpr float RULE_FAINT = 1e-12f;   // so do k and q whose largest value is below it
+constexpr float RULE_FAINT = 1e-24f;   // so do k and q whose squares' sum is below it, where norm_eps is too
 
 // pieces that hold a value of type T, and whether the norm's factor goes in first
 template <typename T> struct RuleType { static constexpr int NP = 1; };
@@ -202,24 +202,22 @@ __device__ __forceinline__ float dr_rows_max(float v) {
     return fmaxf(f(b[0]), f(b[1]));
 }
 
-// x as N bf16 pieces, the first its nearest, the next what is left
-template <int N>
-__device__ __forceinline__ void dr_split(float x, __bf16 (&p)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        p[i] = (__bf16)x;
-        x -= (float)p[i];
-    }
-}
+typedef __bf16 dr_b2 __attribute__((ext_vector_type(2)));
+typedef float dr_f2 __attribute__((ext_vector_type(2)));
+
+// eight values as N bf16 pieces each, the first the nearest, the next what is left (two values an instruction)
 template <int N>
 __device__ __forceinline__ void dr_split8(const float (&x)[8], dr_u4 (&y)[N]) {
-    __bf16 h[8][N];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) dr_split<N>(x[e], h[e]);
+    for (int e = 0; e < 4; ++e) {
+        dr_f2 left = {x[2 * e], x[2 * e + 1]};
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const dr_b8 v = {h[0][i], h[1][i], h[2][i], h[3][i], h[4][i], h[5][i], h[6][i], h[7][i]};
-        y[i] = __builtin_bit_cast(dr_u4, v);
+        for (int i = 0; i < N; ++i) {
+            const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_convertvector(left, dr_b2));
+            y[i][e] = h;
+            left[0] -= __builtin_bit_cast(float, h << 16);
+            left[1] -= __builtin_bit_cast(float, h & 0xffff0000u);
+        }
     }
 }
 // Three pieces by cutting bits off: exact too, a third fewer instructions, and
@@ -260,14 +258,17 @@ __device__ __forceinline__ float dr_exp2(double x) {
     return ldexpf(__builtin_amdgcn_exp2f((float)(x - whole)), (int)fmax(whole, -400.0));
 }
 
-// four or eight adjacent values (aligned to four)
+// four or eight adjacent values (aligned to four), in the lower bits of zeros
 template <typename T, int N>
-__device__ __forceinline__ void dr_load(const T *p, float (&x)[8]) {
-    struct __attribute__((packed, aligned(4 * sizeof(T)))) Raw { T v[N]; };
-    const Raw raw = *reinterpret_cast<const Raw *>(p);
+struct RuleRaw {
+    T v[8];
+    __device__ __forceinline__ void load(const T *p) {
+        struct __attribute__((packed, aligned(4 * sizeof(T)))) Raw { T v[N]; };
+        const Raw raw = *reinterpret_cast<const Raw *>(p);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = i < N ? (float)raw.v[i < N ? i : 0] : 0.0f;
-}
+        for (int i = 0; i < 8; ++i) v[i] = i < N ? raw.v[i < N ? i : 0] : (T)0.0f;
+    }
+};
 
 // one step of an inclusive sum over the wave's lanes, of fp64 values
 template <int CTRL, int ROWS>
@@ -288,7 +289,7 @@ __device__ __forceinline__ double dr_add_from(double v) {
 // the layout in which MFMA leaves two tiles of results, so those are operands
 // as they are.
 template <typename T, int KD>
-__global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
+__global__ __launch_bounds__(256, 2) void delta_piece_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
     typedef RuleKeys<KD> Keys;
     constexpr int NP = RuleType<T>::NP, NS = Keys::STEPS, NT = Keys::NT, LD = 68;
     // K's operands, then A (later T's operands, P, P T) and T
@@ -320,46 +321,45 @@ __global__ __launch_bounds__(256) void delta_piece_kernel(DeltaRule p, DeltaRequ
         const int64_t row = row0 + (in ? 16 * w + m : 0);
         constexpr int V = KD == 64 ? 4 : 8;      // adjacent values of a lane's step
         const T *rows[2] = {(const T *)p.k + row * p.k_ts + kh * p.k_hs + V * g, (const T *)p.q + row * p.q_ts + kh * p.q_hs + V * g};
-        float x[2][NS][8];
+        RuleRaw<T, V> raw[2][NS];
 #pragma unroll
         for (int o = 0; o < 2; ++o)
 #pragma unroll
-            for (int s = 0; s < NS; ++s) dr_load<T, V>(rows[o] + 4 * V * s, x[o][s]);
+            for (int s = 0; s < NS; ++s) raw[o][s].load(rows[o] + 4 * V * s);
         gb = lane < n ? rule_gates(p, row0 + lane, h) : make_float2(0, 0);     // one token a lane
 #pragma unroll
         for (int o = 0; o < 2; ++o) {
-            float ss = 0.0f, top = 0.0f;
+            float x[NS][8], ss = 0.0f;
 #pragma unroll
             for (int s = 0; s < NS; ++s)
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    x[o][s][e] = in ? x[o][s][e] : 0.0f;
-                    ss += x[o][s][e] * x[o][s][e];
-                    top = fmaxf(top, fabsf(x[o][s][e]));
+                    x[s][e] = (float)raw[o][s].v[e];
+                    ss += x[s][e] * x[s][e];
                 }
-            ss = dr_rows_sum(ss);
-            top = dr_rows_max(top);
-            // (a NaN is in the sum, not in the largest)
-            wild |= !(ss <= RULE_WILD * RULE_WILD) || (top > 0.0f && top < RULE_FAINT);
+            ss = in ? dr_rows_sum(ss) : 0.0f;
+            // (values whose squares vanish: what they meet vanishes too, but for a norm that makes them large again)
+            wild |= !(ss <= RULE_WILD * RULE_WILD) || (in && ss < RULE_FAINT && !(p.norm_eps >= RULE_FAINT));
             float inv = norm ? 1.0f / sqrtf(ss + p.norm_eps) : 1.0f;
             if (norm && !(inv <= 3.4e38f)) {     // a row of zeros and norm_eps 0: 0 / 0
                 wild |= in;
                 inv = 0.0f;
             }
             if (!o && g == 0) kn[16 * w + m] = ss * inv * inv;     // |k^|^2
-            if (NP == 3) {
-#pragma unroll
-                for (int s = 0; s < NS; ++s)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) x[o][s][e] *= inv;
-                inv = 1.0f;
-            }
-            if (g == 0) (o ? iq : ik)[16 * w + m] = inv;
+            const float by = !in ? 0.0f : NP == 3 ? inv : 1.0f;
+            if (g == 0) (o ? iq : ik)[16 * w + m] = NP == 3 ? 1.0f : inv;
             dr_u4 *dst = (dr_u4 *)(ws.base + (o ? ws.q : ws.k)) + (((int64_t)local * p.key_heads + kh) * 4 + w) * NS * NP * 64 + lane;
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
                 dr_u4 y[NP];
-                dr_split8<NP>(x[o][s], y);
+                if constexpr (NP == 1) {     // the values' own bits
+                    __builtin_memcpy(y, raw[o][s].v, 16);
+                    if (!in) y[0] = dr_u4{0, 0, 0, 0};
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[s][e] = e < V && in ? x[s][e] * by : 0.0f;
+                    dr_split8<NP>(x[s], y);
+                }
 #pragma unroll
                 for (int i = 0; i < NP; ++i) {
                     if (o) qf[s][i] = y[i];
