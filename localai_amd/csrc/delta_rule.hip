@@ -289,7 +289,7 @@ __device__ __forceinline__ double dr_add_from(double v) {
 // the layout in which MFMA leaves two tiles of results, so those are operands
 // as they are.
 template <typename T, int KD>
-__global__ __launch_bounds__(256, 2) void delta_piece_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
+__global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
     typedef RuleKeys<KD> Keys;
     constexpr int NP = RuleType<T>::NP, NS = Keys::STEPS, NT = Keys::NT, LD = 68;
     // K's operands, then A (later T's operands, P, P T) and T
@@ -620,25 +620,31 @@ __device__ __forceinline__ void dr_hold(X &...x) {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// v of N row tiles from tile t0 on, as R takes it (0 behind the last row)
+// What R takes of N row tiles: v (0 behind the last row) and the factors of K S, with
+// the piece's e^G_last behind its 64.
 template <typename T, int N>
 struct RuleValues {
     T v[N][4];
-    // rows of the call's v from the request's first one on, and how many there are
-    __device__ __forceinline__ void ask(const T *vb, int64_t ts, int row0, int rows) {
+    float c, last;
+    // vb, rows: the request's v and the piece's factors; row0: the lane's first row, of `count`; first: the tiles' in the piece
+    __device__ __forceinline__ void ask(const T *vb, int64_t ts, int row0, int count, const float *rows, int first) {
 #pragma unroll
         for (int t = 0; t < N; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[t][e] = vb[(int64_t)min(row0 + 16 * t + e, rows - 1) * ts];
+            for (int e = 0; e < 4; ++e) v[t][e] = vb[(int64_t)min(row0 + 16 * t + e, count - 1) * ts];
+        c = rows[first + lane_id() % (16 * N)];
+        last = rows[2 * PIECE];
     }
-    __device__ __forceinline__ void give(lq_f4 (*dst)[64], int row0, int rows) {
+    __device__ __forceinline__ void give(lq_f4 (*dst)[64], float *factors, int row0, int count, int first) {
 #pragma unroll
         for (int t = 0; t < N; ++t) {
             lq_f4 x;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = row0 + 16 * t + e < rows ? (float)v[t][e] : 0.0f;
+            for (int e = 0; e < 4; ++e) x[e] = row0 + 16 * t + e < count ? (float)v[t][e] : 0.0f;
             dst[t][lane_id()] = x;
         }
+        if (lane_id() < 16 * N) factors[first + lane_id()] = c;
+        if (first == 0 && lane_id() == 0) factors[PIECE] = last;
     }
 };
 
@@ -649,7 +655,7 @@ struct RuleValues {
 // their quarter of W R. The waves behind them make the outputs of OT tiles of tokens
 // each beside them, from S and R in LDS (two halve what LDS has to give; of 256 key
 // values Q's pieces for one tile are what the registers hold). The last two bring
-// v, of every other piece each: from HBM, it takes longer than a piece (of 256 key
+// v and factors, of every other piece each: from HBM, it takes longer than a piece (of 256 key
 // values the waves with the outputs do: a tenth wave would cost the others registers).
 // Two barriers a piece. Each operand of the next piece is requested as soon as this
 // piece's has been used; nothing between a request and its use is conditional, so
@@ -662,6 +668,7 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
     constexpr int NP = RuleType<T>::NP, NS = Keys::STEPS, NT = Keys::NT, NW = Keys::NW, OT = RULE_OT<KD>;
     __shared__ __align__(16) dr_u4 ss[NS][3][64], rs[2][3][64];
     __shared__ __align__(16) lq_f4 part[4][4][64], vs[2][4][64];
+    __shared__ __align__(16) float cs[2][PIECE + 4];
     __shared__ float red[2][4][2][16], kq[2][2][KD];
     __shared__ int wild_s[4];
     const int group = p.value_heads / p.key_heads, slices = p.vd / 16;
@@ -677,23 +684,27 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
     const int w = wave_id(), lane = lane_id(), m = lane & 15, g = lane >> 4;
     const int h = p.tiled ? gi * p.key_heads + kh : kh * group + gi;
 
-    const T *vb = (const T *)p.v + (int64_t)span.first * p.v_ts + h * p.v_hs + c0 + m;     // (vs[j & 1]: piece j's)
+    // piece j's v and factors, in vs and cs[j & 1]
+    const T *vb = (const T *)p.v + (int64_t)span.first * p.v_ts + h * p.v_hs + c0 + m;
+    const auto rows_of = [&](int j) {
+        return (const float *)(ws.base + ws.rows) + ((int64_t)(base + min(j, to - 1) - ws.first) * p.value_heads + h) * 3 * PIECE;
+    };
     if (w >= 4 + 4 / OT) {
         RuleValues<T, 4> v;
         int mine = from + ((w ^ from) & 1);     // the next piece that is this wave's
-        v.ask(vb, p.v_ts, mine * PIECE + 4 * g, span.count);
+        v.ask(vb, p.v_ts, mine * PIECE + 4 * g, span.count, rows_of(mine), 0);
         for (int j = from - 1; j < to; ++j) {
             if (j >= from) {
                 __syncthreads();     // S
-                __syncthreads();     // R: piece j's v has been read
+                __syncthreads();     // R: piece j's have been read
                 const int bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3];
                 if (__builtin_amdgcn_readfirstlane(bad))
                     for (int t = 0; t < 2 * min(span.count - j * PIECE, PIECE); ++t) __syncthreads();     // the others' token by token
             }
             if (mine == j + 1) {
-                v.give(vs[mine & 1], mine * PIECE + 4 * g, span.count);
+                v.give(vs[mine & 1], cs[mine & 1], mine * PIECE + 4 * g, span.count, 0);
                 mine += 2;
-                v.ask(vb, p.v_ts, mine * PIECE + 4 * g, span.count);
+                v.ask(vb, p.v_ts, mine * PIECE + 4 * g, span.count, rows_of(mine), 0);
             }
         }
         return;
@@ -753,9 +764,9 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
         ask_p();
         dr_hold();
         if constexpr (KD > 128) {
-            v.ask(vb, p.v_ts, from * PIECE + 16 * o + 4 * g, span.count);
-            v.give(vs[from & 1] + o, from * PIECE + 16 * o + 4 * g, span.count);
-            v.ask(vb, p.v_ts, (from + 1) * PIECE + 16 * o + 4 * g, span.count);
+            v.ask(vb, p.v_ts, from * PIECE + 16 * o + 4 * g, span.count, rows_of(from), 16 * o);
+            v.give(vs[from & 1] + o, cs[from & 1], from * PIECE + 16 * o + 4 * g, span.count, 16 * o);
+            v.ask(vb, p.v_ts, (from + 1) * PIECE + 16 * o + 4 * g, span.count, rows_of(from + 1), 16 * o);
         }
         for (int j = from; j < to; ++j) {
             const int n = min(span.count - j * PIECE, PIECE);
@@ -820,8 +831,8 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
             }
             ob += PIECE * p.o_ts;
             if constexpr (KD > 128) {
-                v.give(vs[(j + 1) & 1] + o, (j + 1) * PIECE + 16 * o + 4 * g, span.count);
-                v.ask(vb, p.v_ts, (j + 2) * PIECE + 16 * o + 4 * g, span.count);
+                v.give(vs[(j + 1) & 1] + o, cs[(j + 1) & 1], (j + 1) * PIECE + 16 * o + 4 * g, span.count, 16 * o);
+                v.ask(vb, p.v_ts, (j + 2) * PIECE + 16 * o + 4 * g, span.count, rows_of(j + 2), 16 * o);
             }
         }
         return;
@@ -832,8 +843,6 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
     uint32_t wb = ws.w + (val0 * Keys::TILES + w * NT) * 2 * 3 * 1024;
     const uint32_t w_step = (uint32_t)p.value_heads * Keys::TILES * 2 * 3 * 1024;
     dr_u4 kf[4][NW][NP], wf[NT][2][3];
-    lq_f4 cf;
-    float lf;
     const auto ask_k = [&]() {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -841,10 +850,6 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
             for (int s = 0; s < NW; ++s)
 #pragma unroll
                 for (int i = 0; i < NP; ++i) kf[t][s][i] = block(kb, (t * NS + s) * NP + i);
-    };
-    const auto ask_rows = [&]() {
-        cf = factors(0, 16 * w);
-        lf = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(wsrc, 0, (int)(rb + 8 * PIECE), 0));
     };
     const auto ask_w = [&]() {
 #pragma unroll
@@ -864,14 +869,11 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
     for (int j = from; j < to;) {
         ask_k();
         dr_hold();
-        ask_rows();
-        dr_hold();
         ask_w();
         dr_hold();
         for (; j < to; ++j) {
             const bool more = j + 1 < to;     // the last piece's are asked for again and not used
             lq_f4 c[4] = {};
-            kb += more ? key_step : 0;
 #pragma unroll
             for (int s = 0; s < NW; ++s) {
                 dr_u2 lo[3], hi[3] = {};
@@ -889,21 +891,14 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
                     for (int u = 0; u < NP; ++u)
                         if (u <= i)
 #pragma unroll
-                            for (int t = 0; t < 4; ++t) {
-                                c[t] = dr_mfma(kf[t][s][u], z[i - u], c[t]);
-                                if (i == 0) {     // piece 0 is the last use of a tile's pieces
-                                    dr_hold();
-#pragma unroll
-                                    for (int v = 0; v < NP; ++v) kf[t][s][v] = block(kb, (t * NS + s) * NP + v);
-                                    dr_hold();
-                                }
-                            }
+                            for (int t = 0; t < 4; ++t) c[t] = dr_mfma(kf[t][s][u], z[i - u], c[t]);
             }
 #pragma unroll
             for (int t = 0; t < 4; ++t) part[w][t][lane] = c[t];
             __syncthreads();     // S
             const lq_f4 kS = (part[0][w][lane] + part[1][w][lane]) + (part[2][w][lane] + part[3][w][lane]);
-            const lq_f4 R = vs[j & 1][w][lane] - cf * kS;
+            const lq_f4 R = vs[j & 1][w][lane] - *reinterpret_cast<const lq_f4 *>(&cs[j & 1][16 * w + 4 * g]) * kS;
+            const float lf = cs[j & 1][PIECE];
             lq_f4 next[NT];
 #pragma unroll
             for (int t = 0; t < NT; ++t) next[t] = lf * S[t];
@@ -915,10 +910,6 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
             for (int i = 0; i < 3; ++i) reinterpret_cast<dr_u2 *>(&rs[w >> 1][i][lane])[w & 1] = x[i];
             const bool any = __any(!(size <= RULE_WILD * RULE_WILD));
             if (lane == 0) wild_s[w] = any;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) dr_hold(next[t]);
-            rb += more ? row_step : 0;
-            ask_rows();
             __syncthreads();     // R
             const int bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3];
             dr_u4 y[2][3];
@@ -926,8 +917,10 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int i = 0; i < 3; ++i) y[s][i] = rs[s][i][lane];
+            kb += more ? key_step : 0;
             wb += more ? w_step : 0;
             if (__builtin_amdgcn_readfirstlane(bad)) break;
+            ask_k();
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 lq_f4 d[3] = {next[t]};
@@ -1005,7 +998,9 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
 }
 
 constexpr int RULE_LEAST = 5;              // tokens of a request below which the token kernel takes it
-constexpr int64_t RULE_WINDOW = 64 << 20;  // bytes of workspace that a window of pieces may fill
+// Bytes of workspace that a window of pieces may fill: half of the memory's own cache, from
+// which the chain reads it back (8192 tokens, 32 heads of 128: 32 MB 483 us, 64 MB 400, 128 MB 372, 256 MB 419)
+constexpr int64_t RULE_WINDOW = 128 << 20;
 
 static int64_t key_bytes(int np, int kd) { return 4 * (kd == 64 ? 4 : kd / 32) * np * 1024; }     // a piece's K, or Q
 static int64_t piece_bytes(int np, int key_heads, int value_heads, int kd) {
