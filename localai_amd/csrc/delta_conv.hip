@@ -14,19 +14,36 @@ namespace lq {
 // VEC adjacent channels of a row
 template <typename T, int VEC>
 __device__ __forceinline__ void conv_load(const T *p, float (&y)[VEC]) {
-    if constexpr (VEC == 4) {
-        const float4 v = delta_load4(p);
-        y[0] = v.x; y[1] = v.y; y[2] = v.z; y[3] = v.w;
+    if constexpr (VEC >= 4) {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) {
+            const float4 v = delta_load4(p + i);
+            y[i] = v.x; y[i + 1] = v.y; y[i + 2] = v.z; y[i + 3] = v.w;
+        }
     } else
         y[0] = (float)p[0];
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void conv_store(T *p, const float (&y)[VEC]) {
-    if constexpr (VEC == 4) delta_store4(p, make_float4(y[0], y[1], y[2], y[3]));
+    if constexpr (VEC >= 4)
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) delta_store4(p + i, make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]));
     else p[0] = (T)y[0];
 }
+// a row's values as they lie in memory (requested, not yet used)
+template <typename T, int VEC>
+struct ConvRow {
+    T v[VEC];
+    __device__ __forceinline__ void load(const T *p) {
+        struct __attribute__((packed, aligned(VEC >= 4 ? 4 * sizeof(T) : sizeof(T)))) Raw { T v[VEC]; };
+        const Raw raw = *reinterpret_cast<const Raw *>(p);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = raw.v[i];
+    }
+};
 
 constexpr int CONV_ROWS = 32;     // rows of a piece: its first width - 1 rows before are read twice
+constexpr int CONV_AHEAD = 4;     // rows requested at once
 
 // A workgroup takes one piece of a request's rows and 256 VEC channels. Only a
 // request's first piece reads its state, and writes it: no other workgroup does.
@@ -43,6 +60,12 @@ __global__ __launch_bounds__(256) void delta_conv_kernel(DeltaConv c, DeltaReque
     const T *x = (const T *)c.x + span.first * c.x_stride + ch;
     T *out = (T *)c.out + span.first * c.out_stride + ch;
     float *state = r.state + span.slot * (W - 1) * c.channels + ch;
+    ConvRow<T, VEC> ahead[CONV_AHEAD];
+    const auto ask = [&](int first) {     // (rows behind the piece's last read it)
+#pragma unroll
+        for (int a = 0; a < CONV_AHEAD; ++a) ahead[a].load(x + min(first + a, end - 1) * c.x_stride);
+    };
+    ask(at);
     float w[W][VEC], bias[VEC], line[W][VEC];     // line: the rows under the taps, oldest first
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
@@ -76,19 +99,27 @@ __global__ __launch_bounds__(256) void delta_conv_kernel(DeltaConv c, DeltaReque
 #pragma unroll
         for (int t = 0; t < W - 1; ++t) conv_store<float, VEC>(state + (int64_t)t * c.channels, keep[t]);
     }
-    for (int row = at; row < end; ++row) {
-        conv_load<T, VEC>(x + row * c.x_stride, line[W - 1]);
-        float y[VEC];
+    for (int first = at; first < end; first += CONV_AHEAD) {
+        ConvRow<T, VEC> now[CONV_AHEAD];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            y[i] = bias[i];
+        for (int a = 0; a < CONV_AHEAD; ++a) now[a] = ahead[a];
+        if (first + CONV_AHEAD < end) ask(first + CONV_AHEAD);
 #pragma unroll
-            for (int t = 0; t < W; ++t) y[i] += w[t][i] * line[t][i];
-            if (c.silu) y[i] = y[i] / (1.0f + expf(-y[i]));
+        for (int a = 0; a < CONV_AHEAD; ++a) {
+            if (first + a >= end) break;
+            float y[VEC];
 #pragma unroll
-            for (int t = 0; t < W - 1; ++t) line[t][i] = line[t + 1][i];
+            for (int i = 0; i < VEC; ++i) {
+                line[W - 1][i] = (float)now[a].v[i];
+                y[i] = bias[i];
+#pragma unroll
+                for (int t = 0; t < W; ++t) y[i] += w[t][i] * line[t][i];
+                if (c.silu) y[i] = delta_silu(y[i]);
+#pragma unroll
+                for (int t = 0; t < W - 1; ++t) line[t][i] = line[t + 1][i];
+            }
+            conv_store<T, VEC>(out + (first + a) * c.out_stride, y);
         }
-        conv_store<T, VEC>(out + row * c.out_stride, y);
     }
 }
 

@@ -26,8 +26,6 @@ __device__ __forceinline__ void norm_store(T *p, const float (&y)[VEC]) {
     else p[0] = (T)y[0];
 }
 
-__device__ __forceinline__ float norm_silu(float z) { return z / (1.0f + expf(-z)); }
-
 // Four values of a Q8_0 block whose 8 lanes are adjacent. A block that holds a
 // value that is not finite gets a scale that is not, so all of it is NaN.
 __device__ __forceinline__ void norm_q8(uint8_t *row, int64_t at, const float (&y)[4]) {
@@ -115,7 +113,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsNorm n) {
             float z[VEC];
             norm_load<T, VEC>(gate + at, z);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) y[i] *= norm_silu(z[i]);
+            for (int i = 0; i < VEC; ++i) y[i] *= delta_silu(z[i]);
         }
         if constexpr (Q8) norm_q8((uint8_t *)out, at, y);
         else norm_store<O, VEC>(out + at, y);
@@ -143,6 +141,7 @@ static int norm_launch(const RmsNorm &n, hipStream_t s) {
     if (n.dim <= 64 * VEC) LQ_NORM(64, 1);
     else if (n.dim <= 256 * VEC) LQ_NORM(256, 1);
     else if (n.dim <= 1024 * VEC) LQ_NORM(256, 4);
+    else if (n.dim <= 2048 * VEC) LQ_NORM(256, 8);
     else if (n.dim <= 4096 * VEC) LQ_NORM(256, 16);
     else LQ_NORM(256, 0);
 #undef LQ_NORM
