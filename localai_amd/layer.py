@@ -27,7 +27,7 @@ import struct
 import numpy as np
 
 from . import _lib, device
-from .paged import _device_tensor, _empty, _hold, _ptr, _r, _refuse, _stream
+from .paged import _empty, _hold, _ptr, _r, _refuse, _stream
 
 ORDER = ('attn_output', 'ffn_gate', 'ffn_up', 'ffn_down', 'attn_q', 'attn_k', 'attn_v')
 
@@ -87,7 +87,18 @@ class DecodeLayerChain:
 
 
 _STRIDES = struct.Struct('=8q')
-_TYPES = {}
+
+
+class _Norm:
+    """What rms_norm() needs, looked up once."""
+
+    def __init__(self):
+        t = device.torch()
+        self.types = {t.float32: 0, t.float16: 1, t.bfloat16: 30, 'q8_0': 8}     # GGML numbers
+        self.call = _lib.load().localai_hip_rms_norm
+
+
+_norm = None
 
 
 def _norm_rows(t, name, dtype, shape):
@@ -114,35 +125,47 @@ def rms_norm(x, weight, eps=1e-6, residual=None, gate=None, dtype=None, out=None
     GGML Q8_0 blocks (dequant.dequantize_device reads them; then dim is a multiple of 32,
     and strides of 4 values). Returns the result, in `out` if given: x itself where the types are
     the same, or memory of its own."""
-    _device_tensor(x, 'x')
+    global _norm
     r = _r()
-    if not _TYPES:
-        t = device.torch()
-        _TYPES.update({t.float32: 0, t.float16: 1, t.bfloat16: 30, 'q8_0': 8})
-    kind, out_type = _TYPES.get(x.dtype), _TYPES.get(x.dtype if dtype is None else dtype)
+    if _norm is None:
+        _norm = _Norm()
+    if not isinstance(x, r.Tensor):
+        raise TypeError('x must be a device tensor')
+    given = x.dtype
+    if dtype is None:
+        dtype = given
+    types = _norm.types
+    kind, out_type = types.get(given), types.get(dtype)
     if kind is None:
         raise TypeError('x must be float32, float16 or bfloat16')
     if out_type is None:
         raise TypeError("dtype must be float32, float16, bfloat16 or 'q8_0'")
     shape = x.shape
-    if len(shape) not in (2, 3):
+    if len(shape) == 2:
+        rows, dim = shape
+        heads = 1
+    elif len(shape) == 3:
+        rows, heads, dim = shape
+    else:
         raise ValueError('x must be [rows, dim] or [rows, heads, dim]')
-    dim = shape[-1]
-    xp, *xs = _norm_rows(x, 'x', x.dtype, shape)
+    xp, *xs = _norm_rows(x, 'x', given, shape)
     wp = _ptr(weight, 'weight', r.f32, (dim,))
     rp, *rs = _norm_rows(residual, 'residual', r.f32, shape) if residual is not None else (None, 0, 0)
-    gp, *gs = _norm_rows(gate, 'gate', x.dtype, shape) if gate is not None else (None, 0, 0)
-    q8 = out_type == 8
-    if q8 and dim % 32:
-        raise ValueError("'q8_0' needs dim to be a multiple of 32")
-    out_shape = (*shape[:-1], dim // 32 * 34) if q8 else shape
-    out_dtype = r.u8 if q8 else x.dtype if dtype is None else dtype
+    gp, *gs = _norm_rows(gate, 'gate', given, shape) if gate is not None else (None, 0, 0)
+    if out_type == 8:
+        if dim % 32:
+            raise ValueError("'q8_0' needs dim to be a multiple of 32")
+        width, dtype = dim // 32 * 34, r.u8
+        shape = (*shape[:-1], width)
+    else:
+        width = dim
     if out is None:
-        out = _empty(stream, out_shape, out_dtype)
-    op, *os = _norm_rows(out, 'out', out_dtype, out_shape)
-    status = _lib.load().localai_hip_rms_norm(xp, kind, _STRIDES.pack(*xs, *rs, *gs, *os), shape[0],
-                                              shape[1] if len(shape) == 3 else 1, dim, wp, eps, rp, gp, op, out_type,
-                                              _stream(stream))
+        out = _empty(stream, shape, dtype)
+        op, os = out.data_ptr(), (heads * width, width)
+    else:
+        op, *os = _norm_rows(out, 'out', dtype, shape)
+    status = _norm.call(xp, kind, _STRIDES.pack(*xs, *rs, *gs, *os), rows, heads, dim, wp, eps, rp, gp, op, out_type,
+                        _stream(stream))
     if status:
         _lib.check(status)
     if stream is not None:
