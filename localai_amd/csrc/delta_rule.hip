@@ -341,7 +341,7 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
                 }
             ss = in ? dr_rows_sum(ss) : 0.0f;
             // (values whose squares vanish: what they meet vanishes too, but for a norm that makes them large again)
-            wild |= !(ss <= RULE_WILD * RULE_WILD) || (in && ss < RULE_FAINT && !(p.norm_eps >= RULE_FAINT));
+            wild |= !(ss <= RULE_WILD * RULE_WILD) || (norm && in && ss < RULE_FAINT && p.norm_eps < RULE_FAINT);
             float inv = norm ? 1.0f / sqrtf(ss + p.norm_eps) : 1.0f;
             if (norm && !(inv <= 3.4e38f)) {     // a row of zeros and norm_eps 0: 0 / 0
                 wild |= in;

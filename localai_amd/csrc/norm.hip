@@ -60,7 +60,7 @@ __device__ __forceinline__ void norm_q8(uint8_t *row, int64_t at, const float (&
 // ITEMS values stay in registers, longer ones (ITEMS 0) are read a second time,
 // each lane its own values. Groups of fewer lanes take ROWS rows side by side, all
 // requested at once: heads of 128 (131072 of them, bf16 with a gate: 101 MB) 54 us
-// with a wave a head, ___ so.
+// with a wave a head, 30 so.
 template <typename T, typename O, int VEC, int TPR, int ITEMS, int ROWS>
 __global__ __launch_bounds__(256) void rms_norm_kernel(RmsNorm n) {
     constexpr bool Q8 = sizeof(O) == 1;

@@ -309,3 +309,351 @@ def test_norm_blocks_of_values_that_are_not_finite():
     assert np.isnan(y[0]).all()                                              # the row's norm is NaN
     assert np.isnan(y[1, 32:64]).all() and (y[1, :32] == 0).all() and (y[1, 64:] == 0).all()
     assert np.isnan(y[2, 64:]).all() and np.isfinite(y[2, :64]).all()
+
+
+# ---------------------------------------------------------------- what the rule must not mix
+
+def _finite_case(rng, tokens=150, heads=(2, 4, 128, 32)):
+    import torch
+    hk, hv, kd, vd = heads
+    q, k, v = (torch.tensor(rng.standard_normal((tokens, h, d)), dtype=torch.float32, device='cuda')
+               for h, d in ((hk, kd), (hk, kd), (hv, vd)))
+    decay, beta = -_t(rng.exponential(0.1, (tokens, hv))), _t(rng.random((tokens, hv)))
+    state = _t(rng.standard_normal((1, hv, kd, vd)))
+    return q, k, v, decay, beta, state
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('where,value', [(w, float(x)) for w in ('q', 'k', 'v', 'decay', 'beta') for x in ('nan', 'inf', '-inf')
+                                         if (w, x) != ('decay', '-inf')])     # (that one forgets everything: finite)
+@pytest.mark.parametrize('at', [0, 70, 127])
+def test_rule_values_that_are_not_finite_reach_only_what_follows(at, where, value, dtype):
+    """Tokens before the one that holds it, heads that do not read it and, of a v, other columns are as without it."""
+    import torch
+    from localai_amd import delta
+    rng = np.random.default_rng(at)
+    q, k, v, decay, beta, state = _finite_case(rng)
+    q, k, v = (x.to(getattr(torch, dtype)) for x in (q, k, v))
+    starts = _ints([0, 150])
+    call = lambda s: delta.rule(q, k, v, decay, beta, s, starts=starts, order='grouped')
+    clean_state = state.clone()
+    clean = call(clean_state)
+    {'q': q, 'k': k, 'v': v, 'decay': decay, 'beta': beta}[where][(at, 1) if where in ('decay', 'beta') else (at, 0, 5)] = value
+    got = call(state)
+    heads = {'q': [0, 1], 'k': [0, 1], 'v': [0], 'decay': [1], 'beta': [1]}[where]     # two value heads a key head
+    others = [h for h in range(4) if h not in heads]
+    assert torch.equal(got[:, others], clean[:, others]) and torch.equal(state[:, others], clean_state[:, others])
+    # the piece that holds it goes token by token: rounded elsewhere, no more than that
+    near = dict(rtol=HALF[dtype] * 4 + 1e-5, atol=1e-5)
+    torch.testing.assert_close(got[:at, heads].float(), clean[:at, heads].float(), **near)
+    if where == 'q':
+        if not np.isnan(value):
+            return     # a norm that is infinite makes q zeros, but for 0 times infinity
+        assert torch.isnan(got[at, heads]).all()
+        torch.testing.assert_close(got[at + 1:, heads].float(), clean[at + 1:, heads].float(), **near)
+        torch.testing.assert_close(state, clean_state, rtol=1e-4, atol=1e-5)
+    elif where == 'v':
+        columns = [c for c in range(32) if c != 5]
+        torch.testing.assert_close(got[:, 0][:, columns].float(), clean[:, 0][:, columns].float(), **near)
+        torch.testing.assert_close(state[0, 0][:, columns], clean_state[0, 0][:, columns], rtol=1e-4, atol=1e-5)
+        assert not torch.isfinite(got[at:, 0, 5]).any() and not torch.isfinite(state[0, 0, :, 5]).any()
+    elif where != 'k' or np.isnan(value):
+        assert not torch.isfinite(got[at + 1:, heads]).any() and not torch.isfinite(state[0, heads]).any()
+
+
+def _against_oracle(args, order='grouped', norm_eps=1e-6, tol=2e-5, starts=None):
+    """One request; the 2-norms of output and state within tol of the oracle's largest state."""
+    from localai_amd import delta
+    q, k, v, decay, beta, state = args
+    sizes = np.zeros((len(v), v.shape[1]))
+    want, after = odelta.rule(_np(state)[0], _np(q), _np(k), _np(v), _np(decay), _np(beta), order=order, norm_eps=norm_eps,
+                              sizes=sizes)
+    got = delta.rule(q, k, v, decay, beta, state, starts=_ints([0, len(v)]), order=order, norm_eps=norm_eps)
+    for h in range(v.shape[1]):
+        assert np.linalg.norm(_np(got)[:, h] - want[:, h]) <= tol * np.linalg.norm(sizes[:, h]) * q.shape[-1] ** -0.5, h
+        assert np.linalg.norm(_np(state)[0, h] - after[h]) <= tol * sizes[:, h].max(), h
+
+
+# Tolerance of the cases below: a token rounds (2 sqrt(128) + 16) u = 2.3e-6 of its state, and what
+# it rounds lasts no longer than the state itself, some tens of tokens here: within 2e-5.
+
+def test_rule_forgets_everything():
+    rng = np.random.default_rng(2)
+    args = _finite_case(rng)
+    args[3][40], args[3][64], args[3][100, 1] = -float('inf'), -float('inf'), -3e5
+    _against_oracle(args)
+
+
+def test_rule_equal_keys():
+    """The least comfortable system: every k the same, beta 1, nothing forgotten (a sum of powers of A would cancel
+    numbers of 1e18)."""
+    rng = np.random.default_rng(3)
+    q, k, v, decay, beta, state = _finite_case(rng)
+    k[:] = k[0]
+    decay[:], beta[:] = 0, 1
+    _against_oracle((q, k, v, decay, beta, state))
+    k[70:] = -k[70:]
+    _against_oracle((q, k, v, decay, beta, state))
+
+
+def test_rule_beta_zero_zero_keys_and_growth():
+    rng = np.random.default_rng(4)
+    q, k, v, decay, beta, state = _finite_case(rng)
+    beta[:50] = 0
+    k[60:70], q[65:75] = 0, 0
+    decay[80:90] = 0.2      # a state that grows
+    decay[130] = 1.5        # faster than a piece takes: token by token
+    _against_oracle((q, k, v, decay, beta, state))
+
+
+@pytest.mark.parametrize('size', [1e-20, 1e-3, 1e12, 3e19])
+def test_rule_sizes(size):
+    """v and the state of any size (past 1e30 in v or state: token by token)."""
+    rng = np.random.default_rng(5)
+    q, k, v, decay, beta, state = _finite_case(rng)
+    _against_oracle((q * 1e3, k * 1e-3, v * size, decay, beta, state * size))
+
+
+def test_rule_large_betas():
+    """beta |k|^2 past 2 (a state that overshoots) goes token by token."""
+    rng = np.random.default_rng(6)
+    q, k, v, decay, beta, state = _finite_case(rng, tokens=70)
+    k /= k.norm(dim=-1, keepdim=True)
+    beta[20:23] = 4.0
+    # an error of these three tokens' grows by up to 3 each: 27 times the tolerance
+    _against_oracle((q, k, v, decay, beta, state), norm_eps=None, tol=27 * 2e-5 * 128 ** 0.5)
+
+
+# ---------------------------------------------------------------- together, as a model uses them
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_prompt_at_once_in_pieces_and_token_by_token(dtype):
+    """A layer's convolution, rule and gated norm over a prompt in one call, in two, and its last tokens one by one, with
+    paged.extend's tables: the same states and results but for rounding."""
+    import torch
+    from localai_amd import delta, layer, paged
+    rng = np.random.default_rng(7)
+    hk, hv, kd, vd, width = 2, 4, 64, 64, 4
+    channels, lengths = 2 * hk * kd + hv * vd, [100, 0, 37]
+    total = sum(lengths)
+    x, z = (_random(rng, (total, n), dtype)[0] for n in (channels, hv * vd))
+    w, norm_w = _t(rng.standard_normal((channels, width)) * 0.5), _t(rng.standard_normal(vd))
+    decay, beta = _t(rng.standard_normal((total, hv))), _t(rng.standard_normal((total, hv)))
+    a, dt = _t(-rng.uniform(0.1, 4, hv)), _t(rng.uniform(-4, 0, hv))
+    first = np.concatenate([[0], np.cumsum(lengths)])
+
+    def run(parts):
+        states = delta.DeltaCache(2, hk, hv, kd, vd, rows=len(lengths), width=width)
+        states.rule_state.normal_()       # what is there before a request starts does not matter
+        states.conv_state.normal_()
+        cache = paged.PagedKVCache(1, 1, 64, 32, 16, requests=len(lengths))
+        out, done = torch.zeros((total, hv, vd), dtype=x.dtype, device='cuda'), np.zeros(len(lengths), int)
+        for new in parts:
+            step = cache.extend(_ints(new), sum(new) + 3)
+            rows = np.concatenate([np.arange(first[b] + done[b], first[b] + done[b] + n) for b, n in enumerate(new)])
+            pad = np.concatenate([rows, np.zeros(3, int)])       # three places of padding behind the tokens
+            c = states.conv(1, x[pad], w, step)
+            q, k, v = states.split(c)
+            y = states.rule(1, q, k, v, decay[pad], beta[pad], step, a=a, dt_bias=dt, order='tiled')
+            y = layer.rms_norm(y, norm_w, gate=z[pad].unflatten(-1, (hv, vd)))
+            out[rows] = y[:len(rows)]
+            done += new
+            step.check()
+        return out, states
+
+    whole, states = run([lengths])
+    for parts in ([[64, 0, 30], [36, 0, 7]], [[1, 0, 36], [98, 0, 0], [1, 0, 1]], [[95, 0, 33]] + [[1, 0, 0]] * 5 + [[0, 0, 1]] * 4):
+        got, other = run(parts)
+        torch.testing.assert_close(got.float(), whole.float(), rtol=8 * HALF[dtype] + 1e-4, atol=8 * HALF[dtype] + 1e-4)
+        torch.testing.assert_close(other.rule_state[1, [0, 2]], states.rule_state[1, [0, 2]], rtol=1e-4,
+                                   atol=1e-5 + 8 * HALF[dtype])
+        torch.testing.assert_close(other.conv_state[1, [0, 2]], states.conv_state[1, [0, 2]], rtol=0, atol=0)
+    # against the oracle, the first request
+    xv, n = _np(x)[:100], 100
+    c, _, _ = odelta.conv(np.zeros((width - 1, channels)), xv, _np(w))
+    c = _np(torch.tensor(c).to(x.dtype))
+    q, k, v = (c[:, i:j].reshape(n, -1, 64) for i, j in ((0, 128), (128, 256), (256, 512)))
+    o, S = odelta.rule(np.zeros((hv, kd, vd)), q, k, v, _np(decay)[:n], _np(beta)[:n], _np(a), _np(dt), 'tiled')
+    o, _ = odelta.rms_norm(_np(torch.tensor(o).to(x.dtype)), _np(norm_w), gate=_np(z)[:n].reshape(n, hv, vd))
+    torch.testing.assert_close(whole[:n].double().cpu(), torch.tensor(o), rtol=8 * HALF[dtype] + 1e-4, atol=8 * HALF[dtype] + 1e-4)
+    torch.testing.assert_close(states.rule_state[1, 0].double().cpu(), torch.tensor(S), rtol=1e-4, atol=1e-5 + 8 * HALF[dtype])
+
+
+def _calls(rng, dtype='bfloat16', tokens=200, n=3):
+    import torch
+    heads = (2, 4, 128, 64)
+    q, k, v, decay, beta, a, dt = _rule_inputs(rng, tokens, heads, dtype, True)
+    starts = _ints([0, 130, 133, tokens])
+    state, _ = _random(rng, (n, 4, 128, 64), 'float32')
+    x, _ = _random(rng, (tokens, 512), dtype)
+    w, _ = _random(rng, (512, 4), 'float32')
+    conv_state, _ = _random(rng, (n, 3, 512), 'float32')
+    weight, _ = _random(rng, 64, 'float32')
+    return dict(q=q, k=k, v=v, decay=decay, beta=beta, a=a, dt=dt, starts=starts, state=state, x=x, w=w,
+                conv_state=conv_state, weight=weight, residual=_t(rng.standard_normal((tokens, 512))))
+
+
+def _run_all(c, stream=None):
+    from localai_amd import delta, layer
+    conv = delta.conv(c['x'], c['w'], c['conv_state'], starts=c['starts'], stream=stream)
+    y = delta.rule(c['q'], c['k'], c['v'], c['decay'], c['beta'], c['state'], starts=c['starts'], a=c['a'],
+                   dt_bias=c['dt'], stream=stream)
+    step = delta.rule(c['q'][:3], c['k'][:3], c['v'][:3], c['decay'][:3], c['beta'][:3], c['state'], stream=stream)
+    z = layer.rms_norm(y, c['weight'], gate=y, stream=stream)
+    n = layer.rms_norm(c['x'], c['w'].reshape(-1)[:512], residual=c['residual'], dtype='q8_0', stream=stream)
+    return conv, y, step, z, n, c['state'], c['conv_state'], c['residual']
+
+
+def test_captured_and_replayed():
+    import torch
+    rng = np.random.default_rng(8)
+    c = _calls(rng)
+    kept = [c[k].clone() for k in ('state', 'conv_state', 'residual')]
+
+    def reset():
+        for k, t in zip(('state', 'conv_state', 'residual'), kept):
+            c[k].copy_(t)
+
+    want = [t.clone() for t in _run_all(c)]
+    again = [t.clone() for t in _run_all(c)]         # a second step on the states that the first left
+    graphs, results = [], []
+    for _ in range(2):
+        reset()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            results.append(_run_all(c))
+        graphs.append(g)
+    for _ in range(3):
+        reset()
+        for i, wanted in ((0, want), (1, again)):
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            for t, expected in zip(results[i], wanted):
+                assert torch.equal(t, expected)
+        reset()
+        for t, expected in zip(_run_all(c), want):
+            assert torch.equal(t, expected)
+
+
+def test_streams():
+    """Two streams at once, each with its own inputs; results as on one."""
+    import torch
+    sets = [_calls(np.random.default_rng(s)) for s in (9, 10)]
+    twins = [_calls(np.random.default_rng(s)) for s in (9, 10)]
+    wants = [_run_all(c) for c in twins]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    results = []
+    for c, s in zip(sets, streams):
+        results.append(_run_all(c, s))
+    for s in streams:
+        s.synchronize()
+    for got, want in zip(results, wants):
+        for t, expected in zip(got, want):
+            assert torch.equal(t, expected)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_rule_stays_in_its_workspace(dtype, monkeypatch):
+    """Several windows; what lies behind the workspace stays as it was. (The sizes of a window's pieces differ by type.)"""
+    import torch
+    from localai_amd import delta
+    rng = np.random.default_rng(11)
+    heads, tokens = (8, 128, 128, 16), 1700
+    q, k, v, decay, beta, a, dt = _rule_inputs(rng, tokens, heads, dtype, True)
+    state, _ = _random(rng, (2, heads[1], heads[2], heads[3]), 'float32')
+    behind, made = 8 << 20, []
+
+    def empty(stream, shape, kind):
+        if kind is not torch.uint8:
+            return torch.empty(shape, dtype=kind, device='cuda')
+        made.append(torch.full((shape + behind,), 0xA5, dtype=torch.uint8, device='cuda'))
+        return made[-1][:shape]
+
+    monkeypatch.setattr(delta, '_empty', empty)
+    first = state.clone()
+    y = delta.rule(q, k, v, decay, beta, state, starts=_ints([0, 1600, tokens]), a=a, dt_bias=dt)
+    assert len(made) == 1 and (made[0][-behind:] == 0xA5).all()
+    # the last tokens again, from a call of their own: the first windows carried the state over
+    z = delta.rule(*(t[1600:] for t in (q, k, v, decay, beta)), first[1:], starts=_ints([0, 100]), a=a, dt_bias=dt)
+    torch.testing.assert_close(z.float(), y[1600:].float(), rtol=1e-4 + 2 * HALF[dtype], atol=1e-5)
+    sizes = np.zeros((1600, heads[1]))
+    _, want = odelta.rule(_np(first[0]), *(_np(t[:1600]) for t in (q, k, v, decay, beta)), _np(a), _np(dt), sizes=sizes)
+    for h in range(heads[1]):
+        # (a token's (2 sqrt(128) + 16) u, over the 1600 that may last)
+        assert np.linalg.norm(_np(state[0, h]) - want[h]) <= 2.4e-6 * 40 * sizes[:, h].max()
+
+
+def test_states_past_32_bits():
+    import torch
+    from localai_amd import delta
+    rng = np.random.default_rng(12)
+    rows = 4300                                            # x 32 x 128 x 128 values of 4 bytes: 9 GB
+    state = torch.empty((rows, 32, 128, 128), device='cuda')
+    q, k, v, decay, beta, a, dt = _rule_inputs(rng, 70, (16, 32, 128, 128), 'float32', True)
+    small = torch.zeros((1, 32, 128, 128), device='cuda')
+    for starts, n in ((_ints([0, 70]), 70), (None, 1)):
+        state[rows - 1] = 0
+        small.zero_()
+        args = [t[:n] for t in (q, k, v, decay, beta)]
+        y = delta.rule(*args, state, _ints([rows - 1]), starts, a=a, dt_bias=dt)
+        z = delta.rule(*args, small, None, starts, a=a, dt_bias=dt)
+        assert torch.equal(y, z) and torch.equal(state[rows - 1], small[0])
+
+
+def test_starts_that_do_not_fit_are_cut():
+    """Nothing outside the call's rows is read or written, whatever starts holds."""
+    import torch
+    from localai_amd import delta
+    rng = np.random.default_rng(13)
+    q, k, v, decay, beta, a, dt = _rule_inputs(rng, 40, (1, 2, 64, 32), 'float32', True)
+    state, sv = _random(rng, (3, 2, 64, 32), 'float32')
+    out = torch.full((60, 2, 32), 7.0, device='cuda')
+    delta.rule(q, k, v, decay, beta, state, None, _ints([-5, 20, 20, 1000]), a=a, dt_bias=dt, out=out[10:50])
+    assert (out[:10] == 7).all() and (out[50:] == 7).all() and torch.isfinite(out).all()
+    want, after = odelta.rule(sv[0], *(_np(t)[:20] for t in (q, k, v, decay, beta)), _np(a), _np(dt))
+    np.testing.assert_allclose(_np(out)[10:30], want, atol=1e-4)
+    np.testing.assert_array_equal(_np(state)[1], sv[1])
+    x, _ = _random(rng, (40, 64), 'float32')
+    w, _ = _random(rng, (64, 4), 'float32')
+    cs, _ = _random(rng, (3, 3, 64), 'float32')
+    out = torch.full((60, 64), 7.0, device='cuda')
+    delta.conv(x, w, cs, None, _ints([-5, 20, 20, 1000]), out=out[10:50])
+    assert (out[:10] == 7).all() and (out[50:] == 7).all()
+
+
+def test_refusals_on_the_device():
+    import torch
+    from localai_amd import delta, layer
+    from localai_amd._lib import HipError
+    rng = np.random.default_rng(14)
+    q, k, v, decay, beta, a, dt = _rule_inputs(rng, 6, (1, 2, 64, 32), 'float32', True)
+    state, _ = _random(rng, (6, 2, 64, 32), 'float32')
+    call = lambda **c: delta.rule(**{**dict(q=q, k=k, v=v, decay=decay, beta=beta, state=state), **c})
+    for change, error in [(dict(q=q.double()), TypeError), (dict(q=q.half()), TypeError), (dict(k=k[:5]), ValueError),
+                          (dict(v=v[..., ::2]), ValueError), (dict(beta=beta[:, :1]), ValueError),
+                          (dict(state=state.half()), TypeError), (dict(state=state[:, :, :, :16]), ValueError),
+                          (dict(state=state[:2]), HipError), (dict(a=a), ValueError), (dict(order='other'), ValueError),
+                          (dict(norm_eps=-1.0), ValueError), (dict(scale=float('inf')), HipError),
+                          (dict(slots=_ints([0] * 5)), ValueError), (dict(starts=_ints([0, 6]), lengths=_ints([1, 2])), ValueError),
+                          (dict(starts=_ints(range(9))), ValueError), (dict(out=v[:, :, ::2]), ValueError),
+                          (dict(slots=_ints([0] * 6).long()), TypeError), (dict(q=q[..., :63], k=k[..., :63]), (ValueError, HipError))]:
+        if 'state' in change and change['state'].shape[0] == 2:
+            continue     # rows past the pool are places without a state
+        with pytest.raises(error):
+            call(**change)
+    call()
+    x, w = torch.ones(4, 64, device='cuda'), torch.ones(64, 4, device='cuda')
+    cs = torch.zeros(4, 3, 64, device='cuda')
+    for change, error in [(dict(x=x.double()), TypeError), (dict(x=x.t()), ValueError), (dict(weight=w[:, :3].contiguous()), ValueError),
+                          (dict(state=cs[:, :2]), (TypeError, ValueError)), (dict(bias=w), ValueError),
+                          (dict(out=x.half()), TypeError), (dict(weight=torch.ones(64, 9, device='cuda'),
+                                                                 state=torch.ones(4, 8, 64, device='cuda')), HipError)]:
+        with pytest.raises(error):
+            delta.conv(**{**dict(x=x, weight=w, state=cs), **change})
+    for change, error in [(dict(x=x.double()), TypeError), (dict(weight=w), ValueError), (dict(residual=x.half()), TypeError),
+                          (dict(gate=x[:2]), ValueError), (dict(dtype=torch.int8), TypeError), (dict(dtype='q4_0'), TypeError),
+                          (dict(x=x[:, :40], weight=w.reshape(-1)[:40], dtype='q8_0'), ValueError),
+                          (dict(x=x.reshape(2, 2, 4, 16)), ValueError), (dict(out=x.half()), TypeError)]:
+        with pytest.raises(error):
+            layer.rms_norm(**{**dict(x=x, weight=w.reshape(-1)[:64]), **change})
