@@ -77,19 +77,31 @@ __device__ __forceinline__ DeltaSpan delta_span(const DeltaRequests &r, int b) {
 // starts[b] / size + b + j, so no table is needed: a request of n rows has at
 // most (its last row / size - its first row / size + 1) pieces, and the next
 // request's numbers begin behind those. Numbers below tokens / size + requests.
-// Returns the piece's request, or -1 (no wave-wide value differs): the last b
-// with starts[b] / size + b <= piece, found 64 requests at a time.
-__device__ __forceinline__ int delta_request(const DeltaRequests &r, int piece, int size) {
+// Returns the piece's request, the last b with starts[b] / size + b <= piece, found
+// 64 requests at a time, and its span, from the same requests to memory; -1 if
+// there is none. (No value differs within a wave.)
+__device__ __forceinline__ int delta_request(const DeltaRequests &r, int piece, int size, DeltaSpan *span) {
     const int lane = (int)(threadIdx.x & 63);
-    int b = -1;
-    for (int at = 0; at < r.requests; at += 64) {
-        const int i = at + lane;
-        const bool before = i < r.requests && min(max(r.starts[i], 0), r.tokens) / size + i <= piece;
-        const int n = __popcll(__ballot(before));
-        b += n;
-        if (n < 64) break;
+    int prev_start = 0, prev_slot = -1, prev_length = 0;     // of the 64 before
+    for (int at = 0; at <= r.requests; at += 64) {
+        const int i = min(at + lane, r.requests), own = min(i, r.requests - 1);
+        const int start = min(max(r.starts[i], 0), r.tokens);
+        const int slot = r.slots ? r.slots[own] : own, length = r.lengths ? r.lengths[own] : INT32_MAX;
+        const int n = __popcll(__ballot(at + lane < r.requests && start / size + i <= piece));
+        const auto of = [](int x, int l) { return __builtin_amdgcn_readlane(x, l); };
+        if (n < 64) {
+            if (at + n == 0) return -1;
+            const int first = n ? of(start, n - 1) : of(prev_start, 63), s = n ? of(slot, n - 1) : of(prev_slot, 63);
+            const int end = max(of(start, n), first), rows = end - first;
+            *span = DeltaSpan{first, s >= 0 && s < r.n_slots ? rows : 0, s,
+                              (n ? of(length, n - 1) : of(prev_length, 63)) <= rows};
+            return at + n - 1;
+        }
+        prev_start = start;
+        prev_slot = slot;
+        prev_length = length;
     }
-    return __builtin_amdgcn_readfirstlane(b);
+    return -1;     // (not reached: the last 64 have one behind the last request)
 }
 
 // y / (1 + exp(-y)) to a few fp32 roundings: the exponent's argument in two parts

@@ -51,9 +51,10 @@ template <typename T, int VEC, int W>
 __global__ __launch_bounds__(256) void delta_conv_kernel(DeltaConv c, DeltaRequests r) {
     const int64_t ch = ((int64_t)blockIdx.y * 256 + threadIdx.x) * VEC;
     const int piece = blockIdx.x, size = r.starts ? CONV_ROWS : 1;
-    const int b = r.starts ? delta_request(r, piece, size) : piece;
+    DeltaSpan span;
+    const int b = r.starts ? delta_request(r, piece, size, &span) : piece;
     if (b < 0) return;
-    const DeltaSpan span = delta_span(r, b);
+    if (!r.starts) span = delta_span(r, b);
     const int j = r.starts ? piece - (span.first / size + b) : 0;
     const int at = j * size, end = min(at + size, span.count);
     if (j < 0 || at >= end || ch >= c.channels) return;

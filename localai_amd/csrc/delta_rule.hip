@@ -272,6 +272,12 @@ struct RuleRaw {
     }
 };
 
+// 1 / sqrt(x) to about a rounding, of normal x (others are infinite or NaN: such a piece goes token by token)
+__device__ __forceinline__ float dr_inverse_root(float x) {
+    const float r = __builtin_amdgcn_rsqf(x), e = __builtin_fmaf(-x * r, r, 1.0f);
+    return __builtin_fmaf(0.5f * r, e, r);
+}
+
 // one step of an inclusive sum over the wave's lanes, of fp64 values
 template <int CTRL, int ROWS>
 __device__ __forceinline__ double dr_add_from(double v) {
@@ -302,12 +308,13 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
     dr_u4 (&to)[TRI][3][64] = *reinterpret_cast<dr_u4 (*)[TRI][3][64]>(space);
     float (&tm)[PIECE][LD] = *reinterpret_cast<float (*)[PIECE][LD]>(space + AS);
     __shared__ double gs[PIECE];      // sums of g, in powers of two
-    __shared__ float bs[PIECE], ik[PIECE], iq[PIECE], kn[PIECE], sc[PIECE];
+    __shared__ float bs[PIECE], ik[PIECE], iq[PIECE], kn[PIECE];
+    __shared__ __align__(16) float sc[PIECE];
     __shared__ int wild_s[4];
     const int local = (int)(blockIdx.x / p.key_heads), kh = (int)(blockIdx.x % p.key_heads);
-    const int piece = ws.first + local, b = delta_request(r, piece, PIECE);
+    DeltaSpan span;
+    const int piece = ws.first + local, b = delta_request(r, piece, PIECE, &span);
     if (b < 0) return;
-    const DeltaSpan span = delta_span(r, b);
     const int j0 = (piece - (span.first / PIECE + b)) * PIECE, n = min(span.count - j0, PIECE);
     if (j0 < 0 || n <= 0 || span.count < ws.least) return;
     const int w = wave_id(), lane = lane_id(), m = lane & 15, g = lane >> 4;
@@ -342,7 +349,7 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
             ss = in ? dr_rows_sum(ss) : 0.0f;
             // (values whose squares vanish: what they meet vanishes too, but for a norm that makes them large again)
             wild |= !(ss <= RULE_WILD * RULE_WILD) || (norm && in && ss < RULE_FAINT && p.norm_eps < RULE_FAINT);
-            float inv = norm ? 1.0f / sqrtf(ss + p.norm_eps) : 1.0f;
+            float inv = norm ? dr_inverse_root(ss + p.norm_eps) : 1.0f;
             if (norm && !(inv <= 3.4e38f)) {     // a row of zeros and norm_eps 0: 0 / 0
                 wild |= in;
                 inv = 0.0f;
@@ -457,9 +464,15 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
         for (int e = 0; e < 4; ++e) {
             const int row = 16 * w + 4 * g + e, col = 16 * j + m;
             // (of far tokens the power's argument is rounded to 2^-24 of itself: less of the sum than 2^-25)
-            const float f = row >= col ? __builtin_amdgcn_exp2f((float)(gr[e] - gc[j])) * kc[j] : 0.0f;
-            am[row][col] = row > col ? f * kr[e] * kk[j][e] : 0.0f;
-            qk[j][e] = row >= col ? f * qr[e] * qk[j][e] : 0.0f;
+            const float f = __builtin_amdgcn_exp2f((float)(gr[e] - gc[j])) * kc[j];
+            const float a = f * kr[e] * kk[j][e], b = f * qr[e] * qk[j][e];
+            if (j < w) {
+                am[row][col] = a;
+                qk[j][e] = b;
+            } else {     // the diagonal's tile
+                am[row][col] = row > col ? a : 0.0f;
+                qk[j][e] = row >= col ? b : 0.0f;
+            }
         }
     }
     __syncthreads();
@@ -483,12 +496,13 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
         for (int i = 0; i < 16; ++i) tm[16 * w + i][16 * w + m] = x[i];
     __syncthreads();
     // blocks below it, of column tile w: T_iw = -T_ii (sum_u A_iu T_uw)
+    lq_f4 col[4];
     {
-        lq_f4 col[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) col[0][e] = tm[16 * w + 4 * g + e][16 * w + m];
 #pragma unroll
         for (int i = 1; i < 4; ++i) {
+            col[i] = lq_f4{0, 0, 0, 0};
             if (w + i > 3) continue;
             const int row = 16 * (w + i) + m;
             lq_f4 sum = {0, 0, 0, 0}, res = {0, 0, 0, 0};
@@ -509,20 +523,29 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
         }
     }
     __syncthreads();
-    // W^T = T^T diag K: the scaled T with tokens contracted, column tile c, tokens 32 s .., in A's place
-    for (int i = w; i < TRI; i += 4) {
-        const int c = i < 4 ? i >> 1 : i - 2, s = i < 4 ? i & 1 : 1;
-        const float bc = bs[16 * c + m];
-        float y8[8];
+    // W^T = T^T diag K: column tile w of the scaled T with tokens contracted is what the wave
+    // holds, tile by tile; in A's place
+    {
+        const bool odd = w & 1;
+        const float bc = bs[16 * w + m];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int token = 32 * s + 16 * (e >> 2) + 4 * g + (e & 3);
-            y8[e] = 2 * s + (e >> 2) >= c ? tm[token][16 * c + m] * (bc * sc[token]) : 0.0f;
+        for (int s = 0; s < 2; ++s) {     // tokens 32 (w / 2 + s) ..
+            if (w / 2 + s > 1) continue;
+            float y8[8];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                // tile 2 (w / 2 + s) + u is the wave's 2 s + u - odd, zero ahead of its first
+                const lq_f4 tile = odd ? (2 * s + u ? col[2 * s + u - 1 < 0 ? 0 : 2 * s + u - 1] : lq_f4{0, 0, 0, 0}) : col[2 * s + u];
+                const float4 f = *reinterpret_cast<const float4 *>(&sc[32 * (w / 2 + s) + 16 * u + 4 * g]);
+                const float by[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y8[4 * u + e] = tile[e] * (bc * by[e]);
+            }
+            dr_u4 y[3];
+            dr_split8<3>(y8, y);
+#pragma unroll
+            for (int pc = 0; pc < 3; ++pc) to[w < 2 ? 2 * w + s : w + 2][pc][lane] = y[pc];
         }
-        dr_u4 y[3];
-        dr_split8<3>(y8, y);
-#pragma unroll
-        for (int pc = 0; pc < 3; ++pc) to[i][pc][lane] = y[pc];
     }
     __syncthreads();
     {
