@@ -140,9 +140,12 @@ __global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequ
 // request's pieces is a second one, each workgroup with 16 value columns of one
 // head, whose S stays in registers (delta_chain_kernel).
 //
-// Precision: everything is fp32's. MFMA takes bf16 operands, so each fp32 value
-// goes in as three bf16 pieces (24 bits), q and k of 16 bits as they are (bf16:
-// one piece, f16: two); of the products those up to 2^-16 of the largest are
+// Precision: everything is fp32's. MFMA takes 16-bit operands, so each fp32 value
+// goes in as several. S as three bf16 pieces (24 bits), q and k of 16 bits as they
+// are (bf16: one piece, f16: two), of fp32 three. W, P T and R, whose size is known
+// ahead, as two f16 pieces (22 bits of each value, and 2^-35 of the largest that it
+// may be: they are scaled by a power of two below that bound), a third fewer bytes
+// and half the products of three bf16 ones. Products up to 2^-16 (f16: 2^-11) of the largest are
 // kept. The norms' factors are applied to the sums (fp32 q and k: before). G is
 // summed in fp64, so that a difference keeps its bits behind a token that
 // forgets everything. The inverse goes by forward substitution in blocks of 16,
@@ -157,6 +160,7 @@ typedef uint32_t dr_u2 __attribute__((ext_vector_type(2)));
 
 constexpr int PIECE = 64;
 constexpr int TRI = 6;                 // 16 x 32 blocks of a lower triangular 64 x 64: row tile w has w / 2 + 1
+// W's and P T's bounds hold while a state cannot grow: beta |k^|^2 <= 2 and g <= 0, but for roundings
 constexpr float RULE_WILD = 1e15f;     // values of q, k, v (squared: of S) past it go token by token
 constexpr float RULE_FAINT = 1e-24f;   // so do k and q whose squares' sum is below it, where norm_eps is too
 
@@ -176,13 +180,16 @@ template <int KD> struct RuleKeys {
     }
 };
 
+// the last row's: e^G_last (NaN: the piece goes token by token), what W and P T are divided by, the largest e^G |k^|
+enum { RULE_LAST = 0, RULE_W = 1, RULE_P = 2, RULE_K = 3 };
+
 // workspace of one window of pieces: byte offsets of arrays of 1 KB blocks (64 lanes x 16 bytes: an MFMA operand)
 struct RuleWork {
     char *base;
     uint32_t bytes;
     uint32_t k, q;         // [piece, key head][row tile][step][np]
-    uint32_t w, p;         // [piece, value head]: [key tile][2][3], [TRI][3]
-    uint32_t rows;         // [piece, value head][3][64] fp32: e^G / |k|, scale e^G / |q|; e^G_last, NaN: token by token
+    uint32_t w, p;         // [piece, value head]: [key tile][2][2], [TRI][2]
+    uint32_t rows;         // [piece, value head][3][64] fp32: e^G / |k|, scale e^G / |q|, RULE_LAST ..
     int first, pieces;     // the window
     int least;             // requests of fewer tokens are the token kernel's
 };
@@ -238,6 +245,43 @@ __device__ __forceinline__ void dr_split4(const lq_f4 &x, dr_u2 (&y)[3]) {
 #pragma unroll
     for (int i = 0; i < 3; ++i)     // the upper halves of two values
         y[i] = dr_u2{__builtin_amdgcn_perm(h[i][1], h[i][0], 0x07060302u), __builtin_amdgcn_perm(h[i][3], h[i][2], 0x07060302u)};
+}
+
+typedef _Float16 dr_h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 dr_h8 __attribute__((ext_vector_type(8)));
+
+// two values as two f16 pieces each
+__device__ __forceinline__ void dr_split2(float a, float b, uint32_t (&y)[2]) {
+    const dr_h2 h = __builtin_convertvector(dr_f2{a, b}, dr_h2);
+    const dr_h2 m = __builtin_convertvector(dr_f2{a - (float)h[0], b - (float)h[1]}, dr_h2);
+    y[0] = __builtin_bit_cast(uint32_t, h);
+    y[1] = __builtin_bit_cast(uint32_t, m);
+}
+__device__ __forceinline__ void dr_split8h(const float (&x)[8], dr_u4 (&y)[2]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        uint32_t u[2];
+        dr_split2(x[2 * e], x[2 * e + 1], u);
+        y[0][e] = u[0];
+        y[1][e] = u[1];
+    }
+}
+// the power of two that takes values below `bound` below 2^bits
+__device__ __forceinline__ float dr_scale(float bound, int bits) {
+    return ldexpf(1.0f, min(bits - __builtin_amdgcn_frexp_expf(bound), 120));
+}
+__device__ __forceinline__ float dr_wave_max(float x) {     // x >= 0
+    return __builtin_bit_cast(float, wave_max_u32(__builtin_bit_cast(uint32_t, x)));
+}
+
+__device__ __forceinline__ lq_f4 dr_mfma_h(const dr_u4 &a, const dr_u4 &b, const lq_f4 &c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(dr_h8, a), __builtin_bit_cast(dr_h8, b), c, 0, 0, 0);
+}
+// c[0] += the first pieces' product, c[1] += those of a first and a second
+__device__ __forceinline__ void dr_product_h(const dr_u4 (&a)[2], const dr_u4 (&b)[2], lq_f4 (&c)[2]) {
+    c[1] = dr_mfma_h(a[0], b[1], c[1]);
+    c[0] = dr_mfma_h(a[0], b[0], c[0]);
+    c[1] = dr_mfma_h(a[1], b[0], c[1]);
 }
 
 __device__ __forceinline__ lq_f4 dr_mfma(const dr_u4 &a, const dr_u4 &b, const lq_f4 &c) {
@@ -308,7 +352,7 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
     dr_u4 (&to)[TRI][3][64] = *reinterpret_cast<dr_u4 (*)[TRI][3][64]>(space);
     float (&tm)[PIECE][LD] = *reinterpret_cast<float (*)[PIECE][LD]>(space + AS);
     __shared__ double gs[PIECE];      // sums of g, in powers of two
-    __shared__ float bs[PIECE], ik[PIECE], iq[PIECE], kn[PIECE];
+    __shared__ float bs[PIECE], ik[PIECE], iq[PIECE], kn[PIECE], qn[PIECE];
     __shared__ __align__(16) float sc[PIECE];
     __shared__ int wild_s[4];
     const int local = (int)(blockIdx.x / p.key_heads), kh = (int)(blockIdx.x % p.key_heads);
@@ -354,7 +398,7 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
                 wild |= in;
                 inv = 0.0f;
             }
-            if (!o && g == 0) kn[16 * w + m] = ss * inv * inv;     // |k^|^2
+            if (g == 0) (o ? qn : kn)[16 * w + m] = ss * inv * inv;     // |k^|^2, |q^|^2 / scale^2
             const float by = !in ? 0.0f : NP == 3 ? inv : 1.0f;
             if (g == 0) (o ? iq : ik)[16 * w + m] = NP == 3 ? 1.0f : inv;
             dr_u4 *dst = (dr_u4 *)(ws.base + (o ? ws.q : ws.k)) + (((int64_t)local * p.key_heads + kh) * 4 + w) * NS * NP * 64 + lane;
@@ -391,17 +435,24 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
         bs[lane] = gb.y;
     }
     // (a state that grows by itself would make T grow to what the piece's sums cancel)
-    wild |= !(gb.y >= 0.0f && gb.y <= 1e3f) || !(gb.x <= 0.3f);
+    wild |= !(gb.y >= 0.0f && gb.y <= 1e3f) || !(gb.x <= 0.01f);
     const bool any = __any(wild);
     if (lane == 0) wild_s[w] = any;
     __syncthreads();
     const double last = gs[63];
-    const bool bad = (wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3]) || __any(!(gb.y * kn[lane] <= 2.1f));
+    const bool bad = (wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3]) || __any(!(gb.y * kn[lane] <= 2.001f));
+    // a column of W is beta_j k^_j through contractions (e^0.64 for the g's that round above 0), a row of P T meets q^
+    const float size_k = 1.001f * __builtin_amdgcn_sqrtf(kn[lane]), size_w = 2.0f * dr_wave_max(gb.y * size_k);
+    const float size_p = size_w * fabsf(p.scale) * dr_wave_max(1.001f * __builtin_amdgcn_sqrtf(qn[lane]));
+    const float by_w = dr_scale(size_w, 13), by_p = dr_scale(size_p, 13);
     if (w == 0) {
         float *rows = (float *)(ws.base + ws.rows) + at * 3 * PIECE;
         rows[lane] = dr_exp2(total) * ik[lane];
         rows[PIECE + lane] = dr_exp2(total) * iq[lane] * p.scale;
-        if (lane == 0) rows[2 * PIECE] = bad ? __builtin_nanf("") : dr_exp2(last);
+        const float size_r = dr_wave_max(dr_exp2(total) * size_k);
+        if (lane < 4)
+            rows[2 * PIECE + lane] = lane == RULE_LAST ? bad ? __builtin_nanf("") : dr_exp2(last)
+                                     : lane == RULE_W ? 1.0f / by_w : lane == RULE_P ? 1.0f / by_p : size_r;
         sc[lane] = dr_exp2(last - total) * ik[lane];
     }
     if (bad) return;     // nothing else of it is read
@@ -564,17 +615,18 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
 #pragma unroll
             for (int i = 0; i < NT; ++i) wt[i][c] = dr_total(acc[i]);
         }
-        dr_u4 *dst = (dr_u4 *)(ws.base + ws.w) + (at * Keys::TILES + w * NT) * 2 * 3 * 64 + lane;
+        dr_u4 *dst = (dr_u4 *)(ws.base + ws.w) + (at * Keys::TILES + w * NT) * 2 * 2 * 64 + lane;
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                const float y8[8] = {wt[i][2 * s][0], wt[i][2 * s][1], wt[i][2 * s][2], wt[i][2 * s][3],
-                                     wt[i][2 * s + 1][0], wt[i][2 * s + 1][1], wt[i][2 * s + 1][2], wt[i][2 * s + 1][3]};
-                dr_u4 y[3];
-                dr_split8<3>(y8, y);
+                float y8[8];
 #pragma unroll
-                for (int pc = 0; pc < 3; ++pc) dst[((i * 2 + s) * 3 + pc) * 64] = y[pc];
+                for (int e = 0; e < 8; ++e) y8[e] = wt[i][2 * s + (e >> 2)][e & 3] * by_w;
+                dr_u4 y[2];
+                dr_split8h(y8, y);
+#pragma unroll
+                for (int pc = 0; pc < 2; ++pc) dst[((i * 2 + s) * 2 + pc) * 64] = y[pc];
             }
     }
     __syncthreads();     // T's operands have been read
@@ -612,7 +664,7 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
     }
     __syncthreads();
     // P T's operands of row tile w (columns behind the tile's last are zero)
-    dr_u4 *dst = (dr_u4 *)(ws.base + ws.p) + (at * TRI + (w < 2 ? w : 2 * w - 2)) * 3 * 64 + lane;
+    dr_u4 *dst = (dr_u4 *)(ws.base + ws.p) + (at * TRI + (w < 2 ? w : 2 * w - 2)) * 2 * 64 + lane;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         if (s > w / 2) continue;
@@ -623,12 +675,12 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
             const float4 v = *reinterpret_cast<const float4 *>(&am[16 * w + m][col]);
             const float e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y8[4 * u + i] = 2 * s + u <= w ? e[i] * bs[col + i] : 0.0f;
+            for (int i = 0; i < 4; ++i) y8[4 * u + i] = 2 * s + u <= w ? e[i] * (bs[col + i] * by_p) : 0.0f;
         }
-        dr_u4 y[3];
-        dr_split8<3>(y8, y);
+        dr_u4 y[2];
+        dr_split8h(y8, y);
 #pragma unroll
-        for (int i = 0; i < 3; ++i) dst[(s * 3 + i) * 64] = y[i];
+        for (int i = 0; i < 2; ++i) dst[(s * 2 + i) * 64] = y[i];
     }
 }
 
@@ -650,7 +702,7 @@ __device__ __forceinline__ void dr_hold(X &...x) {
 template <typename T, int N>
 struct RuleValues {
     T v[N][4];
-    float c, last;
+    float c, last;     // last: the last row's four, in lanes 0 to 3
     // vb, rows: the request's v and the piece's factors; row0: the lane's first row, of `count`; first: the tiles' in the piece
     __device__ __forceinline__ void ask(const T *vb, int64_t ts, int row0, int count, const float *rows, int first) {
 #pragma unroll
@@ -658,18 +710,23 @@ struct RuleValues {
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[t][e] = vb[(int64_t)min(row0 + 16 * t + e, count - 1) * ts];
         c = rows[first + lane_id() % (16 * N)];
-        last = rows[2 * PIECE];
+        last = rows[2 * PIECE + (lane_id() & 3)];
     }
-    __device__ __forceinline__ void give(lq_f4 (*dst)[64], float *factors, int row0, int count, int first) {
+    // largest: of |v|, by column
+    __device__ __forceinline__ void give(lq_f4 (*dst)[64], float *factors, float (*largest)[16], int row0, int count, int first) {
+        float top = 0.0f;
 #pragma unroll
         for (int t = 0; t < N; ++t) {
             lq_f4 x;
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = row0 + 16 * t + e < count ? (float)v[t][e] : 0.0f;
+            top = fmaxf(top, fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
             dst[t][lane_id()] = x;
         }
+        top = dr_rows_max(top);
+        if (lane_id() < 16) largest[first / 16][lane_id()] = top;
         if (lane_id() < 16 * N) factors[first + lane_id()] = c;
-        if (first == 0 && lane_id() == 0) factors[PIECE] = last;
+        if (first == 0 && lane_id() < 4) factors[PIECE + lane_id()] = last;
     }
 };
 
@@ -691,9 +748,10 @@ template <typename T, int KD>
 __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
     typedef RuleKeys<KD> Keys;
     constexpr int NP = RuleType<T>::NP, NS = Keys::STEPS, NT = Keys::NT, NW = Keys::NW, OT = RULE_OT<KD>;
-    __shared__ __align__(16) dr_u4 ss[NS][3][64], rs[2][3][64];
+    __shared__ __align__(16) dr_u4 ss[NS][3][64], rs[2][2][64];
     __shared__ __align__(16) lq_f4 part[4][4][64], vs[2][4][64];
     __shared__ __align__(16) float cs[2][PIECE + 4];
+    __shared__ float vm[2][OT == 1 ? 4 : 1][16], sm[4][16], rf[16];     // largest |v|, |S| by column; what R was divided by
     __shared__ float red[2][4][2][16], kq[2][2][KD];
     __shared__ int wild_s[4];
     const int group = p.value_heads / p.key_heads, slices = p.vd / 16;
@@ -727,7 +785,7 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
                     for (int t = 0; t < 2 * min(span.count - j * PIECE, PIECE); ++t) __syncthreads();     // the others' token by token
             }
             if (mine == j + 1) {
-                v.give(vs[mine & 1], cs[mine & 1], mine * PIECE + 4 * g, span.count, 0);
+                v.give(vs[mine & 1], cs[mine & 1], vm[mine & 1], mine * PIECE + 4 * g, span.count, 0);
                 mine += 2;
                 v.ask(vb, p.v_ts, mine * PIECE + 4 * g, span.count, rows_of(mine), 0);
             }
@@ -757,12 +815,12 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
         const int o = w - 4;
         const auto tile = [&](int t) { return t ? 3 - o : o; };
         const bool upper = o > 1;                                      // its one tile has two blocks
-        uint32_t qb = ws.q + key0, pb = ws.p + val0 * TRI * 3 * 1024;
-        const uint32_t tri_step = (uint32_t)p.value_heads * TRI * 3 * 1024;
+        uint32_t qb = ws.q + key0, pb = ws.p + val0 * TRI * 2 * 1024;
+        const uint32_t tri_step = (uint32_t)p.value_heads * TRI * 2 * 1024;
         T *ob = (T *)p.out + ((int64_t)span.first + from * PIECE) * p.o_ts + h * p.o_hs + c0;
         const int o_ts = (int)p.o_ts;
         constexpr int PB = OT + 1;      // blocks of P T: the first tile's, the last one's two
-        dr_u4 qf[OT][NS][NP], pf[PB][3];
+        dr_u4 qf[OT][NS][NP], pf[PB][2];
         lq_f4 of[OT];
         const auto ask_q = [&]() {
 #pragma unroll
@@ -780,8 +838,8 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
 #pragma unroll
             for (int s = 0; s < PB; ++s)
 #pragma unroll
-                for (int i = 0; i < 3; ++i)
-                    pf[s][i] = block(pb + 3072 * (OT == 1 ? first(o) + (upper ? s : 0) : s ? first(3 - o) + s - 1 : o), i);
+                for (int i = 0; i < 2; ++i)
+                    pf[s][i] = block(pb + 2048 * (OT == 1 ? first(o) + (upper ? s : 0) : s ? first(3 - o) + s - 1 : o), i);
         };
         RuleValues<T, OT> v;      // of 256 key values
         ask_q();
@@ -790,7 +848,7 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
         dr_hold();
         if constexpr (KD > 128) {
             v.ask(vb, p.v_ts, from * PIECE + 16 * o + 4 * g, span.count, rows_of(from), 16 * o);
-            v.give(vs[from & 1] + o, cs[from & 1], from * PIECE + 16 * o + 4 * g, span.count, 16 * o);
+            v.give(vs[from & 1] + o, cs[from & 1], vm[from & 1], from * PIECE + 16 * o + 4 * g, span.count, 16 * o);
             v.ask(vb, p.v_ts, (from + 1) * PIECE + 16 * o + 4 * g, span.count, rows_of(from + 1), 16 * o);
         }
         for (int j = from; j < to; ++j) {
@@ -820,17 +878,18 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
             __syncthreads();     // R
             const int bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3];
             {
-                lq_f4 c[OT][3] = {};
-                dr_u4 y[2][3];
+                lq_f4 c[OT][2] = {};
+                dr_u4 y[2][2];
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) y[s][i] = rs[s][i][lane];
+                    for (int i = 0; i < 2; ++i) y[s][i] = rs[s][i][lane];
+                const float by = rf[m] * cs[j & 1][PIECE + RULE_P];
 #pragma unroll
                 for (int t = 0; t < OT; ++t) {
-                    dr_product<3, 3>(pf[t], y[0], c[t]);
-                    if (OT == 1 ? upper : t) dr_product<3, 3>(pf[t + 1], y[1], c[t]);
-                    O[t] = O[t] + dr_total(c[t]);
+                    dr_product_h(pf[t], y[0], c[t]);
+                    if (OT == 1 ? upper : t) dr_product_h(pf[t + 1], y[1], c[t]);
+                    O[t] = O[t] + (c[t][0] + c[t][1]) * by;
                     dr_hold(O[t]);
                 }
             }
@@ -856,7 +915,7 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
             }
             ob += PIECE * p.o_ts;
             if constexpr (KD > 128) {
-                v.give(vs[(j + 1) & 1] + o, cs[(j + 1) & 1], (j + 1) * PIECE + 16 * o + 4 * g, span.count, 16 * o);
+                v.give(vs[(j + 1) & 1] + o, cs[(j + 1) & 1], vm[(j + 1) & 1], (j + 1) * PIECE + 16 * o + 4 * g, span.count, 16 * o);
                 v.ask(vb, p.v_ts, (j + 2) * PIECE + 16 * o + 4 * g, span.count, rows_of(j + 2), 16 * o);
             }
         }
@@ -865,9 +924,9 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
 
     __builtin_amdgcn_s_setprio(3);      // ahead of the other waves, which have time to spare
     uint32_t kb = ws.k + key0 + w * NW * NP * 1024;
-    uint32_t wb = ws.w + (val0 * Keys::TILES + w * NT) * 2 * 3 * 1024;
-    const uint32_t w_step = (uint32_t)p.value_heads * Keys::TILES * 2 * 3 * 1024;
-    dr_u4 kf[4][NW][NP], wf[NT][2][3];
+    uint32_t wb = ws.w + (val0 * Keys::TILES + w * NT) * 2 * 2 * 1024;
+    const uint32_t w_step = (uint32_t)p.value_heads * Keys::TILES * 2 * 2 * 1024;
+    dr_u4 kf[4][NW][NP], wf[NT][2][2];
     const auto ask_k = [&]() {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -882,7 +941,7 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int i = 0; i < 3; ++i) wf[t][s][i] = block(wb, (t * 2 + s) * 3 + i);
+                for (int i = 0; i < 2; ++i) wf[t][s][i] = block(wb, (t * 2 + s) * 2 + i);
     };
     float *state = r.state + (span.slot * p.value_heads + h) * (int64_t)KD * p.vd + c0 + m;
     lq_f4 S[NT];
@@ -920,44 +979,61 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
             }
 #pragma unroll
             for (int t = 0; t < 4; ++t) part[w][t][lane] = c[t];
+            float top = 0.0f;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                top = fmaxf(top, fmaxf(fmaxf(fabsf(S[t][0]), fabsf(S[t][1])), fmaxf(fabsf(S[t][2]), fabsf(S[t][3]))));
+            top = dr_rows_max(top);
+            if (g == 0) sm[w][m] = top;
             __syncthreads();     // S
             const lq_f4 kS = (part[0][w][lane] + part[1][w][lane]) + (part[2][w][lane] + part[3][w][lane]);
             const lq_f4 R = vs[j & 1][w][lane] - *reinterpret_cast<const lq_f4 *>(&cs[j & 1][16 * w + 4 * g]) * kS;
-            const float lf = cs[j & 1][PIECE];
+            const float lf = cs[j & 1][PIECE + RULE_LAST];
             lq_f4 next[NT];
 #pragma unroll
             for (int t = 0; t < NT; ++t) next[t] = lf * S[t];
             // of v, or of S, whose products with k are in it; NaN where lf is
             const float size = fabsf(R[0]) + fabsf(R[1]) + fabsf(R[2]) + (fabsf(R[3]) + lf);
-            dr_u2 x[3];
-            dr_split4(R, x);
+            // what R of the column may be: |v|, and k^ . S at most the root of KD times the largest of S
+            constexpr float ROOT = 1.001f * (KD == 64 ? 8.0f : KD == 128 ? 11.3137085f : 16.0f);
+            const float most = fmaxf(fmaxf(sm[0][m], sm[1][m]), fmaxf(sm[2][m], sm[3][m])) * (ROOT * cs[j & 1][PIECE + RULE_K]);
+            const float v_top = OT > 1 ? vm[j & 1][0][m]
+                                       : fmaxf(fmaxf(vm[j & 1][0][m], vm[j & 1][OT > 1 ? 0 : 1][m]),
+                                               fmaxf(vm[j & 1][OT > 1 ? 0 : 2][m], vm[j & 1][OT > 1 ? 0 : 3][m]));
+            const int e14 = min(14 - __builtin_amdgcn_frexp_expf(most + v_top), 120);
+            const float scale = ldexpf(1.0f, e14), unscale = ldexpf(1.0f, -e14);
+            if (w == 0 && g == 0) rf[m] = unscale;
+            uint32_t x[2][2];
+            dr_split2(R[0] * scale, R[1] * scale, x[0]);
+            dr_split2(R[2] * scale, R[3] * scale, x[1]);
 #pragma unroll
-            for (int i = 0; i < 3; ++i) reinterpret_cast<dr_u2 *>(&rs[w >> 1][i][lane])[w & 1] = x[i];
+            for (int i = 0; i < 2; ++i) reinterpret_cast<dr_u2 *>(&rs[w >> 1][i][lane])[w & 1] = dr_u2{x[0][i], x[1][i]};
+            const float by = unscale * cs[j & 1][PIECE + RULE_W];
             const bool any = __any(!(size <= RULE_WILD * RULE_WILD));
             if (lane == 0) wild_s[w] = any;
             __syncthreads();     // R
             const int bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3];
-            dr_u4 y[2][3];
+            dr_u4 y[2][2];
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int i = 0; i < 3; ++i) y[s][i] = rs[s][i][lane];
+                for (int i = 0; i < 2; ++i) y[s][i] = rs[s][i][lane];
             kb += more ? key_step : 0;
             wb += more ? w_step : 0;
             if (__builtin_amdgcn_readfirstlane(bad)) break;
             ask_k();
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                lq_f4 d[3] = {next[t]};
+                lq_f4 d[2] = {};
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    dr_product<3, 3>(wf[t][s], y[s], d);
-                    dr_hold(d[0], d[1], d[2]);
+                    dr_product_h(wf[t][s], y[s], d);
+                    dr_hold(d[0], d[1]);
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) wf[t][s][i] = block(wb, (t * 2 + s) * 3 + i);
+                    for (int i = 0; i < 2; ++i) wf[t][s][i] = block(wb, (t * 2 + s) * 2 + i);
                     dr_hold();
                 }
-                S[t] = dr_total(d);
+                S[t] = next[t] + (d[0] + d[1]) * by;
             }
         }
         if (j >= to) break;
@@ -1029,7 +1105,7 @@ constexpr int64_t RULE_WINDOW = 128 << 20;
 
 static int64_t key_bytes(int np, int kd) { return 4 * (kd == 64 ? 4 : kd / 32) * np * 1024; }     // a piece's K, or Q
 static int64_t piece_bytes(int np, int key_heads, int value_heads, int kd) {
-    return 2 * key_heads * key_bytes(np, kd) + value_heads * ((kd / 16 * 2 + TRI) * 3 * 1024 + 12 * PIECE);
+    return 2 * key_heads * key_bytes(np, kd) + value_heads * ((kd / 16 * 2 + TRI) * 2 * 1024 + 12 * PIECE);
 }
 static int64_t all_pieces(int64_t tokens, int requests) { return tokens / PIECE + requests; }
 
@@ -1063,7 +1139,7 @@ static void rule_launch(const DeltaRule &p, const DeltaRequests &r, void *ws, hi
     const int64_t bytes = piece_bytes(NP, p.key_heads, p.value_heads, KD), all = all_pieces(r.tokens, r.requests);
     const int64_t window = std::min(all, delta_rule_workspace_bytes(r.tokens, r.requests, false, p.key_heads, p.value_heads, KD, p.vd) / bytes);
     RuleWork w{};
-    const int64_t keys = window * p.key_heads * key_bytes(NP, KD), tiles = window * p.value_heads * 3 * 1024;
+    const int64_t keys = window * p.key_heads * key_bytes(NP, KD), tiles = window * p.value_heads * 2 * 1024;
     uint32_t at = 0;     // (a window is far below 4 GB)
     w.base = (char *)ws;
     w.k = at;
