@@ -141,11 +141,13 @@ __global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequ
 // head, whose S stays in registers (delta_chain_kernel).
 //
 // Precision: everything is fp32's. MFMA takes 16-bit operands, so each fp32 value
-// goes in as several. S as three bf16 pieces (24 bits), q and k of 16 bits as they
-// are (bf16: one piece, f16: two), of fp32 three. W, P T and R, whose size is known
-// ahead, as two f16 pieces (22 bits of each value, and 2^-35 of the largest that it
-// may be: they are scaled by a power of two below that bound), a third fewer bytes
-// and half the products of three bf16 ones. Products up to 2^-16 (f16: 2^-11) of the largest are
+// goes in as several. bf16 q and k as they are, beside S and T in three bf16 pieces
+// (24 bits); f16 q and k as they are, fp32 ones in two f16 pieces, beside S and T in
+// two. W, P T and R are two f16 pieces always. Two f16 pieces hold 22 bits of a
+// value, and 2^-35 of the largest that it may be: they are scaled by a power of two
+// below a bound that is known ahead (rows of k and q their own, columns of S and T
+// theirs). They are a third fewer bytes and half the products of three bf16 ones.
+// Of the products those up to 2^-16 (f16: 2^-11) of the largest are
 // kept. The norms' factors are applied to the sums (fp32 q and k: before). G is
 // summed in fp64, so that a difference keeps its bits behind a token that
 // forgets everything. The inverse goes by forward substitution in blocks of 16,
@@ -164,10 +166,19 @@ constexpr int TRI = 6;                 // 16 x 32 blocks of a lower triangular 6
 constexpr float RULE_WILD = 1e15f;     // values of q, k, v (squared: of S) past it go token by token
 constexpr float RULE_FAINT = 1e-24f;   // so do k and q whose squares' sum is below it, where norm_eps is too
 
-// pieces that hold a value of type T, and whether the norm's factor goes in first
-template <typename T> struct RuleType { static constexpr int NP = 1; };
-template <> struct RuleType<_Float16> { static constexpr int NP = 2; };
-template <> struct RuleType<float> { static constexpr int NP = 3; };
+// pieces that hold a q or k of type T, whether they are f16, and pieces of S and T beside them
+template <typename T> struct RuleType {     // bf16
+    static constexpr bool HALF = false;
+    static constexpr int NP = 1, SP = 3;
+};
+template <> struct RuleType<_Float16> {
+    static constexpr bool HALF = true;
+    static constexpr int NP = 1, SP = 2;
+};
+template <> struct RuleType<float> {
+    static constexpr bool HALF = true;
+    static constexpr int NP = 2, SP = 2;
+};
 
 // Key values in the order of S's tiles of 16: tile t, row 4 g + e is key value
 // 32 (t / 2) + 8 g + 4 (t % 2) + e, so that a lane's eight values of two tiles are
@@ -287,16 +298,21 @@ __device__ __forceinline__ void dr_product_h(const dr_u4 (&a)[2], const dr_u4 (&
 __device__ __forceinline__ lq_f4 dr_mfma(const dr_u4 &a, const dr_u4 &b, const lq_f4 &c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dr_b8, a), __builtin_bit_cast(dr_b8, b), c, 0, 0, 0);
 }
-// c[i] += the products of pieces i apart in size, up to 2^-16 of the largest (NA, NB: pieces of a and b)
-template <int NA, int NB>
-__device__ __forceinline__ void dr_product(const dr_u4 (&a)[NA], const dr_u4 (&b)[NB], lq_f4 (&c)[3]) {
+// c[i] += the products of pieces i apart in size, of either kind (f16: up to 2^-11 of the largest)
+template <bool HALF, int NA, int NB>
+__device__ __forceinline__ void dr_any_product(const dr_u4 (&a)[NA], const dr_u4 (&b)[NB], lq_f4 (&c)[HALF ? 2 : 3]) {
 #pragma unroll
     for (int i = 0; i < NA; ++i)
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
-            if (i + j < 3) c[i + j] = dr_mfma(a[i], b[j], c[i + j]);
+        for (int j = 0; j < NB; ++j) {
+            if constexpr (HALF) {
+                if (i + j < 2) c[i + j] = dr_mfma_h(a[i], b[j], c[i + j]);
+            } else if (i + j < 3)
+                c[i + j] = dr_mfma(a[i], b[j], c[i + j]);
+        }
 }
 __device__ __forceinline__ lq_f4 dr_total(const lq_f4 (&c)[3]) { return c[0] + (c[1] + c[2]); }
+__device__ __forceinline__ lq_f4 dr_total(const lq_f4 (&c)[2]) { return c[0] + c[1]; }
 
 // 2^x for fp64 x, to fp32's last bit or so however large x is
 __device__ __forceinline__ float dr_exp2(double x) {
@@ -343,17 +359,18 @@ __device__ __forceinline__ double dr_add_from(double v) {
 template <typename T, int KD>
 __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
     typedef RuleKeys<KD> Keys;
-    constexpr int NP = RuleType<T>::NP, NS = Keys::STEPS, NT = Keys::NT, LD = 68;
+    constexpr bool HALF = RuleType<T>::HALF;
+    constexpr int NP = RuleType<T>::NP, SP = RuleType<T>::SP, CP = HALF ? 2 : 3, NS = Keys::STEPS, NT = Keys::NT, LD = 68;
     // K's operands, then A (later T's operands, P, P T) and T
-    constexpr int KS = 4 * NS * NP * 1024, AS = TRI * 3 * 1024, MS = PIECE * LD * 4;
+    constexpr int KS = 4 * NS * NP * 1024, AS = TRI * SP * 1024 > PIECE * LD * 4 ? TRI * SP * 1024 : PIECE * LD * 4, MS = PIECE * LD * 4;
     __shared__ __align__(16) char space[KS > AS + MS ? KS : AS + MS];
     dr_u4 (&ks)[4][NS][NP][64] = *reinterpret_cast<dr_u4 (*)[4][NS][NP][64]>(space);
     float (&am)[PIECE][LD] = *reinterpret_cast<float (*)[PIECE][LD]>(space);
-    dr_u4 (&to)[TRI][3][64] = *reinterpret_cast<dr_u4 (*)[TRI][3][64]>(space);
+    dr_u4 (&to)[TRI][SP][64] = *reinterpret_cast<dr_u4 (*)[TRI][SP][64]>(space);
     float (&tm)[PIECE][LD] = *reinterpret_cast<float (*)[PIECE][LD]>(space + AS);
     __shared__ double gs[PIECE];      // sums of g, in powers of two
     __shared__ float bs[PIECE], ik[PIECE], iq[PIECE], kn[PIECE], qn[PIECE];
-    __shared__ __align__(16) float sc[PIECE];
+    __shared__ __align__(16) float sc[PIECE], tw[PIECE];     // tw: of f16, what T's columns are divided by for W
     __shared__ int wild_s[4];
     const int local = (int)(blockIdx.x / p.key_heads), kh = (int)(blockIdx.x % p.key_heads);
     DeltaSpan span;
@@ -399,8 +416,9 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
                 inv = 0.0f;
             }
             if (g == 0) (o ? qn : kn)[16 * w + m] = ss * inv * inv;     // |k^|^2, |q^|^2 / scale^2
-            const float by = !in ? 0.0f : NP == 3 ? inv : 1.0f;
-            if (g == 0) (o ? iq : ik)[16 * w + m] = NP == 3 ? 1.0f : inv;
+            // fp32 rows: by a power of two to at most 2^13
+            const float by = NP == 2 ? dr_scale(1.001f * __builtin_amdgcn_sqrtf(ss), 13) : 1.0f;
+            if (g == 0) (o ? iq : ik)[16 * w + m] = NP == 2 ? inv / by : inv;
             dr_u4 *dst = (dr_u4 *)(ws.base + (o ? ws.q : ws.k)) + (((int64_t)local * p.key_heads + kh) * 4 + w) * NS * NP * 64 + lane;
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
@@ -411,7 +429,7 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[s][e] = e < V && in ? x[s][e] * by : 0.0f;
-                    dr_split8<NP>(x[s], y);
+                    dr_split8h(x[s], y);
                 }
 #pragma unroll
                 for (int i = 0; i < NP; ++i) {
@@ -454,6 +472,9 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
             rows[2 * PIECE + lane] = lane == RULE_LAST ? bad ? __builtin_nanf("") : dr_exp2(last)
                                      : lane == RULE_W ? 1.0f / by_w : lane == RULE_P ? 1.0f / by_p : size_r;
         sc[lane] = dr_exp2(last - total) * ik[lane];
+        // |T_ij| b_j e^.. / |k_i| of column j: its own row, or what row i makes of it
+        const float rows_at_most = dr_wave_max(ik[lane] * fmaxf(1.0f, gb.y * size_k));
+        if (HALF) tw[lane] = dr_scale(2.0f * rows_at_most * gb.y * fmaxf(1.0f, size_k), 13);
     }
     if (bad) return;     // nothing else of it is read
     // K with tokens contracted: lane (key value (t, m), tokens 4 g + 0..3 and 16 + 4 g + 0..3 of 32), the wave's key tiles
@@ -480,7 +501,7 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
     for (int j = 0; j < 4; ++j) {
         kk[j] = qk[j] = lq_f4{0, 0, 0, 0};
         if (j <= w) {
-            lq_f4 a[3] = {}, c[3] = {};
+            lq_f4 a[CP] = {}, c[CP] = {};
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
                 dr_u4 x[NP], y[NP];
@@ -489,8 +510,8 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
                     x[i] = ks[w][s][i][lane];
                     y[i] = ks[j][s][i][lane];
                 }
-                dr_product<NP, NP>(x, y, a);
-                dr_product<NP, NP>(qf[s], y, c);
+                dr_any_product<HALF, NP, NP>(x, y, a);
+                dr_any_product<HALF, NP, NP>(qf[s], y, c);
             }
             kk[j] = dr_total(a);
             qk[j] = dr_total(c);
@@ -578,7 +599,7 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
     // holds, tile by tile; in A's place
     {
         const bool odd = w & 1;
-        const float bc = bs[16 * w + m];
+        const float bc = bs[16 * w + m] * (HALF ? tw[16 * w + m] : 1.0f);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {     // tokens 32 (w / 2 + s) ..
             if (w / 2 + s > 1) continue;
@@ -592,10 +613,11 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y8[4 * u + e] = tile[e] * (bc * by[e]);
             }
-            dr_u4 y[3];
-            dr_split8<3>(y8, y);
+            dr_u4 y[SP];
+            if constexpr (HALF) dr_split8h(y8, y);
+            else dr_split8<3>(y8, y);
 #pragma unroll
-            for (int pc = 0; pc < 3; ++pc) to[w < 2 ? 2 * w + s : w + 2][pc][lane] = y[pc];
+            for (int pc = 0; pc < SP; ++pc) to[w < 2 ? 2 * w + s : w + 2][pc][lane] = y[pc];
         }
     }
     __syncthreads();
@@ -603,17 +625,21 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
         lq_f4 wt[NT][4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            lq_f4 acc[NT][3] = {};
+            lq_f4 acc[NT][CP] = {};
 #pragma unroll
             for (int s = c >> 1; s < 2; ++s) {
-                dr_u4 y[3];
+                dr_u4 y[SP];
 #pragma unroll
-                for (int pc = 0; pc < 3; ++pc) y[pc] = to[c < 2 ? 2 * c + s : c + 2][pc][lane];
+                for (int pc = 0; pc < SP; ++pc) y[pc] = to[c < 2 ? 2 * c + s : c + 2][pc][lane];
 #pragma unroll
-                for (int i = 0; i < NT; ++i) dr_product<3, NP>(y, kt[i][s], acc[i]);
+                for (int i = 0; i < NT; ++i) dr_any_product<HALF, SP, NP>(y, kt[i][s], acc[i]);
             }
+            lq_f4 by = {by_w, by_w, by_w, by_w};
+            if (HALF)
 #pragma unroll
-            for (int i = 0; i < NT; ++i) wt[i][c] = dr_total(acc[i]);
+                for (int e = 0; e < 4; ++e) by[e] /= tw[16 * c + 4 * g + e];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) wt[i][c] = dr_total(acc[i]) * by;
         }
         dr_u4 *dst = (dr_u4 *)(ws.base + ws.w) + (at * Keys::TILES + w * NT) * 2 * 2 * 64 + lane;
 #pragma unroll
@@ -622,7 +648,7 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
             for (int s = 0; s < 2; ++s) {
                 float y8[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y8[e] = wt[i][2 * s + (e >> 2)][e & 3] * by_w;
+                for (int e = 0; e < 8; ++e) y8[e] = wt[i][2 * s + (e >> 2)][e & 3];
                 dr_u4 y[2];
                 dr_split8h(y8, y);
 #pragma unroll
@@ -747,11 +773,14 @@ constexpr int RULE_CHAIN = 512;      // threads
 template <typename T, int KD>
 __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
     typedef RuleKeys<KD> Keys;
-    constexpr int NP = RuleType<T>::NP, NS = Keys::STEPS, NT = Keys::NT, NW = Keys::NW, OT = RULE_OT<KD>;
-    __shared__ __align__(16) dr_u4 ss[NS][3][64], rs[2][2][64];
+    constexpr bool HALF = RuleType<T>::HALF;
+    constexpr int NP = RuleType<T>::NP, SP = RuleType<T>::SP, CP = HALF ? 2 : 3;
+    constexpr int NS = Keys::STEPS, NT = Keys::NT, NW = Keys::NW, OT = RULE_OT<KD>;
+    __shared__ __align__(16) dr_u4 ss[NS][SP][64], rs[2][2][64];
     __shared__ __align__(16) lq_f4 part[4][4][64], vs[2][4][64];
     __shared__ __align__(16) float cs[2][PIECE + 4];
-    __shared__ float vm[2][OT == 1 ? 4 : 1][16], sm[4][16], rf[16];     // largest |v|, |S| by column; what R was divided by
+    __shared__ float vm[2][OT == 1 ? 4 : 1][16], sm[4][16], su[4][16], rf[16];
+    // (largest |v|, |S| of a wave's quarter by column; what S, of f16, and R were divided by)
     __shared__ float red[2][4][2][16], kq[2][2][KD];
     __shared__ int wild_s[4];
     const int group = p.value_heads / p.key_heads, slices = p.vd / 16;
@@ -857,18 +886,30 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
             __syncthreads();     // S
             lq_f4 O[OT];
             {
-                lq_f4 c[OT][3] = {};
+                lq_f4 c[OT][CP] = {}, sum[OT] = {};
 #pragma unroll
                 for (int s = 0; s < NS; ++s) {
-                    dr_u4 z[3];
+                    dr_u4 z[SP];
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) z[i] = ss[s][i][lane];
+                    for (int i = 0; i < SP; ++i) z[i] = ss[s][i][lane];
 #pragma unroll
-                    for (int t = 0; t < OT; ++t) dr_product<NP, 3>(qf[t][s], z, c[t]);
+                    for (int t = 0; t < OT; ++t) dr_any_product<HALF, NP, SP>(qf[t][s], z, c[t]);
+                    if (HALF && s % NW == NW - 1) {     // a wave's quarter, with its own scale
+                        const float by = su[s / NW][m];
+#pragma unroll
+                        for (int t = 0; t < OT; ++t) {
+                            sum[t] = sum[t] + dr_total(c[t]) * by;
+#pragma unroll
+                            for (int i = 0; i < CP; ++i) c[t][i] = lq_f4{0, 0, 0, 0};
+                        }
+                    }
                 }
 #pragma unroll
+                for (int t = 0; t < OT; ++t)
+                    if (!HALF) sum[t] = dr_total(c[t]);
+#pragma unroll
                 for (int t = 0; t < OT; ++t) {
-                    O[t] = dr_total(c[t]) * of[t];
+                    O[t] = sum[t] * of[t];
                     dr_hold(O[t]);
                 }
             }
@@ -957,34 +998,43 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
         dr_hold();
         for (; j < to; ++j) {
             const bool more = j + 1 < to;     // the last piece's are asked for again and not used
-            lq_f4 c[4] = {};
-#pragma unroll
-            for (int s = 0; s < NW; ++s) {
-                dr_u2 lo[3], hi[3] = {};
-                dr_split4(S[NT > 1 ? 2 * s : 0], lo);
-                if (NT > 1) dr_split4(S[NT > 1 ? 2 * s + 1 : 0], hi);
-                dr_u4 z[3];
-#pragma unroll
-                for (int i = 0; i < 3; ++i) {
-                    z[i] = dr_u4{lo[i][0], lo[i][1], hi[i][0], hi[i][1]};
-                    ss[w * NW + s][i][lane] = z[i];
-                }
-#pragma unroll
-                for (int i = 2; i >= 0; --i)     // the smallest products first
-#pragma unroll
-                    for (int u = 0; u < NP; ++u)
-                        if (u <= i)
-#pragma unroll
-                            for (int t = 0; t < 4; ++t) c[t] = dr_mfma(kf[t][s][u], z[i - u], c[t]);
-            }
-#pragma unroll
-            for (int t = 0; t < 4; ++t) part[w][t][lane] = c[t];
-            float top = 0.0f;
+            float top = 0.0f;     // of |S|, of the wave's quarter of the column
 #pragma unroll
             for (int t = 0; t < NT; ++t)
                 top = fmaxf(top, fmaxf(fmaxf(fabsf(S[t][0]), fabsf(S[t][1])), fmaxf(fabsf(S[t][2]), fabsf(S[t][3]))));
             top = dr_rows_max(top);
             if (g == 0) sm[w][m] = top;
+            const int e14 = min(14 - __builtin_amdgcn_frexp_expf(top), 120);
+            const float up = ldexpf(1.0f, e14), down = ldexpf(1.0f, -e14);
+            if (HALF && g == 0) su[w][m] = down;
+            lq_f4 c[4] = {};
+#pragma unroll
+            for (int s = 0; s < NW; ++s) {
+                dr_u4 z[SP];
+                if constexpr (HALF) {
+                    const lq_f4 lo = S[NT > 1 ? 2 * s : 0] * up, hi = NT > 1 ? S[NT > 1 ? 2 * s + 1 : 0] * up : lq_f4{0, 0, 0, 0};
+                    const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                    dr_split8h(x, z);
+                } else {
+                    dr_u2 lo[3], hi[3] = {};
+                    dr_split4(S[NT > 1 ? 2 * s : 0], lo);
+                    if (NT > 1) dr_split4(S[NT > 1 ? 2 * s + 1 : 0], hi);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) z[i] = dr_u4{lo[i][0], lo[i][1], hi[i][0], hi[i][1]};
+                }
+#pragma unroll
+                for (int i = 0; i < SP; ++i) ss[w * NW + s][i][lane] = z[i];
+#pragma unroll
+                for (int i = SP - 1; i >= 0; --i)     // the smallest products first
+#pragma unroll
+                    for (int u = 0; u < NP; ++u)
+                        if (u <= i)
+#pragma unroll
+                            for (int t = 0; t < 4; ++t)
+                                c[t] = HALF ? dr_mfma_h(kf[t][s][u], z[i - u], c[t]) : dr_mfma(kf[t][s][u], z[i - u], c[t]);
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) part[w][t][lane] = HALF ? c[t] * down : c[t];
             __syncthreads();     // S
             const lq_f4 kS = (part[0][w][lane] + part[1][w][lane]) + (part[2][w][lane] + part[3][w][lane]);
             const lq_f4 R = vs[j & 1][w][lane] - *reinterpret_cast<const lq_f4 *>(&cs[j & 1][16 * w + 4 * g]) * kS;
@@ -1000,8 +1050,8 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
             const float v_top = OT > 1 ? vm[j & 1][0][m]
                                        : fmaxf(fmaxf(vm[j & 1][0][m], vm[j & 1][OT > 1 ? 0 : 1][m]),
                                                fmaxf(vm[j & 1][OT > 1 ? 0 : 2][m], vm[j & 1][OT > 1 ? 0 : 3][m]));
-            const int e14 = min(14 - __builtin_amdgcn_frexp_expf(most + v_top), 120);
-            const float scale = ldexpf(1.0f, e14), unscale = ldexpf(1.0f, -e14);
+            const int r14 = min(14 - __builtin_amdgcn_frexp_expf(most + v_top), 120);
+            const float scale = ldexpf(1.0f, r14), unscale = ldexpf(1.0f, -r14);
             if (w == 0 && g == 0) rf[m] = unscale;
             uint32_t x[2][2];
             dr_split2(R[0] * scale, R[1] * scale, x[0]);
@@ -1113,7 +1163,7 @@ static int64_t all_pieces(int64_t tokens, int requests) { return tokens / PIECE 
 int64_t delta_rule_workspace_bytes(int64_t tokens, int requests, bool step, int key_heads, int value_heads, int kd,
                                    int vd) {
     if (step) return 0;
-    const int64_t bytes = piece_bytes(3, key_heads, value_heads, kd), all = all_pieces(tokens, requests);
+    const int64_t bytes = piece_bytes(2, key_heads, value_heads, kd), all = all_pieces(tokens, requests);
     return std::min(all, std::max<int64_t>(RULE_WINDOW / bytes, 1)) * bytes;
 }
 
