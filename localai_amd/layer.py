@@ -27,7 +27,7 @@ import struct
 import numpy as np
 
 from . import _lib, device
-from .paged import _empty, _hold, _ptr, _r, _refuse, _stream
+from .paged import _device_tensor, _empty, _hold, _ptr, _r, _refuse, _stream
 
 ORDER = ('attn_output', 'ffn_gate', 'ffn_up', 'ffn_down', 'attn_q', 'attn_k', 'attn_v')
 
@@ -126,11 +126,10 @@ def rms_norm(x, weight, eps=1e-6, residual=None, gate=None, dtype=None, out=None
     and strides of 4 values). Returns the result, in `out` if given: x itself where the types are
     the same, or memory of its own."""
     global _norm
+    _device_tensor(x, 'x')
     r = _r()
     if _norm is None:
         _norm = _Norm()
-    if not isinstance(x, r.Tensor):
-        raise TypeError('x must be a device tensor')
     given = x.dtype
     if dtype is None:
         dtype = given
