@@ -164,6 +164,7 @@ constexpr int PIECE = 64;
 constexpr int TRI = 6;                 // 16 x 32 blocks of a lower triangular 64 x 64: row tile w has w / 2 + 1
 // W's and P T's bounds hold while a state cannot grow: beta |k^|^2 <= 2 and g <= 0, but for roundings
 constexpr float RULE_WILD = 1e15f;     // values of q, k, v (squared: of S) past it go token by token
+constexpr float RULE_SQUARE = 1e-36f;   // more than what 256 squares lose below fp32's range
 constexpr float RULE_FAINT = 1e-24f;   // so do k and q whose squares' sum is below it, where norm_eps is too
 
 // pieces that hold a q or k of type T, whether they are f16, and pieces of S and T beside them
@@ -415,9 +416,11 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
                 wild |= in;
                 inv = 0.0f;
             }
-            if (g == 0) (o ? qn : kn)[16 * w + m] = ss * inv * inv;     // |k^|^2, |q^|^2 / scale^2
+            // bounds of |k^|^2, |q^|^2 / scale^2, also where the squares vanish
+            const float bound = ss + RULE_SQUARE;
+            if (g == 0) (o ? qn : kn)[16 * w + m] = bound * inv * inv;
             // fp32 rows: by a power of two to at most 2^13
-            const float by = NP == 2 ? dr_scale(1.001f * __builtin_amdgcn_sqrtf(ss), 13) : 1.0f;
+            const float by = NP == 2 ? dr_scale(1.001f * __builtin_amdgcn_sqrtf(bound), 13) : 1.0f;
             if (g == 0) (o ? iq : ik)[16 * w + m] = NP == 2 ? inv / by : inv;
             dr_u4 *dst = (dr_u4 *)(ws.base + (o ? ws.q : ws.k)) + (((int64_t)local * p.key_heads + kh) * 4 + w) * NS * NP * 64 + lane;
 #pragma unroll
@@ -963,7 +966,6 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
         return;
     }
 
-    __builtin_amdgcn_s_setprio(3);      // ahead of the other waves, which have time to spare
     uint32_t kb = ws.k + key0 + w * NW * NP * 1024;
     uint32_t wb = ws.w + (val0 * Keys::TILES + w * NT) * 2 * 2 * 1024;
     const uint32_t w_step = (uint32_t)p.value_heads * Keys::TILES * 2 * 2 * 1024;
@@ -1059,7 +1061,7 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
 #pragma unroll
             for (int i = 0; i < 2; ++i) reinterpret_cast<dr_u2 *>(&rs[w >> 1][i][lane])[w & 1] = dr_u2{x[0][i], x[1][i]};
             const float by = unscale * cs[j & 1][PIECE + RULE_W];
-            const bool any = __any(!(size <= RULE_WILD * RULE_WILD));
+            const bool any = __any(!(size <= RULE_WILD * RULE_WILD) || !(most + v_top <= RULE_WILD * RULE_WILD));
             if (lane == 0) wild_s[w] = any;
             __syncthreads();     // R
             const int bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3];

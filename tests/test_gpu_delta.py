@@ -414,6 +414,41 @@ def test_rule_sizes(size):
     _against_oracle((q * 1e3, k * 1e-3, v * size, decay, beta, state * size))
 
 
+@pytest.mark.parametrize('dtype', ['float32', 'bfloat16'])
+@pytest.mark.parametrize('small', [1e-15, 1e-18, 1e-20, 1e-23])
+def test_rule_small_keys_and_a_large_state(small, dtype):
+    """Keys whose squares leave fp32's range, and a state whose products with them are far above v."""
+    import torch
+    rng = np.random.default_rng(7)
+    q, k, v, decay, beta, state = _finite_case(rng)
+    q, k, v = (x.to(getattr(torch, dtype)) for x in (q, k * small, v))
+    # (the result's type adds its half step)
+    _against_oracle((q, k, v, decay, beta, state * 1e25), tol=2e-5 + 2 * HALF[dtype])
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_rule_state_values_that_no_key_meets(dtype):
+    """One key value is zero in every k and q: what the state holds there, up to fp32's largest, reaches nothing."""
+    import torch
+    from localai_amd import delta
+    rng = np.random.default_rng(8)
+    q, k, v, decay, beta, state = _finite_case(rng)
+    k[:, :, 5], q[:, :, 5] = 0, 0
+    q, k, v = (x.to(getattr(torch, dtype)) for x in (q, k, v))
+    decay *= 1e-3
+    want_state = state.clone()
+    state[:, :, 5] = 3e38
+    want_state[:, :, 5] = 0
+    starts = _ints([0, 150])
+    want = delta.rule(q, k, v, decay, beta, want_state, starts=starts)
+    got = delta.rule(q, k, v, decay, beta, state, starts=starts)
+    # both within the tolerance above, which is of the norm of a head's state
+    rows = [i for i in range(128) if i != 5]
+    size = want_state.norm(dim=(2, 3)).max().item()
+    assert (state - want_state)[:, :, rows].norm().item() <= 4e-5 * 2 * size
+    assert (got.float() - want.float()).norm().item() <= 2 * (2e-5 + 2 * HALF[dtype]) * (want.float().norm().item() + size)
+
+
 def test_rule_large_betas():
     """beta |k|^2 past 2 (a state that overshoots) goes token by token."""
     rng = np.random.default_rng(6)
