@@ -140,15 +140,14 @@ __global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequ
 // request's pieces is a second one, each workgroup with 16 value columns of one
 // head, whose S stays in registers (delta_chain_kernel).
 //
-// Precision: everything is fp32's. MFMA takes 16-bit operands, so each fp32 value
-// goes in as several. bf16 q and k as they are, beside S and T in three bf16 pieces
-// (24 bits); f16 q and k as they are, fp32 ones in two f16 pieces, beside S and T in
-// two. W, P T and R are two f16 pieces always. Two f16 pieces hold 22 bits of a
-// value, and 2^-35 of the largest that it may be: they are scaled by a power of two
-// below a bound that is known ahead (rows of k and q their own, columns of S and T
-// theirs). They are a third fewer bytes and half the products of three bf16 ones.
-// Of the products those up to 2^-16 (f16: 2^-11) of the largest are
-// kept. The norms' factors are applied to the sums (fp32 q and k: before). G is
+// Precision: fp32's, up to two bits. MFMA takes 16-bit operands, so each fp32 value
+// goes in as two f16 pieces: 22 bits of it, and 2^-35 of the largest that it may be
+// (operands are scaled by a power of two below a bound that is known ahead: rows
+// of q and k, columns of S, T, W, P T and R have their own). bf16 q and k are one
+// such piece, f16 ones one as they are. Of the products those up to 2^-11 of the
+// largest are kept, in fp32 sums; norms and decays are applied to the sums. Three
+// bf16 pieces of the unscaled values would hold 24 bits, in half as many bytes and
+// products again (8192 tokens, 32 heads of 128, bf16: 318 us). G is
 // summed in fp64, so that a difference keeps its bits behind a token that
 // forgets everything. The inverse goes by forward substitution in blocks of 16,
 // whose numbers stay as small as the rule's own.
@@ -156,7 +155,6 @@ __global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequ
 // range, goes through its tokens one by one instead: NaN times a zero of T or
 // P T would reach tokens before it.
 
-typedef __bf16 dr_b8 __attribute__((ext_vector_type(8)));
 typedef uint32_t dr_u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t dr_u2 __attribute__((ext_vector_type(2)));
 
@@ -167,19 +165,10 @@ constexpr float RULE_WILD = 1e15f;     // values of q, k, v (squared: of S) past
 constexpr float RULE_SQUARE = 1e-36f;   // more than what 256 squares lose below fp32's range
 constexpr float RULE_FAINT = 1e-24f;   // so do k and q whose squares' sum is below it, where norm_eps is too
 
-// pieces that hold a q or k of type T, whether they are f16, and pieces of S and T beside them
-template <typename T> struct RuleType {     // bf16
-    static constexpr bool HALF = false;
-    static constexpr int NP = 1, SP = 3;
-};
-template <> struct RuleType<_Float16> {
-    static constexpr bool HALF = true;
-    static constexpr int NP = 1, SP = 2;
-};
-template <> struct RuleType<float> {
-    static constexpr bool HALF = true;
-    static constexpr int NP = 2, SP = 2;
-};
+// f16 pieces of a q or k of type T, and whether their rows are scaled
+template <typename T> constexpr int RULE_NP = sizeof(T) == 4 ? 2 : 1;
+template <typename T> constexpr bool RULE_SCALED = true;
+template <> constexpr bool RULE_SCALED<_Float16> = false;
 
 // Key values in the order of S's tiles of 16: tile t, row 4 g + e is key value
 // 32 (t / 2) + 8 g + 4 (t % 2) + e, so that a lane's eight values of two tiles are
@@ -223,42 +212,7 @@ __device__ __forceinline__ float dr_rows_max(float v) {
     return fmaxf(f(b[0]), f(b[1]));
 }
 
-typedef __bf16 dr_b2 __attribute__((ext_vector_type(2)));
 typedef float dr_f2 __attribute__((ext_vector_type(2)));
-
-// eight values as N bf16 pieces each, the first the nearest, the next what is left (two values an instruction)
-template <int N>
-__device__ __forceinline__ void dr_split8(const float (&x)[8], dr_u4 (&y)[N]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        dr_f2 left = {x[2 * e], x[2 * e + 1]};
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_convertvector(left, dr_b2));
-            y[i][e] = h;
-            left[0] -= __builtin_bit_cast(float, h << 16);
-            left[1] -= __builtin_bit_cast(float, h & 0xffff0000u);
-        }
-    }
-}
-// Three pieces by cutting bits off: exact too, a third fewer instructions, and
-// the pieces one bit larger (the dropped products 2^-25 of the largest instead
-// of 2^-26: the other operand's pieces are the nearest).
-__device__ __forceinline__ void dr_split4(const lq_f4 &x, dr_u2 (&y)[3]) {
-    uint32_t h[3][4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float a = x[e], b = a - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, a) & 0xffff0000u);
-        const float c = b - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, b) & 0xffff0000u);
-        h[0][e] = __builtin_bit_cast(uint32_t, a);
-        h[1][e] = __builtin_bit_cast(uint32_t, b);
-        h[2][e] = __builtin_bit_cast(uint32_t, c);
-    }
-#pragma unroll
-    for (int i = 0; i < 3; ++i)     // the upper halves of two values
-        y[i] = dr_u2{__builtin_amdgcn_perm(h[i][1], h[i][0], 0x07060302u), __builtin_amdgcn_perm(h[i][3], h[i][2], 0x07060302u)};
-}
-
 typedef _Float16 dr_h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 dr_h8 __attribute__((ext_vector_type(8)));
 
@@ -269,7 +223,7 @@ __device__ __forceinline__ void dr_split2(float a, float b, uint32_t (&y)[2]) {
     y[0] = __builtin_bit_cast(uint32_t, h);
     y[1] = __builtin_bit_cast(uint32_t, m);
 }
-__device__ __forceinline__ void dr_split8h(const float (&x)[8], dr_u4 (&y)[2]) {
+__device__ __forceinline__ void dr_split8(const float (&x)[8], dr_u4 (&y)[2]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         uint32_t u[2];
@@ -286,33 +240,16 @@ __device__ __forceinline__ float dr_wave_max(float x) {     // x >= 0
     return __builtin_bit_cast(float, wave_max_u32(__builtin_bit_cast(uint32_t, x)));
 }
 
-__device__ __forceinline__ lq_f4 dr_mfma_h(const dr_u4 &a, const dr_u4 &b, const lq_f4 &c) {
+__device__ __forceinline__ lq_f4 dr_mfma(const dr_u4 &a, const dr_u4 &b, const lq_f4 &c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(dr_h8, a), __builtin_bit_cast(dr_h8, b), c, 0, 0, 0);
 }
 // c[0] += the first pieces' product, c[1] += those of a first and a second
-__device__ __forceinline__ void dr_product_h(const dr_u4 (&a)[2], const dr_u4 (&b)[2], lq_f4 (&c)[2]) {
-    c[1] = dr_mfma_h(a[0], b[1], c[1]);
-    c[0] = dr_mfma_h(a[0], b[0], c[0]);
-    c[1] = dr_mfma_h(a[1], b[0], c[1]);
+template <int NA, int NB>
+__device__ __forceinline__ void dr_product(const dr_u4 (&a)[NA], const dr_u4 (&b)[NB], lq_f4 (&c)[2]) {
+    if constexpr (NB > 1) c[1] = dr_mfma(a[0], b[1], c[1]);
+    c[0] = dr_mfma(a[0], b[0], c[0]);
+    if constexpr (NA > 1) c[1] = dr_mfma(a[1], b[0], c[1]);
 }
-
-__device__ __forceinline__ lq_f4 dr_mfma(const dr_u4 &a, const dr_u4 &b, const lq_f4 &c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dr_b8, a), __builtin_bit_cast(dr_b8, b), c, 0, 0, 0);
-}
-// c[i] += the products of pieces i apart in size, of either kind (f16: up to 2^-11 of the largest)
-template <bool HALF, int NA, int NB>
-__device__ __forceinline__ void dr_any_product(const dr_u4 (&a)[NA], const dr_u4 (&b)[NB], lq_f4 (&c)[HALF ? 2 : 3]) {
-#pragma unroll
-    for (int i = 0; i < NA; ++i)
-#pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            if constexpr (HALF) {
-                if (i + j < 2) c[i + j] = dr_mfma_h(a[i], b[j], c[i + j]);
-            } else if (i + j < 3)
-                c[i + j] = dr_mfma(a[i], b[j], c[i + j]);
-        }
-}
-__device__ __forceinline__ lq_f4 dr_total(const lq_f4 (&c)[3]) { return c[0] + (c[1] + c[2]); }
 __device__ __forceinline__ lq_f4 dr_total(const lq_f4 (&c)[2]) { return c[0] + c[1]; }
 
 // 2^x for fp64 x, to fp32's last bit or so however large x is
@@ -358,20 +295,20 @@ __device__ __forceinline__ double dr_add_from(double v) {
 // the layout in which MFMA leaves two tiles of results, so those are operands
 // as they are.
 template <typename T, int KD>
-__global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
+__global__ __launch_bounds__(256, RULE_NP<T> == 1 ? 2 : 1) void delta_piece_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
     typedef RuleKeys<KD> Keys;
-    constexpr bool HALF = RuleType<T>::HALF;
-    constexpr int NP = RuleType<T>::NP, SP = RuleType<T>::SP, CP = HALF ? 2 : 3, NS = Keys::STEPS, NT = Keys::NT, LD = 68;
+    constexpr int NP = RULE_NP<T>, NS = Keys::STEPS, NT = Keys::NT, LD = 68;
     // K's operands, then A (later T's operands, P, P T) and T
-    constexpr int KS = 4 * NS * NP * 1024, AS = TRI * SP * 1024 > PIECE * LD * 4 ? TRI * SP * 1024 : PIECE * LD * 4, MS = PIECE * LD * 4;
+    constexpr int KS = 4 * NS * NP * 1024, AS = PIECE * LD * 4, MS = AS;
+    static_assert(AS >= TRI * 2 * 1024);
     __shared__ __align__(16) char space[KS > AS + MS ? KS : AS + MS];
     dr_u4 (&ks)[4][NS][NP][64] = *reinterpret_cast<dr_u4 (*)[4][NS][NP][64]>(space);
     float (&am)[PIECE][LD] = *reinterpret_cast<float (*)[PIECE][LD]>(space);
-    dr_u4 (&to)[TRI][SP][64] = *reinterpret_cast<dr_u4 (*)[TRI][SP][64]>(space);
+    dr_u4 (&to)[TRI][2][64] = *reinterpret_cast<dr_u4 (*)[TRI][2][64]>(space);
     float (&tm)[PIECE][LD] = *reinterpret_cast<float (*)[PIECE][LD]>(space + AS);
     __shared__ double gs[PIECE];      // sums of g, in powers of two
     __shared__ float bs[PIECE], ik[PIECE], iq[PIECE], kn[PIECE], qn[PIECE];
-    __shared__ __align__(16) float sc[PIECE], tw[PIECE];     // tw: of f16, what T's columns are divided by for W
+    __shared__ __align__(16) float sc[PIECE], tw[PIECE];     // tw: what T's columns are multiplied by for W
     __shared__ int wild_s[4];
     const int local = (int)(blockIdx.x / p.key_heads), kh = (int)(blockIdx.x % p.key_heads);
     DeltaSpan span;
@@ -419,20 +356,24 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
             // bounds of |k^|^2, |q^|^2 / scale^2, also where the squares vanish
             const float bound = ss + RULE_SQUARE;
             if (g == 0) (o ? qn : kn)[16 * w + m] = bound * inv * inv;
-            // fp32 rows: by a power of two to at most 2^13
-            const float by = NP == 2 ? dr_scale(1.001f * __builtin_amdgcn_sqrtf(bound), 13) : 1.0f;
-            if (g == 0) (o ? iq : ik)[16 * w + m] = NP == 2 ? inv / by : inv;
+            // rows by a power of two to at most 2^13
+            const float by = RULE_SCALED<T> ? dr_scale(1.001f * __builtin_amdgcn_sqrtf(bound), 13) : 1.0f;
+            if (g == 0) (o ? iq : ik)[16 * w + m] = RULE_SCALED<T> ? inv / by : inv;
             dr_u4 *dst = (dr_u4 *)(ws.base + (o ? ws.q : ws.k)) + (((int64_t)local * p.key_heads + kh) * 4 + w) * NS * NP * 64 + lane;
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
                 dr_u4 y[NP];
-                if constexpr (NP == 1) {     // the values' own bits
+                if constexpr (!RULE_SCALED<T>) {     // the values' own bits
                     __builtin_memcpy(y, raw[o][s].v, 16);
                     if (!in) y[0] = dr_u4{0, 0, 0, 0};
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[s][e] = e < V && in ? x[s][e] * by : 0.0f;
-                    dr_split8h(x[s], y);
+                    if constexpr (NP == 2) dr_split8(x[s], y);
+                    else
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            y[0][e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(dr_f2{x[s][2 * e], x[s][2 * e + 1]}, dr_h2));
                 }
 #pragma unroll
                 for (int i = 0; i < NP; ++i) {
@@ -477,7 +418,7 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
         sc[lane] = dr_exp2(last - total) * ik[lane];
         // |T_ij| b_j e^.. / |k_i| of column j: its own row, or what row i makes of it
         const float rows_at_most = dr_wave_max(ik[lane] * fmaxf(1.0f, gb.y * size_k));
-        if (HALF) tw[lane] = dr_scale(2.0f * rows_at_most * gb.y * fmaxf(1.0f, size_k), 13);
+        tw[lane] = dr_scale(2.0f * rows_at_most * gb.y * fmaxf(1.0f, size_k), 13);
     }
     if (bad) return;     // nothing else of it is read
     // K with tokens contracted: lane (key value (t, m), tokens 4 g + 0..3 and 16 + 4 g + 0..3 of 32), the wave's key tiles
@@ -504,7 +445,7 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
     for (int j = 0; j < 4; ++j) {
         kk[j] = qk[j] = lq_f4{0, 0, 0, 0};
         if (j <= w) {
-            lq_f4 a[CP] = {}, c[CP] = {};
+            lq_f4 a[2] = {}, c[2] = {};
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
                 dr_u4 x[NP], y[NP];
@@ -513,8 +454,8 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
                     x[i] = ks[w][s][i][lane];
                     y[i] = ks[j][s][i][lane];
                 }
-                dr_any_product<HALF, NP, NP>(x, y, a);
-                dr_any_product<HALF, NP, NP>(qf[s], y, c);
+                dr_product(x, y, a);
+                dr_product(qf[s], y, c);
             }
             kk[j] = dr_total(a);
             qk[j] = dr_total(c);
@@ -602,7 +543,7 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
     // holds, tile by tile; in A's place
     {
         const bool odd = w & 1;
-        const float bc = bs[16 * w + m] * (HALF ? tw[16 * w + m] : 1.0f);
+        const float bc = bs[16 * w + m] * tw[16 * w + m];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {     // tokens 32 (w / 2 + s) ..
             if (w / 2 + s > 1) continue;
@@ -616,11 +557,10 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
 #pragma unroll
                 for (int e = 0; e < 4; ++e) y8[4 * u + e] = tile[e] * (bc * by[e]);
             }
-            dr_u4 y[SP];
-            if constexpr (HALF) dr_split8h(y8, y);
-            else dr_split8<3>(y8, y);
+            dr_u4 y[2];
+            dr_split8(y8, y);
 #pragma unroll
-            for (int pc = 0; pc < SP; ++pc) to[w < 2 ? 2 * w + s : w + 2][pc][lane] = y[pc];
+            for (int pc = 0; pc < 2; ++pc) to[w < 2 ? 2 * w + s : w + 2][pc][lane] = y[pc];
         }
     }
     __syncthreads();
@@ -628,19 +568,18 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
         lq_f4 wt[NT][4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            lq_f4 acc[NT][CP] = {};
+            lq_f4 acc[NT][2] = {};
 #pragma unroll
             for (int s = c >> 1; s < 2; ++s) {
-                dr_u4 y[SP];
+                dr_u4 y[2];
 #pragma unroll
-                for (int pc = 0; pc < SP; ++pc) y[pc] = to[c < 2 ? 2 * c + s : c + 2][pc][lane];
+                for (int pc = 0; pc < 2; ++pc) y[pc] = to[c < 2 ? 2 * c + s : c + 2][pc][lane];
 #pragma unroll
-                for (int i = 0; i < NT; ++i) dr_any_product<HALF, SP, NP>(y, kt[i][s], acc[i]);
+                for (int i = 0; i < NT; ++i) dr_product(y, kt[i][s], acc[i]);
             }
-            lq_f4 by = {by_w, by_w, by_w, by_w};
-            if (HALF)
+            lq_f4 by;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) by[e] /= tw[16 * c + 4 * g + e];
+            for (int e = 0; e < 4; ++e) by[e] = by_w / tw[16 * c + 4 * g + e];
 #pragma unroll
             for (int i = 0; i < NT; ++i) wt[i][c] = dr_total(acc[i]) * by;
         }
@@ -653,7 +592,7 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
 #pragma unroll
                 for (int e = 0; e < 8; ++e) y8[e] = wt[i][2 * s + (e >> 2)][e & 3];
                 dr_u4 y[2];
-                dr_split8h(y8, y);
+                dr_split8(y8, y);
 #pragma unroll
                 for (int pc = 0; pc < 2; ++pc) dst[((i * 2 + s) * 2 + pc) * 64] = y[pc];
             }
@@ -707,7 +646,7 @@ __global__ __launch_bounds__(256, RuleType<T>::NP == 1 ? 2 : 1) void delta_piece
             for (int i = 0; i < 4; ++i) y8[4 * u + i] = 2 * s + u <= w ? e[i] * (bs[col + i] * by_p) : 0.0f;
         }
         dr_u4 y[2];
-        dr_split8h(y8, y);
+        dr_split8(y8, y);
 #pragma unroll
         for (int i = 0; i < 2; ++i) dst[(s * 2 + i) * 64] = y[i];
     }
@@ -776,14 +715,13 @@ constexpr int RULE_CHAIN = 512;      // threads
 template <typename T, int KD>
 __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
     typedef RuleKeys<KD> Keys;
-    constexpr bool HALF = RuleType<T>::HALF;
-    constexpr int NP = RuleType<T>::NP, SP = RuleType<T>::SP, CP = HALF ? 2 : 3;
+    constexpr int NP = RULE_NP<T>;
     constexpr int NS = Keys::STEPS, NT = Keys::NT, NW = Keys::NW, OT = RULE_OT<KD>;
-    __shared__ __align__(16) dr_u4 ss[NS][SP][64], rs[2][2][64];
+    __shared__ __align__(16) dr_u4 ss[NS][2][64], rs[2][2][64];
     __shared__ __align__(16) lq_f4 part[4][4][64], vs[2][4][64];
     __shared__ __align__(16) float cs[2][PIECE + 4];
     __shared__ float vm[2][OT == 1 ? 4 : 1][16], sm[4][16], su[4][16], rf[16];
-    // (largest |v|, |S| of a wave's quarter by column; what S, of f16, and R were divided by)
+    // (largest |v|, |S| of a wave's quarter by column; what S and R are to be multiplied by)
     __shared__ float red[2][4][2][16], kq[2][2][KD];
     __shared__ int wild_s[4];
     const int group = p.value_heads / p.key_heads, slices = p.vd / 16;
@@ -889,27 +827,24 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
             __syncthreads();     // S
             lq_f4 O[OT];
             {
-                lq_f4 c[OT][CP] = {}, sum[OT] = {};
+                lq_f4 c[OT][2] = {}, sum[OT] = {};
 #pragma unroll
                 for (int s = 0; s < NS; ++s) {
-                    dr_u4 z[SP];
+                    dr_u4 z[2];
 #pragma unroll
-                    for (int i = 0; i < SP; ++i) z[i] = ss[s][i][lane];
+                    for (int i = 0; i < 2; ++i) z[i] = ss[s][i][lane];
 #pragma unroll
-                    for (int t = 0; t < OT; ++t) dr_any_product<HALF, NP, SP>(qf[t][s], z, c[t]);
-                    if (HALF && s % NW == NW - 1) {     // a wave's quarter, with its own scale
+                    for (int t = 0; t < OT; ++t) dr_product(qf[t][s], z, c[t]);
+                    if (s % NW == NW - 1) {     // a wave's quarter, with its own scale
                         const float by = su[s / NW][m];
 #pragma unroll
                         for (int t = 0; t < OT; ++t) {
                             sum[t] = sum[t] + dr_total(c[t]) * by;
 #pragma unroll
-                            for (int i = 0; i < CP; ++i) c[t][i] = lq_f4{0, 0, 0, 0};
+                            for (int i = 0; i < 2; ++i) c[t][i] = lq_f4{0, 0, 0, 0};
                         }
                     }
                 }
-#pragma unroll
-                for (int t = 0; t < OT; ++t)
-                    if (!HALF) sum[t] = dr_total(c[t]);
 #pragma unroll
                 for (int t = 0; t < OT; ++t) {
                     O[t] = sum[t] * of[t];
@@ -931,8 +866,8 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
                 const float by = rf[m] * cs[j & 1][PIECE + RULE_P];
 #pragma unroll
                 for (int t = 0; t < OT; ++t) {
-                    dr_product_h(pf[t], y[0], c[t]);
-                    if (OT == 1 ? upper : t) dr_product_h(pf[t + 1], y[1], c[t]);
+                    dr_product(pf[t], y[0], c[t]);
+                    if (OT == 1 ? upper : t) dr_product(pf[t + 1], y[1], c[t]);
                     O[t] = O[t] + (c[t][0] + c[t][1]) * by;
                     dr_hold(O[t]);
                 }
@@ -1008,35 +943,27 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
             if (g == 0) sm[w][m] = top;
             const int e14 = min(14 - __builtin_amdgcn_frexp_expf(top), 120);
             const float up = ldexpf(1.0f, e14), down = ldexpf(1.0f, -e14);
-            if (HALF && g == 0) su[w][m] = down;
+            if (g == 0) su[w][m] = down;
             lq_f4 c[4] = {};
 #pragma unroll
             for (int s = 0; s < NW; ++s) {
-                dr_u4 z[SP];
-                if constexpr (HALF) {
-                    const lq_f4 lo = S[NT > 1 ? 2 * s : 0] * up, hi = NT > 1 ? S[NT > 1 ? 2 * s + 1 : 0] * up : lq_f4{0, 0, 0, 0};
-                    const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                    dr_split8h(x, z);
-                } else {
-                    dr_u2 lo[3], hi[3] = {};
-                    dr_split4(S[NT > 1 ? 2 * s : 0], lo);
-                    if (NT > 1) dr_split4(S[NT > 1 ? 2 * s + 1 : 0], hi);
+                dr_u4 z[2];
+                const lq_f4 lo = S[NT > 1 ? 2 * s : 0] * up, hi = NT > 1 ? S[NT > 1 ? 2 * s + 1 : 0] * up : lq_f4{0, 0, 0, 0};
+                const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                dr_split8(x, z);
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) z[i] = dr_u4{lo[i][0], lo[i][1], hi[i][0], hi[i][1]};
-                }
+                for (int i = 0; i < 2; ++i) ss[w * NW + s][i][lane] = z[i];
 #pragma unroll
-                for (int i = 0; i < SP; ++i) ss[w * NW + s][i][lane] = z[i];
-#pragma unroll
-                for (int i = SP - 1; i >= 0; --i)     // the smallest products first
+                for (int i = 1; i >= 0; --i)     // the smallest products first
 #pragma unroll
                     for (int u = 0; u < NP; ++u)
                         if (u <= i)
 #pragma unroll
                             for (int t = 0; t < 4; ++t)
-                                c[t] = HALF ? dr_mfma_h(kf[t][s][u], z[i - u], c[t]) : dr_mfma(kf[t][s][u], z[i - u], c[t]);
+                                c[t] = dr_mfma(kf[t][s][u], z[i - u], c[t]);
             }
 #pragma unroll
-            for (int t = 0; t < 4; ++t) part[w][t][lane] = HALF ? c[t] * down : c[t];
+            for (int t = 0; t < 4; ++t) part[w][t][lane] = c[t] * down;
             __syncthreads();     // S
             const lq_f4 kS = (part[0][w][lane] + part[1][w][lane]) + (part[2][w][lane] + part[3][w][lane]);
             const lq_f4 R = vs[j & 1][w][lane] - *reinterpret_cast<const lq_f4 *>(&cs[j & 1][16 * w + 4 * g]) * kS;
@@ -1079,7 +1006,7 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
                 lq_f4 d[2] = {};
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    dr_product_h(wf[t][s], y[s], d);
+                    dr_product(wf[t][s], y[s], d);
                     dr_hold(d[0], d[1]);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) wf[t][s][i] = block(wb, (t * 2 + s) * 2 + i);
@@ -1187,7 +1114,7 @@ static void token_columns(const DeltaRule &p, const DeltaRequests &r, int most, 
 template <typename T, int KD>
 static void rule_launch(const DeltaRule &p, const DeltaRequests &r, void *ws, hipStream_t s) {
     if (!r.starts) return token_columns<T, KD>(p, r, INT32_MAX, s);
-    constexpr int NP = RuleType<T>::NP;
+    constexpr int NP = RULE_NP<T>;
     const int64_t bytes = piece_bytes(NP, p.key_heads, p.value_heads, KD), all = all_pieces(r.tokens, r.requests);
     const int64_t window = std::min(all, delta_rule_workspace_bytes(r.tokens, r.requests, false, p.key_heads, p.value_heads, KD, p.vd) / bytes);
     RuleWork w{};
