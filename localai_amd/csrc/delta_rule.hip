@@ -1077,9 +1077,9 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
         for (int e = 0; e < 4; ++e) state[(int64_t)Keys::at(w * NT + t, 4 * g + e) * p.vd] = S[t][e];
 }
 
-constexpr int RULE_LEAST = 5;              // tokens of a request below which the token kernel takes it
 // Bytes of workspace that a window of pieces may fill: half of the memory's own cache, from
-// which the chain reads it back (8192 tokens, 32 heads of 128: 32 MB 483 us, 64 MB 400, 128 MB 372, 256 MB 419)
+// which the chain reads it back (8192 tokens, 32 heads of 128, bf16: 32 MB 344 us, 64 MB 288, 128 MB 269, 192 MB 313,
+// 256 MB 341; fp32: 500, 446, 413, 447, 470)
 constexpr int64_t RULE_WINDOW = 128 << 20;
 
 static int64_t key_bytes(int np, int kd) { return 4 * (kd == 64 ? 4 : kd / 32) * np * 1024; }     // a piece's K, or Q
@@ -1104,10 +1104,14 @@ static void token_launch(const DeltaRule &p, const DeltaRequests &r, int most, h
 
 template <typename T, int KD>
 static void token_columns(const DeltaRule &p, const DeltaRequests &r, int most, hipStream_t s) {
-    const int64_t all = (int64_t)r.requests * p.value_heads * p.vd;     // value columns of the call
-    if (p.vd % 128 == 0 && all >= 128 * 512) token_launch<T, KD, 128>(p, r, most, s);
-    else if (p.vd % 64 == 0 && all >= 64 * 512) token_launch<T, KD, 64>(p, r, most, s);
-    else if (p.vd % 32 == 0 && all >= 32 * 256) token_launch<T, KD, 32>(p, r, most, s);
+    // Value columns of the call: few go in narrow slices, for the workgroups' number, many in wide
+    // ones, for the rows' length in memory. Heads of 128 x 128, one token of each request, columns -> us
+    // of slices of 32, 64, 128: 2^12 4.9, 5.2, 5.7; 2^14 6.5, 6.3, 6.9; 2^16 13.2, 11.2, 11.2;
+    // 2^18 48.2, 48.2, 49.4; 2^20 217, 210, 178. (16: 6.1 and 289 at the ends; for value_dims of no multiple of 32.)
+    const int64_t all = (int64_t)r.requests * p.value_heads * p.vd;
+    if (p.vd % 128 == 0 && all >= 1 << 19) token_launch<T, KD, 128>(p, r, most, s);
+    else if (p.vd % 64 == 0 && all >= 1 << 14) token_launch<T, KD, 64>(p, r, most, s);
+    else if (p.vd % 32 == 0) token_launch<T, KD, 32>(p, r, most, s);
     else token_launch<T, KD, 16>(p, r, most, s);
 }
 
@@ -1115,6 +1119,14 @@ template <typename T, int KD>
 static void rule_launch(const DeltaRule &p, const DeltaRequests &r, void *ws, hipStream_t s) {
     if (!r.starts) return token_columns<T, KD>(p, r, INT32_MAX, s);
     constexpr int NP = RULE_NP<T>;
+    // Requests of fewer tokens go token by token: for each, that takes a token's latency, or its share of
+    // the vector units, and a chain its start and the piece's operands. With 32 heads of 128, us of n tokens
+    // a request in pieces and token by token, by workgroups of the chain: 256 (one request) 8: 16.2, 15.6,
+    // 12: 16.2, 21.4; 1024 8: 28, 18, 16: 28, 30; 2048 16: 46, 33, 24: 47, 47; 8192 16: 140, 93, 24: 141, 132,
+    // 32: 142, 190.
+    const int64_t groups = (int64_t)r.requests * p.value_heads * (p.vd / 16);
+    const int least = (int)std::min<int64_t>(std::max<int64_t>(groups / 80, 9), 25);
+    if (r.tokens < least) return token_columns<T, KD>(p, r, INT32_MAX, s);
     const int64_t bytes = piece_bytes(NP, p.key_heads, p.value_heads, KD), all = all_pieces(r.tokens, r.requests);
     const int64_t window = std::min(all, delta_rule_workspace_bytes(r.tokens, r.requests, false, p.key_heads, p.value_heads, KD, p.vd) / bytes);
     RuleWork w{};
@@ -1127,8 +1139,8 @@ static void rule_launch(const DeltaRule &p, const DeltaRequests &r, void *ws, hi
     w.p = at += (uint32_t)(tiles * (KD / 16 * 2));
     w.rows = at += (uint32_t)(tiles * TRI);
     w.bytes = (uint32_t)(window * bytes);
-    // (one request may also have few tokens: its pieces serve any number)
-    w.least = r.requests > 1 ? RULE_LEAST : 1;
+    // (one request's tokens are the call's, or fewer by a few: its pieces serve any number)
+    w.least = r.requests > 1 ? least : 1;
     if (w.least > 1) token_columns<T, KD>(p, r, w.least - 1, s);
     const int group = p.value_heads / p.key_heads;
     for (int64_t first = 0; first < all; first += window) {
