@@ -4,6 +4,9 @@
 //   y = y z / (1 + exp(-z))  (gate z);  y rounded once, or in Q8_0 blocks:
 //   d = fp16(max |y| / 127) of 32 values, quants rint(y / d), ties to even
 // fp32 throughout.
+// Bound by memory: x, the residual and the gate once, the results once (2^24 fp32
+// values in rows of 4096, in and out: 134 MB, 21.6 us, out of the memory's own cache).
+// A row's values stay in registers between the sum and the results.
 #include "delta.h"
 #include "dev_common.h"
 #include "internal.h"
@@ -58,123 +61,109 @@ __device__ __forceinline__ void norm_q8(uint8_t *row, int64_t at, const float (&
 
 // TPR lanes a row (16 to 64, or 256), VEC values a lane and pass; rows of up to TPR VEC
 // ITEMS values stay in registers, longer ones (ITEMS 0) are read a second time,
-// each lane its own values. Groups of fewer lanes take ROWS rows side by side, all
-// requested at once: heads of 128 (131072 of them, bf16 with a gate: 101 MB) 54 us
-// with a wave a head, 30 so.
-template <typename T, typename O, int VEC, int TPR, int ITEMS, int ROWS>
+// each lane its own values.
+template <typename T, typename O, int VEC, int TPR, int ITEMS>
 __global__ __launch_bounds__(256) void rms_norm_kernel(RmsNorm n) {
     constexpr bool Q8 = sizeof(O) == 1;
-    constexpr int GROUPS = 256 / TPR, KEEP = ITEMS ? ITEMS : 1;
+    constexpr int KEEP = ITEMS ? ITEMS : 1;
     const int lane = threadIdx.x % TPR;
-    const uint32_t rows = (uint32_t)(n.rows * n.heads), row0 = blockIdx.x * (GROUPS * ROWS) + threadIdx.x / TPR;
-    const int64_t step = (int64_t)TPR * VEC;
-    const T *x[ROWS];
-    float *res[ROWS];
-    int64_t t[ROWS], h[ROWS], dim[ROWS];     // dim: 0 past the last row
-    float keep[ROWS][KEEP][VEC], old[ROWS][KEEP][VEC], sum[ROWS];
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        const uint32_t row = row0 + i * GROUPS, at = row < rows ? row : rows - 1;
-        const uint32_t heads = (uint32_t)n.heads, q = heads == 1 ? at : at / heads;
-        t[i] = q;
-        h[i] = at - q * heads;
-        dim[i] = row < rows ? n.dim : 0;
-        x[i] = (const T *)n.x + t[i] * n.x_rs + h[i] * n.x_hs;
-        res[i] = n.residual ? n.residual + t[i] * n.r_rs + h[i] * n.r_hs : nullptr;
-        sum[i] = 0.0f;
-    }
-    const auto ask = [&](int i, int64_t at, float (&y)[VEC], float (&z)[VEC]) {
-        norm_load<T, VEC>(x[i] + at, y);
-        if (res[i]) norm_load<float, VEC>(res[i] + at, z);
+    const uint32_t rows = (uint32_t)(n.rows * n.heads), row = blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const uint32_t heads = (uint32_t)n.heads, at_row = row < rows ? row : rows - 1, quot = heads == 1 ? at_row : at_row / heads;
+    const int64_t step = (int64_t)TPR * VEC, t = quot, h = at_row - quot * heads;
+    const int64_t dim = row < rows ? n.dim : 0;
+    const T *x = (const T *)n.x + t * n.x_rs + h * n.x_hs;
+    float *res = n.residual ? n.residual + t * n.r_rs + h * n.r_hs : nullptr;
+    const T *gate = n.gate ? (const T *)n.gate + t * n.g_rs + h * n.g_hs : nullptr;
+    O *out = (O *)n.out + t * n.o_rs + h * n.o_hs;
+    float keep[KEEP][VEC], old[KEEP][VEC], sum = 0.0f;
+    const auto ask = [&](int64_t at, float (&y)[VEC], float (&z)[VEC]) {
+        norm_load<T, VEC>(x + at, y);
+        if (res) norm_load<float, VEC>(res + at, z);
     };
-    const auto take = [&](int i, int64_t at, float (&y)[VEC], float (&z)[VEC]) {
-        if (res[i]) {
+    const auto take = [&](int64_t at, float (&y)[VEC], float (&z)[VEC]) {
+        if (res) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) y[e] += z[e];
-            norm_store<float, VEC>(res[i] + at, y);
+            norm_store<float, VEC>(res + at, y);
         }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) sum[i] += y[e] * y[e];
+        for (int e = 0; e < VEC; ++e) sum += y[e] * y[e];
     };
     if constexpr (ITEMS > 0) {
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i)
-#pragma unroll
-            for (int u = 0; u < ITEMS; ++u) {
-                const int64_t at = u * step + lane * VEC;
-                if (at < dim[i]) ask(i, at, keep[i][u], old[i][u]);
-            }
-#pragma unroll
-        for (int i = 0; i < ROWS; ++i)
-#pragma unroll
-            for (int u = 0; u < ITEMS; ++u) {
-                const int64_t at = u * step + lane * VEC;
-                if (at < dim[i]) take(i, at, keep[i][u], old[i][u]);
-            }
-    } else
-        for (int64_t at = lane * VEC; at < dim[0]; at += step) {
-            ask(0, at, keep[0][0], old[0][0]);
-            take(0, at, keep[0][0], old[0][0]);
+        for (int u = 0; u < ITEMS; ++u) {     // all requested at once
+            const int64_t at = u * step + lane * VEC;
+            if (at < dim) ask(at, keep[u], old[u]);
         }
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) sum[i] = group_sum<(TPR < 64 ? TPR : 64)>(sum[i]);
+        for (int u = 0; u < ITEMS; ++u) {
+            const int64_t at = u * step + lane * VEC;
+            if (at < dim) take(at, keep[u], old[u]);
+        }
+    } else
+        for (int64_t at = lane * VEC; at < dim; at += step) {
+            ask(at, keep[0], old[0]);
+            take(at, keep[0], old[0]);
+        }
+    sum = group_sum<(TPR < 64 ? TPR : 64)>(sum);
     if constexpr (TPR > 64) {
         __shared__ float part[TPR / 64];
-        if (lane % 64 == 0) part[lane / 64] = sum[0];
+        if (lane % 64 == 0) part[lane / 64] = sum;
         __syncthreads();
-        sum[0] = 0.0f;
+        sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < TPR / 64; ++i) sum[0] += part[i];
+        for (int i = 0; i < TPR / 64; ++i) sum += part[i];
     }
+    const float inv = 1.0f / sqrtf(sum / (float)n.dim + n.eps);
+    const auto give = [&](int64_t at, float (&y)[VEC]) {
+        float w[VEC];
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        const float inv = 1.0f / sqrtf(sum[i] / (float)n.dim + n.eps);
-        const T *gate = n.gate ? (const T *)n.gate + t[i] * n.g_rs + h[i] * n.g_hs : nullptr;
-        O *out = (O *)n.out + t[i] * n.o_rs + h[i] * n.o_hs;
-        const auto give = [&](int64_t at, float (&y)[VEC]) {
-            float w[VEC];
+        for (int e = 0; e < VEC; ++e) w[e] = n.weight[at + e];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) w[e] = n.weight[at + e];
+        for (int e = 0; e < VEC; ++e) y[e] = y[e] * inv * w[e];
+        if (gate) {
+            float z[VEC];
+            norm_load<T, VEC>(gate + at, z);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) y[e] = y[e] * inv * w[e];
-            if (gate) {
-                float z[VEC];
-                norm_load<T, VEC>(gate + at, z);
+            for (int e = 0; e < VEC; ++e) y[e] *= delta_silu(z[e]);
+        }
+        if constexpr (Q8) norm_q8((uint8_t *)out, at, y);
+        else norm_store<O, VEC>(out + at, y);
+    };
+    if constexpr (ITEMS > 0) {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) y[e] *= delta_silu(z[e]);
-            }
-            if constexpr (Q8) norm_q8((uint8_t *)out, at, y);
-            else norm_store<O, VEC>(out + at, y);
-        };
-        if constexpr (ITEMS > 0) {
-#pragma unroll
-            for (int u = 0; u < ITEMS; ++u) {
-                const int64_t at = u * step + lane * VEC;
-                if (at < dim[i]) give(at, keep[i][u]);
-            }
-        } else
-            for (int64_t at = lane * VEC; at < dim[0]; at += step) {
-                if (res[0]) norm_load<float, VEC>(res[0] + at, keep[0][0]);
-                else norm_load<T, VEC>(x[0] + at, keep[0][0]);
-                give(at, keep[0][0]);
-            }
-    }
+        for (int u = 0; u < ITEMS; ++u) {
+            const int64_t at = u * step + lane * VEC;
+            if (at < dim) give(at, keep[u]);
+        }
+    } else
+        for (int64_t at = lane * VEC; at < dim; at += step) {
+            if (res) norm_load<float, VEC>(res + at, keep[0]);
+            else norm_load<T, VEC>(x + at, keep[0]);
+            give(at, keep[0]);
+        }
 }
 
 template <typename T, typename O, int VEC>
 static int norm_launch(const RmsNorm &n, hipStream_t s) {
     const int64_t rows = n.rows * n.heads;
-#define LQ_NORM(TPR, ITEMS, ROWS)                                                                            \
-    hipLaunchKernelGGL((rms_norm_kernel<T, O, VEC, TPR, ITEMS, ROWS>),                                       \
-                       dim3((unsigned)((rows + 256 / TPR * ROWS - 1) / (256 / TPR * ROWS))), dim3(256), 0, s, n)
-    if (n.dim <= 16 * VEC) LQ_NORM(16, 1, 4);
-    else if (n.dim <= 32 * VEC) LQ_NORM(32, 1, 4);
-    else if (n.dim <= 64 * VEC) LQ_NORM(64, 1, 4);
-    else if (n.dim <= 256 * VEC) LQ_NORM(256, 1, 1);
-    else if (n.dim <= 1024 * VEC) LQ_NORM(256, 4, 1);
-    else if (n.dim <= 2048 * VEC) LQ_NORM(256, 8, 1);
-    else if (n.dim <= 4096 * VEC) LQ_NORM(256, 16, 1);
-    else LQ_NORM(256, 0, 1);
+#define LQ_NORM(TPR, ITEMS)                                                                                  \
+    hipLaunchKernelGGL((rms_norm_kernel<T, O, VEC, TPR, ITEMS>), dim3((unsigned)((rows + 256 / TPR - 1) / (256 / TPR))), \
+                       dim3(256), 0, s, n)
+    // Lanes a row: short rows share waves, so that no lane is idle (heads of 64, 131072 of them, bf16 with
+    // a gate: 16 lanes 14.8 us, a wave 43.5; of 128: 32 lanes 26.5, a wave 44.7); rows of up to two passes of
+    // a wave stay in one (512 fp32: 21.5 us, a workgroup a row 28.3). Longer ones take a workgroup: a single
+    // row of 1024 has 2.7 us so, 4.0 in a wave, many the same. As few values a lane as the row needs (rows
+    // of 4096 with the residual: 4 passes' registers 30.8 us, 16 39.9, none and a second reading 36.0).
+    if (n.dim <= 16 * VEC) LQ_NORM(16, 1);
+    else if (n.dim <= 32 * VEC) LQ_NORM(32, 1);
+    else if (n.dim <= 64 * VEC) LQ_NORM(64, 1);
+    else if (n.dim <= 128 * VEC) LQ_NORM(64, 2);
+    else if (n.dim <= 256 * VEC) LQ_NORM(256, 1);
+    else if (n.dim <= 1024 * VEC) LQ_NORM(256, 4);
+    else if (n.dim <= 2048 * VEC) LQ_NORM(256, 8);
+    else if (n.dim <= 4096 * VEC) LQ_NORM(256, 16);
+    else LQ_NORM(256, 0);
 #undef LQ_NORM
     LQ_HIP(hipGetLastError());
     return LOCALAI_OK;
@@ -189,6 +178,7 @@ static int norm_aligned(const RmsNorm &n, hipStream_t s) {
         };
         const bool ok = n.dim % 4 == 0 && four(n.x, n.x_rs, n.x_hs, sizeof(T)) && four(n.gate, n.g_rs, n.g_hs, sizeof(T)) &&
                         four(n.residual, n.r_rs, n.r_hs, 4) && four(n.out, n.o_rs, n.o_hs, sizeof(O));
+        // (four values a lane: 131072 heads of 128 26.5 us, one 97.9)
         return ok ? norm_launch<T, O, 4>(n, s) : norm_launch<T, O, 1>(n, s);
     }
 }
