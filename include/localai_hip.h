@@ -438,9 +438,12 @@ int64_t localai_hip_delta_rule_workspace_size(int64_t tokens, int64_t requests, 
  * key_dim 64, 128 or 256; value_dim a multiple of 16, at most 1024; q, k, v and
  * out aligned to 4 values, state and workspace to 16 bytes. out shares memory
  * with no other buffer. requests times value_heads times value_dim / 16 below 2^24.
- * fp32 results whatever the type (out rounded once). What is not finite reaches
- * the tokens behind it, of a v the one column alone, and none before it; which of NaN and
- * infinity they show is not defined. */
+ * States and sums are fp32; of several tokens at once the products' operands hold
+ * 22 bits, and no less than 2^-35 of the largest of their row or column; out is
+ * rounded once. A state that could grow by itself (g > 0.01, b < 0 or b |k^|^2 > 2)
+ * and values past 1e15 cost the 64 tokens they are among each a token's own time.
+ * What is not finite reaches the tokens behind it, of a v the one column alone,
+ * and none before it; which of NaN and infinity they show is not defined. */
 int localai_hip_delta_rule(const void *q_dev, const void *k_dev, const void *v_dev, int type,
                            const int64_t *strides, int64_t tokens, int key_heads, int value_heads, int key_dim,
                            int value_dim, const float *decay_dev, const float *beta_dev, const float *a_dev,

@@ -129,9 +129,10 @@ __global__ __launch_bounds__(256) void delta_conv_kernel(DeltaConv c, DeltaReque
 // Rows of a piece: its first width - 1 rows before are read twice, so long pieces read
 // less, and short ones are more workgroups with fewer rows one behind the other. 8192
 // bf16 channels, us of pieces of 8, 16, 32: 64 rows 5.6, 8.1, 12.4; 1024 13.9, 15.8, 18.8;
-// 2048 21.5, 21.3, 24.8; 4096 36.2, 33.1, 35.8; 8192 65.3, 57.6, 56.3.
+// 2048 21.5, 21.3, 24.8; 4096 36.2, 33.1, 35.8; 8192 65.3, 57.6, 56.3 (fp32, out of HBM: 146, 132, 126).
 static int conv_rows(const DeltaConv &c, const DeltaRequests &r) {
-    return !r.starts ? 1 : r.tokens * c.channels <= 1 << 24 ? 8 : 16;
+    const int64_t values = r.tokens * c.channels;
+    return !r.starts ? 1 : values <= 1 << 24 ? 8 : values <= 1 << 25 ? 16 : 32;
 }
 
 template <typename T, int VEC>

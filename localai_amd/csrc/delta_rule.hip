@@ -4,7 +4,7 @@
 //   k^ = k / sqrt(|k|^2 + eps), q^ = scale q / sqrt(|q|^2 + eps)
 //   S <- e^g S;  d = beta (v - S^T k^);  S <- S + k^ d^T;  o = S^T q^
 // g = decay, beta as given, or from projections: g = a softplus(decay + dt_bias),
-// beta = 1 / (1 + exp(-beta)). fp32 throughout; o rounded once to its type.
+// beta = 1 / (1 + exp(-beta)). fp32 sums and states; o rounded once to its type.
 #include <algorithm>
 
 #include "delta.h"
@@ -33,7 +33,9 @@ __device__ __forceinline__ int rule_key_head(const DeltaRule &p, int h) {
 // A workgroup owns VS value columns of one head of one request: KD x VS values
 // of S in registers, each lane 4 adjacent columns of KD VS / 1024 rows. With
 // S' = e^g S, one pass over the rows gives S'^T k and S'^T q; the token's result
-// needs no second one: o = S'^T q^ + d (k^ . q^).
+// needs no second one: o = S'^T q^ + d (k^ . q^). Bound by memory, the state in and
+// out once: 256 requests of 32 heads of 128 x 128, fp32, 1.07 GB in 203 us, 5.3 TB/s;
+// 16 of 16-bit types 11 us. One request: latency, 4.9 us.
 template <typename T, int KD, int VS>
 __global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequests r, int most) {
     constexpr int LPR = VS / 4, RW = 64 / LPR, NR = KD * VS / 1024;   // lanes a row, rows a wave's pass, passes
@@ -293,7 +295,9 @@ __device__ __forceinline__ double dr_add_from(double v) {
 // 16 w .. 16 w + 15. An operand's lane l holds row or column l & 15 and of each
 // 32 contracted values x the eight 4 (l >> 4) + 0..3 and 16 + 4 (l >> 4) + 0..3:
 // the layout in which MFMA leaves two tiles of results, so those are operands
-// as they are.
+// as they are. Bound by latency and LDS: eleven barriers between products of one or
+// two tiles a wave, four workgroups a CU (37 KB of LDS each); 8192 tokens of 16/32 heads
+// of 128, bf16: 100 us for 4096 workgroups, 0.3 GB of workspace written.
 template <typename T, int KD>
 __global__ __launch_bounds__(256, RULE_NP<T> == 1 ? 2 : 1) void delta_piece_kernel(DeltaRule p, DeltaRequests r, RuleWork ws) {
     typedef RuleKeys<KD> Keys;
@@ -654,8 +658,8 @@ __global__ __launch_bounds__(256, RULE_NP<T> == 1 ? 2 : 1) void delta_piece_kern
 
 // Requests stay behind what makes the values x, the last uses of what they
 // replace: moved ahead of one, they need registers of their own, and copies at the
-// loop's end that wait for all of them (8192 tokens, 32 heads of 128: 2.0 us a piece
-// so, 1.8 as it is).
+// loop's end that wait for all of them (before S and R were f16: 2.0 us a piece so,
+// 1.8 with them held).
 template <typename X>
 __device__ __forceinline__ void dr_pin(X &x) { asm volatile("" : "+v"(x)); }
 template <typename... X>
@@ -707,7 +711,9 @@ struct RuleValues {
 // values Q's pieces for one tile are what the registers hold). The last two bring
 // v and factors, of every other piece each: from HBM, it takes longer than a piece (of 256 key
 // values the waves with the outputs do: a tenth wave would cost the others registers).
-// Two barriers a piece. Each operand of the next piece is requested as soon as this
+// Bound by that chain of exchanges: two barriers a piece, 1.55 us of 64 tokens (8192
+// tokens, 32 heads of 128, bf16: 128 pieces one behind the other, 200 us; 16 columns a workgroup, so that
+// one request's heads fill the chip: 256 workgroups). Each operand of the next piece is requested as soon as this
 // piece's has been used; nothing between a request and its use is conditional, so
 // the compiler's count of what is in flight is exact.
 template <int KD> constexpr int RULE_OT = KD > 128 ? 1 : 2;
@@ -1107,9 +1113,10 @@ static void token_columns(const DeltaRule &p, const DeltaRequests &r, int most, 
     // Value columns of the call: few go in narrow slices, for the workgroups' number, many in wide
     // ones, for the rows' length in memory. Heads of 128 x 128, one token of each request, columns -> us
     // of slices of 32, 64, 128: 2^12 4.9, 5.2, 5.7; 2^14 6.5, 6.3, 6.9; 2^16 13.2, 11.2, 11.2;
-    // 2^18 48.2, 48.2, 49.4; 2^20 217, 210, 178. (16: 6.1 and 289 at the ends; for value_dims of no multiple of 32.)
+    // 2^18 48.2, 48.2, 49.4 (calls one by one instead of from a graph: 58.5,
+    // 52.7 of 64, 128); 2^20 217, 210, 178. (16: 6.1 and 289 at the ends; for value_dims of no multiple of 32.)
     const int64_t all = (int64_t)r.requests * p.value_heads * p.vd;
-    if (p.vd % 128 == 0 && all >= 1 << 19) token_launch<T, KD, 128>(p, r, most, s);
+    if (p.vd % 128 == 0 && all >= 1 << 18) token_launch<T, KD, 128>(p, r, most, s);
     else if (p.vd % 64 == 0 && all >= 1 << 14) token_launch<T, KD, 64>(p, r, most, s);
     else if (p.vd % 32 == 0) token_launch<T, KD, 32>(p, r, most, s);
     else token_launch<T, KD, 16>(p, r, most, s);

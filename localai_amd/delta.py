@@ -102,7 +102,7 @@ def _requests(tokens, state, slots, starts, lengths):
             break
     if starts is None and n != tokens:
         raise ValueError('without starts there is one token per request')
-    if starts is not None and slots is None and n > state.shape[0]:
+    if slots is None and n > state.shape[0]:
         raise ValueError('more requests than rows of the state')
     return _REQUESTS.pack(state.data_ptr(), state.shape[0], _ptr(slots, 'slots', i32, (n,)) if slots is not None else 0,
                           _ptr(starts, 'starts', i32, (n + 1,)) if starts is not None else 0,

@@ -15,7 +15,9 @@ products' 2-norm, which is at most the state's norm times |k^| or |q^| (the sum
 itself may cancel to nothing, so it is no measure), with a few u from the norms and
 the gates. So with s_t the larger norm of the state after the decay and after the
 update, in u: r_t = (2 sqrt(key_dim) + 16) s_t is what token t rounds, and E_t^2 =
-(e^g E_(t-1))^2 + r_t^2 bounds the state, scale (E_t + r_t) the output, in 2-norms.
+(e^g E_(t-1))^2 + r_t^2 bounds the state, scale (E_t + r_t) the output, in 2-norms. 64 tokens at once round each operand of a
+product to 22 bits (2 u) instead, once, and sum 64 or key_dim products in fp32: of a
+token's share fewer and no larger roundings than the three a token of its own.
 
 Norm: the mean square is off by at most (32 + 8) u where no lane sums more than 32
 squares and the rest is a tree; half of it reaches the root; root, quotient, two
@@ -668,13 +670,11 @@ def test_refusals_on_the_device():
     for change, error in [(dict(q=q.double()), TypeError), (dict(q=q.half()), TypeError), (dict(k=k[:5]), ValueError),
                           (dict(v=v[..., ::2]), ValueError), (dict(beta=beta[:, :1]), ValueError),
                           (dict(state=state.half()), TypeError), (dict(state=state[:, :, :, :16]), ValueError),
-                          (dict(state=state[:2]), HipError), (dict(a=a), ValueError), (dict(order='other'), ValueError),
+                          (dict(state=state[:2]), ValueError), (dict(a=a), ValueError), (dict(order='other'), ValueError),
                           (dict(norm_eps=-1.0), ValueError), (dict(scale=float('inf')), HipError),
                           (dict(slots=_ints([0] * 5)), ValueError), (dict(starts=_ints([0, 6]), lengths=_ints([1, 2])), ValueError),
                           (dict(starts=_ints(range(9))), ValueError), (dict(out=v[:, :, ::2]), ValueError),
                           (dict(slots=_ints([0] * 6).long()), TypeError), (dict(q=q[..., :63], k=k[..., :63]), (ValueError, HipError))]:
-        if 'state' in change and change['state'].shape[0] == 2:
-            continue     # rows past the pool are places without a state
         with pytest.raises(error):
             call(**change)
     call()
