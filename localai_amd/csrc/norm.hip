@@ -7,6 +7,8 @@
 // Bound by memory: x, the residual and the gate once, the results once (2^24 fp32
 // values in rows of 4096, in and out: 134 MB, 21.6 us, out of the memory's own cache).
 // A row's values stay in registers between the sum and the results.
+#include <algorithm>
+
 #include "delta.h"
 #include "dev_common.h"
 #include "internal.h"
@@ -15,18 +17,21 @@ namespace lq {
 
 enum { NORM_Q8_0 = 8 };
 
+// VEC adjacent values (aligned to VEC, to four of fp32)
 template <typename T, int VEC>
 __device__ __forceinline__ void norm_load(const T *p, float (&y)[VEC]) {
-    if constexpr (VEC == 4) {
-        const float4 v = delta_load4(p);
-        y[0] = v.x; y[1] = v.y; y[2] = v.z; y[3] = v.w;
-    } else
-        y[0] = (float)p[0];
+    struct alignas(sizeof(T) * VEC < 16 ? sizeof(T) * VEC : 16) Raw { T v[VEC]; };
+    const Raw raw = *reinterpret_cast<const Raw *>(p);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) y[i] = (float)raw.v[i];
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void norm_store(T *p, const float (&y)[VEC]) {
-    if constexpr (VEC == 4) delta_store4(p, make_float4(y[0], y[1], y[2], y[3]));
-    else p[0] = (T)y[0];
+    struct alignas(sizeof(T) * VEC < 16 ? sizeof(T) * VEC : 16) Raw { T v[VEC]; };
+    Raw raw;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) raw.v[i] = (T)y[i];
+    *reinterpret_cast<Raw *>(p) = raw;
 }
 
 // Four values of a Q8_0 block whose 8 lanes are adjacent. A block that holds a
@@ -59,7 +64,7 @@ __device__ __forceinline__ void norm_q8(uint8_t *row, int64_t at, const float (&
     if (at % 32 == 0) *reinterpret_cast<uint16_t *>(block) = __builtin_bit_cast(uint16_t, d16);
 }
 
-// TPR lanes a row (16 to 64, or 256), VEC values a lane and pass; rows of up to TPR VEC
+// TPR lanes a row (8 to 64, or 256), VEC values a lane and pass; rows of up to TPR VEC
 // ITEMS values stay in registers, longer ones (ITEMS 0) are read a second time,
 // each lane its own values.
 template <typename T, typename O, int VEC, int TPR, int ITEMS>
@@ -117,8 +122,11 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsNorm n) {
     const float inv = 1.0f / sqrtf(sum / (float)n.dim + n.eps);
     const auto give = [&](int64_t at, float (&y)[VEC]) {
         float w[VEC];
+        if constexpr (Q8) {     // (its weight may be aligned to one value)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) w[e] = n.weight[at + e];
+            for (int e = 0; e < VEC; ++e) w[e] = n.weight[at + e];
+        } else
+            norm_load<float, VEC>(n.weight + at, w);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) y[e] = y[e] * inv * w[e];
         if (gate) {
@@ -150,12 +158,14 @@ static int norm_launch(const RmsNorm &n, hipStream_t s) {
 #define LQ_NORM(TPR, ITEMS)                                                                                  \
     hipLaunchKernelGGL((rms_norm_kernel<T, O, VEC, TPR, ITEMS>), dim3((unsigned)((rows + 256 / TPR - 1) / (256 / TPR))), \
                        dim3(256), 0, s, n)
-    // Lanes a row: short rows share waves, so that no lane is idle (heads of 64, 131072 of them, bf16 with
-    // a gate: 16 lanes 14.8 us, a wave 43.5; of 128: 32 lanes 26.5, a wave 44.7); rows of up to two passes of
+    // Lanes a row: short rows share waves, so that no lane is idle (131072 heads of 64 with a gate, bf16,
+    // four values a lane: 16 lanes 14.8 us, a wave 43.5; of 128: 32 lanes 26.5, a wave 44.7; eight a lane, heads of
+    // 64: 8 lanes 12.7, 16 18.2); rows of up to two passes of
     // a wave stay in one (512 fp32: 21.5 us, a workgroup a row 28.3). Longer ones take a workgroup: a single
     // row of 1024 has 2.7 us so, 4.0 in a wave, many the same. As few values a lane as the row needs (rows
     // of 4096 with the residual: 4 passes' registers 30.8 us, 16 39.9, none and a second reading 36.0).
-    if (n.dim <= 16 * VEC) LQ_NORM(16, 1);
+    if (n.dim <= 8 * VEC) LQ_NORM(8, 1);
+    else if (n.dim <= 16 * VEC) LQ_NORM(16, 1);
     else if (n.dim <= 32 * VEC) LQ_NORM(32, 1);
     else if (n.dim <= 64 * VEC) LQ_NORM(64, 1);
     else if (n.dim <= 128 * VEC) LQ_NORM(64, 2);
@@ -173,13 +183,18 @@ template <typename T, typename O>
 static int norm_aligned(const RmsNorm &n, hipStream_t s) {
     if constexpr (sizeof(O) == 1) return norm_launch<T, O, 4>(n, s);
     else {
-        const auto four = [](const void *p, int64_t rs, int64_t hs, size_t size) {
-            return !p || (reinterpret_cast<uintptr_t>(p) % (4 * size) == 0 && rs % 4 == 0 && hs % 4 == 0);
+        const auto fits = [&](int vec) {
+            const auto all = [&](const void *p, int64_t rs, int64_t hs, size_t size) {
+                return !p || (reinterpret_cast<uintptr_t>(p) % std::min<size_t>(vec * size, 16) == 0 && rs % vec == 0 && hs % vec == 0);
+            };
+            return n.dim % vec == 0 && all(n.x, n.x_rs, n.x_hs, sizeof(T)) && all(n.gate, n.g_rs, n.g_hs, sizeof(T)) &&
+                   all(n.residual, n.r_rs, n.r_hs, 4) && all(n.weight, 0, 0, 4) && all(n.out, n.o_rs, n.o_hs, sizeof(O));
         };
-        const bool ok = n.dim % 4 == 0 && four(n.x, n.x_rs, n.x_hs, sizeof(T)) && four(n.gate, n.g_rs, n.g_hs, sizeof(T)) &&
-                        four(n.residual, n.r_rs, n.r_hs, 4) && four(n.out, n.o_rs, n.o_hs, sizeof(O));
-        // (four values a lane: 131072 heads of 128 26.5 us, one 97.9)
-        return ok ? norm_launch<T, O, 4>(n, s) : norm_launch<T, O, 1>(n, s);
+        // Values a lane: as many as 16 bytes hold (131072 bf16 heads of 128 with a gate: 8 21.5 us, 4 28.3, 1
+        // 97.9; 2^25 values in rows of 1024: 22.4, 31.7), but 4 beside a residual, whose are 16 bytes
+        // then (2^24 in rows of 4096: 30.5 us, with 8 33.7).
+        if (sizeof(T) == 2 && !n.residual && fits(8)) return norm_launch<T, O, sizeof(T) == 2 ? 8 : 4>(n, s);
+        return fits(4) ? norm_launch<T, O, 4>(n, s) : norm_launch<T, O, 1>(n, s);
     }
 }
 

@@ -286,6 +286,27 @@ def test_norm_of_odd_rows(dtype, dim):
     _check_norm((3, dim), dtype, dtype, False, gate=False, cut=1)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('dim', [32, 64, 100, 128, 1032, 2056])
+def test_norm_of_rows_at_any_alignment(dim, dtype):
+    """Rows, gate, result and weight that begin 0, 1, 4 or 8 values behind an aligned place."""
+    import torch
+    from localai_amd import layer
+    rng = np.random.default_rng(dim)
+    base, bv = _random(rng, (5, 3, dim + 8), dtype)
+    gate, gv = _random(rng, (5, 3, dim + 8), dtype)
+    weight, wv = _random(rng, (dim + 8,), 'float32')
+    for x0, g0, w0, o0 in [(0, 0, 0, 0), (8, 0, 4, 8), (4, 8, 0, 0), (0, 4, 4, 8), (8, 8, 1, 0), (1, 0, 0, 0), (0, 0, 0, 4)]:
+        out = torch.full((5, 3, dim + 8), 3.0, dtype=base.dtype, device='cuda')
+        view = out[..., o0:o0 + dim]
+        layer.rms_norm(base[..., x0:x0 + dim], weight[w0:w0 + dim], 1e-6, gate=gate[..., g0:g0 + dim], out=view)
+        want, _ = odelta.rms_norm(bv[..., x0:x0 + dim], wv[w0:w0 + dim], 1e-6, gate=gv[..., g0:g0 + dim])
+        tol = 40 * U * np.abs(want).max(-1, keepdims=True) + HALF[dtype] * np.abs(want) * (1 + 40 * U) + FLOOR[dtype]
+        assert (np.abs(_np(view) - want) <= tol).all(), (x0, g0, w0, o0)
+        view[:] = 3.0
+        assert (out == 3).all()
+
+
 def test_norm_in_place_and_of_zeros():
     import torch
     from localai_amd import layer
@@ -426,6 +447,13 @@ def test_rule_small_keys_and_a_large_state(small, dtype):
     q, k, v = (x.to(getattr(torch, dtype)) for x in (q, k * small, v))
     # (the result's type adds its half step)
     _against_oracle((q, k, v, decay, beta, state * 1e25), tol=2e-5 + 2 * HALF[dtype])
+
+
+def test_rule_keys_below_the_types_normal_values():
+    """f16 keys and queries of a few of its smallest steps."""
+    rng = np.random.default_rng(9)
+    q, k, v, decay, beta, state = _finite_case(rng)
+    _against_oracle(((q * 1e-6).half(), (k * 1e-6).half(), v.half(), decay, beta, state), norm_eps=1e-13, tol=2e-5 + 2 * HALF['float16'])
 
 
 @pytest.mark.parametrize('dtype', TYPES)
