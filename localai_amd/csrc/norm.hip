@@ -34,27 +34,30 @@ __device__ __forceinline__ void norm_store(T *p, const float (&y)[VEC]) {
     *reinterpret_cast<Raw *>(p) = raw;
 }
 
+template <int CTRL>
+__device__ __forceinline__ float norm_max_from(float x) {     // with another lane's of the 8
+    return fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, false)));
+}
+
 // Four values of a Q8_0 block whose 8 lanes are adjacent. A block that holds a
-// value that is not finite gets a scale that is not, so all of it is NaN.
+// value that is not finite gets a scale that is not, so all of it is NaN. The
+// quotients are a reciprocal's, corrected once: exact but for ties by 2^-23 of
+// themselves (2049 rows of 5120 bf16 with the residual: 25.6 us, with a division each 27.9).
 __device__ __forceinline__ void norm_q8(uint8_t *row, int64_t at, const float (&y)[4]) {
-    float top = 0.0f;
-    bool bad = false;
+    float top = 0.0f;     // infinite: a value that is not finite
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        top = fmaxf(top, fabsf(y[i]));
-        bad |= !(fabsf(y[i]) <= 3.402823466e38f);
-    }
-#pragma unroll
-    for (int m = 1; m < 8; m <<= 1) {
-        top = fmaxf(top, __shfl_xor(top, m, 64));
-        bad |= __shfl_xor((int)bad, m, 64) != 0;
-    }
+    for (int i = 0; i < 4; ++i) top = fabsf(y[i]) <= 3.402823466e38f ? fmaxf(top, fabsf(y[i])) : __builtin_inff();
+    top = norm_max_from<0xB1>(top);      // the next lane, the next two, the four behind
+    top = norm_max_from<0x4E>(top);
+    top = norm_max_from<0x141>(top);
+    const bool bad = top > 3.402823466e38f;
     const _Float16 d16 = bad ? (_Float16)__builtin_nanf("") : (_Float16)(top / 127.0f);
-    const float d = (float)d16;
+    const float d = (float)d16, r = __builtin_amdgcn_rcpf(d);
+    const bool some = d > 0.0f && d <= 65504.0f;
     uint8_t q[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float t = d > 0.0f && !bad ? rintf(y[i] / d) : 0.0f;
+        const float q0 = y[i] * r, t = some ? rintf(__builtin_fmaf(__builtin_fmaf(-q0, d, y[i]), r, q0)) : 0.0f;
         q[i] = (uint8_t)(int8_t)fminf(fmaxf(t, -127.0f), 127.0f);
     }
     uint8_t *block = row + at / 32 * 34;
