@@ -226,6 +226,24 @@ def test_rule_many_requests():
     _check_rule((1, 2, 64, 32), [0] * 64 + [70] + [0] * 63 + [1, 100], 'float32', True, 'grouped')
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('counts', [[8], [9], [1, 2, 3], [8, 9, 10], [25, 0, 24, 7, 64]], ids=str)
+def test_rule_few_tokens_a_request(counts, dtype):
+    """On both sides of what goes token by token in a call of prompts."""
+    _check_rule((2, 4, 128, 128), counts, dtype, True, 'tiled')
+
+
+def test_rule_many_short_requests():
+    rng = np.random.default_rng(3)
+    _check_rule((1, 4, 64, 64), rng.integers(0, 40, 130).tolist(), 'bfloat16', True, 'grouped')
+    _check_rule((1, 4, 64, 64), rng.integers(20, 30, 130).tolist(), 'float32', True, 'grouped')
+
+
+def test_rule_step_of_many_requests():
+    """The widest slices of columns."""
+    _check_rule((2, 4, 128, 128), [1] * 520, 'float32', True, 'grouped', pad=0, step=True)
+
+
 def test_rule_long_prompt():
     _check_rule((1, 2, 128, 32), [3000], 'float32', True, 'grouped')
 
