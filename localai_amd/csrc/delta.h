@@ -107,16 +107,17 @@ __device__ __forceinline__ int delta_request(const DeltaRequests &r, int piece, 
 // y / (1 + exp(-y)) to a few fp32 roundings: the exponent's argument in two parts
 // (its rounding alone would cost |y| of them), a reciprocal corrected once. A third
 // of the instructions of expf and a division, which bound 16-bit rows of the
-// convolution (7941 rows of 8192: 66 us, 54 so) and the gated norm. NaN stays, as
-// do the results of infinities: inf, and NaN for -inf.
+// convolution (7941 rows of 8192: 66 us, 54 so) and the gated norm. Below -87.3, where
+// 1 + exp(-y) passes what has a reciprocal or is infinite itself, the result is 0 (less than 2^-119 is
+// lost); the corrections, which are inf - inf there, are left out. inf gives inf, NaN and -inf give NaN.
 __device__ __forceinline__ float delta_silu(float y) {
     const float a = fminf(fmaxf(y, -100.0f), 100.0f);
     const float hi = a * -1.4426950408889634f;
     const float lo = __builtin_fmaf(a, -1.4426950408889634f, -hi) - a * 1.9259629911266174e-8f;
-    const float power = __builtin_amdgcn_exp2f(hi);
-    const float d = 1.0f + __builtin_fmaf(power, lo * 0.6931471805599453f, power);
-    const float r = __builtin_amdgcn_rcpf(d), q = y * r;
-    return d < 1e37f ? __builtin_fmaf(__builtin_fmaf(-q, d, y), r, q) : q;
+    const float power = __builtin_amdgcn_exp2f(hi), exact = __builtin_fmaf(power, lo * 0.6931471805599453f, power);
+    const float d = 1.0f + (power < __builtin_inff() ? exact : power);
+    const float r = __builtin_amdgcn_rcpf(d), q = y * r, off = __builtin_fmaf(-q, d, y);
+    return off == off ? __builtin_fmaf(off, r, q) : q;     // (NaN: d or y is infinite)
 }
 
 template <typename T> struct DeltaVec;
