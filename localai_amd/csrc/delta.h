@@ -109,13 +109,13 @@ __device__ __forceinline__ int delta_request(const DeltaRequests &r, int piece, 
 // of the instructions of expf and a division, which bound 16-bit rows of the
 // convolution (7941 rows of 8192: 66 us, 54 so) and the gated norm. Below -87.3, where
 // 1 + exp(-y) passes what has a reciprocal or is infinite itself, the result is 0 (less than 2^-119 is
-// lost); the corrections, which are inf - inf there, are left out. inf gives inf, NaN and -inf give NaN.
+// lost); the quotient's correction, which is NaN there, is left out. inf gives inf, NaN and -inf give NaN.
 __device__ __forceinline__ float delta_silu(float y) {
     const float a = fminf(fmaxf(y, -100.0f), 100.0f);
     const float hi = a * -1.4426950408889634f;
     const float lo = __builtin_fmaf(a, -1.4426950408889634f, -hi) - a * 1.9259629911266174e-8f;
-    const float power = __builtin_amdgcn_exp2f(hi), exact = __builtin_fmaf(power, lo * 0.6931471805599453f, power);
-    const float d = 1.0f + (power < __builtin_inff() ? exact : power);
+    // (power may be infinite; the factor beside it is 1 but for 2^-17)
+    const float d = __builtin_fmaf(__builtin_amdgcn_exp2f(hi), __builtin_fmaf(lo, 0.6931471805599453f, 1.0f), 1.0f);
     const float r = __builtin_amdgcn_rcpf(d), q = y * r, off = __builtin_fmaf(-q, d, y);
     return off == off ? __builtin_fmaf(off, r, q) : q;     // (NaN: d or y is infinite)
 }
