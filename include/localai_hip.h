@@ -437,7 +437,8 @@ int64_t localai_hip_delta_rule_workspace_size(int64_t tokens, int64_t requests, 
  * stride of decay and beta.
  * key_dim 64, 128 or 256; value_dim a multiple of 16, at most 1024; q, k, v and
  * out aligned to 4 values, state and workspace to 16 bytes. out shares memory
- * with no other buffer. requests times value_heads times value_dim / 16 below 2^24.
+ * with no other buffer. requests times value_heads times value_dim / 16 below 2^24;
+ * with starts below 2^23, requests times key_heads rounded up to a multiple of 8.
  * States and sums are fp32; of several tokens at once the products' operands hold
  * 22 bits, and no less than 2^-35 of the largest of their row or column; out is
  * rounded once. A state that could grow by itself (g > 0.01, b < 0 or b |k^|^2 > 2)

@@ -796,12 +796,14 @@ int localai_hip_delta_conv(const void *x, int type, int64_t tokens, int64_t chan
                              (hipStream_t)stream);
 }
 
-static int delta_rule_sizes(int64_t requests, int key_heads, int value_heads, int kd, int vd) {
+static int delta_rule_sizes(int64_t requests, bool starts, int key_heads, int value_heads, int kd, int vd) {
     if (key_heads < 1 || value_heads < 1 || value_heads > 4096 || value_heads % key_heads)
         return fail(LOCALAI_EARG, "delta rule: value_heads must be a multiple of key_heads, at most 4096");
     if (kd != 64 && kd != 128 && kd != 256) return fail(LOCALAI_ETYPE, "delta rule: key_dim 64, 128 or 256");
     if (vd < 16 || vd > 1024 || vd % 16) return fail(LOCALAI_ETYPE, "delta rule: value_dim a multiple of 16, at most 1024");
-    if (requests * value_heads * (vd / 16) >= 1 << 24)     // workgroups of a launch
+    // a launch has fewer than 2^32 threads: 256 a workgroup of a step, 512 of prompts, whose key heads are rounded up to 8
+    const int64_t groups = (int64_t)(value_heads / key_heads) * (vd / 16), units = requests * key_heads;
+    if (starts ? (units + 7) / 8 * 8 * groups >= 1 << 23 : units * groups >= 1 << 24)
         return fail(LOCALAI_EARG, "delta rule: too many requests times heads for one call");
     return LOCALAI_OK;
 }
@@ -809,7 +811,7 @@ static int delta_rule_sizes(int64_t requests, int key_heads, int value_heads, in
 int64_t localai_hip_delta_rule_workspace_size(int64_t tokens, int64_t requests, int starts, int key_heads,
                                               int value_heads, int key_dim, int value_dim) {
     if (tokens < 0 || tokens >= 1 << 24 || requests < 1 || requests > DELTA_MAX_REQUESTS ||
-        delta_rule_sizes(requests, key_heads, value_heads, key_dim, value_dim))
+        delta_rule_sizes(requests, starts, key_heads, value_heads, key_dim, value_dim))
         return -1;
     return delta_rule_workspace_bytes(tokens, (int)requests, !starts, key_heads, value_heads, key_dim, value_dim);
 }
@@ -822,7 +824,7 @@ int localai_hip_delta_rule(const void *q, const void *k, const void *v, int type
     clear_error();
     DeltaRequests r;
     if (int st = delta_requests_of("delta rule", requests, tokens, &r)) return st;
-    if (int st = delta_rule_sizes(r.requests, key_heads, value_heads, key_dim, value_dim)) return st;
+    if (int st = delta_rule_sizes(r.requests, r.starts, key_heads, value_heads, key_dim, value_dim)) return st;
     if (!delta_type(type)) return fail(LOCALAI_ETYPE, "delta rule: q, k, v and out are fp32 (0), fp16 (1) or bf16 (30)");
     if (tiled != 0 && tiled != 1) return fail(LOCALAI_EARG, "delta rule: tiled is 0 or 1");
     if (!(std::fabs(scale) <= FLT_MAX) || !(norm_eps <= FLT_MAX))

@@ -152,6 +152,25 @@ def test_rule_workspace_size():
         assert size(*bad) == -1, bad
 
 
+def test_rule_sizes_that_no_launch_holds():
+    """Workgroups of 512 threads for prompts, 256 for a step: fewer than 2^32 threads; refused before anything is queued."""
+    size = _lib.load().localai_hip_delta_rule_workspace_size
+    for n, starts, hk, hv, vd, fits in [
+            (4096, 1, 64, 64, 512, False), (4095, 1, 64, 64, 512, True), (4096, 0, 64, 64, 512, True),
+            (4096, 0, 64, 64, 1024, False), (4095, 0, 64, 64, 1024, True), (4096, 1, 4, 64, 512, False),
+            (4095, 1, 1, 64, 512, False), (4088, 1, 1, 64, 512, True),      # (4095 key heads are launched as 4096)
+            (2048, 1, 128, 128, 512, False), (2047, 1, 128, 128, 512, True)]:
+        case = n, starts, hk, hv, vd
+        assert (size(n, n, starts, hk, hv, 64, vd) >= 0) == fits, case
+        r = requests(requests=n, **({} if starts else {'starts_dev': None}))
+        s = (hk * 64, 64, hk * 64, 64, hv * vd, vd, hv * vd, vd, hv, hv)
+        # (what fits goes on to the next check: an address that is not aligned)
+        assert refused(rule(r, s, tokens=n, key_heads=hk, value_heads=hv, key_dim=64, value_dim=vd,
+                            q=ctypes.c_void_p(20))) == 'EARG'
+        message = _lib.load().localai_hip_last_error().decode()
+        assert ('aligned' if fits else 'too many') in message, (case, message)
+
+
 def norm(strides=(64, 0, 64, 0, 64, 0, 64, 0), **change):
     a = dict(x=ONE, type=0, strides=(ctypes.c_int64 * 8)(*strides), rows=3, heads=1, dim=64, weight=ONE,
              eps=ctypes.c_float(1e-6), residual=None, gate=None, out=ONE, out_type=0, stream=None)
