@@ -440,7 +440,8 @@ int64_t localai_hip_delta_rule_workspace_size(int64_t tokens, int64_t requests, 
  * with no other buffer. requests times value_heads times value_dim / 16 below 2^24;
  * with starts below 2^23, requests times key_heads rounded up to a multiple of 8.
  * States and sums are fp32; of several tokens at once the products' operands hold
- * 22 bits, and no less than 2^-35 of the largest of their row or column; out is
+ * 22 bits of values within 2^24 of the largest of their row, column or 64 tokens, of smaller
+ * ones 2^-46 of that, and where a v needs more, the 64 tokens it is among go token by token; out is
  * rounded once. A state that could grow by itself (g > 0.01, b < 0 or b |k^|^2 > 2)
  * and values past 1e15 cost the 64 tokens they are among each a token's own time.
  * What is not finite reaches the tokens behind it, of a v the one column alone,

@@ -143,13 +143,16 @@ __global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequ
 // head, whose S stays in registers (delta_chain_kernel).
 //
 // Precision: fp32's, up to two bits. MFMA takes 16-bit operands, so each fp32 value
-// goes in as two f16 pieces: 22 bits of it, and 2^-35 of the largest that it may be
-// (operands are scaled by a power of two below a bound that is known ahead: rows
-// of q and k, columns of S, T, W, P T and R have their own). bf16 q and k are one
-// such piece, f16 ones one as they are. Of the products those up to 2^-11 of the
-// largest are kept, in fp32 sums; norms and decays are applied to the sums. Three
-// bf16 pieces of the unscaled values would hold 24 bits, in half as many bytes and
-// products again (8192 tokens, 32 heads of 128, bf16: 318 us). G is
+// goes in as two f16 pieces, the second 2^11 times itself and summed apart: 22 bits of a
+// value within 2^24 of the largest that it may be, of smaller ones 2^-46 of that (operands are
+// scaled by a power of two below a bound that is known ahead: rows of q and k, columns
+// of S, T and R, a piece's W and P T have their own). R takes v, of whatever sizes:
+// a piece with a smaller value that the column's state at that token needs goes token
+// by token. bf16 q and k are one such piece, f16 ones one as they are. Of the products
+// those up to 2^-11 of the largest are kept, in fp32 sums; norms and decays are applied
+// to the sums. Three bf16 pieces of the unscaled values would hold 24 bits at any size, in half
+// as many bytes and products again (8192 tokens, 32 heads of 128, bf16: 318 us, so 272; with
+// second pieces that are not 2^11 times themselves, which hold 2^-35, 269). G is
 // summed in fp64, so that a difference keeps its bits behind a token that
 // forgets everything. The inverse goes by forward substitution in blocks of 16,
 // whose numbers stay as small as the rule's own.
@@ -183,8 +186,9 @@ template <int KD> struct RuleKeys {
     }
 };
 
-// the last row's: e^G_last (NaN: the piece goes token by token), what W and P T are divided by, the largest e^G |k^|
-enum { RULE_LAST = 0, RULE_W = 1, RULE_P = 2, RULE_K = 3 };
+// the last row's: e^G_last (NaN: the piece goes token by token), what W and P T are divided by, the largest e^G |k^|,
+// the least and the largest |k^|
+enum { RULE_LAST = 0, RULE_W = 1, RULE_P = 2, RULE_K = 3, RULE_LEAST_K = 4, RULE_MOST_K = 5 };
 
 // workspace of one window of pieces: byte offsets of arrays of 1 KB blocks (64 lanes x 16 bytes: an MFMA operand)
 struct RuleWork {
@@ -218,10 +222,11 @@ typedef float dr_f2 __attribute__((ext_vector_type(2)));
 typedef _Float16 dr_h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 dr_h8 __attribute__((ext_vector_type(8)));
 
-// two values as two f16 pieces each
+// two values as two f16 pieces each: x = y0 + y1 / LOW
+constexpr float LOW = 2048.0f;
 __device__ __forceinline__ void dr_split2(float a, float b, uint32_t (&y)[2]) {
     const dr_h2 h = __builtin_convertvector(dr_f2{a, b}, dr_h2);
-    const dr_h2 m = __builtin_convertvector(dr_f2{a - (float)h[0], b - (float)h[1]}, dr_h2);
+    const dr_h2 m = __builtin_convertvector(dr_f2{(a - (float)h[0]) * LOW, (b - (float)h[1]) * LOW}, dr_h2);
     y[0] = __builtin_bit_cast(uint32_t, h);
     y[1] = __builtin_bit_cast(uint32_t, m);
 }
@@ -245,14 +250,14 @@ __device__ __forceinline__ float dr_wave_max(float x) {     // x >= 0
 __device__ __forceinline__ lq_f4 dr_mfma(const dr_u4 &a, const dr_u4 &b, const lq_f4 &c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(dr_h8, a), __builtin_bit_cast(dr_h8, b), c, 0, 0, 0);
 }
-// c[0] += the first pieces' product, c[1] += those of a first and a second
+// c[0] += the first pieces' product, c[1] += LOW times those of a first and a second
 template <int NA, int NB>
 __device__ __forceinline__ void dr_product(const dr_u4 (&a)[NA], const dr_u4 (&b)[NB], lq_f4 (&c)[2]) {
     if constexpr (NB > 1) c[1] = dr_mfma(a[0], b[1], c[1]);
     c[0] = dr_mfma(a[0], b[0], c[0]);
     if constexpr (NA > 1) c[1] = dr_mfma(a[1], b[0], c[1]);
 }
-__device__ __forceinline__ lq_f4 dr_total(const lq_f4 (&c)[2]) { return c[0] + c[1]; }
+__device__ __forceinline__ lq_f4 dr_total(const lq_f4 (&c)[2]) { return c[0] + c[1] * (1.0f / LOW); }
 
 // 2^x for fp64 x, to fp32's last bit or so however large x is
 __device__ __forceinline__ float dr_exp2(double x) {
@@ -416,9 +421,11 @@ __global__ __launch_bounds__(256, RULE_NP<T> == 1 ? 2 : 1) void delta_piece_kern
         rows[lane] = dr_exp2(total) * ik[lane];
         rows[PIECE + lane] = dr_exp2(total) * iq[lane] * p.scale;
         const float size_r = dr_wave_max(dr_exp2(total) * size_k);
-        if (lane < 4)
+        const float most_k = dr_wave_max(size_k), less_k = dr_wave_max(lane < n ? most_k - size_k : 0.0f);
+        if (lane < 6)
             rows[2 * PIECE + lane] = lane == RULE_LAST ? bad ? __builtin_nanf("") : dr_exp2(last)
-                                     : lane == RULE_W ? 1.0f / by_w : lane == RULE_P ? 1.0f / by_p : size_r;
+                                     : lane == RULE_W ? 1.0f / by_w : lane == RULE_P ? 1.0f / by_p
+                                     : lane == RULE_K ? size_r : lane == RULE_LEAST_K ? most_k - less_k : most_k;
         sc[lane] = dr_exp2(last - total) * ik[lane];
         // |T_ij| b_j e^.. / |k_i| of column j: its own row, or what row i makes of it
         const float rows_at_most = dr_wave_max(ik[lane] * fmaxf(1.0f, gb.y * size_k));
@@ -874,7 +881,7 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
                 for (int t = 0; t < OT; ++t) {
                     dr_product(pf[t], y[0], c[t]);
                     if (OT == 1 ? upper : t) dr_product(pf[t + 1], y[1], c[t]);
-                    O[t] = O[t] + (c[t][0] + c[t][1]) * by;
+                    O[t] = O[t] + dr_total(c[t]) * by;
                     dr_hold(O[t]);
                 }
             }
@@ -934,6 +941,36 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             S[t][e] = from == 0 && span.fresh ? 0.0f : state[(int64_t)Keys::at(w * NT + t, 4 * g + e) * p.vd];
+    // Whether a value of R below `normal`, of token i, is needed to more bits than the pieces hold: not where the
+    // column of the state, of its own or of a token up to i, holds as much as its largest rounding then (so it
+    // is for the values that are small by chance, about one in 2^25, which one step back shows).
+    const auto loses = [&](int j, const lq_f4 &R, float normal) {
+        const float *size_k = rows_of(j) + 2 * PIECE;
+        const float least_k = size_k[RULE_LEAST_K], most_k = size_k[RULE_MOST_K];
+        const bool in = lane < span.count - j * PIECE;     // a token a lane
+        const float2 gb = in ? rule_gates(p, (int64_t)span.first + j * PIECE + lane, h) : make_float2(0, 0);
+        const float factor = expf(gb.x), adds = gb.y * least_k;
+        const float before = fmaxf(fmaxf(sm[0][m], sm[1][m]), fmaxf(sm[2][m], sm[3][m]));
+        bool lost = false;
+        for (int e = 0; e < 4; ++e) {
+            int i = 16 * w + 4 * g + e;
+            const float r = fabsf(e & 2 ? (e & 1 ? R[3] : R[2]) : (e & 1 ? R[1] : R[0]));
+            const float needed = __shfl(gb.y, i, 64) * most_k * normal;
+            float held = __shfl(adds, i, 64) * r, left = 1.0f;
+            bool open = r > 0.0f && r < normal && !(held >= needed);
+            while (__any(open)) {
+                left *= __shfl(factor, i, 64);
+                i = max(i - 1, -1);
+                const float size = __shfl(adds, max(i, 0), 64) * fabsf(vs[j & 1][max(i, 0) >> 4][(max(i, 0) >> 2 & 3) * 16 + m][max(i, 0) & 3]);
+                if (open && left * (i < 0 ? before : size) >= needed) open = false;
+                if (open && (i < 0 || !(left > 0.0f))) {
+                    open = false;
+                    lost = true;
+                }
+            }
+        }
+        return lost;
+    };
     for (int j = from; j < to;) {
         ask_k();
         dr_hold();
@@ -950,7 +987,7 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
             const int e14 = min(14 - __builtin_amdgcn_frexp_expf(top), 120);
             const float up = ldexpf(1.0f, e14), down = ldexpf(1.0f, -e14);
             if (g == 0) su[w][m] = down;
-            lq_f4 c[4] = {};
+            lq_f4 c[4][2] = {};
 #pragma unroll
             for (int s = 0; s < NW; ++s) {
                 dr_u4 z[2];
@@ -960,16 +997,16 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
 #pragma unroll
                 for (int i = 0; i < 2; ++i) ss[w * NW + s][i][lane] = z[i];
 #pragma unroll
-                for (int i = 1; i >= 0; --i)     // the smallest products first
+                for (int i = 1; i >= 0; --i)
 #pragma unroll
                     for (int u = 0; u < NP; ++u)
                         if (u <= i)
 #pragma unroll
                             for (int t = 0; t < 4; ++t)
-                                c[t] = dr_mfma(kf[t][s][u], z[i - u], c[t]);
+                                c[t][i] = dr_mfma(kf[t][s][u], z[i - u], c[t][i]);
             }
 #pragma unroll
-            for (int t = 0; t < 4; ++t) part[w][t][lane] = c[t] * down;
+            for (int t = 0; t < 4; ++t) part[w][t][lane] = dr_total(c[t]) * down;
             __syncthreads();     // S
             const lq_f4 kS = (part[0][w][lane] + part[1][w][lane]) + (part[2][w][lane] + part[3][w][lane]);
             const lq_f4 R = vs[j & 1][w][lane] - *reinterpret_cast<const lq_f4 *>(&cs[j & 1][16 * w + 4 * g]) * kS;
@@ -994,7 +1031,13 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
 #pragma unroll
             for (int i = 0; i < 2; ++i) reinterpret_cast<dr_u2 *>(&rs[w >> 1][i][lane])[w & 1] = dr_u2{x[0][i], x[1][i]};
             const float by = unscale * cs[j & 1][PIECE + RULE_W];
-            const bool any = __any(!(size <= RULE_WILD * RULE_WILD) || !(most + v_top <= RULE_WILD * RULE_WILD));
+            bool any = __any(!(size <= RULE_WILD * RULE_WILD) || !(most + v_top <= RULE_WILD * RULE_WILD));
+            // a value of R, not 0, that has fewer bits for the largest of its column: below f16's normal ones
+            const float normal = ldexpf(1.0f, -14 - r14);
+            uint32_t least = ~0u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) least = min(least, (__builtin_bit_cast(uint32_t, R[e]) << 1) - 1);
+            if (__any(least < (__builtin_bit_cast(uint32_t, normal) << 1) - 1) && !any) any = __any(loses(j, R, normal));
             if (lane == 0) wild_s[w] = any;
             __syncthreads();     // R
             const int bad = wild_s[0] | wild_s[1] | wild_s[2] | wild_s[3];
@@ -1018,7 +1061,7 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
                     for (int i = 0; i < 2; ++i) wf[t][s][i] = block(wb, (t * 2 + s) * 2 + i);
                     dr_hold();
                 }
-                S[t] = next[t] + (d[0] + d[1]) * by;
+                S[t] = next[t] + dr_total(d) * by;
             }
         }
         if (j >= to) break;

@@ -87,3 +87,81 @@ def test_norm_with_gates_of_every_value(dtype):
     top = np.repeat(np.abs(want).reshape(-1, 32).max(-1), 32).reshape(want.shape)
     # half a step of the scale, its own rounding to f16 (normal, or by 2^-25) at 127 steps of it
     assert (np.abs(got - want) <= top / 127 * (0.5 + 127 * 2.0 ** -11) * (1 + 2.0 ** -9) + 128 * 2.0 ** -25 + 14 * U * top).all()
+
+
+# ---------------------------------------------------------------- values of mixed sizes in the rule
+
+def _columns(state, q, k, v, g, b, scale):
+    """One head in 64 bits, token after token: results [tokens, value dim], the state after, and how far fp32 may be off
+    in each, column by column.
+
+    A column of the state is a recurrence of its own: s <- e^g s; d = b (v - k^ . s); s <- s + k^ d. With |k^| = 1 and
+    0 <= b <= 1 its step is e^g times a contraction, so what a token rounds is not enlarged behind it: with s_t the larger of
+    the column's norms after the decay and after the update, r_t = (2 sqrt(key dim) + 16) u s_t is rounded (three
+    roundings a value, two sums of key dim products), E_t^2 = (e^g E)^2 + r_t^2, and E_t + r_t, times q^'s scale, bounds the
+    result. Operands of 22 bits (4 u each) are fewer roundings than these."""
+    S, E, c = state.copy(), np.zeros(v.shape[1]), (2 * k.shape[1] ** 0.5 + 16) * U
+    out, off = np.zeros(v.shape), np.zeros(v.shape)
+    for t in range(len(v)):
+        S *= np.exp(g[t])
+        size = np.linalg.norm(S, axis=0)
+        S += np.outer(k[t], b[t] * (v[t] - k[t] @ S))
+        r = c * np.maximum(size, np.linalg.norm(S, axis=0))
+        E = np.hypot(np.exp(g[t]) * E, r)
+        out[t], off[t] = scale * (q[t] @ S), scale * (E + r)
+    return out, S, off, E
+
+
+def _mixed(case, rng, q, k, v, g, b, state, big):
+    """Puts values `big` times the others into one or more columns of v [tokens, heads, value dim] or of the state."""
+    if case == 'one':              # behind and ahead of tokens of 1
+        v[40, 0, 5], v[100, -1, 7] = big, -big
+    elif case == 'rows':           # whole tokens
+        v[[20, 75]] *= big
+    elif case == 'forgotten':      # large, then everything forgotten within the same 64
+        v[10] *= big
+        g[15] = -200
+        v[80, -1, 3] = big
+        g[81] = -np.inf
+    elif case == 'faint':          # large v that a small beta takes down to the others' size
+        v[[3, 70]] *= big
+        b[[3, 70]] = 1 / big
+    elif case == 'state':          # a state that is forgotten in time
+        state *= big
+        g[5] = -np.log(big) - 3
+    elif case == 'zeros':          # ahead of the first value, and between
+        v[:30], v[50:60] = 0, 0
+        state[:] = 0
+        v[33] *= big
+    else:                          # of every size, column by column
+        v *= big ** rng.uniform(-0.5, 0.5, v.shape)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('big', [1e4, 1e6, 1e8, 1e10, 1e12])
+@pytest.mark.parametrize('case', ['one', 'rows', 'forgotten', 'faint', 'state', 'zeros', 'any'])
+@pytest.mark.parametrize('heads', [(2, 4, 128, 32), (1, 2, 64, 16), (1, 1, 256, 48)], ids=str)
+def test_rule_mixed_sizes_in_64_tokens(heads, case, big, dtype):
+    """A value beside one that is far larger, in the same column and the same 64 tokens, keeps its bits."""
+    import torch
+    from localai_amd import delta
+    if dtype == 'float16':
+        big = min(big, 1e4)       # (f16 holds none larger beside 1)
+    rng = np.random.default_rng(sum(heads) + len(case))
+    hk, hv, kd, vd = heads
+    n = 150
+    q, k, v = (rng.standard_normal((n, h, d)) for h, d in ((hk, kd), (hk, kd), (hv, vd)))
+    g, b, state = -rng.exponential(0.05, (n, hv)), rng.random((n, hv)), rng.standard_normal((hv, kd, vd)) * 0.1
+    with np.errstate(divide='ignore'):
+        _mixed(case, rng, q, k, v, g, b, state, big)
+    q, k, v = (torch.tensor(x, dtype=torch.float32).to(getattr(torch, dtype)).cuda() for x in (q, k, v))
+    assert torch.isfinite(v).all()
+    g, b, state = (torch.tensor(x, dtype=torch.float32, device='cuda') for x in (g, b, state[None]))
+    qv, kv, vv, gv, bv, sv = (_np(x) for x in (q, k, v, g, b, state[0]))
+    got = _np(delta.rule(q, k, v, g, b, state, starts=_ints([0, n])))
+    qv, kv = (x / np.sqrt((x * x).sum(-1, keepdims=True) + 1e-6) for x in (qv, kv))
+    for h in range(hv):
+        key = h // (hv // hk)
+        want, after, off, off_state = _columns(sv[h], qv[:, key], kv[:, key], vv[:, h], gv[:, h], bv[:, h], kd ** -0.5)
+        assert (np.abs(got[:, h] - want) <= off + (HALF[dtype] * np.abs(want) if dtype != 'float32' else 0) + 2.0 ** -25 * (dtype == 'float16')).all(), ('out', h)
+        assert (np.linalg.norm(_np(state[0, h]) - after, axis=0) <= off_state).all(), ('state', h)
