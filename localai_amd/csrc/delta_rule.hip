@@ -34,8 +34,8 @@ __device__ __forceinline__ int rule_key_head(const DeltaRule &p, int h) {
 // of S in registers, each lane 4 adjacent columns of KD VS / 1024 rows. With
 // S' = e^g S, one pass over the rows gives S'^T k and S'^T q; the token's result
 // needs no second one: o = S'^T q^ + d (k^ . q^). Bound by memory, the state in and
-// out once: 256 requests of 32 heads of 128 x 128, fp32, 1.07 GB in 203 us, 5.3 TB/s;
-// 16 of 16-bit types 11 us. One request: latency, 4.9 us.
+// out once: 256 requests of 32 heads of 128 x 128, fp32, 1.07 GB in 211 us, 5.1 TB/s;
+// 16 16.7 us, 4.0 TB/s. One request: latency, 5.4 us. (States of other layers between, so none is in a cache.)
 template <typename T, int KD, int VS>
 __global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequests r, int most) {
     constexpr int LPR = VS / 4, RW = 64 / LPR, NR = KD * VS / 1024;   // lanes a row, rows a wave's pass, passes
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequ
         }
     }
 #pragma unroll
-    for (int i = 0; i < NR; ++i)     // (not read again in this step: past the caches, 256 requests 203 us in place of 220)
+    for (int i = 0; i < NR; ++i)     // (not read again in this step: past the caches, 70 requests 61.3 us in place of 62.2, 256 211, 207)
         __builtin_nontemporal_store(lq_f4{S[i].x, S[i].y, S[i].z, S[i].w},
                                     reinterpret_cast<lq_f4 *>(state + (int64_t)i * 4 * RW * p.vd));
 }
@@ -1153,14 +1153,14 @@ static void token_launch(const DeltaRule &p, const DeltaRequests &r, int most, h
 
 template <typename T, int KD>
 static void token_columns(const DeltaRule &p, const DeltaRequests &r, int most, hipStream_t s) {
-    // Value columns of the call: few go in narrow slices, for the workgroups' number, many in wide
-    // ones, for the rows' length in memory. Heads of 128 x 128, one token of each request, columns -> us
-    // of slices of 32, 64, 128: 2^12 4.9, 5.2, 5.7; 2^14 6.5, 6.3, 6.9; 2^16 13.2, 11.2, 11.2;
-    // 2^18 48.2, 48.2, 49.4 (calls one by one instead of from a graph: 58.5,
-    // 52.7 of 64, 128); 2^20 217, 210, 178. (16: 6.1 and 289 at the ends; for value_dims of no multiple of 32.)
+    // Value columns of the call: few go in narrow slices, for the workgroups' number, many in wider
+    // ones, for the rows' length in memory. Heads of 128 x 128, one token of each request, the states of many
+    // layers one behind the other, so that none is in a cache; columns -> us of slices of 32, 64, 128: 2^12 5.5,
+    // 5.7, 6.7; 2^14 8.0, 7.9, 8.5; 2^16 18.8, 16.8, 17.3; 2^18 56.0, 56.8, 58.5; 2^19 108.7, 106.9,
+    // 109.9; 2^20 220, 211, 220. (128 are ahead only where the same 150 MB are called
+    // again and again; 16 are for value_dims of no multiple of 32.)
     const int64_t all = (int64_t)r.requests * p.value_heads * p.vd;
-    if (p.vd % 128 == 0 && all >= 1 << 18) token_launch<T, KD, 128>(p, r, most, s);
-    else if (p.vd % 64 == 0 && all >= 1 << 14) token_launch<T, KD, 64>(p, r, most, s);
+    if (p.vd % 64 == 0 && all >= 1 << 14) token_launch<T, KD, 64>(p, r, most, s);
     else if (p.vd % 32 == 0) token_launch<T, KD, 32>(p, r, most, s);
     else token_launch<T, KD, 16>(p, r, most, s);
 }
