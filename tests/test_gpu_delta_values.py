@@ -165,3 +165,42 @@ def test_rule_mixed_sizes_in_64_tokens(heads, case, big, dtype):
         want, after, off, off_state = _columns(sv[h], qv[:, key], kv[:, key], vv[:, h], gv[:, h], bv[:, h], kd ** -0.5)
         assert (np.abs(got[:, h] - want) <= off + (HALF[dtype] * np.abs(want) if dtype != 'float32' else 0) + 2.0 ** -25 * (dtype == 'float16')).all(), ('out', h)
         assert (np.linalg.norm(_np(state[0, h]) - after, axis=0) <= off_state).all(), ('state', h)
+
+
+# ---------------------------------------------------------------- long pieces of the convolution
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('width', [2, 4, 8])
+@pytest.mark.parametrize('channels', [1 << 20, (1 << 20) - 3])
+@pytest.mark.parametrize('counts', [[13, 0, 17], [0, 3, 16, 1, 7, 2], [31, 0, 33, 1], [2, 64, 32, 5]], ids=str)
+def test_conv_of_many_values(counts, channels, width, dtype):
+    """Pieces of 16 rows (past 2^24 values) and of 32 (past 2^25), with requests on both sides of their ends. (width + 1) u of
+    the terms' sizes, passed on by silu with a slope below 1.1, and 6 u of the result."""
+    import torch
+    from localai_amd import delta
+    gen = torch.Generator('cuda').manual_seed(sum(counts) + width)
+    normal = lambda *shape: torch.randn(shape, generator=gen, device='cuda')
+    n, starts = len(counts), np.concatenate([[0], np.cumsum(counts)])
+    x, w, state = normal(sum(counts) + 2, channels).to(getattr(torch, dtype)), normal(channels, width), normal(n + 1, width - 1, channels)
+    assert (len(x) * channels > 1 << 25) == (counts[0] not in (0, 13)) and len(x) * channels > 1 << 24
+    before, out, slots = state.clone(), torch.full_like(x, 7.0), [(b + 1) % (n + 1) for b in range(n)]
+    lengths = [c + b % 2 for b, c in enumerate(counts)]      # every other request starts from zeros
+    delta.conv(x, w, state, _ints(slots), _ints(starts), _ints(lengths), out=out)
+    assert (out[sum(counts):] == 7).all()
+    busy = {s for s, c in zip(slots, counts) if c}
+    for s in set(range(n + 1)) - busy:
+        assert torch.equal(state[s], before[s])
+    for b, c in enumerate(counts):
+        if not c:
+            continue
+        old = before[slots[b]].double() * (b % 2)
+        line = torch.cat([old, x[starts[b]:starts[b + 1]].double()])
+        want, size = torch.zeros(2, c, channels, dtype=torch.float64, device='cuda')
+        for j in range(width):
+            term = line[j:j + c] * w[:, j].double()
+            want += term
+            size += term.abs()
+        want = want / (1 + torch.exp(-want))
+        off = (out[starts[b]:starts[b + 1]].double() - want).abs()
+        assert (off <= 1.1 * (width + 1) * U * size + (6 * U + HALF[dtype]) * want.abs() + FLOOR[dtype]).all(), b
+        assert torch.equal(state[slots[b]].double(), line[c:]), b
