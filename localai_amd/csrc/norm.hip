@@ -3,7 +3,7 @@
 //   h = x + residual (kept in residual);  y = h / sqrt(mean(h^2) + eps) w
 //   y = y z / (1 + exp(-z))  (gate z);  y rounded once, or in Q8_0 blocks:
 //   d = fp16(max |y| / 127) of 32 values, quants rint(y / d), ties to even
-// fp32 throughout.
+// fp32 throughout, but for the sum of the squares of rows that registers do not hold (fp64).
 // Bound by memory: x, the residual and the gate once, the results once (2^24 fp32
 // values in rows of 4096, in and out: 134 MB, 21.6 us, out of the memory's own cache).
 // A row's values stay in registers between the sum and the results.
@@ -83,7 +83,9 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsNorm n) {
     float *res = n.residual ? n.residual + t * n.r_rs + h * n.r_hs : nullptr;
     const T *gate = n.gate ? (const T *)n.gate + t * n.g_rs + h * n.g_hs : nullptr;
     O *out = (O *)n.out + t * n.o_rs + h * n.o_hs;
-    float keep[KEEP][VEC], old[KEEP][VEC], sum = 0.0f;
+    // A lane's squares: sums of up to 16 of them, one for each place of a vector, or in fp64 of longer rows
+    // (equal values of 2^20: one sum was off by 130 roundings).
+    float keep[KEEP][VEC], old[KEEP][VEC], part[VEC] = {}, sum = 0.0f;
     const auto ask = [&](int64_t at, float (&y)[VEC], float (&z)[VEC]) {
         norm_load<T, VEC>(x + at, y);
         if (res) norm_load<float, VEC>(res + at, z);
@@ -95,7 +97,13 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsNorm n) {
             norm_store<float, VEC>(res + at, y);
         }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) sum += y[e] * y[e];
+        for (int e = 0; e < VEC; ++e) part[e] += y[e] * y[e];
+    };
+    const auto parts = [&]() {
+        float y = part[0];
+#pragma unroll
+        for (int e = 1; e < VEC; ++e) y += part[e];
+        return y;
     };
     if constexpr (ITEMS > 0) {
 #pragma unroll
@@ -108,19 +116,26 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsNorm n) {
             const int64_t at = u * step + lane * VEC;
             if (at < dim) take(at, keep[u], old[u]);
         }
-    } else
+        sum = parts();
+    } else {
+        double all = 0.0;
         for (int64_t at = lane * VEC; at < dim; at += step) {
             ask(at, keep[0], old[0]);
             take(at, keep[0], old[0]);
+            all += parts();
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) part[e] = 0.0f;
         }
+        sum = (float)all;
+    }
     sum = group_sum<(TPR < 64 ? TPR : 64)>(sum);
     if constexpr (TPR > 64) {
-        __shared__ float part[TPR / 64];
-        if (lane % 64 == 0) part[lane / 64] = sum;
+        __shared__ float waves[TPR / 64];
+        if (lane % 64 == 0) waves[lane / 64] = sum;
         __syncthreads();
         sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < TPR / 64; ++i) sum += part[i];
+        for (int i = 0; i < TPR / 64; ++i) sum += waves[i];
     }
     const float inv = 1.0f / sqrtf(sum / (float)n.dim + n.eps);
     const auto give = [&](int64_t at, float (&y)[VEC]) {

@@ -204,3 +204,34 @@ def test_conv_of_many_values(counts, channels, width, dtype):
         off = (out[starts[b]:starts[b + 1]].double() - want).abs()
         assert (off <= 1.1 * (width + 1) * U * size + (6 * U + HALF[dtype]) * want.abs() + FLOOR[dtype]).all(), b
         assert torch.equal(state[slots[b]].double(), line[c:]), b
+
+
+# ---------------------------------------------------------------- long rows of the norm
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('kind', ['equal', 'random', 'first'])
+@pytest.mark.parametrize('dim', [4095, 4096, 32768, 100001, (1 << 20) - 1, 1 << 20])
+def test_norm_of_long_rows(dim, kind, dtype):
+    """Rows whose squares' roundings all go one way, or are lost behind a large one. A lane's squares (u each) are summed
+    in runs of at most 16 and 8 of those (23 u), or in 64 bits; lanes and waves in a tree (10 u): half of 34 u reaches the
+    root, root and products are 4 u; in all below 24 u of the result."""
+    import torch
+    from localai_amd import layer
+    gen = torch.Generator('cuda').manual_seed(dim)
+    for value in ([1.1, 0.77, 3.3e-5] if kind == 'equal' else [1.0]):
+        x = torch.full((3, dim), value, device='cuda')
+        if kind != 'equal':
+            x = torch.randn((3, dim), generator=gen, device='cuda')
+        if kind == 'first':
+            x[:, :16] *= 1e4
+        x = x.to(getattr(torch, dtype))
+        w = torch.rand(dim, generator=gen, device='cuda') + 0.5
+        h = x.double()
+        want = h / torch.sqrt((h * h).mean(-1, keepdim=True) + 1e-10) * w.double()
+        got = layer.rms_norm(x, w, eps=1e-10, dtype=torch.float32)
+        off = ((got.double() - want).abs() / want.abs().clamp(min=2.0 ** -100)).max().item()
+        assert off <= 24 * U, (value, off / U)
+        residual = torch.zeros(3, dim, device='cuda')
+        got = layer.rms_norm(x, w, eps=1e-10, residual=residual, dtype=torch.float32)     # (four values a lane)
+        off = ((got.double() - want).abs() / want.abs().clamp(min=2.0 ** -100)).max().item()
+        assert off <= 24 * U, ('residual', value, off / U)
