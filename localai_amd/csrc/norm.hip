@@ -34,6 +34,16 @@ __device__ __forceinline__ void norm_store(T *p, const float (&y)[VEC]) {
     *reinterpret_cast<Raw *>(p) = raw;
 }
 
+// 1 / sqrt(x) to a rounding and 2^-6 of one: an approximation, corrected by what x r r leaves of 1 (a root and
+// a quotient are two roundings, which was an eighth of the result's error). Of 0 and infinity the correction is NaN.
+__device__ __forceinline__ float norm_inverse_root(float x) {
+    const bool tiny = x < 0x1p-100f;     // the approximation takes no subnormal values
+    const float y = tiny ? x * 0x1p100f : x, r = __builtin_amdgcn_rsqf(y);
+    const float t = y * r, low = __builtin_fmaf(y, r, -t);
+    const float z = __builtin_fmaf(0.5f * r, __builtin_fmaf(-low, r, __builtin_fmaf(-t, r, 1.0f)), r);
+    return (z == z ? z : r) * (tiny ? 0x1p50f : 1.0f);
+}
+
 template <int CTRL>
 __device__ __forceinline__ float norm_max_from(float x) {     // with another lane's of the 8
     return fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, false)));
@@ -137,7 +147,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsNorm n) {
 #pragma unroll
         for (int i = 0; i < TPR / 64; ++i) sum += waves[i];
     }
-    const float inv = 1.0f / sqrtf(sum / (float)n.dim + n.eps);
+    const float inv = norm_inverse_root(sum / (float)n.dim + n.eps);
     const auto give = [&](int64_t at, float (&y)[VEC]) {
         float w[VEC];
         if constexpr (Q8) {     // (its weight may be aligned to one value)

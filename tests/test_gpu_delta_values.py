@@ -235,3 +235,26 @@ def test_norm_of_long_rows(dim, kind, dtype):
         got = layer.rms_norm(x, w, eps=1e-10, residual=residual, dtype=torch.float32)     # (four values a lane)
         off = ((got.double() - want).abs() / want.abs().clamp(min=2.0 ** -100)).max().item()
         assert off <= 24 * U, ('residual', value, off / U)
+
+
+def test_norm_rounds_its_inverse_root_once():
+    """Values of 2^-70, whose squares are nothing beside eps: the result is the inverse root of eps, 2^-70 of it. One rounding,
+    and 2^-6 of one for what is left of the approximation; past fp32's middle range, 1e-37 and 1e37, a quotient's too where it is
+    computed so and, as their square 2^-140 is 2^-17 of 1e-37, half of the sum's: 2.5 u; 2^-70 / sqrt(1e37) = 2.7e-40 is subnormal, rounded to
+    steps of 2^-149: half of one, 2^70 times, besides."""
+    import torch
+    from localai_amd import layer
+    rng = np.random.default_rng(0)
+    x, w = torch.full((1, 64), 2.0 ** -70, device='cuda'), torch.ones(64, device='cuda')
+    eps = np.concatenate([np.float32(10.0) ** rng.uniform(-30, 30, 300).astype(np.float32), np.float32([1, 2, 3, 0.25, 1e-37, 1e37])])
+    got = torch.stack([layer.rms_norm(x, w, eps=float(e))[0, 0] for e in eps])
+    want = 1 / np.sqrt(eps.astype(np.float64) + 2.0 ** -140)
+    off = np.where((eps >= 1e-30) & (eps <= 1e30), 1 + 2.0 ** -6, 2.5) * U * want + 2.0 ** (70 - 150) * (want < 2.0 ** (70 - 126))
+    assert (np.abs(_np(got) * 2.0 ** 70 - want) <= off).all()
+    x[:] = 0
+    for e in (0.0, 1e-45, 3e38):
+        y = _np(layer.rms_norm(x, w, eps=e))
+        assert np.isnan(y).all() if e == 0 else not y.any()      # 0 / 0
+    x[:] = 1
+    np.testing.assert_allclose(_np(layer.rms_norm(x, w, eps=3e38)), 1 / np.sqrt(3e38), rtol=3 * U)
+    assert not _np(layer.rms_norm(x * 1e30, w)).any()             # squares past fp32: 1 / inf
