@@ -443,7 +443,9 @@ int64_t localai_hip_delta_rule_workspace_size(int64_t tokens, int64_t requests, 
  * 22 bits of values within 2^24 of the largest of their row, column or 64 tokens, of smaller
  * ones 2^-46 of that, and where a v needs more, the 64 tokens it is among go token by token; out is
  * rounded once. A state that could grow by itself (g > 0.01, b < 0 or b |k^|^2 > 2)
- * and values past 1e15 cost the 64 tokens they are among each a token's own time.
+ * q and k of a length past 1e15, v and products of the state with k past 1e30 cost the 64 tokens
+ * they are among each a token's own time. Squares of q and k are summed in fp32: a row whose
+ * sum passes its range, or is 0 with a norm_eps of 0, has no defined result.
  * What is not finite reaches the tokens behind it, of a v the one column alone,
  * and none before it; which of NaN and infinity they show is not defined. */
 int localai_hip_delta_rule(const void *q_dev, const void *k_dev, const void *v_dev, int type,

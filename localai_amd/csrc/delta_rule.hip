@@ -34,8 +34,8 @@ __device__ __forceinline__ int rule_key_head(const DeltaRule &p, int h) {
 // of S in registers, each lane 4 adjacent columns of KD VS / 1024 rows. With
 // S' = e^g S, one pass over the rows gives S'^T k and S'^T q; the token's result
 // needs no second one: o = S'^T q^ + d (k^ . q^). Bound by memory, the state in and
-// out once: 256 requests of 32 heads of 128 x 128, fp32, 1.07 GB in 211 us, 5.1 TB/s;
-// 16 16.7 us, 4.0 TB/s. One request: latency, 5.4 us. (States of other layers between, so none is in a cache.)
+// out once: 256 requests of 32 heads of 128 x 128, fp32, 1.07 GB in 204 us, 5.3 TB/s;
+// 16 17.5 us, 3.8 TB/s. One request: latency, 5.3 us. (States of other layers between, so none is in a cache.)
 template <typename T, int KD, int VS>
 __global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequests r, int most) {
     constexpr int LPR = VS / 4, RW = 64 / LPR, NR = KD * VS / 1024;   // lanes a row, rows a wave's pass, passes
@@ -60,17 +60,17 @@ __global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequ
     T *op = (T *)p.out + (int64_t)span.first * p.o_ts + h * p.o_hs + c0 + c;
     for (int t = 0; t < span.count; ++t) {
         const int par = t & 1;
-        // each wave sums the squares for itself; one of them leaves k, one q
+        // each wave sums the squares for itself; one of them leaves k^, one q^ (products with k and q as they are
+        // could leave fp32's range where the results do not)
         constexpr int E = KD / 64;
-        float kk = 0.0f, qq = 0.0f, kdq = 0.0f;
+        float kv[E], qv[E], kk = 0.0f, qq = 0.0f, kdq = 0.0f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const float kv = (float)kp[t * p.k_ts + lane * E + e], qv = (float)qp[t * p.q_ts + lane * E + e];
-            if (w == 0) kq[par][0][lane * E + e] = kv;
-            if (w == 1) kq[par][1][lane * E + e] = qv;
-            kk += kv * kv;
-            qq += qv * qv;
-            kdq += kv * qv;
+            kv[e] = (float)kp[t * p.k_ts + lane * E + e];
+            qv[e] = (float)qp[t * p.q_ts + lane * E + e];
+            kk += kv[e] * kv[e];
+            qq += qv[e] * qv[e];
+            kdq += kv[e] * qv[e];
         }
         const float2 gb = rule_gates(p, span.first + t, h);
         const float4 v = delta_load4(vp + t * p.v_ts);
@@ -79,6 +79,11 @@ __global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequ
         kdq = group_sum<64>(kdq);
         const float ik = p.norm_eps >= 0.0f ? 1.0f / sqrtf(kk + p.norm_eps) : 1.0f;
         const float iq = (p.norm_eps >= 0.0f ? 1.0f / sqrtf(qq + p.norm_eps) : 1.0f) * p.scale;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (w == 0) kq[par][0][lane * E + e] = kv[e] * ik;
+            if (w == 1) kq[par][1][lane * E + e] = qv[e] * iq;
+        }
         const float f = expf(gb.x);
         __syncthreads();
         float4 pk = make_float4(0, 0, 0, 0), pq = pk;
@@ -110,21 +115,21 @@ __global__ __launch_bounds__(256) void delta_token_kernel(DeltaRule p, DeltaRequ
             pk.x += x.x; pk.y += x.y; pk.z += x.z; pk.w += x.w;
             pq.x += y.x; pq.y += y.y; pq.z += y.z; pq.w += y.w;
         }
-        const float4 d = make_float4((v.x - pk.x * ik) * gb.y, (v.y - pk.y * ik) * gb.y, (v.z - pk.z * ik) * gb.y,
-                                     (v.w - pk.w * ik) * gb.y);
+        const float4 d = make_float4((v.x - pk.x) * gb.y, (v.y - pk.y) * gb.y, (v.z - pk.z) * gb.y, (v.w - pk.w) * gb.y);
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
-            const float kr = kq[par][0][i * 4 * RW + row0] * ik;
+            const float kr = kq[par][0][i * 4 * RW + row0];
             S[i].x += kr * d.x; S[i].y += kr * d.y; S[i].z += kr * d.z; S[i].w += kr * d.w;
         }
         if (tid < LPR) {
             const float x = kdq * ik * iq;
-            delta_store4(op + t * p.o_ts, make_float4(pq.x * iq + d.x * x, pq.y * iq + d.y * x, pq.z * iq + d.z * x,
-                                                      pq.w * iq + d.w * x));
+            delta_store4(op + t * p.o_ts, make_float4(pq.x + d.x * x, pq.y + d.y * x, pq.z + d.z * x, pq.w + d.w * x));
         }
     }
+    // Not read again in this step, so past the caches: as they are, and past them, 12 requests in states of 24 layers 13.1,
+    // 12.7 us, 70 57.2, 57.4, 128 98.0, 101.7, 256 200, 203; 70 in the same states again and again 59.5, 57.2.
 #pragma unroll
-    for (int i = 0; i < NR; ++i)     // (not read again in this step: past the caches, 70 requests 61.3 us in place of 62.2, 256 211, 207)
+    for (int i = 0; i < NR; ++i)
         __builtin_nontemporal_store(lq_f4{S[i].x, S[i].y, S[i].z, S[i].w},
                                     reinterpret_cast<lq_f4 *>(state + (int64_t)i * 4 * RW * p.vd));
 }
@@ -166,7 +171,7 @@ typedef uint32_t dr_u2 __attribute__((ext_vector_type(2)));
 constexpr int PIECE = 64;
 constexpr int TRI = 6;                 // 16 x 32 blocks of a lower triangular 64 x 64: row tile w has w / 2 + 1
 // W's and P T's bounds hold while a state cannot grow: beta |k^|^2 <= 2 and g <= 0, but for roundings
-constexpr float RULE_WILD = 1e15f;     // values of q, k, v (squared: of S) past it go token by token
+constexpr float RULE_WILD = 1e15f;     // q and k longer than it, and R (v, and S times k) past its square, go token by token
 constexpr float RULE_SQUARE = 1e-36f;   // more than what 256 squares lose below fp32's range
 constexpr float RULE_FAINT = 1e-24f;   // so do k and q whose squares' sum is below it, where norm_eps is too
 
@@ -1074,21 +1079,25 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
         for (int t = 0; t < n; ++t) {
             const int par = t & 1;
             constexpr int E = KD / 64;
-            float kk = 0.0f, qq = 0.0f, kdq = 0.0f;
+            float kv[E], qv[E], kk = 0.0f, qq = 0.0f, kdq = 0.0f;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float kv = (float)kp[t * p.k_ts + lane * E + e], qv = (float)qp[t * p.q_ts + lane * E + e];
-                if (w == 0) kq[par][0][lane * E + e] = kv;
-                if (w == 1) kq[par][1][lane * E + e] = qv;
-                kk += kv * kv;
-                qq += qv * qv;
-                kdq += kv * qv;
+                kv[e] = (float)kp[t * p.k_ts + lane * E + e];
+                qv[e] = (float)qp[t * p.q_ts + lane * E + e];
+                kk += kv[e] * kv[e];
+                qq += qv[e] * qv[e];
+                kdq += kv[e] * qv[e];
             }
             kk = group_sum<64>(kk);
             qq = group_sum<64>(qq);
             kdq = group_sum<64>(kdq);
             const float nk = p.norm_eps >= 0.0f ? 1.0f / sqrtf(kk + p.norm_eps) : 1.0f;
             const float nq = (p.norm_eps >= 0.0f ? 1.0f / sqrtf(qq + p.norm_eps) : 1.0f) * p.scale;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                if (w == 0) kq[par][0][lane * E + e] = kv[e] * nk;
+                if (w == 1) kq[par][1][lane * E + e] = qv[e] * nq;
+            }
             const float2 gb = rule_gates(p, row0 + t, h);
             const float f = expf(gb.x), v = (float)vp[t * p.v_ts];
             __syncthreads();
@@ -1111,12 +1120,12 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
             __syncthreads();
             pk = (red[par][0][0][m] + red[par][1][0][m]) + (red[par][2][0][m] + red[par][3][0][m]);
             pq = (red[par][0][1][m] + red[par][1][1][m]) + (red[par][2][1][m] + red[par][3][1][m]);
-            const float d = (v - pk * nk) * gb.y;
+            const float d = (v - pk) * gb.y;
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) S[i][e] += kq[par][0][Keys::at(w * NT + i, 4 * g + e)] * nk * d;
-            if (threadIdx.x < 16) op[(int64_t)t * p.o_ts] = (T)(pq * nq + d * (kdq * nk * nq));
+                for (int e = 0; e < 4; ++e) S[i][e] += kq[par][0][Keys::at(w * NT + i, 4 * g + e)] * d;
+            if (threadIdx.x < 16) op[(int64_t)t * p.o_ts] = (T)(pq + d * (kdq * nk * nq));
         }
         ++j;     // (the operands' places are the next piece's already)
     }
@@ -1155,10 +1164,9 @@ template <typename T, int KD>
 static void token_columns(const DeltaRule &p, const DeltaRequests &r, int most, hipStream_t s) {
     // Value columns of the call: few go in narrow slices, for the workgroups' number, many in wider
     // ones, for the rows' length in memory. Heads of 128 x 128, one token of each request, the states of many
-    // layers one behind the other, so that none is in a cache; columns -> us of slices of 32, 64, 128: 2^12 5.5,
-    // 5.7, 6.7; 2^14 8.0, 7.9, 8.5; 2^16 18.8, 16.8, 17.3; 2^18 56.0, 56.8, 58.5; 2^19 108.7, 106.9,
-    // 109.9; 2^20 220, 211, 220. (128 are ahead only where the same 150 MB are called
-    // again and again; 16 are for value_dims of no multiple of 32.)
+    // layers one behind the other, so that none is in a cache; columns -> us of slices of 32, 64, 128: 2^12 5.3,
+    // 5.6, 6.6; 2^14 7.8, 7.8, 8.5; 2^16 17.9, 17.5, 17.0; 2^18 54.3, 52.8, 55.8; 2^19 105.5, 101.8,
+    // 106.7; 2^20 216, 203, 218. (16 are for value_dims of no multiple of 32.)
     const int64_t all = (int64_t)r.requests * p.value_heads * p.vd;
     if (p.vd % 64 == 0 && all >= 1 << 14) token_launch<T, KD, 64>(p, r, most, s);
     else if (p.vd % 32 == 0) token_launch<T, KD, 32>(p, r, most, s);

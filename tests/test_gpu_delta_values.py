@@ -258,3 +258,25 @@ def test_norm_rounds_its_inverse_root_once():
     x[:] = 1
     np.testing.assert_allclose(_np(layer.rms_norm(x, w, eps=3e38)), 1 / np.sqrt(3e38), rtol=3 * U)
     assert not _np(layer.rms_norm(x * 1e30, w)).any()             # squares past fp32: 1 / inf
+
+
+@pytest.mark.parametrize('dtype', ['float32', 'bfloat16'])
+@pytest.mark.parametrize('q_size,k_size,v_size', [(3e13, 3e13, 1e28), (1e14, 3e15, 1), (3e15, 1e14, 1), (1e17, 1e17, 1e29),
+                                                  (1, 1, 3e31), (1, 1, 1e34), (1e-12, 1e14, 1e-30)])
+@pytest.mark.parametrize('n', [150, 7])     # in pieces, token by token
+def test_rule_on_both_sides_of_its_largest_values(n, q_size, k_size, v_size, dtype):
+    """Lengths of q and k around 1e15, v around 1e30; the rule is the same but for v's factor."""
+    import torch
+    from localai_amd import delta
+    rng = np.random.default_rng(1)
+    q, k, v = (torch.tensor(rng.standard_normal((n, h, d)) * s, dtype=torch.float32).to(getattr(torch, dtype)).cuda()
+               for h, d, s in ((1, 128, q_size), (1, 128, k_size), (2, 32, v_size)))
+    g, b = (torch.tensor(x, dtype=torch.float32, device='cuda') for x in (-rng.exponential(0.05, (n, 2)), rng.random((n, 2))))
+    state = torch.tensor(rng.standard_normal((1, 2, 128, 32)) * 0.1 * v_size, dtype=torch.float32, device='cuda')
+    qv, kv, vv, gv, bv, sv = (_np(x) for x in (q, k, v, g, b, state[0]))
+    got = _np(delta.rule(q, k, v, g, b, state, starts=_ints([0, n]), norm_eps=0))
+    qv, kv = (x / np.sqrt((x * x).sum(-1, keepdims=True)) for x in (qv, kv))
+    for h in range(2):
+        want, after, off, off_state = _columns(sv[h], qv[:, 0], kv[:, 0], vv[:, h], gv[:, h], bv[:, h], 128 ** -0.5)
+        assert (np.abs(got[:, h] - want) <= off + (HALF[dtype] * np.abs(want) if dtype != 'float32' else 0)).all()
+        assert (np.linalg.norm(_np(state[0, h]) - after, axis=0) <= off_state).all()
