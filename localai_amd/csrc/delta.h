@@ -104,6 +104,30 @@ __device__ __forceinline__ int delta_request(const DeltaRequests &r, int piece, 
     return -1;     // (not reached: the last 64 have one behind the last request)
 }
 
+// The same for requests of `least` rows or more alone, whose piece j, of 64 rows, has the number (starts[b] >> shift)
+// + b + j, with shift 6, or (starts[b] >> shift) + j (`many`), with a shift for which 2^shift <= least <= 32: n >= least rows
+// have no more pieces than n >> shift, so these numbers are below tokens >> shift however many requests there are.
+__device__ __forceinline__ int delta_long_request(const DeltaRequests &r, int piece, int least, int shift, bool many,
+                                                  DeltaSpan *span) {
+    const int lane = (int)(threadIdx.x & 63);
+    int b = -1;
+    for (int at = 0; at < r.requests; at += 64) {
+        const int i = min(at + lane, r.requests - 1);
+        const int start = min(max(r.starts[i], 0), r.tokens), end = min(max(r.starts[i + 1], start), r.tokens);
+        const int slot = r.slots ? r.slots[i] : i, length = r.lengths ? r.lengths[i] : INT32_MAX;
+        const int number = (start >> shift) + (many ? 0 : i);
+        const auto found = __ballot(at + lane < r.requests && end - start >= least && number <= piece);
+        const auto of = [](int x, int l) { return __builtin_amdgcn_readlane(x, l); };
+        if (found) {
+            const int l = 63 - __clzll(found), first = of(start, l), rows = of(end, l) - first, s = of(slot, l);
+            b = at + l;
+            *span = DeltaSpan{first, s >= 0 && s < r.n_slots ? rows : 0, s, of(length, l) <= rows};
+        }
+        if (of(number, 63) > piece) break;
+    }
+    return b;
+}
+
 // y / (1 + exp(-y)) to a few fp32 roundings: the exponent's argument in two parts
 // (its rounding alone would cost |y| of them), a reciprocal corrected once. A third
 // of the instructions of expf and a division, which bound 16-bit rows of the

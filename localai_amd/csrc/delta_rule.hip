@@ -204,7 +204,13 @@ struct RuleWork {
     uint32_t rows;         // [piece, value head][3][64] fp32: e^G / |k|, scale e^G / |q|, RULE_LAST ..
     int first, pieces;     // the window
     int least;             // requests of fewer tokens are the token kernel's
+    int shift;             // of delta_long_request's numbers
+    bool many;
+    bool by_piece;         // a chain for each piece of the window that is a request's first there, not for each request
 };
+
+// the number of a request's first piece
+__device__ __forceinline__ int rule_base(const RuleWork &ws, int first, int b) { return (first >> ws.shift) + (ws.many ? 0 : b); }
 
 __device__ __forceinline__ float dr_rows_sum(float v) {     // over lanes l, l ^ 16, l ^ 32, l ^ 48
     const auto f = [](uint32_t u) { return __builtin_bit_cast(float, u); };
@@ -326,10 +332,10 @@ __global__ __launch_bounds__(256, RULE_NP<T> == 1 ? 2 : 1) void delta_piece_kern
     __shared__ int wild_s[4];
     const int local = (int)(blockIdx.x / p.key_heads), kh = (int)(blockIdx.x % p.key_heads);
     DeltaSpan span;
-    const int piece = ws.first + local, b = delta_request(r, piece, PIECE, &span);
+    const int piece = ws.first + local, b = delta_long_request(r, piece, ws.least, ws.shift, ws.many, &span);
     if (b < 0) return;
-    const int j0 = (piece - (span.first / PIECE + b)) * PIECE, n = min(span.count - j0, PIECE);
-    if (j0 < 0 || n <= 0 || span.count < ws.least) return;
+    const int j0 = (piece - rule_base(ws, span.first, b)) * PIECE, n = min(span.count - j0, PIECE);
+    if (j0 < 0 || n <= 0) return;
     const int w = wave_id(), lane = lane_id(), m = lane & 15, g = lane >> 4;
     const int group = p.value_heads / p.key_heads, gi = blockIdx.y;
     const int h = p.tiled ? gi * p.key_heads + kh : kh * group + gi;
@@ -745,11 +751,16 @@ __global__ __launch_bounds__(RULE_CHAIN, 1) void delta_chain_kernel(DeltaRule p,
     const int group = p.value_heads / p.key_heads, slices = p.vd / 16;
     // a key head's workgroups on one XCD: they read the same operands
     const int xcd = blockIdx.x & 7, in = blockIdx.x >> 3, unit = in / (group * slices) * 8 + xcd, rest = in % (group * slices);
-    if (unit >= r.requests * p.key_heads) return;
-    const int b = unit / p.key_heads, kh = unit % p.key_heads, gi = rest / slices, c0 = rest % slices * 16;
-    const DeltaSpan span = delta_span(r, b);
-    if (!span.count || span.count < ws.least) return;
-    const int base = span.first / PIECE + b, pieces = (span.count + PIECE - 1) / PIECE;
+    if (unit >= (ws.by_piece ? ws.pieces : r.requests) * p.key_heads) return;
+    const int own = unit / p.key_heads, kh = unit % p.key_heads, gi = rest / slices, c0 = rest % slices * 16;
+    DeltaSpan span;
+    int b = own;
+    if (ws.by_piece) b = delta_long_request(r, ws.first + own, ws.least, ws.shift, ws.many, &span);
+    else span = delta_span(r, b);
+    if (b < 0 || !span.count || span.count < ws.least) return;
+    const int base = rule_base(ws, span.first, b);
+    if (ws.by_piece && own && ws.first + own != base) return;      // an earlier piece's chain has it
+    const int pieces = (span.count + PIECE - 1) / PIECE;
     const int from = max(ws.first - base, 0), to = min(ws.first + ws.pieces - base, pieces);
     if (from >= to) return;
     const int w = wave_id(), lane = lane_id(), m = lane & 15, g = lane >> 4;
@@ -1144,14 +1155,33 @@ static int64_t key_bytes(int np, int kd) { return 4 * (kd == 64 ? 4 : kd / 32) *
 static int64_t piece_bytes(int np, int key_heads, int value_heads, int kd) {
     return 2 * key_heads * key_bytes(np, kd) + value_heads * ((kd / 16 * 2 + TRI) * 2 * 1024 + 12 * PIECE);
 }
-static int64_t all_pieces(int64_t tokens, int requests) { return tokens / PIECE + requests; }
+
+// Requests of fewer tokens go token by token: for each, that takes a token's latency, or its share of
+// the vector units, and a chain its start and the piece's operands. With 32 heads of 128, us of n tokens
+// a request in pieces and token by token, by workgroups of the chain: 256 (one request) 8: 16.2, 15.6,
+// 12: 16.2, 21.4; 1024 8: 28, 18, 16: 28, 30; 2048 16: 46, 33, 24: 47, 47; 8192 16: 140, 93, 24: 141, 132,
+// 32: 142, 190.
+static int rule_least(int requests, int value_heads, int vd) {
+    const int64_t groups = (int64_t)requests * value_heads * (vd / 16);
+    return (int)std::min<int64_t>(std::max<int64_t>(groups / 80, 9), 25);
+}
+// Numbers of pieces, by rows and requests, or by rows alone where that is fewer (a step of one token each of 256
+// requests: 16, not 260; with the chains of these 225 us, 680 with those of 260 and of each request in each window;
+// without starts 217).
+static int many_shift(int least) { return least >= 16 ? 4 : 3; }
+static bool many_requests(int64_t tokens, int requests, int least) {
+    return requests > 1 && tokens >> many_shift(least) < tokens / PIECE + requests;
+}
+static int64_t all_pieces(int64_t tokens, int requests, int least) {
+    return many_requests(tokens, requests, least) ? std::max<int64_t>(tokens >> many_shift(least), 1) : tokens / PIECE + requests;
+}
 
 // room for a window of fp32's pieces; 16-bit types' are smaller, so theirs may be longer
 int64_t delta_rule_workspace_bytes(int64_t tokens, int requests, bool step, int key_heads, int value_heads, int kd,
                                    int vd) {
     if (step) return 0;
-    const int64_t bytes = piece_bytes(2, key_heads, value_heads, kd), all = all_pieces(tokens, requests);
-    return std::min(all, std::max<int64_t>(RULE_WINDOW / bytes, 1)) * bytes;
+    const int64_t bytes = piece_bytes(2, key_heads, value_heads, kd);
+    return std::min(all_pieces(tokens, requests, rule_least(requests, value_heads, vd)), std::max<int64_t>(RULE_WINDOW / bytes, 1)) * bytes;
 }
 
 template <typename T, int KD, int VS>
@@ -1177,15 +1207,10 @@ template <typename T, int KD>
 static void rule_launch(const DeltaRule &p, const DeltaRequests &r, void *ws, hipStream_t s) {
     if (!r.starts) return token_columns<T, KD>(p, r, INT32_MAX, s);
     constexpr int NP = RULE_NP<T>;
-    // Requests of fewer tokens go token by token: for each, that takes a token's latency, or its share of
-    // the vector units, and a chain its start and the piece's operands. With 32 heads of 128, us of n tokens
-    // a request in pieces and token by token, by workgroups of the chain: 256 (one request) 8: 16.2, 15.6,
-    // 12: 16.2, 21.4; 1024 8: 28, 18, 16: 28, 30; 2048 16: 46, 33, 24: 47, 47; 8192 16: 140, 93, 24: 141, 132,
-    // 32: 142, 190.
-    const int64_t groups = (int64_t)r.requests * p.value_heads * (p.vd / 16);
-    const int least = (int)std::min<int64_t>(std::max<int64_t>(groups / 80, 9), 25);
+    const int least = rule_least(r.requests, p.value_heads, p.vd);
     if (r.tokens < least) return token_columns<T, KD>(p, r, INT32_MAX, s);
-    const int64_t bytes = piece_bytes(NP, p.key_heads, p.value_heads, KD), all = all_pieces(r.tokens, r.requests);
+    static_assert(PIECE == 1 << 6);
+    const int64_t bytes = piece_bytes(NP, p.key_heads, p.value_heads, KD), all = all_pieces(r.tokens, r.requests, least);
     const int64_t window = std::min(all, delta_rule_workspace_bytes(r.tokens, r.requests, false, p.key_heads, p.value_heads, KD, p.vd) / bytes);
     RuleWork w{};
     const int64_t keys = window * p.key_heads * key_bytes(NP, KD), tiles = window * p.value_heads * 2 * 1024;
@@ -1199,6 +1224,8 @@ static void rule_launch(const DeltaRule &p, const DeltaRequests &r, void *ws, hi
     w.bytes = (uint32_t)(window * bytes);
     // (one request's tokens are the call's, or fewer by a few: its pieces serve any number)
     w.least = r.requests > 1 ? least : 1;
+    w.many = many_requests(r.tokens, r.requests, least);
+    w.shift = w.many ? many_shift(least) : 6;
     if (w.least > 1) token_columns<T, KD>(p, r, w.least - 1, s);
     const int group = p.value_heads / p.key_heads;
     for (int64_t first = 0; first < all; first += window) {
@@ -1206,7 +1233,8 @@ static void rule_launch(const DeltaRule &p, const DeltaRequests &r, void *ws, hi
         w.pieces = (int)(all - first < window ? all - first : window);
         const dim3 grid((unsigned)(w.pieces * p.key_heads), (unsigned)group);
         hipLaunchKernelGGL((delta_piece_kernel<T, KD>), grid, dim3(256), 0, s, p, r, w);
-        const int64_t units = ((int64_t)r.requests * p.key_heads + 7) / 8 * 8;
+        w.by_piece = r.requests > w.pieces;
+        const int64_t units = ((int64_t)(w.by_piece ? w.pieces : r.requests) * p.key_heads + 7) / 8 * 8;
         hipLaunchKernelGGL((delta_chain_kernel<T, KD>), dim3((unsigned)(units * group * (p.vd / 16))), dim3(RULE_CHAIN), 0, s, p, r,
                            w);
     }

@@ -738,3 +738,35 @@ def test_refusals_on_the_device():
                           (dict(x=x.reshape(2, 2, 4, 16)), ValueError), (dict(out=x.half()), TypeError)]:
         with pytest.raises(error):
             layer.rms_norm(**{**dict(x=x, weight=w.reshape(-1)[:64]), **change})
+
+
+# ---------------------------------------------------------------- steps of many requests, with starts
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('n', [25, 64, 65, 200])
+def test_rule_one_token_each_with_starts(n, dtype):
+    """A decoding step as paged.extend's tables have it, some requests without a token."""
+    counts = [1] * n
+    counts[3], counts[n - 2] = 0, 0
+    _check_rule((2, 4, 128, 32), counts, dtype, True, 'grouped')
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_rule_many_requests_with_prompts_among_them(dtype):
+    """Pieces numbered by rows alone: prompts of every length beside single tokens, at the ends of 64 requests too."""
+    rng = np.random.default_rng(5)
+    counts = [1] * 260
+    for b in (0, 63, 64, 65, 127, 128, 200, 259):
+        counts[b] = int(rng.choice([24, 25, 26, 49, 50, 63, 64, 65, 100, 129, 200]))
+    counts[30:50] = [0] * 20
+    _check_rule((1, 4, 64, 64), counts, dtype, True, 'grouped')
+    _check_rule((1, 4, 64, 64), [25] * 70, dtype, True, 'grouped')
+    _check_rule((1, 4, 64, 64), [64] * 3 + [24] * 100 + [65, 64, 25, 128], dtype, True, 'tiled')
+
+
+@pytest.mark.parametrize('dtype', ['float32', 'bfloat16'])
+@pytest.mark.parametrize('counts', [[1] * 60 + [30] * 20 + [100] * 10 + [400] + [1] * 9, [90] * 28 + [400, 1], [2500] + [1] * 40],
+                         ids=['by rows', 'by rows and requests', 'one long'])
+def test_rule_more_requests_than_a_window_has_pieces(counts, dtype):
+    """Windows of 20 pieces and more (128 heads); requests that begin, go on and end in any of them."""
+    _check_rule((8, 128, 128, 16), counts, dtype, True, 'grouped')
