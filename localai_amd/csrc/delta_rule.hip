@@ -311,7 +311,7 @@ __device__ __forceinline__ double dr_add_from(double v) {
 // 16 w .. 16 w + 15. An operand's lane l holds row or column l & 15 and of each
 // 32 contracted values x the eight 4 (l >> 4) + 0..3 and 16 + 4 (l >> 4) + 0..3:
 // the layout in which MFMA leaves two tiles of results, so those are operands
-// as they are. Bound by latency and LDS: eleven barriers between products of one or
+// as they are. Bound by latency and LDS: ten barriers between products of one or
 // two tiles a wave, four workgroups a CU (37 KB of LDS each); 8192 tokens of 16/32 heads
 // of 128, bf16: 100 us for 4096 workgroups, 0.3 GB of workspace written.
 template <typename T, int KD>
@@ -729,8 +729,8 @@ struct RuleValues {
 // values Q's pieces for one tile are what the registers hold). The last two bring
 // v and factors, of every other piece each: from HBM, it takes longer than a piece (of 256 key
 // values the waves with the outputs do: a tenth wave would cost the others registers).
-// Bound by that chain of exchanges: two barriers a piece, 1.55 us of 64 tokens (8192
-// tokens, 32 heads of 128, bf16: 128 pieces one behind the other, 200 us; 16 columns a workgroup, so that
+// Bound by that chain: two barriers a piece, 1.3 to 1.6 us of 64 tokens (8192
+// tokens, 32 heads of 128, bf16: 128 pieces one behind the other, 170 to 200 us of 273; 16 columns a workgroup, so that
 // one request's heads fill the chip: 256 workgroups). Each operand of the next piece is requested as soon as this
 // piece's has been used; nothing between a request and its use is conditional, so
 // the compiler's count of what is in flight is exact.
