@@ -770,3 +770,41 @@ def test_rule_many_requests_with_prompts_among_them(dtype):
 def test_rule_more_requests_than_a_window_has_pieces(counts, dtype):
     """Windows of 20 pieces and more (128 heads); requests that begin, go on and end in any of them."""
     _check_rule((8, 128, 128, 16), counts, dtype, True, 'grouped')
+
+
+def test_captured_step_takes_any_lengths():
+    """One graph of 100 requests and 256 tokens, replayed with other tables: single tokens, a prompt among them, all prompts."""
+    import torch
+    from localai_amd import delta
+    rng = np.random.default_rng(15)
+    n, tokens = 100, 256
+    q, k, v, decay, beta, a, dt = _rule_inputs(rng, tokens, (2, 4, 128, 64), 'bfloat16', True)
+    first, _ = _random(rng, (n, 4, 128, 64), 'float32')
+    starts, lengths, state = _ints([0] * (n + 1)), _ints([500] * n), first.clone()
+    out = torch.zeros((tokens, 4, 64), dtype=v.dtype, device='cuda')
+    run = lambda: delta.rule(q, k, v, decay, beta, state, None, starts, lengths, a, dt, out=out)
+    run()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        run()
+    for counts in ([1] * n, [1] * 50 + [157] + [1] * 49, [25] * 10 + [0] * 89 + [6], [0] * 99 + [256], [24, 0] * 10 + [0] * 80, [1] * n):
+        starts.copy_(_ints(np.concatenate([[0], np.cumsum(counts)])))
+        results = []
+        for call in (g.replay, run):
+            state.copy_(first)
+            out.fill_(7)
+            call()
+            torch.cuda.synchronize()
+            results.append((out.clone(), state.clone()))
+        for got, expected in zip(*results):
+            assert torch.equal(got, expected)
+        assert (results[0][0][sum(counts):] == 7).all() and torch.isfinite(results[0][0]).all()
+        at = 0
+        for b, c in enumerate(counts):
+            if c > 1:
+                rows = slice(at, at + c)
+                alone = first[b:b + 1].clone()
+                y = delta.rule(q[rows], k[rows], v[rows], decay[rows], beta[rows], alone, starts=_ints([0, c]), a=a, dt_bias=dt)
+                torch.testing.assert_close(results[0][0][rows].float(), y.float(), rtol=4 * HALF['bfloat16'], atol=1e-4)
+                torch.testing.assert_close(results[0][1][b:b + 1], alone, rtol=1e-4, atol=1e-4)
+            at += c
